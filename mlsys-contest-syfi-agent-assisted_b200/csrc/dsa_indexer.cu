@@ -31,6 +31,7 @@
 #include "dsa_bins.h"
 #include "moe_internal.h"
 #include "ptx.cuh"
+#include "stream_scratch.h"
 
 namespace syfi {
 
@@ -576,40 +577,6 @@ dsa_select_kernel(const float* __restrict__ scores, const uint2* __restrict__ ra
   for (int i = k + tid; i < kKeep; i += kSelectThreads) o[i] = -1;
 }
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-typedef CUresult (*IsCapturingFn)(CUstream, CUstreamCaptureStatus*);
-typedef CUresult (*StreamIdFn)(CUstream, unsigned long long*);
-
-// Driver functions without a link to libcuda.  (The runtime has the two on streams as well; it takes 40 ns for each instead
-// of 11, and a short batch is bound by the host's part of the call.)
-struct Driver {
-  EncodeTiledFn encode_tiled = nullptr;
-  IsCapturingFn is_capturing = nullptr;
-  StreamIdFn stream_id = nullptr;
-};
-
-template <typename Fn>
-void driver_fn(const char* name, Fn* fn) {
-  void* p = nullptr;
-  cudaDriverEntryPointQueryResult q;
-  if (cudaGetDriverEntryPoint(name, &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
-    *fn = reinterpret_cast<Fn>(p);
-}
-
-const Driver& driver() {
-  static Driver d;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    driver_fn("cuTensorMapEncodeTiled", &d.encode_tiled);
-    driver_fn("cuStreamIsCapturing", &d.is_capturing);
-    driver_fn("cuStreamGetId", &d.stream_id);
-  });
-  return d;
-}
-
 // rows of 128 bytes, boxes of 64 rows, 128-byte swizzle
 bool rows128_map(CUtensorMap* m, const void* base, uint64_t rows) {
   const EncodeTiledFn fn = driver().encode_tiled;
@@ -666,23 +633,9 @@ cudaError_t launch_select(const float* scores, const uint2* ranges, int runs, in
   return c16 == 1 ? run(launch_select_as<16, false>, 1) : run(launch_select_as<16, true>, c16);
 }
 
-// The scores of every token of every sequence with their ranges, one buffer per stream: calls on one stream follow each
-// other, calls on two may run at the same time.  A stream is known by its id, which is never given out twice (a handle
-// may be, after the stream was destroyed); a stream that is being captured cannot be asked for it and is known by its
-// handle.
-struct Scratch {
-  cudaStream_t handle = nullptr;
-  unsigned long long id = 0; // 0: not known yet
-  uint64_t last_use = 0;     // 0: free
-  float* scores = nullptr;
-  size_t floats = 0;
-  bool captured = false;     // a graph may use it
-};
-constexpr int kMaxScratch = 8;   // streams of a device that hold one at a time; the next one takes over the least recently used
-
+// Scratch: the scores of every token of every sequence with their ranges.
 struct Device {
-  Scratch scratch[kMaxScratch];
-  uint64_t calls = 0;
+  ScratchPool scratch;
   int* status = nullptr;
   long long next_wait_limit = 0;   // syfi_dsa_debug_wait_limit: applies to the next call, then clears itself
   bool checked = false;
@@ -692,80 +645,6 @@ std::mutex g_mu;
 Device g_devices[64];
 
 int fail(int code, const char* msg) { return set_last_error(code, msg); }
-
-// Allocation must not end a capture that is going on, on this stream or another.
-struct RelaxedCapture {
-  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-  RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
-  ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
-};
-
-// The stream's buffer of at least `need` floats; null with the error code in *rc when there is none.
-Scratch* scratch_of(Device& d, cudaStream_t st, size_t need, int* rc) {
-  const Driver& drv = driver();
-  CUstreamCaptureStatus capture = CU_STREAM_CAPTURE_STATUS_NONE;
-  unsigned long long id = 0;
-  bool known = drv.is_capturing && drv.stream_id;
-  if (known && drv.is_capturing(st, &capture) != CUDA_SUCCESS) capture = CU_STREAM_CAPTURE_STATUS_NONE;   // the default stream beside a capture: the launch will say so
-  const bool capturing = capture != CU_STREAM_CAPTURE_STATUS_NONE;
-  if (known && !capturing) known = drv.stream_id(st, &id) == CUDA_SUCCESS;
-  if (!known) {
-    *rc = fail(SYFI_DSA_ERR_CUDA, "not a stream of the current device");
-    return nullptr;
-  }
-  // The stream's own; of two (below) the larger.
-  Scratch *s = nullptr, *spare = nullptr;
-  for (Scratch& c : d.scratch) {
-    if (c.last_use == 0) spare = &c;
-    else if ((capturing || c.id == 0 ? c.handle == st : c.id == id) && (!s || c.floats > s->floats)) s = &c;
-  }
-  if (s && s->floats < need && (capturing || s->captured) && spare) s = nullptr;   // a graph keeps the small one
-  if (capturing && !spare && (!s || s->floats < need)) {
-    // Nothing may wait now, so nothing can be freed: whichever is large enough, as if the two streams were one.
-    s = nullptr;
-    for (Scratch& c : d.scratch)
-      if (c.floats >= need && (!s || c.last_use < s->last_use)) s = &c;
-    if (!s) *rc = fail(SYFI_DSA_ERR_CUDA, "no scratch buffer is large enough, and none can be had during a capture");
-    else s->captured = true;
-    return s;
-  }
-  if (!s) {
-    s = spare;
-    if (!s) {   // the one that was not used for longest, of those that no graph needs, if there is one
-      for (Scratch& c : d.scratch)
-        if (!s || (c.captured != s->captured ? s->captured : c.last_use < s->last_use)) s = &c;
-      if (cudaDeviceSynchronize() != cudaSuccess) {
-        *rc = fail(SYFI_DSA_ERR_CUDA, "device synchronisation failed");
-        return nullptr;
-      }
-    }
-    s->handle = st;
-    s->id = 0;
-    s->captured = false;
-  }
-  if (need > s->floats) {
-    if (s->scores) {
-      if (cudaDeviceSynchronize() != cudaSuccess) {
-        *rc = fail(SYFI_DSA_ERR_CUDA, "device synchronisation failed");
-        return nullptr;
-      }
-      cudaFree(s->scores);
-    }
-    s->scores = nullptr;
-    s->floats = 0;
-    RelaxedCapture relaxed;
-    if (cudaMalloc(&s->scores, need * sizeof(float)) != cudaSuccess) {
-      s->last_use = 0;
-      *rc = fail(SYFI_DSA_ERR_CUDA, "out of device memory for the scores");
-      return nullptr;
-    }
-    s->floats = need;
-  }
-  if (id != 0) s->id = id;
-  if (capturing) s->captured = true;
-  s->last_use = ++d.calls;
-  return s;
-}
 
 }  // namespace
 
@@ -800,7 +679,7 @@ extern "C" int syfi_dsa_topk_indexer(const void* q_index_fp8, const void* k_inde
   const size_t n_scores = static_cast<size_t>(batch) * max_ls;
   const size_t need = n_scores + 2 * static_cast<size_t>(batch) * ((max_ls + kTokTile - 1) / kTokTile);
   int rc = SYFI_DSA_OK;
-  Scratch* const s = scratch_of(d, st, need, &rc);
+  Scratch* const s = d.scratch.get(st, need * sizeof(float), 0, SYFI_DSA_ERR_CUDA, &rc);
   if (!s) return rc;
   if (!d.status) {
     if (cudaMalloc(&d.status, 16) != cudaSuccess) return fail(SYFI_DSA_ERR_CUDA, "out of device memory");
@@ -826,12 +705,13 @@ extern "C" int syfi_dsa_topk_indexer(const void* q_index_fp8, const void* k_inde
   // 24.2, 16 (8192) 63.9 / 44.0 / 37.8 / 37.5, 40 (20480) 114.7 / 66.2 / 46.0 / 40.0.
   const int per_cta = tiles <= 1024 ? 1 : tiles <= 2048 ? 2 : tiles <= 12288 ? 4 : kMaxTilesPerCta;
   const int runs = (max_ls + per_cta * kTokTile - 1) / (per_cta * kTokTile);
-  uint2* ranges = reinterpret_cast<uint2*>(s->scores + n_scores);
+  float* const scores = static_cast<float*>(s->memory);
+  uint2* ranges = reinterpret_cast<uint2*>(scores + n_scores);
   if (launch_dependent(dsa_score_kernel, dim3(runs, batch), dim3(kScoreThreads), kScoreSmem, st, tm_q, tm_k,
                        static_cast<const uint8_t*>(k_index_cache_fp8), weights, seq_lens, block_table, max_pages,
-                       s->scores, max_ls, per_cta, ranges, d.status, wait_limit) != cudaSuccess)
+                       scores, max_ls, per_cta, ranges, d.status, wait_limit) != cudaSuccess)
     return fail(SYFI_DSA_ERR_CUDA, "score kernel launch failed");
-  if (launch_select(s->scores, ranges, runs, per_cta * kTokTile, max_ls, seq_lens, block_table, batch, max_pages,
+  if (launch_select(scores, ranges, runs, per_cta * kTokTile, max_ls, seq_lens, block_table, batch, max_pages,
                     topk_indices, d.num_sms, st) != cudaSuccess)
     return fail(SYFI_DSA_ERR_CUDA, "select kernel launch failed");
   return SYFI_DSA_OK;

@@ -1,101 +1,505 @@
 // Attention of new tokens over the quantised paged KV cache (include/syfi_kv.h).
 //
-//   x_j = scale * kscale_j * sum_d q_d k_jd,   m = max x_j,   l = sum exp(x_j - m),   out_d = sum exp(x_j - m) vscale_j v_jd / l
-// over the visible positions j, in one pass over the cache: m, l and the sum are corrected by exp(m_old - m_new) when m grows.
+//   x_j = scale * kscale_j * sum_d q_d k_jd,   out_d = sum_j exp(x_j) vscale_j v_jd / sum_j exp(x_j)   over the visible positions j
+// in one pass over the cache.  With x in units of log2 and references m (of the sum l) and n (of the sum o) that follow the largest
+// terms,   l = sum 2^(x_j - m),   o_d = sum 2^(x_j + log2 vscale_j - n) v_jd,   out_d = o_d 2^(n - m) / l :
+// the values' scales go into the weights, so the products are made with the cache's e4m3 bytes as they are, which f16 holds exactly.
+#include <mutex>
+
+#include "attention_plan.cuh"
 #include "kv_internal.h"
+#include "stream_scratch.h"
 
 namespace syfi {
 
 namespace {
 
-constexpr int kWarps = 4;
+struct AttentionArgs {
+  const __nv_bfloat16* q;
+  __nv_bfloat16* out;
+  long long q_stride, out_stride;
+  KvCache cache;
+  KvBatch batch;
+  int group, window;
+  float scale_log2;
+  int* tickets;          // [CTAs] zero between calls
+  float* partial;        // [2 * CTAs][rows][D] sums, then [2 * CTAs][rows] of (m, l, n, -)
+};
 
-// One warp per query and head.  A lane has two of a page's 64 tokens while the scores are made and D / 32 dimensions while the
-// values are added up.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t bytes) {   // the lower two
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(bytes)));
+  return h;
+}
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float quad_max(float v) {
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+  v += __shfl_xor_sync(0xffffffffu, v, 1);
+  return v + __shfl_xor_sync(0xffffffffu, v, 2);
+}
+__device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.0f : m; }
+
+// ---------------------------------------------------------------- few rows per sequence and key head: decoding
+// A CTA walks its piece of the pages through a ring of stages filled by cp.async.  Four warps share a page, 16 positions each, for
+// every 16 rows (MT row groups of four warps); mma.sync m16n8k16 in f16, whose operands the lanes make from the bytes in
+// registers.  What bounds it is the cache's bytes, so the shape is chosen for loads in flight: three CTAs of three stages per SM.
+//   scores: rows x positions; a lane's K operand is 16 bytes of a position's row, the dimensions of the MMAs' k index being
+//           permuted alike in q;
+//   values: rows x dimensions; a lane's V operand pairs the bytes of two positions (prmt), its 16 dimensions are 16 MMAs' n.
+// Which position an n index of the scores stands for is chosen so that both reads of the swizzled rows are free of bank
+// conflicts: even n is position n, odd n is position (n - 1) ^ 5.
+template <int D, int MT>
+struct DecodeShape {
+  static constexpr int kRows = 16 * MT;
+  static constexpr int kThreads = 128 * MT;
+  static constexpr int kBlocks = MT == 1 ? 3 : 1;                       // per SM
+  static constexpr int kStages = MT == 1 ? (D == 128 ? 3 : 5) : (D == 128 ? 6 : 10);
+  static constexpr int kBlockBytes = kKvPage * D;
+  static constexpr int kStageBytes = 2 * kBlockBytes + 2 * kKvPage * 4;
+  static constexpr int kMerge = MT * 2 * 16 * D;                        // floats
+  static constexpr int kSmem = kStages * kStageBytes + kMerge * 4;
+};
+constexpr float kHeadroom = 7.0f;     // weights are kept times 2^7 in f16 ...
+constexpr float kGrowth = 8.0f;       // ... and may grow to 2^15 before their reference follows
+
 template <int D>
-__global__ void __launch_bounds__(kWarps * 32)
-attention_rows_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, KvCache cache, KvBatch batch, int q_heads,
-                      float scale_log2, int window, __nv_bfloat16* __restrict__ out, long long out_stride) {
-  __shared__ float s_q[kWarps][D], s_p[kWarps][kKvPage];
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const long long id = static_cast<long long>(blockIdx.x) * kWarps + warp;
-  if (id >= static_cast<long long>(batch.tokens) * q_heads) return;
-  const int t = static_cast<int>(id / q_heads), head = static_cast<int>(id - static_cast<long long>(t) * q_heads);
-  int b = -1;
-  KvSequence s = {};
-  for (int at = 0; at < batch.batch && b < 0; at += 32) {
-    KvSequence mine = {};
-    if (at + lane < batch.batch) mine = kv_sequence(batch, at + lane);
-    const unsigned holds = __ballot_sync(0xffffffffu, t >= mine.first && t < mine.first + mine.count);
-    if (holds != 0u) b = at + __ffs(holds) - 1;
+__device__ __forceinline__ int swizzled(int row, int chunk) {   // byte offset of a row's 16-byte chunk
+  return row * D + ((D == 128 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3)) << 4);
+}
+
+// Adds up a split unit's parts: out = sum o_p 2^(n_p - n) 2^(n - m) / sum l_p 2^(m_p - m).
+template <int D, int ROWS>
+__device__ void join_parts(const AttentionArgs& a, const KvSequence& s, int rt, int head, int rows, long long total, int ctas, int first, int last,
+                           long long unit_start) {
+  const float4* stats = reinterpret_cast<const float4*>(a.partial + 2ll * ctas * ROWS * D);
+  for (int i = threadIdx.x; i < rows * (D / 4); i += blockDim.x) {
+    const int row = i / (D / 4), d = (i % (D / 4)) * 4;
+    auto slot = [&](int c) { return 2 * c + (piece_start(total, ctas, c) >= unit_start ? 0 : 1); };
+    float m = -INFINITY, n = -INFINITY;
+    for (int c = first; c <= last; ++c) {
+      const float4 st = __ldcg(stats + static_cast<long long>(slot(c)) * ROWS + row);
+      m = fmaxf(m, st.x);
+      n = fmaxf(n, st.z);
+    }
+    const float m_ref = finite_or_zero(m), n_ref = finite_or_zero(n);
+    float l = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int c = first; c <= last; ++c) {
+      const long long at = static_cast<long long>(slot(c)) * ROWS + row;
+      const float4 st = __ldcg(stats + at);
+      const float4 part = __ldcg(reinterpret_cast<const float4*>(a.partial + at * D + d));
+      l += st.y * ex2(st.x - m_ref);
+      const float f = ex2(st.z - n_ref);
+      o.x = fmaf(part.x, f, o.x);
+      o.y = fmaf(part.y, f, o.y);
+      o.z = fmaf(part.z, f, o.z);
+      o.w = fmaf(part.w, f, o.w);
+    }
+    const float f = l == 0.0f ? 0.0f : ex2(n_ref - m_ref - kHeadroom) / l;
+    const int r = rt * ROWS + row;
+    __nv_bfloat16* to = a.out + (s.first + r / a.group) * a.out_stride + (head * a.group + r % a.group) * D + d;
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(o.x * f, o.y * f), hi = __floats2bfloat162_rn(o.z * f, o.w * f);
+    *reinterpret_cast<uint2*>(to) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
   }
-  if (b < 0) return;
-  s = kv_sequence(batch, b);
-  const int position = s.length - s.count + (t - s.first);
-  const int low = window > 0 ? max(position - window + 1, 0) : 0;
-  const int kv_head = head / (q_heads / cache.heads);
-  for (int d = lane; d < D; d += 32) s_q[warp][d] = __bfloat162float(q[t * q_stride + head * D + d]);
-  __syncwarp();
-  float m = -INFINITY, l = 0.0f, acc[D / 32] = {};
-  for (int page = low / kKvPage; page * kKvPage <= position; ++page) {
-    const int at = batch.block_table[static_cast<long long>(b) * batch.max_pages + page];
-    if (at < 0 || at >= cache.num_pages) continue;
-    const uint8_t* keys = kv_block<D>(cache, at, 0, kv_head);
-    const uint8_t* values = kv_block<D>(cache, at, 1, kv_head);
-    float x[2];
+}
+
+template <int D, int MT>
+__global__ void __launch_bounds__(DecodeShape<D, MT>::kThreads, DecodeShape<D, MT>::kBlocks) attention_decode_kernel(const __grid_constant__ AttentionArgs a) {
+  using Shape = DecodeShape<D, MT>;
+  constexpr int kRows = Shape::kRows, kStages = Shape::kStages, kSteps = D / 16, kMmas = D / 8;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ PlanShared s_plan;
+  __shared__ int s_there[kStages];
+  __shared__ float4 s_stat[4 * MT][16];
+  float* const s_merge = reinterpret_cast<float*>(smem + kStages * Shape::kStageBytes);
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, c = lane % 4;
+  const int mt = warp / 4, quarter = warp % 4;
+
+  pdl_wait();
+  pdl_trigger();
+  const Plan<kKvPage, kRows> plan = {a.batch, a.cache.heads, a.group, a.window};
+  const long long total = plan.total(s_plan);
+  const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
+  if (static_cast<int>(blockIdx.x) >= ctas) return;
+  const long long w0 = piece_start(total, ctas, blockIdx.x), w1 = piece_start(total, ctas, blockIdx.x + 1);
+  const int count = static_cast<int>(w1 - w0);
+  plan.locate(s_plan, w0);
+
+  Cursor<kKvPage, kRows> load, use;
+  load.start(plan, s_plan);
+  use = load;
+  int loaded = 0;
+  auto entry_of = [&](const Cursor<kKvPage, kRows>& at) {
+    return __ldg(a.batch.block_table + static_cast<long long>(at.b) * a.batch.max_pages + at.span.first + at.tile);
+  };
+  int entry = entry_of(load);                // of the page to ask for next: read one page ahead
+  auto ask = [&]() {
+    if (loaded < count) {
+      const int stage = loaded % kStages;
+      const bool there = entry >= 0 && entry < a.cache.num_pages;
+      if (there) {
+        const uint32_t dst = smem_u32(smem) + stage * Shape::kStageBytes;
+        const uint8_t* block = kv_block<D>(a.cache, entry, 0, load.head);
+        const long long to_values = static_cast<long long>(a.cache.heads) * (kKvPage * (D + 4));
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int token = lane + 32 * i, j = page * kKvPage + token;
-      x[i] = -INFINITY;
-      if (j >= low && j <= position) {
-        float sum = 0.0f;
-        for (int d = 0; d < D; d += 16) {
-          const uint4 p = *reinterpret_cast<const uint4*>(keys + token * D + d);
-          const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+        for (int i = 0; i < 2 * Shape::kBlockBytes / 16 / Shape::kThreads; ++i) {
+          const int at = tid + i * Shape::kThreads, kind = at / (Shape::kBlockBytes / 16), chunk = at % (Shape::kBlockBytes / 16);
+          cp_async16(dst + kind * Shape::kBlockBytes + swizzled<D>(chunk / (D / 16), chunk % (D / 16)), block + kind * to_values + chunk * 16);
+        }
+        if (tid < 32) cp_async16(dst + 2 * Shape::kBlockBytes + tid * 16, block + tid / 16 * to_values + Shape::kBlockBytes + tid % 16 * 16);
+      }
+      if (tid == 0) s_there[stage] = there;
+      ++loaded;
+      if (loaded < count) {
+        if (++load.tile == load.span.tiles) load.next_unit(plan);
+        entry = entry_of(load);
+      }
+    }
+    cp_async_commit();
+  };
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float2 f = e4m3x2_to_float2(static_cast<uint16_t>(w[e / 2] >> (16 * (e % 2))));
-            sum = fmaf(s_q[warp][d + 2 * e], f.x, fmaf(s_q[warp][d + 2 * e + 1], f.y, sum));
+  for (int i = 0; i < kStages - 1; ++i) ask();
+
+  uint32_t qa[kSteps][4];
+  float unit[2], m[2], l[2], n[2], o[kMmas][4];
+  int low[2], high[2];                       // positions that this lane's two rows see
+  int all_low = 0, all_high = 0, any_low = 0, any_high = 0;   // positions that all / any of the unit's rows see
+  bool fresh = true;
+  int begun = use.tile;                      // the segment's first tile
+
+  for (int done = 0; done < count; ++done) {
+    cp_async_wait<kStages - 2>();
+    __syncthreads();
+    ask();
+    if (fresh) {
+      fresh = false;
+      begun = use.tile;
+      const int rows = use.rows(a.group), base = use.s.length - use.s.count, r0 = use.rt * kRows;
+      const int first = base + r0 / a.group, last = base + (r0 + rows - 1) / a.group;
+      all_low = a.window > 0 ? max(last - a.window + 1, 0) : 0;
+      any_low = a.window > 0 ? max(first - a.window + 1, 0) : 0;
+      all_high = first;
+      any_high = last;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = mt * 16 + g + 8 * i, r = r0 + row;
+        const bool real = row < rows;
+        const int position = base + (real ? r / a.group : 0);
+        low[i] = a.window > 0 ? max(position - a.window + 1, 0) : 0;
+        high[i] = real ? position : -1;
+        m[i] = n[i] = -INFINITY;
+        l[i] = 0.0f;
+        // 2^k that brings the row's largest magnitude to 2^14 .. 2^15: f16 then holds bf16 values exactly down to 2^-29 of it
+        const __nv_bfloat16* from = a.q + (use.s.first + (real ? r / a.group : 0)) * a.q_stride + (use.head * a.group + (real ? r % a.group : 0)) * D;
+        uint2 raw[kSteps];
+        unsigned top = 0u;
+#pragma unroll
+        for (int step = 0; step < kSteps; ++step) {
+          raw[step] = real ? __ldg(reinterpret_cast<const uint2*>(from + 16 * (c + 4 * (step / 4)) + 4 * (step % 4))) : make_uint2(0u, 0u);
+          top = max(max(top, raw[step].x & 0x7fffu), (raw[step].x >> 16) & 0x7fffu);
+          top = max(max(top, raw[step].y & 0x7fffu), (raw[step].y >> 16) & 0x7fffu);
+        }
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int k = top == 0u ? 0 : min(14 - (static_cast<int>(top >> 7) - 127), 120);
+        const float up = __int_as_float((k + 127) << 23);
+        unit[i] = top >= 0x7f80u ? __int_as_float(0x7fffffff) : a.scale_log2 * __int_as_float((127 - k) << 23);
+#pragma unroll
+        for (int step = 0; step < kSteps; ++step) {
+          qa[step][i] = pack_half2(__uint_as_float(raw[step].x << 16) * up, __uint_as_float(raw[step].x & 0xffff0000u) * up);
+          qa[step][2 + i] = pack_half2(__uint_as_float(raw[step].y << 16) * up, __uint_as_float(raw[step].y & 0xffff0000u) * up);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kMmas; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
+    }
+
+    const int stage = done % kStages;
+    uint8_t* const keys = smem + stage * Shape::kStageBytes;
+    uint8_t* const values = keys + Shape::kBlockBytes;
+    float* const k_scale = reinterpret_cast<float*>(keys + 2 * Shape::kBlockBytes);
+    float* const v_scale = k_scale + kKvPage;
+    const int position0 = (use.span.first + use.tile) * kKvPage;
+    const bool plain = position0 >= all_low && position0 + kKvPage - 1 <= all_high;    // every row sees every position of the page
+    if (s_there[stage]) {
+      if (!plain) {
+        // What a row does not see must not reach its sums, and zero times NaN is NaN: positions that no row sees lose their bytes, and
+        // where some rows see a value that is not finite, the NaN goes by way of its score to those rows alone.
+        for (int t = tid / 2; t < kKvPage; t += Shape::kThreads / 2) {
+          const int half = tid % 2, position = position0 + t;
+          const bool unseen = position < any_low || position > any_high;
+          bool bad = false;
+          uint4* const chunk0 = reinterpret_cast<uint4*>(values);
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) {
+            const uint4 w = chunk0[swizzled<D>(t, half * (D / 32) + i) / 16];
+            const uint32_t over = ((w.x & 0x7f7f7f7fu) + 0x01010101u) | ((w.y & 0x7f7f7f7fu) + 0x01010101u) |
+                                  ((w.z & 0x7f7f7f7fu) + 0x01010101u) | ((w.w & 0x7f7f7f7fu) + 0x01010101u);
+            bad |= (over & 0x80808080u) != 0u;
+          }
+          bad = __shfl_xor_sync(0xffffffffu, static_cast<int>(bad), 1) | static_cast<int>(bad);
+          bad |= !(fabsf(v_scale[t]) <= 3.402823466e38f);
+          __syncwarp();
+          if (bad || unseen) {
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) chunk0[swizzled<D>(t, half * (D / 32) + i) / 16] = make_uint4(0u, 0u, 0u, 0u);
+            if (half == 0) {
+              v_scale[t] = 1.0f;
+              if (bad) k_scale[t] = __int_as_float(0x7fffffff);
+            }
           }
         }
-        x[i] = sum * *reinterpret_cast<const float*>(keys + kKvPage * D + token * 4) * scale_log2;
+        __syncthreads();
+      }
+      float x[2][4] = {};
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int row = quarter * 16 + 8 * u + ((g & 1) ? (g - 1) ^ 5 : g);
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) {
+          const uint4 p = *reinterpret_cast<const uint4*>(keys + swizzled<D>(row, c + 4 * j));
+          const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mma_f16(x[u], qa[4 * j + i], e4m3x2_to_half2(w[i]), e4m3x2_to_half2(w[i] >> 16));
+        }
+      }
+      float y[2][4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int t = quarter * 16 + 8 * u + (e ? (2 * c) ^ 5 : 2 * c);
+          const float ks = k_scale[t], lv = __log2f(v_scale[t]);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float& v = x[u][2 * i + e];
+            v *= ks * unit[i];
+            if (!plain && (position0 + t < low[i] || position0 + t > high[i])) v = -INFINITY;
+            y[u][2 * i + e] = v == -INFINITY ? -INFINITY : v + lv;
+          }
+        }
+      }
+      float fade[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        // l by lane, for its own positions; the lanes of a row meet at the unit's end
+        const float top = fmaxf(fmaxf(x[0][2 * i], x[0][2 * i + 1]), fmaxf(x[1][2 * i], x[1][2 * i + 1]));
+        const float m_new = fmaxf(m[i], top), m_ref = finite_or_zero(m_new);
+        l[i] = l[i] * ex2(m[i] - m_ref) + ((ex2(x[0][2 * i] - m_ref) + ex2(x[0][2 * i + 1] - m_ref)) + (ex2(x[1][2 * i] - m_ref) + ex2(x[1][2 * i + 1] - m_ref)));
+        m[i] = m_new;
+        const float y_top = quad_max(fmaxf(fmaxf(y[0][2 * i], y[0][2 * i + 1]), fmaxf(y[1][2 * i], y[1][2 * i + 1])));
+        fade[i] = 1.0f;
+        if (y_top > n[i] + kGrowth) {
+          fade[i] = ex2(n[i] - y_top);
+          n[i] = y_top;
+        }
+        const float shift = kHeadroom - finite_or_zero(n[i]);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          y[u][2 * i] = ex2(y[u][2 * i] + shift);
+          y[u][2 * i + 1] = ex2(y[u][2 * i + 1] + shift);
+        }
+      }
+      if (__any_sync(0xffffffffu, fade[0] != 1.0f || fade[1] != 1.0f)) {
+#pragma unroll
+        for (int j = 0; j < kMmas; ++j) {
+          o[j][0] *= fade[0];
+          o[j][1] *= fade[0];
+          o[j][2] *= fade[1];
+          o[j][3] *= fade[1];
+        }
+      }
+      const uint32_t pa[4] = {pack_half2(y[0][0], y[0][1]), pack_half2(y[0][2], y[0][3]), pack_half2(y[1][0], y[1][1]), pack_half2(y[1][2], y[1][3])};
+      uint32_t even[2][D / 32], odd[2][D / 32];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int t0 = quarter * 16 + 8 * u + 2 * c, t1 = quarter * 16 + 8 * u + ((2 * c) ^ 5);
+        if constexpr (D == 128) {
+          const uint4 p = *reinterpret_cast<const uint4*>(values + swizzled<D>(t0, g)), r = *reinterpret_cast<const uint4*>(values + swizzled<D>(t1, g));
+          even[u][0] = p.x; even[u][1] = p.y; even[u][2] = p.z; even[u][3] = p.w;
+          odd[u][0] = r.x; odd[u][1] = r.y; odd[u][2] = r.z; odd[u][3] = r.w;
+        } else {
+          const uint2 p = *reinterpret_cast<const uint2*>(values + swizzled<D>(t0, g / 2) + (g & 1) * 8), r = *reinterpret_cast<const uint2*>(values + swizzled<D>(t1, g / 2) + (g & 1) * 8);
+          even[u][0] = p.x; even[u][1] = p.y;
+          odd[u][0] = r.x; odd[u][1] = r.y;
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < D / 32; ++w) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t b0 = __byte_perm(even[0][w], odd[0][w], h ? 0x7362 : 0x5140), b1 = __byte_perm(even[1][w], odd[1][w], h ? 0x7362 : 0x5140);
+          mma_f16(o[4 * w + 2 * h], pa, e4m3x2_to_half2(b0), e4m3x2_to_half2(b1));
+          mma_f16(o[4 * w + 2 * h + 1], pa, e4m3x2_to_half2(b0 >> 16), e4m3x2_to_half2(b1 >> 16));
+        }
       }
     }
-    float top = fmaxf(x[0], x[1]);
+
+    const bool unit_ends = use.tile + 1 == use.span.tiles;
+    if (unit_ends || done + 1 == count) {
+      // ---- the segment's end: lanes, then the four warps of a row group, then the unit's other pieces
+      const int rows = use.rows(a.group);
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    const float m_new = fmaxf(m, top), reference = m_new == -INFINITY ? 0.0f : m_new;
-    const float fade = exp2f(m - reference);
-    l *= fade;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) acc[i] *= fade;
-    m = m_new;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float p = exp2f(x[i] - reference);
-      l += p;
-      s_p[warp][lane + 32 * i] = p;
-    }
-    __syncwarp();
-    const int first = max(low - page * kKvPage, 0), last = min(position - page * kKvPage, kKvPage - 1);
-    for (int token = first; token <= last; ++token) {
-      const float p = s_p[warp][token] * *reinterpret_cast<const float*>(values + kKvPage * D + token * 4);
-#pragma unroll
-      for (int i = 0; i < D / 64; ++i) {
-        const float2 f = e4m3x2_to_float2(*reinterpret_cast<const uint16_t*>(values + token * D + i * 64 + lane * 2));
-        acc[2 * i] = fmaf(p, f.x, acc[2 * i]);
-        acc[2 * i + 1] = fmaf(p, f.y, acc[2 * i + 1]);
+      for (int i = 0; i < 2; ++i) {
+        const float top = quad_max(m[i]);
+        l[i] = quad_sum(l[i] * ex2(m[i] - finite_or_zero(top)));
+        m[i] = top;
+        if (c == 0) s_stat[warp][g + 8 * i] = make_float4(m[i], l[i], n[i], 0.0f);
       }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float m_all = -INFINITY, n_all = -INFINITY, l_all = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          m_all = fmaxf(m_all, s_stat[mt * 4 + w][g + 8 * i].x);
+          n_all = fmaxf(n_all, s_stat[mt * 4 + w][g + 8 * i].z);
+        }
+#pragma unroll
+        for (int w = 0; w < 4; ++w) l_all += s_stat[mt * 4 + w][g + 8 * i].y * ex2(s_stat[mt * 4 + w][g + 8 * i].x - finite_or_zero(m_all));
+        const float f = ex2(n[i] - finite_or_zero(n_all));
+#pragma unroll
+        for (int j = 0; j < kMmas; ++j) {
+          o[j][2 * i] *= f;
+          o[j][2 * i + 1] *= f;
+        }
+        m[i] = m_all;
+        n[i] = n_all;
+        l[i] = l_all;
+      }
+      float* const mine = s_merge + (mt * 2 + (quarter & 1)) * 16 * D;
+      if (quarter >= 2) {
+#pragma unroll
+        for (int j = 0; j < kMmas; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mine[(j * 4 + e) * 32 + lane] = o[j][e];
+      }
+      __syncthreads();
+      if (quarter < 2) {
+#pragma unroll
+        for (int j = 0; j < kMmas; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[j][e] += mine[(j * 4 + e) * 32 + lane];
+        if (quarter == 1) {
+#pragma unroll
+          for (int j = 0; j < kMmas; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mine[(j * 4 + e) * 32 + lane] = o[j][e];
+        }
+      }
+      __syncthreads();
+      const bool whole = begun == 0 && unit_ends;
+      const long long unit_start = w0 + done - use.tile;
+      if (quarter == 0) {
+        const float* other = s_merge + (mt * 2 + 1) * 16 * D;
+        const int slot = 2 * static_cast<int>(blockIdx.x) + (w0 >= unit_start ? 0 : 1);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int row = mt * 16 + g + 8 * i, r = use.rt * kRows + row;
+          if (row >= rows) continue;
+          // this lane's dimensions: D / 4 in a row, the MMAs' first columns, then their second ones
+          float v[D / 4];
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int j = 0; j < kMmas; ++j) v[e * kMmas + j] = o[j][2 * i + e] + other[(j * 4 + 2 * i + e) * 32 + lane];
+          if (whole) {
+            const float f = l[i] == 0.0f ? 0.0f : ex2(finite_or_zero(n[i]) - finite_or_zero(m[i]) - kHeadroom) / l[i];
+            uint4* to = reinterpret_cast<uint4*>(a.out + (use.s.first + r / a.group) * a.out_stride + (use.head * a.group + r % a.group) * D + c * (D / 4));
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j) {
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(v[8 * j + 2 * e] * f, v[8 * j + 2 * e + 1] * f);
+                w[e] = *reinterpret_cast<const uint32_t*>(&h);
+              }
+              to[j] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          } else {
+            const long long at = static_cast<long long>(slot) * kRows + row;
+            float4* to = reinterpret_cast<float4*>(a.partial + at * D + c * (D / 4));
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j) to[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+            if (c == 0) reinterpret_cast<float4*>(a.partial + 2ll * ctas * kRows * D)[at] = make_float4(m[i], l[i], n[i], 0.0f);
+          }
+        }
+      }
+      if (!whole) {
+        const int first = piece_of(total, ctas, unit_start), last = piece_of(total, ctas, unit_start + use.span.tiles - 1);
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) {
+          const bool is_last = atomicAdd(a.tickets + first, 1) == last - first;
+          if (is_last) a.tickets[first] = 0;
+          s_plan.last = is_last;
+        }
+        __syncthreads();
+        if (s_plan.last) {
+          __threadfence();
+          join_parts<D, kRows>(a, use.s, use.rt, use.head, rows, total, ctas, first, last, unit_start);
+        }
+      }
+      fresh = true;
+      if (unit_ends) use.next_unit(plan);
+    } else {
+      ++use.tile;
     }
-    __syncwarp();
   }
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-  for (int i = 0; i < D / 64; ++i)
-    *reinterpret_cast<__nv_bfloat162*>(out + t * out_stride + head * D + i * 64 + lane * 2) =
-        __floats2bfloat162_rn(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+}
+
+// ---------------------------------------------------------------- host
+struct Device {
+  ScratchPool scratch;
+  bool ready = false;      // the kernels' shared memory is allowed
+};
+std::mutex g_mu;
+Device g_devices[64];
+
+template <int D, int MT>
+bool raise_decode() {
+  return cudaFuncSetAttribute(attention_decode_kernel<D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeShape<D, MT>::kSmem) == cudaSuccess;
+}
+
+constexpr size_t kTicketBytes = 4096;      // 1024 CTAs
+
+template <int D, int MT>
+int launch_decode(AttentionArgs a, Device& d, int sms, cudaStream_t st) {
+  using Shape = DecodeShape<D, MT>;
+  const int ctas = sms * Shape::kBlocks;
+  const size_t need = kTicketBytes + 2ull * ctas * Shape::kRows * (D + 4) * sizeof(float);
+  int rc = SYFI_KV_OK;
+  Scratch* const s = d.scratch.get(st, need, kTicketBytes, SYFI_KV_ERR_CUDA, &rc);
+  if (!s) return rc;
+  a.tickets = static_cast<int*>(s->memory);
+  a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(s->memory) + kTicketBytes);
+  return launch_dependent(attention_decode_kernel<D, MT>, dim3(ctas), dim3(Shape::kThreads), Shape::kSmem, st, a) == cudaSuccess
+             ? SYFI_KV_OK : kv_fail(SYFI_KV_ERR_CUDA, "attention kernel launch failed");
 }
 
 }  // namespace
@@ -112,7 +516,7 @@ extern "C" int syfi_paged_attention(const void* q, int64_t q_stride, const void*
   if (const char* wrong = kv_cache_error(cache, num_pages, page_stride, 2, kv_heads, head_dim)) return kv_fail(SYFI_KV_ERR_INVALID, wrong);
   if (q_heads < 1 || q_heads > 4096 || q_heads % kv_heads != 0) return kv_fail(SYFI_KV_ERR_INVALID, "q_heads must be a multiple of kv_heads");
   if (batch < 0 || batch > (1 << 16)) return kv_fail(SYFI_KV_ERR_INVALID, "batch out of range");
-  if (tokens < 0 || tokens * q_heads > 0x3fffffffll) return kv_fail(SYFI_KV_ERR_INVALID, "tokens out of range");
+  if (tokens < 0 || tokens > 0x3fffffffll / q_heads) return kv_fail(SYFI_KV_ERR_INVALID, "tokens out of range");
   if (max_pages < 1 || max_pages > (1 << 20)) return kv_fail(SYFI_KV_ERR_INVALID, "max_pages (block table width) out of range");
   if (window < 0) return kv_fail(SYFI_KV_ERR_INVALID, "window must not be negative");
   if (!(scale > -1e30 && scale < 1e30)) return kv_fail(SYFI_KV_ERR_INVALID, "scale is not a finite float");
@@ -122,13 +526,31 @@ extern "C" int syfi_paged_attention(const void* q, int64_t q_stride, const void*
   const int64_t width = static_cast<int64_t>(q_heads) * head_dim;
   if (!kv_stride_ok(q_stride, width) || !kv_stride_ok(out_stride, width))
     return kv_fail(SYFI_KV_ERR_INVALID, "a token stride is smaller than the token's heads or no multiple of 8");
-  if (!kv_device_sms()) return SYFI_KV_ERR_CUDA;
-  const KvCache c = {static_cast<uint8_t*>(const_cast<void*>(cache)), page_stride, static_cast<int>(num_pages), 2, kv_heads};
-  const KvBatch batch_args = {block_table, seq_lens, q_starts, batch, max_pages, static_cast<int>(tokens)};
-  const float scale_log2 = static_cast<float>(scale * 1.4426950408889634);
-  const unsigned grid = static_cast<unsigned>((tokens * q_heads + kWarps - 1) / kWarps);
-  auto* kernel = head_dim == 128 ? attention_rows_kernel<128> : attention_rows_kernel<64>;
-  kernel<<<grid, kWarps * 32, 0, static_cast<cudaStream_t>(stream)>>>(static_cast<const __nv_bfloat16*>(q), q_stride, c, batch_args, q_heads,
-                                                                      scale_log2, window, static_cast<__nv_bfloat16*>(out), out_stride);
-  return cudaGetLastError() == cudaSuccess ? SYFI_KV_OK : kv_fail(SYFI_KV_ERR_CUDA, "attention kernel launch failed");
+  const int sms = kv_device_sms();
+  if (!sms) return SYFI_KV_ERR_CUDA;
+  AttentionArgs a = {};
+  a.q = static_cast<const __nv_bfloat16*>(q);
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.q_stride = q_stride;
+  a.out_stride = out_stride;
+  a.cache = {static_cast<uint8_t*>(const_cast<void*>(cache)), page_stride, static_cast<int>(num_pages), 2, kv_heads};
+  a.batch = {block_table, seq_lens, q_starts, batch, max_pages, static_cast<int>(tokens)};
+  a.group = q_heads / kv_heads;
+  a.window = window;
+  a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::lock_guard<std::mutex> lock(g_mu);
+  Device& d = g_devices[dev];
+  if (!d.ready) {
+    if (!raise_decode<128, 1>() || !raise_decode<128, 2>() || !raise_decode<128, 4>() || !raise_decode<64, 1>() || !raise_decode<64, 2>() || !raise_decode<64, 4>())
+      return kv_fail(SYFI_KV_ERR_CUDA, "cannot raise the shared-memory limit of the attention kernels");
+    d.ready = true;
+  }
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // Rows per sequence and key head, on average (the lengths themselves are on the device): row tiles of 16, 32 or 64.
+  const int64_t rows = (tokens * a.group + batch - 1) / batch;
+  if (head_dim == 128)
+    return rows <= 16 ? launch_decode<128, 1>(a, d, sms, st) : rows <= 32 ? launch_decode<128, 2>(a, d, sms, st) : launch_decode<128, 4>(a, d, sms, st);
+  return rows <= 16 ? launch_decode<64, 1>(a, d, sms, st) : rows <= 32 ? launch_decode<64, 2>(a, d, sms, st) : launch_decode<64, 4>(a, d, sms, st);
 }
