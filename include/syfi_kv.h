@@ -26,6 +26,7 @@ extern "C" {
 #define SYFI_KV_OK 0
 #define SYFI_KV_ERR_INVALID 1   /* bad argument */
 #define SYFI_KV_ERR_CUDA 2      /* a CUDA call failed, no CUDA device, or not an sm_100 device */
+#define SYFI_KV_ERR_DEVICE 3    /* a kernel gave up on a bounded wait (syfi_kv_check) */
 #define SYFI_KV_PAGE 64
 
 /* New tokens' queries, keys and values: head norms, rotation, quantisation and the scatter into the cache in one pass.
@@ -63,11 +64,20 @@ int syfi_kv_read(const void* cache, int64_t num_pages, int64_t page_stride, int3
  *       Rows of no sequence are left alone.
  * The query at position p sees the positions j <= p that are there, with window > 0 only those with j > p - window:
  *   out = sum_j softmax_j(scale * q . key_j) * value_j;  a query that sees nothing gets zeros.
- * Positions that a query does not see do not touch its result, whatever the cache holds there. */
+ * Positions that a query does not see do not touch its result, whatever the cache holds there.  Scales are not negative.
+ * Calls on different streams may run at the same time: every stream has a scratch buffer of its own (up to 45 MB), which
+ * grows on demand (that waits for the device).  Up to eight streams of a device hold one; a ninth waits for the device and takes
+ * over the least recently used.  A captured graph keeps using the buffer that its stream had then: do not replay two graphs
+ * captured on one stream at the same time, nor beside calls on that stream; and where more than eight streams call, capture
+ * after a call of the same kind, and replay beside no other call. */
 int syfi_paged_attention(const void* q, int64_t q_stride, const void* cache, int64_t num_pages, int64_t page_stride,
                          const int32_t* block_table, int32_t max_pages, const int32_t* seq_lens, const int32_t* q_starts,
                          int32_t batch, int64_t tokens, int32_t q_heads, int32_t kv_heads, int32_t head_dim, double scale,
                          int32_t window, void* out, int64_t out_stride, void* stream);
+
+/* Synchronises `stream` and reports whether an attention kernel gave up on a bounded wait on the current device since the last
+ * check (status 301; the rows that it had not finished are NaN). */
+int syfi_kv_check(void* stream);
 
 #ifdef __cplusplus
 }

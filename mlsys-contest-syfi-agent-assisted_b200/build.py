@@ -15,8 +15,8 @@ import sys
 CSRC = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc")
 LIB = os.path.join(CSRC, "libsyfi_moe.so")
 SOURCES = ["api.cu", "router.cu", "permute.cu", "grouped_gemm.cu", "grouped_gemm_pair.cu", "combine.cu", "ep_exchange.cu", "prepack.cu", "dsa_indexer.cu",
-           "kv_cache.cu", "paged_attention.cu"]
-HEADERS = ["moe_internal.h", "kv_internal.h", "attention_plan.cuh", "stream_scratch.h", "ptx.cuh", "dsa_bins.h", os.path.join("..", "..", "include", "syfi_moe.h"),
+           "kv_cache.cu", "paged_attention.cu", "paged_attention_chunk.cu"]
+HEADERS = ["moe_internal.h", "kv_internal.h", "attention_plan.cuh", "attention_common.cuh", "stream_scratch.h", "ptx.cuh", "dsa_bins.h", os.path.join("..", "..", "include", "syfi_moe.h"),
            os.path.join("..", "..", "include", "syfi_dsa.h"), os.path.join("..", "..", "include", "syfi_kv.h")]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-shared", "-Xptxas", "-v"]

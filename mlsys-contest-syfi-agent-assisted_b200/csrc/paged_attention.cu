@@ -4,27 +4,15 @@
 // in one pass over the cache.  With x in units of log2 and references m (of the sum l) and n (of the sum o) that follow the largest
 // terms,   l = sum 2^(x_j - m),   o_d = sum 2^(x_j + log2 vscale_j - n) v_jd,   out_d = o_d 2^(n - m) / l :
 // the values' scales go into the weights, so the products are made with the cache's e4m3 bytes as they are, which f16 holds exactly.
+#include <cstdio>
 #include <mutex>
 
-#include "attention_plan.cuh"
-#include "kv_internal.h"
+#include "attention_common.cuh"
 #include "stream_scratch.h"
 
 namespace syfi {
 
 namespace {
-
-struct AttentionArgs {
-  const __nv_bfloat16* q;
-  __nv_bfloat16* out;
-  long long q_stride, out_stride;
-  KvCache cache;
-  KvBatch batch;
-  int group, window;
-  float scale_log2;
-  int* tickets;          // [CTAs] zero between calls
-  float* partial;        // [2 * CTAs][rows][D] sums, then [2 * CTAs][rows] of (m, l, n, -)
-};
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -32,20 +20,6 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t bytes) {   // the lower two
-  uint32_t h;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(bytes)));
-  return h;
-}
-__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -59,8 +33,6 @@ __device__ __forceinline__ float quad_sum(float v) {
   v += __shfl_xor_sync(0xffffffffu, v, 1);
   return v + __shfl_xor_sync(0xffffffffu, v, 2);
 }
-__device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.0f : m; }
-
 // ---------------------------------------------------------------- few rows per sequence and key head: decoding
 // A CTA walks its piece of the pages through a ring of stages filled by cp.async.  Four warps share a page, 16 positions each, for
 // every 16 rows (MT row groups of four warps); mma.sync m16n8k16 in f16, whose operands the lanes make from the bytes in
@@ -81,51 +53,6 @@ struct DecodeShape {
   static constexpr int kMerge = MT * 2 * 16 * D;                        // floats
   static constexpr int kSmem = kStages * kStageBytes + kMerge * 4;
 };
-constexpr float kHeadroom = 7.0f;     // weights are kept times 2^7 in f16 ...
-constexpr float kGrowth = 8.0f;       // ... and may grow to 2^15 before their reference follows
-
-template <int D>
-__device__ __forceinline__ int swizzled(int row, int chunk) {   // byte offset of a row's 16-byte chunk
-  return row * D + ((D == 128 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3)) << 4);
-}
-
-// Adds up a split unit's parts: out = sum o_p 2^(n_p - n) 2^(n - m) / sum l_p 2^(m_p - m).
-template <int D, int ROWS>
-__device__ void join_parts(const AttentionArgs& a, const KvSequence& s, int rt, int head, int rows, long long total, int ctas, int first, int last,
-                           long long unit_start) {
-  const float4* stats = reinterpret_cast<const float4*>(a.partial + 2ll * ctas * ROWS * D);
-  for (int i = threadIdx.x; i < rows * (D / 4); i += blockDim.x) {
-    const int row = i / (D / 4), d = (i % (D / 4)) * 4;
-    auto slot = [&](int c) { return 2 * c + (piece_start(total, ctas, c) >= unit_start ? 0 : 1); };
-    float m = -INFINITY, n = -INFINITY;
-    for (int c = first; c <= last; ++c) {
-      const float4 st = __ldcg(stats + static_cast<long long>(slot(c)) * ROWS + row);
-      m = fmaxf(m, st.x);
-      n = fmaxf(n, st.z);
-    }
-    const float m_ref = finite_or_zero(m), n_ref = finite_or_zero(n);
-    float l = 0.0f;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-    for (int c = first; c <= last; ++c) {
-      const long long at = static_cast<long long>(slot(c)) * ROWS + row;
-      const float4 st = __ldcg(stats + at);
-      const float4 part = __ldcg(reinterpret_cast<const float4*>(a.partial + at * D + d));
-      l += st.y * ex2(st.x - m_ref);
-      const float f = ex2(st.z - n_ref);
-      o.x = fmaf(part.x, f, o.x);
-      o.y = fmaf(part.y, f, o.y);
-      o.z = fmaf(part.z, f, o.z);
-      o.w = fmaf(part.w, f, o.w);
-    }
-    const float f = l == 0.0f ? 0.0f : ex2(n_ref - m_ref - kHeadroom) / l;
-    const int r = rt * ROWS + row;
-    __nv_bfloat16* to = a.out + (s.first + r / a.group) * a.out_stride + (head * a.group + r % a.group) * D + d;
-    const __nv_bfloat162 lo = __floats2bfloat162_rn(o.x * f, o.y * f), hi = __floats2bfloat162_rn(o.z * f, o.w * f);
-    *reinterpret_cast<uint2*>(to) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-  }
-}
-
 template <int D, int MT>
 __global__ void __launch_bounds__(DecodeShape<D, MT>::kThreads, DecodeShape<D, MT>::kBlocks) attention_decode_kernel(const __grid_constant__ AttentionArgs a) {
   using Shape = DecodeShape<D, MT>;
@@ -462,7 +389,7 @@ __global__ void __launch_bounds__(DecodeShape<D, MT>::kThreads, DecodeShape<D, M
         __syncthreads();
         if (s_plan.last) {
           __threadfence();
-          join_parts<D, kRows>(a, use.s, use.rt, use.head, rows, total, ctas, first, last, unit_start);
+          join_parts<D, kRows>(a, use.s, use.rt, use.head, rows, total, ctas, first, last, unit_start, tid, Shape::kThreads);
         }
       }
       fresh = true;
@@ -476,8 +403,10 @@ __global__ void __launch_bounds__(DecodeShape<D, MT>::kThreads, DecodeShape<D, M
 // ---------------------------------------------------------------- host
 struct Device {
   ScratchPool scratch;
-  bool ready = false;      // the kernels' shared memory is allowed
+  int* status = nullptr;
+  long long next_wait_limit = 0;   // syfi_kv_debug_wait_limit: applies to the next call, then clears itself
 };
+constexpr long long kWaitLimit = 1ll << 32;   // SM clocks (about two seconds)
 std::mutex g_mu;
 Device g_devices[64];
 
@@ -488,16 +417,20 @@ bool raise_decode() {
 
 constexpr size_t kTicketBytes = 4096;      // 1024 CTAs
 
+bool take_scratch(AttentionArgs& a, Device& d, size_t partial, cudaStream_t st, int* rc) {
+  Scratch* const s = d.scratch.get(st, kTicketBytes + partial, kTicketBytes, SYFI_KV_ERR_CUDA, rc);
+  if (!s) return false;
+  a.tickets = static_cast<int*>(s->memory);
+  a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(s->memory) + kTicketBytes);
+  return true;
+}
+
 template <int D, int MT>
 int launch_decode(AttentionArgs a, Device& d, int sms, cudaStream_t st) {
   using Shape = DecodeShape<D, MT>;
   const int ctas = sms * Shape::kBlocks;
-  const size_t need = kTicketBytes + 2ull * ctas * Shape::kRows * (D + 4) * sizeof(float);
   int rc = SYFI_KV_OK;
-  Scratch* const s = d.scratch.get(st, need, kTicketBytes, SYFI_KV_ERR_CUDA, &rc);
-  if (!s) return rc;
-  a.tickets = static_cast<int*>(s->memory);
-  a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(s->memory) + kTicketBytes);
+  if (!take_scratch(a, d, 2ull * ctas * Shape::kRows * (D + 4) * sizeof(float), st, &rc)) return rc;
   return launch_dependent(attention_decode_kernel<D, MT>, dim3(ctas), dim3(Shape::kThreads), Shape::kSmem, st, a) == cudaSuccess
              ? SYFI_KV_OK : kv_fail(SYFI_KV_ERR_CUDA, "attention kernel launch failed");
 }
@@ -542,15 +475,54 @@ extern "C" int syfi_paged_attention(const void* q, int64_t q_stride, const void*
   cudaGetDevice(&dev);
   std::lock_guard<std::mutex> lock(g_mu);
   Device& d = g_devices[dev];
-  if (!d.ready) {
-    if (!raise_decode<128, 1>() || !raise_decode<128, 2>() || !raise_decode<128, 4>() || !raise_decode<64, 1>() || !raise_decode<64, 2>() || !raise_decode<64, 4>())
+  if (!d.status) {
+    if (!raise_decode<128, 1>() || !raise_decode<128, 2>() || !raise_decode<128, 4>() || !raise_decode<64, 1>() || !raise_decode<64, 2>() || !raise_decode<64, 4>() ||
+        chunk_set_attributes() != cudaSuccess)
       return kv_fail(SYFI_KV_ERR_CUDA, "cannot raise the shared-memory limit of the attention kernels");
-    d.ready = true;
+    RelaxedCapture relaxed;
+    if (cudaMalloc(&d.status, 16) != cudaSuccess || !zero_now(d.status, 16)) return kv_fail(SYFI_KV_ERR_CUDA, "out of device memory");
   }
+  const long long wait_limit = d.next_wait_limit > 0 ? d.next_wait_limit : kWaitLimit;
+  d.next_wait_limit = 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // Rows per sequence and key head, on average (the lengths themselves are on the device): row tiles of 16, 32 or 64.
+  // Rows per sequence and key head, on average (the lengths themselves are on the device): row tiles of 16, 32 or 64, beyond that
+  // the tensor memory kernel's of 256.
   const int64_t rows = (tokens * a.group + batch - 1) / batch;
+  if (rows > 64) {
+    int rc = SYFI_KV_OK;
+    if (!take_scratch(a, d, chunk_partial_bytes(head_dim, sms), st, &rc)) return rc;
+    return launch_chunk(a, head_dim, sms, d.status, wait_limit, st) == cudaSuccess ? SYFI_KV_OK : kv_fail(SYFI_KV_ERR_CUDA, "attention kernel launch failed");
+  }
   if (head_dim == 128)
     return rows <= 16 ? launch_decode<128, 1>(a, d, sms, st) : rows <= 32 ? launch_decode<128, 2>(a, d, sms, st) : launch_decode<128, 4>(a, d, sms, st);
   return rows <= 16 ? launch_decode<64, 1>(a, d, sms, st) : rows <= 32 ? launch_decode<64, 2>(a, d, sms, st) : launch_decode<64, 4>(a, d, sms, st);
+}
+
+// Test hook for the bounded waits, no part of the interface: a wait of the next attention call's kernel on the current device may
+// take this many SM clocks (0: the normal limit).
+extern "C" int syfi_kv_debug_wait_limit(int64_t clocks) {
+  if (clocks < 0) return kv_fail(SYFI_KV_ERR_INVALID, "a wait limit must not be negative");
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return kv_fail(SYFI_KV_ERR_CUDA, "no current CUDA device");
+  std::lock_guard<std::mutex> lock(g_mu);
+  g_devices[dev].next_wait_limit = clocks;
+  return SYFI_KV_OK;
+}
+
+extern "C" int syfi_kv_check(void* stream) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return kv_fail(SYFI_KV_ERR_CUDA, "no current CUDA device");
+  if (cudaStreamSynchronize(static_cast<cudaStream_t>(stream)) != cudaSuccess) return kv_fail(SYFI_KV_ERR_CUDA, "stream synchronisation failed");
+  std::lock_guard<std::mutex> lock(g_mu);
+  Device& d = g_devices[dev];
+  if (!d.status) return SYFI_KV_OK;
+  int status = 0;
+  if (cudaMemcpy(&status, d.status, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess) return kv_fail(SYFI_KV_ERR_CUDA, "cannot read the status word");
+  if (status != 0) {
+    cudaMemset(d.status, 0, sizeof(int));
+    char msg[128];
+    snprintf(msg, sizeof(msg), "a kernel reported status %d (301: a bounded wait of the attention ran out; its rows are NaN)", status);
+    return kv_fail(SYFI_KV_ERR_DEVICE, msg);
+  }
+  return SYFI_KV_OK;
 }

@@ -26,6 +26,7 @@ ABI = {
     "syfi_kv_read": (ctypes.c_int, [_vp, _i64, _i64, _i32, _i32, _i32, _vp, _i64, _i32, _vp, _vp, _vp]),
     "syfi_paged_attention": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i64, _vp, _i32, _vp, _vp, _i32, _i64, _i32, _i32, _i32, _f64,
                                             _i32, _vp, _i64, _vp]),
+    "syfi_kv_check": (ctypes.c_int, [_vp]),
 }
 _bound = None      # the library once these functions are declared
 
@@ -216,4 +217,11 @@ def run_paged_attention(q, kv_cache, block_table, seq_lens, q_starts, out, *, sc
     return out
 
 
-__all__ = ["kv_cache_shape", "run_kv_read", "run_kv_write", "run_paged_attention"]
+def kv_check(device=None, stream=None):
+    """Synchronise and raise :class:`MoeError` if an attention kernel gave up on a bounded wait."""
+    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    with torch.cuda.device(dev):
+        _check(_lib().syfi_kv_check(_stream_ptr(stream, dev.index)))
+
+
+__all__ = ["kv_cache_shape", "kv_check", "run_kv_read", "run_kv_write", "run_paged_attention"]
