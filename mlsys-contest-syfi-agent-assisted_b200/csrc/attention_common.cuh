@@ -48,40 +48,61 @@ __device__ __forceinline__ int swizzled(int row, int chunk) {   // byte offset o
   return row * D + ((D == 128 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3)) << 4);
 }
 
-// Adds up a split unit's parts: out = sum o_p 2^(n_p - n) 2^(n - m) / sum l_p 2^(m_p - m).
-template <int D, int ROWS>
-__device__ __forceinline__ void join_parts(const AttentionArgs& a, const KvSequence& s, int rt, int head, int rows, long long total, int ctas, int first, int last,
-                           long long unit_start, int thread, int threads) {
-  const float4* stats = reinterpret_cast<const float4*>(a.partial + 2ll * ctas * ROWS * D);
-  for (int i = thread; i < rows * (D / 4); i += threads) {
-    const int row = i / (D / 4), d = (i % (D / 4)) * 4;
-    auto slot = [&](int c) { return 2 * c + (piece_start(total, ctas, c) >= unit_start ? 0 : 1); };
-    float m = -INFINITY, n = -INFINITY;
-    for (int c = first; c <= last; ++c) {
-      const float4 st = __ldcg(stats + static_cast<long long>(slot(c)) * ROWS + row);
-      m = fmaxf(m, st.x);
-      n = fmaxf(n, st.z);
+// The parts of a split unit [unit_start, unit_start + tiles) of the line: CTAs first .. last, of which all but perhaps the first have it
+// at the start of their piece.
+struct Parts {
+  int first, last, first_slot;
+  __device__ Parts(long long total, int ctas, long long unit_start, int tiles)
+      : first(piece_of(total, ctas, unit_start)), last(piece_of(total, ctas, unit_start + tiles - 1)),
+        first_slot(2 * first + (piece_start(total, ctas, first) < unit_start)) {}
+  __device__ int slot(int c) const { return c == first ? first_slot : 2 * c; }
+};
+
+// Adds up a split unit's parts: out = sum o_p 2^(n_p - n) 2^(n - m) / sum l_p 2^(m_p - m).  A group of D / 4 threads has a row, four
+// dimensions each, and BATCH rows at once, so that their loads are under way together.
+template <int D, int ROWS, int BATCH>
+__device__ __forceinline__ void join_parts(const AttentionArgs& a, int q_first, int unit_row0, int head, int rows, int ctas, const Parts& parts,
+                                           int thread, int threads) {
+  const float4* const stats = reinterpret_cast<const float4*>(a.partial + 2ll * ctas * ROWS * D);
+  const int d = thread % (D / 4) * 4, groups = threads / (D / 4);
+  for (int row0 = thread / (D / 4); row0 < rows; row0 += groups * BATCH) {
+    float m[BATCH], n[BATCH], l[BATCH];
+    float4 o[BATCH];
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      m[k] = n[k] = -INFINITY;
+      l[k] = 0.0f;
+      o[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
-    const float m_ref = finite_or_zero(m), n_ref = finite_or_zero(n);
-    float l = 0.0f;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-    for (int c = first; c <= last; ++c) {
-      const long long at = static_cast<long long>(slot(c)) * ROWS + row;
-      const float4 st = __ldcg(stats + at);
-      const float4 part = __ldcg(reinterpret_cast<const float4*>(a.partial + at * D + d));
-      l += st.y * ex2(st.x - m_ref);
-      const float f = ex2(st.z - n_ref);
-      o.x = fmaf(part.x, f, o.x);
-      o.y = fmaf(part.y, f, o.y);
-      o.z = fmaf(part.z, f, o.z);
-      o.w = fmaf(part.w, f, o.w);
+#pragma unroll 2
+    for (int c = parts.first; c <= parts.last; ++c) {
+      const long long base = static_cast<long long>(parts.slot(c)) * ROWS;
+      float4 st[BATCH], part[BATCH];
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {
+        const long long at = base + min(row0 + groups * k, rows - 1);
+        st[k] = __ldcg(stats + at);
+        part[k] = __ldcg(reinterpret_cast<const float4*>(a.partial + at * D + d));
+      }
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {
+        const float m_new = fmaxf(m[k], st[k].x), n_new = fmaxf(n[k], st[k].z), m_ref = finite_or_zero(m_new), n_ref = finite_or_zero(n_new);
+        l[k] = l[k] * ex2(m[k] - m_ref) + st[k].y * ex2(st[k].x - m_ref);
+        const float f = ex2(n[k] - n_ref), g = ex2(st[k].z - n_ref);
+        o[k] = make_float4(o[k].x * f + part[k].x * g, o[k].y * f + part[k].y * g, o[k].z * f + part[k].z * g, o[k].w * f + part[k].w * g);
+        m[k] = m_new;
+        n[k] = n_new;
+      }
     }
-    const float f = l == 0.0f ? 0.0f : ex2(n_ref - m_ref - kHeadroom) / l;
-    const int r = rt * ROWS + row;
-    __nv_bfloat16* to = a.out + (s.first + r / a.group) * a.out_stride + (head * a.group + r % a.group) * D + d;
-    const __nv_bfloat162 lo = __floats2bfloat162_rn(o.x * f, o.y * f), hi = __floats2bfloat162_rn(o.z * f, o.w * f);
-    *reinterpret_cast<uint2*>(to) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      const int row = row0 + groups * k, r = unit_row0 + row;
+      if (row >= rows) break;
+      const float f = l[k] == 0.0f ? 0.0f : ex2(finite_or_zero(n[k]) - finite_or_zero(m[k]) - kHeadroom) / l[k];
+      __nv_bfloat16* to = a.out + (q_first + r / a.group) * a.out_stride + (head * a.group + r % a.group) * D + d;
+      const __nv_bfloat162 lo = __floats2bfloat162_rn(o[k].x * f, o[k].y * f), hi = __floats2bfloat162_rn(o[k].z * f, o[k].w * f);
+      *reinterpret_cast<uint2*>(to) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+    }
   }
 }
 

@@ -378,18 +378,18 @@ __global__ void __launch_bounds__(DecodeShape<D, MT>::kThreads, DecodeShape<D, M
         }
       }
       if (!whole) {
-        const int first = piece_of(total, ctas, unit_start), last = piece_of(total, ctas, unit_start + use.span.tiles - 1);
+        const Parts parts(total, ctas, unit_start, use.span.tiles);
         __threadfence();
         __syncthreads();
         if (tid == 0) {
-          const bool is_last = atomicAdd(a.tickets + first, 1) == last - first;
-          if (is_last) a.tickets[first] = 0;
+          const bool is_last = atomicAdd(a.tickets + parts.first, 1) == parts.last - parts.first;
+          if (is_last) a.tickets[parts.first] = 0;
           s_plan.last = is_last;
         }
         __syncthreads();
         if (s_plan.last) {
           __threadfence();
-          join_parts<D, kRows>(a, use.s, use.rt, use.head, rows, total, ctas, first, last, unit_start, tid, Shape::kThreads);
+          join_parts<D, kRows, 1>(a, use.s.first, use.rt * kRows, use.head, rows, ctas, parts, tid, Shape::kThreads);
         }
       }
       fresh = true;

@@ -23,7 +23,6 @@ constexpr int kTile = 128;             // positions per tile: two pages
 constexpr int kChunkRows = 256;
 constexpr int kChunkThreads = 512;
 constexpr int kScaleStages = 4;
-constexpr int kFlagRing = 4;
 constexpr int kStatusChunkTimeout = 301;
 constexpr int kUnitShift = 5;          // the largest value scale becomes 2^4 .. 2^5 when the unit's reference is set, ...
 constexpr int kUnitGrowth = 2;         // ... and may grow to 2^7 (448 * 2^7 < 65504) before the reference follows
@@ -45,30 +44,36 @@ struct ChunkShape {
   static constexpr int kSmem = 1024 + kRedo + 8 * (D + kKvPage) * 4;
 };
 
+// A piece of a unit, as the planning warp describes it to the others.
+struct Segment {
+  int tile0, tiles;                    // tiles [tile0, tile0 + tiles) of the sequence's positions
+  int rows, row0;                      // rows [row0, row0 + rows) of the sequence's count * group
+  int head, b, q_first;                // key head, sequence, its first row of q
+  int base;                            // position of the sequence's first query
+  int any_low, any_high, all_low, all_high;   // positions that any / all of the rows see
+  int whole;                           // the unit lies in this piece alone
+  int unit_tiles;
+  long long unit_start;                // on the line
+};
+constexpr int kSegmentRing = 4;
+constexpr int kSegmentReaders = 14;    // arrivals that free an entry: loads, MMAs, 4 converting and 8 softmax warps
+
 struct ChunkShared {
+  Segment segment[kSegmentRing];
+  uint64_t segment_full[kSegmentRing], segment_empty[kSegmentRing];
   uint64_t scale_full[kScaleStages], scale_clean[kScaleStages], scale_empty[kScaleStages], k_full[4], k_empty[4], v_full[2], v_empty[2], half_full[2], half_empty[2];
   uint64_t q_full[2], s_full[2], p_full[2], o_full[2], o_empty[2], idle;
   uint32_t tmem;
   int there[kScaleStages];             // bit p: page p of the tile is there
-  volatile int redo[kFlagRing];        // of the segment: f16 did not hold a value
+  volatile int redo[kSegmentRing];     // of the segment: f16 did not hold a value
   volatile int abort_code;
   int finished;                        // segments of this CTA whose results are written
   int asked_k, asked_v, asked_scales;  // loads that the producer has issued
 };
 
-// The row tile's positions, as every role sees them.
-struct Seen {
-  int any_low, any_high, all_low, all_high;
-};
-__device__ __forceinline__ Seen seen_by(const Cursor<kTile, kChunkRows>& at, int group, int window) {
-  const int rows = at.rows(group), base = at.s.length - at.s.count, r0 = at.rt * kChunkRows;
-  const int first = base + r0 / group, last = base + (r0 + rows - 1) / group;
-  return {window > 0 ? max(first - window + 1, 0) : 0, last, window > 0 ? max(last - window + 1, 0) : 0, first};
-}
-
 // The unit's reference after a tile: 2^e above every finite scale of a position that is there and seen by any row; whole warp.
 // Roles that need it follow it by themselves.
-__device__ __forceinline__ int tile_exponent(const float* v_scale, int there, int position0, const Seen& seen, int lane) {
+__device__ __forceinline__ int tile_exponent(const float* v_scale, int there, int position0, int any_low, int any_high, int lane) {
   const float4 v = reinterpret_cast<const float4*>(v_scale)[lane];
   const float x[4] = {v.x, v.y, v.z, v.w};
   unsigned top = 0u;
@@ -77,7 +82,7 @@ __device__ __forceinline__ int tile_exponent(const float* v_scale, int there, in
   for (int i = 0; i < 4; ++i) {
     const unsigned bits = __float_as_uint(x[i]) & 0x7fffffffu;
     const int position = position0 + 4 * lane + i;
-    if (here && position >= seen.any_low && position <= seen.any_high && bits < 0x7f800000u) top = max(top, bits);
+    if (here && position >= any_low && position <= any_high && bits < 0x7f800000u) top = max(top, bits);
   }
   top = __reduce_max_sync(0xffffffffu, top);
   return max(static_cast<int>(top >> 23) - 126, -100);
@@ -99,11 +104,11 @@ __device__ __forceinline__ bool softmax_bar_any(bool p) {
 
 // One row in f32 by one warp, for what the tiles cannot hold: a lane has two of a page's positions, then D / 32 dimensions.
 template <int D>
-__device__ __noinline__ void exact_row(const AttentionArgs& a, const KvSequence& s, int b, int head, int r, float* s_q, float* s_p) {
+__device__ __noinline__ void exact_row(const AttentionArgs& a, int base, int q_first, int b, int head, int r, float* s_q, float* s_p) {
   const int lane = threadIdx.x % 32, t = r / a.group;
-  const int position = s.length - s.count + t, low = a.window > 0 ? max(position - a.window + 1, 0) : 0;
+  const int position = base + t, low = a.window > 0 ? max(position - a.window + 1, 0) : 0;
   const long long column = static_cast<long long>(head * a.group + r % a.group) * D;
-  const __nv_bfloat16* q = a.q + (s.first + t) * a.q_stride + column;
+  const __nv_bfloat16* q = a.q + (q_first + t) * a.q_stride + column;
   for (int d = lane; d < D; d += 32) s_q[d] = __bfloat162float(q[d]);
   __syncwarp();
   float m = -INFINITY, l = 0.0f, acc[D / 32] = {};
@@ -155,8 +160,544 @@ __device__ __noinline__ void exact_row(const AttentionArgs& a, const KvSequence&
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
   for (int i = 0; i < D / 64; ++i)
-    *reinterpret_cast<__nv_bfloat162*>(a.out + (s.first + t) * a.out_stride + column + i * 64 + lane * 2) =
+    *reinterpret_cast<__nv_bfloat162*>(a.out + (q_first + t) * a.out_stride + column + i * 64 + lane * 2) =
         __floats2bfloat162_rn(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+}
+
+__device__ __forceinline__ bool wait_for(ChunkShared& sh, uint64_t* bar, uint32_t parity, long long limit) {
+  return mbar_wait_bounded(bar, parity, &sh.abort_code, kStatusChunkTimeout, limit);
+}
+__device__ __forceinline__ void wait_whole_warp(ChunkShared& sh, bool& ok, uint64_t* bar, uint32_t parity, long long limit) {
+  mbar_wait_or_clear(ok, bar, parity, &sh.abort_code, kStatusChunkTimeout, limit);
+}
+
+// A place in a ring of stages: its index, and the parity of its use.
+template <int N>
+struct Ring {
+  int stage = 0;
+  uint32_t parity = 0;
+  __device__ void next() {
+    if (++stage == N) {
+      stage = 0;
+      parity ^= 1u;
+    }
+  }
+};
+
+// ---------------------------------------------------------------- planning (one thread)
+__device__ __forceinline__ void plan_role(const AttentionArgs& a, const Plan<kTile, kChunkRows>& plan, const PlanShared& s_plan, ChunkShared& sh, int count,
+                                       long long w0, long long limit) {
+  Cursor<kTile, kChunkRows> at;
+  at.start(plan, s_plan);
+  Ring<kSegmentRing> ring;
+  for (int i = 0; i < count;) {
+    if (!wait_for(sh, &sh.segment_empty[ring.stage], ring.parity ^ 1u, limit)) return;
+    Segment& g = sh.segment[ring.stage];
+    const int rows = at.rows(a.group), base = at.s.length - at.s.count, row0 = at.rt * kChunkRows;
+    const int first = base + row0 / a.group, last = base + (row0 + rows - 1) / a.group;
+    g.tile0 = at.span.first + at.tile;
+    g.tiles = min(at.span.tiles - at.tile, count - i);
+    g.rows = rows;
+    g.row0 = row0;
+    g.head = at.head;
+    g.b = at.b;
+    g.q_first = at.s.first;
+    g.base = base;
+    g.any_low = a.window > 0 ? max(first - a.window + 1, 0) : 0;
+    g.any_high = last;
+    g.all_low = a.window > 0 ? max(last - a.window + 1, 0) : 0;
+    g.all_high = first;
+    g.whole = g.tiles == at.span.tiles;
+    g.unit_tiles = at.span.tiles;
+    g.unit_start = w0 + i - at.tile;
+    mbar_arrive(&sh.segment_full[ring.stage]);
+    i += g.tiles;
+    ring.next();
+    if (i < count) at.next_unit(plan);
+  }
+}
+
+// ---------------------------------------------------------------- loads (one thread)
+template <int D>
+__device__ __forceinline__ void load_role(const CUtensorMap& map, const AttentionArgs& a, ChunkShared& sh, uint8_t* smem, int count, long long limit) {
+  using Shape = ChunkShape<D>;
+  const uint64_t keep = l2_policy_evict_normal();          // other row tiles of the sequence read the same pages
+  Ring<kSegmentRing> segments;
+  Ring<kScaleStages> scales;
+  Ring<Shape::kKStages> keys;
+  Ring<Shape::kVStages> values;
+  int head = 0, next_tile = 0, left = 0, any_low = 0, any_high = 0;
+  const int32_t* table = nullptr;
+  int entry0 = -1, entry1 = -1;
+  // table entries of the tile to ask for next: read one tile ahead
+  auto entries = [&]() {
+    if (left == 0) {
+      if (!wait_for(sh, &sh.segment_full[segments.stage], segments.parity, limit)) return false;
+      const Segment& g = sh.segment[segments.stage];
+      next_tile = g.tile0;
+      left = g.tiles;
+      any_low = g.any_low;
+      any_high = g.any_high;
+      head = g.head;
+      table = a.batch.block_table + static_cast<long long>(g.b) * a.batch.max_pages;
+      mbar_arrive(&sh.segment_empty[segments.stage]);
+      segments.next();
+    }
+    const int page = 2 * next_tile;
+    entry0 = page < a.batch.max_pages && page * kKvPage <= any_high && (page + 1) * kKvPage > any_low ? __ldg(table + page) : -1;
+    entry1 = page + 1 < a.batch.max_pages && (page + 1) * kKvPage <= any_high && (page + 2) * kKvPage > any_low ? __ldg(table + page + 1) : -1;
+    ++next_tile;
+    --left;
+    return true;
+  };
+  bool alive = entries();
+  for (int i = 0; i < count && alive; ++i) {
+    const int entry[2] = {entry0, entry1}, h = head;
+    const bool here[2] = {entry0 >= 0 && entry0 < a.cache.num_pages, entry1 >= 0 && entry1 < a.cache.num_pages};
+    const int pages = here[0] + here[1];
+    if (i + 1 < count && !entries()) return;
+    if (!wait_for(sh, &sh.scale_empty[scales.stage], scales.parity ^ 1u, limit)) return;
+    sh.there[scales.stage] = here[0] | here[1] << 1;
+    mbar_arrive_expect_tx(&sh.scale_full[scales.stage], pages * 2 * kKvPage * 4);
+    float* const scale = reinterpret_cast<float*>(smem + Shape::kScales) + scales.stage * 2 * kTile;
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      if (!here[p]) continue;
+      bulk_load(scale + p * kKvPage, kv_block<D>(a.cache, entry[p], 0, h) + kKvPage * D, kKvPage * 4, &sh.scale_full[scales.stage], keep);
+      bulk_load(scale + kTile + p * kKvPage, kv_block<D>(a.cache, entry[p], 1, h) + kKvPage * D, kKvPage * 4, &sh.scale_full[scales.stage], keep);
+    }
+    sh.asked_scales = i + 1;
+    scales.next();
+    if (!wait_for(sh, &sh.k_empty[keys.stage], keys.parity ^ 1u, limit)) return;
+    mbar_arrive_expect_tx(&sh.k_full[keys.stage], pages * kKvPage * D);
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+      if (here[p]) tma_load_4d(smem + Shape::kK + keys.stage * Shape::kTileBytes + p * kKvPage * D, &map, &sh.k_full[keys.stage], 0, 0, h, entry[p], keep);
+    sh.asked_k = i + 1;
+    keys.next();
+    if (!wait_for(sh, &sh.v_empty[values.stage], values.parity ^ 1u, limit)) return;
+    mbar_arrive_expect_tx(&sh.v_full[values.stage], pages * kKvPage * D);
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+      if (here[p]) tma_load_4d(smem + Shape::kV + values.stage * Shape::kTileBytes + p * kKvPage * D, &map, &sh.v_full[values.stage], 0, 0, a.cache.heads + h, entry[p], keep);
+    sh.asked_v = i + 1;
+    values.next();
+  }
+}
+
+// ---------------------------------------------------------------- MMAs (one thread)
+template <int D>
+__device__ __forceinline__ void mma_role(ChunkShared& sh, uint8_t* smem, uint32_t tmem, int count, long long limit) {
+  using Shape = ChunkShape<D>;
+  const uint32_t qk_desc = umma_idesc_e4m3_m128(kTile), pv_desc = umma_idesc_f16_m128_n_major(D);
+  const uint64_t q_desc = D == 128 ? umma_smem_desc_sw128(smem_u32(smem + Shape::kQ)) : umma_smem_desc_sw64(smem_u32(smem + Shape::kQ));
+  const uint64_t v_desc = umma_smem_desc_n_major_sw128(smem_u32(smem + Shape::kHalf), kTile * 128);
+  const uint32_t q0 = static_cast<uint32_t>(q_desc), k0 = q0 + (Shape::kK - Shape::kQ) / 16, qk_hi = static_cast<uint32_t>(q_desc >> 32);
+  const uint32_t v0 = static_cast<uint32_t>(v_desc), v_hi = static_cast<uint32_t>(v_desc >> 32);
+  auto scores = [&](int slot, int stage) {
+    const uint32_t k = k0 + stage * (Shape::kTileBytes / 16), q = q0 + slot * (2 * Shape::kTileBytes / 16), to = tmem + slot * 128;
+#pragma unroll
+    for (int term = 0; term < 2; ++term)
+#pragma unroll
+      for (int step = 0; step < D / 32; ++step)
+        umma_f8_words(to, q + term * (Shape::kTileBytes / 16) + 2 * step, k + 2 * step, qk_hi, qk_desc, term + step > 0 ? 1u : 0u);
+    umma_commit(&sh.s_full[slot]);
+  };
+  auto values = [&](int slot, int stage, uint32_t add) {
+    const uint32_t v = v0 + stage * (Shape::kHalfBytes / 16), p = tmem + slot * 128;
+#pragma unroll
+    for (int step = 0; step < kTile / 16; ++step) umma_f16_ts_words(p + 256, p + 8 * step, v + 128 * step, v_hi, pv_desc, step == 0 ? add : 1u);
+  };
+  Ring<kSegmentRing> segments;
+  Ring<Shape::kKStages> keys;
+  Ring<Shape::kHalfStages> halves;
+  uint32_t tile_parity = 0, segment_parity = 0;    // bit s: of slot s
+  for (int i = 0; i < count;) {
+    if (!wait_for(sh, &sh.segment_full[segments.stage], segments.parity, limit)) return;
+    const int n = sh.segment[segments.stage].tiles, slots = sh.segment[segments.stage].rows > 128 ? 2 : 1;
+    mbar_arrive(&sh.segment_empty[segments.stage]);
+    segments.next();
+    for (int s = 0; s < slots; ++s)
+      if (!wait_for(sh, &sh.q_full[s], segment_parity >> s & 1u, limit)) return;
+    if (!wait_for(sh, &sh.k_full[keys.stage], keys.parity, limit)) return;
+    tc_fence_after();
+    for (int s = 0; s < slots; ++s) scores(s, keys.stage);
+    umma_commit(&sh.k_empty[keys.stage]);
+    keys.next();
+    for (int j = 0; j < n; ++j) {
+      const bool more = j + 1 < n;
+      if (more && !wait_for(sh, &sh.k_full[keys.stage], keys.parity, limit)) return;
+      if (!wait_for(sh, &sh.half_full[halves.stage], halves.parity, limit)) return;
+#pragma unroll 1
+      for (int s = 0; s < slots; ++s) {
+        if (j == 0 && !wait_for(sh, &sh.o_empty[s], (segment_parity >> s & 1u) ^ 1u, limit)) return;
+        if (!wait_for(sh, &sh.p_full[s], tile_parity >> s & 1u, limit)) return;
+        tile_parity ^= 1u << s;
+        tc_fence_after();
+        values(s, halves.stage, j > 0 ? 1u : 0u);
+        if (s + 1 == slots) umma_commit(&sh.half_empty[halves.stage]);
+        if (more) scores(s, keys.stage);
+        else umma_commit(&sh.o_full[s]);
+      }
+      halves.next();
+      if (more) {
+        umma_commit(&sh.k_empty[keys.stage]);
+        keys.next();
+      }
+    }
+    segment_parity ^= slots == 2 ? 3u : 1u;
+    i += n;
+  }
+}
+
+// ---------------------------------------------------------------- values to f16, a thread per position (four warps)
+template <int D>
+__device__ __forceinline__ void convert_role(ChunkShared& sh, uint8_t* smem, int count, long long limit) {
+  using Shape = ChunkShape<D>;
+  const int t = threadIdx.x - 8 * 32, lane = threadIdx.x % 32;
+  Ring<kSegmentRing> segments;
+  Ring<kScaleStages> scales;
+  Ring<Shape::kVStages> raw;
+  Ring<Shape::kHalfStages> halves;
+  bool ok = true;
+  for (int i = 0; i < count;) {
+    wait_whole_warp(sh, ok, &sh.segment_full[segments.stage], segments.parity, limit);
+    if (!__all_sync(0xffffffffu, ok)) return;
+    const Segment& g = sh.segment[segments.stage];
+    const int n = g.tiles;
+    int unit = -100;
+    for (int j = 0; j < n; ++j) {
+      float* const k_scale = reinterpret_cast<float*>(smem + Shape::kScales) + scales.stage * 2 * kTile;
+      wait_whole_warp(sh, ok, &sh.scale_full[scales.stage], scales.parity, limit);
+      const int there = sh.there[scales.stage], position0 = (g.tile0 + j) * kTile, any_low = g.any_low, any_high = g.any_high;
+      const int e = tile_exponent(k_scale + kTile, there, position0, any_low, any_high, lane);
+      if (j == 0 || e > unit + kUnitGrowth) unit = e;
+      const float scale = k_scale[kTile + t];
+      const bool valid = (there >> (t / kKvPage) & 1) && position0 + t >= any_low && position0 + t <= any_high;
+      const bool mixed = position0 < g.all_low || position0 + kTile - 1 > g.all_high;     // some rows may see what others do not
+      const float r = scale * __int_as_float((kUnitShift - unit + 127) << 23);
+      // r as two f16 terms, so that the product with a byte's value is rounded once
+      const __half hi = __float2half_rn(r);
+      const __half2 r_hi = __half2half2(hi), r_lo = __half2half2(__float2half_rn(r - __half2float(hi)));
+      wait_whole_warp(sh, ok, &sh.v_full[raw.stage], raw.parity, limit);
+      const uint8_t* const from = smem + Shape::kV + raw.stage * Shape::kTileBytes;
+      // Zero times NaN is NaN: where some rows see a value that is not finite and others do not, its bytes become zeros and the NaN
+      // goes by way of its score to the rows that see it.
+      bool bad = false;
+      if (mixed && valid) {
+        uint32_t over = 0u;
+#pragma unroll 2
+        for (int chunk = 0; chunk < D / 16; ++chunk) {
+          const uint4 p = *reinterpret_cast<const uint4*>(from + swizzled<D>(t, chunk));
+          over |= ((p.x & 0x7f7f7f7fu) + 0x01010101u) | ((p.y & 0x7f7f7f7fu) + 0x01010101u) | ((p.z & 0x7f7f7f7fu) + 0x01010101u) | ((p.w & 0x7f7f7f7fu) + 0x01010101u);
+        }
+        bad = (over & 0x80808080u) != 0u || !(fabsf(scale) <= 3.402823466e38f);
+        if (bad) k_scale[t] = __int_as_float(0x7fffffff);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.scale_clean[scales.stage]);
+      wait_whole_warp(sh, ok, &sh.half_empty[halves.stage], halves.parity ^ 1u, limit);
+      uint8_t* const to = smem + Shape::kHalf + halves.stage * Shape::kHalfBytes + t * 128;
+      if (valid && !bad) {
+        uint32_t any = 0u;
+#pragma unroll 2
+        for (int chunk = 0; chunk < D / 16; ++chunk) {
+          const uint4 p = *reinterpret_cast<const uint4*>(from + swizzled<D>(t, chunk));
+          const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+          uint32_t h[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const uint32_t bits = e4m3x2_to_half2(w[k / 2] >> (16 * (k % 2)));
+            const __half2 v = *reinterpret_cast<const __half2*>(&bits);
+            const __half2 y = __hfma2(v, r_hi, __hmul2(v, r_lo));
+            h[k] = *reinterpret_cast<const uint32_t*>(&y);
+          }
+          any |= (p.x | p.y | p.z | p.w) & 0x7f7f7f7fu;
+          uint8_t* const row = to + chunk / 4 * (kTile * 128);
+          *reinterpret_cast<uint4*>(row + (((2 * chunk) % 8 ^ (t & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+          *reinterpret_cast<uint4*>(row + (((2 * chunk + 1) % 8 ^ (t & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
+        }
+        if (any != 0u && fabsf(r) < kSmallestUnit) sh.redo[segments.stage] = 1;
+      } else {
+#pragma unroll 2
+        for (int chunk = 0; chunk < D / 8; ++chunk) *reinterpret_cast<uint4*>(to + chunk / 8 * (kTile * 128) + chunk % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&sh.half_full[halves.stage]);
+        mbar_arrive(&sh.v_empty[raw.stage]);
+        mbar_arrive(&sh.scale_empty[scales.stage]);
+      }
+      if (!__all_sync(0xffffffffu, ok)) return;
+      scales.next();
+      raw.next();
+      halves.next();
+    }
+    if (lane == 0) mbar_arrive(&sh.segment_empty[segments.stage]);
+    segments.next();
+    i += n;
+  }
+}
+
+// ---------------------------------------------------------------- softmax, a thread per row (eight warps, four to a slot)
+// One tile: scores from tensor memory, weights back into it, the row's reference m and sum l2 (in two halves).  `fade`: what the
+// unit's reference has become smaller by.
+__device__ __forceinline__ void softmax_tile(uint32_t t_s, uint32_t t_o, int o_columns, const float* k_scale, bool masked, int low, int high, int there,
+                                             float unit, float fade, bool first, float& m, uint64_t& l2) {
+  uint32_t s[4][32];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) tmem_ld32(t_s + 32 * c, s[c]);
+  tmem_ld_wait_for(s[0]);
+#pragma unroll
+  for (int c = 1; c < 4; ++c) tmem_landed(s[c]);
+  // times the key's scale: scores in units of the row's
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const ulonglong2 ks = *reinterpret_cast<const ulonglong2*>(k_scale + 32 * c + 4 * e);
+      float x0, x1, x2, x3;
+      f32x2_unpack(f32x2_mul(f32x2_pack_bits(s[c][4 * e], s[c][4 * e + 1]), ks.x), x0, x1);
+      f32x2_unpack(f32x2_mul(f32x2_pack_bits(s[c][4 * e + 2], s[c][4 * e + 3]), ks.y), x2, x3);
+      s[c][4 * e] = __float_as_uint(x0);
+      s[c][4 * e + 1] = __float_as_uint(x1);
+      s[c][4 * e + 2] = __float_as_uint(x2);
+      s[c][4 * e + 3] = __float_as_uint(x3);
+    }
+  }
+  if (masked) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      // bit b: the tile's position 32 c + b is there and seen (low and high count from the tile's first)
+      const int first_bit = low - 32 * c, last_bit = high - 32 * c;
+      uint32_t bits = last_bit < 0 || first_bit > 31 || !(there >> (c / 2) & 1) ? 0u : 0xffffffffu;
+      if (last_bit >= 0 && last_bit < 31) bits &= (2u << last_bit) - 1u;
+      if (first_bit > 0 && first_bit <= 31) bits &= 0xffffffffu << first_bit;
+#pragma unroll
+      for (int b = 0; b < 32; ++b)
+        if (!(bits >> b & 1u)) s[c][b] = 0xff800000u;
+    }
+  }
+  float top4[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    top4[c] = __uint_as_float(s[c][0]);
+#pragma unroll
+    for (int b = 1; b < 32; ++b) top4[c] = fmaxf(top4[c], __uint_as_float(s[c][b]));
+  }
+  const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * unit;
+  if (top > m + kGrowth) {
+    const float f = ex2(m - top);       // (0 for a row that had seen nothing)
+    fade *= f;
+    l2 = f32x2_mul(l2, f32x2_pack(f, f));
+    m = top;
+  }
+  if (!first && __any_sync(0xffffffffu, fade != 1.0f)) {
+    for (int c = 0; c < o_columns; c += 16) {
+      uint32_t o[16];
+      tmem_ld16(t_o + c, o);
+      tmem_ld_wait_for(o);
+#pragma unroll
+      for (int b = 0; b < 16; ++b) o[b] = __float_as_uint(__uint_as_float(o[b]) * fade);
+      tmem_st16(t_o + c, o);
+    }
+  }
+  const float shift = kHeadroom - finite_or_zero(m);
+  const uint64_t unit2 = f32x2_pack(unit, unit), shift2 = f32x2_pack(shift, shift);
+  uint64_t more = 0ull;
+#pragma unroll
+  for (int h = 0; h < 4; ++h) {
+    uint32_t p[16];
+#pragma unroll
+    for (int b = 0; b < 16; ++b) {
+      float x0, x1;
+      f32x2_unpack(f32x2_fma(f32x2_pack_bits(s[h][2 * b], s[h][2 * b + 1]), unit2, shift2), x0, x1);
+      x0 = ex2(x0);
+      x1 = ex2(x1);
+      uint64_t& sum = b & 1 ? more : l2;
+      sum = f32x2_add(sum, f32x2_pack(x0, x1));
+      p[b] = pack_half2(x0, x1);
+    }
+    tmem_st16(t_s + 16 * h, p);
+  }
+  l2 = f32x2_add(l2, more);
+  tmem_st_wait();
+}
+
+// The row's part of q as two e4m3 terms of q * 2^k, its largest at 2^7 .. 2^8, into the slot's tiles; returns what a score's unit is.
+template <int D>
+__device__ __forceinline__ float put_query(const __nv_bfloat16* q, bool real, float scale_log2, uint8_t* hi_tile, int row) {
+  uint4 raw[D / 8];
+  unsigned top = 0u;
+#pragma unroll
+  for (int c = 0; c < D / 8; ++c) {
+    raw[c] = real ? __ldg(reinterpret_cast<const uint4*>(q) + c) : make_uint4(0u, 0u, 0u, 0u);
+    const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top = max(top, max(w[e] & 0x7fffu, w[e] >> 16 & 0x7fffu));
+  }
+  const int k = top == 0u ? 0 : min(7 - (static_cast<int>(top >> 7) - 127), 120);
+  const float up = copysignf(__int_as_float((k + 127) << 23), scale_log2);
+#pragma unroll
+  for (int c = 0; c < D / 16; ++c) {
+    const uint32_t w[8] = {raw[2 * c].x, raw[2 * c].y, raw[2 * c].z, raw[2 * c].w, raw[2 * c + 1].x, raw[2 * c + 1].y, raw[2 * c + 1].z, raw[2 * c + 1].w};
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float x0 = __uint_as_float(w[2 * e] << 16) * up, x1 = __uint_as_float(w[2 * e] & 0xffff0000u) * up;
+      const float x2 = __uint_as_float(w[2 * e + 1] << 16) * up, x3 = __uint_as_float(w[2 * e + 1] & 0xffff0000u) * up;
+      const uint16_t h01 = cvt_e4m3x2(x0, x1), h23 = cvt_e4m3x2(x2, x3);
+      const float2 f01 = e4m3x2_to_float2(h01), f23 = e4m3x2_to_float2(h23);
+      hi[e] = h01 | static_cast<uint32_t>(h23) << 16;
+      lo[e] = cvt_e4m3x2(x0 - f01.x, x1 - f01.y) | static_cast<uint32_t>(cvt_e4m3x2(x2 - f23.x, x3 - f23.y)) << 16;
+    }
+    const int to = swizzled<D>(row, c);
+    *reinterpret_cast<uint4*>(hi_tile + to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    *reinterpret_cast<uint4*>(hi_tile + ChunkShape<D>::kTileBytes + to) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+  }
+  // (a scale of zero keeps a factor, so that -infinity stays what it is)
+  return top >= 0x7f80u ? __int_as_float(0x7fffffff) : fmaxf(fabsf(scale_log2) * __int_as_float((127 - k) << 23), 1e-30f);
+}
+
+template <int D>
+__device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared& sh, PlanShared& s_plan, uint8_t* smem, uint32_t tmem, int count, int ctas,
+                                             long long total, long long limit) {
+  using Shape = ChunkShape<D>;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, slot = warp / 4;
+  const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
+  const uint32_t t_s = tmem + lanes + slot * 128, t_o = tmem + lanes + 256 + slot * 128;
+  Ring<kSegmentRing> segments;
+  Ring<kScaleStages> scales;
+  uint32_t tile_parity = 0, segment_parity = 0;     // of this slot
+  bool ok = true;
+  int done = 0;                                     // segments
+  for (int i = 0; i < count;) {
+    wait_whole_warp(sh, ok, &sh.segment_full[segments.stage], segments.parity, limit);
+    __syncwarp();
+    const Segment& g = sh.segment[segments.stage];
+    const int n = ok ? g.tiles : 0;
+    const bool active = slot * 128 < g.rows;
+    const bool real = tid < g.rows;
+    float unit = 0.0f, m = -INFINITY;
+    uint64_t l2 = 0ull;
+    int exponent = -100;
+    if (n > 0) {
+      const int r = g.row0 + (real ? tid : g.rows - 1), token = r / a.group;        // (rows beyond the last copy its bounds)
+      const int high = g.base + token, low = a.window > 0 ? max(high - a.window + 1, 0) : 0;
+      if (active) {
+        unit = put_query<D>(a.q + (g.q_first + token) * a.q_stride + (g.head * a.group + r % a.group) * D, real, a.scale_log2,
+                            smem + Shape::kQ + 2 * slot * Shape::kTileBytes, tid % 128);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.q_full[slot]);
+      }
+      const int warp_low = __reduce_max_sync(0xffffffffu, low), warp_high = __reduce_min_sync(0xffffffffu, high);   // seen by every row of the warp
+      for (int j = 0; j < n; ++j) {
+        wait_whole_warp(sh, ok, &sh.scale_full[scales.stage], scales.parity, limit);
+        wait_whole_warp(sh, ok, &sh.scale_clean[scales.stage], scales.parity, limit);
+        if (active) {
+          const float* const k_scale = reinterpret_cast<const float*>(smem + Shape::kScales) + scales.stage * 2 * kTile;
+          const int there = sh.there[scales.stage], position0 = (g.tile0 + j) * kTile;
+          const int e = tile_exponent(k_scale + kTile, there, position0, g.any_low, g.any_high, lane);
+          float fade = 1.0f;
+          if (j == 0) {
+            exponent = e;
+          } else if (e > exponent + kUnitGrowth) {
+            fade = ex2(static_cast<float>(exponent - e));
+            exponent = e;
+          }
+          wait_whole_warp(sh, ok, &sh.s_full[slot], tile_parity, limit);
+          __syncwarp();
+          tc_fence_after();
+          softmax_tile(t_s, t_o, D, k_scale, position0 < warp_low || position0 + kTile - 1 > warp_high || there != 3, low - position0, high - position0,
+                       there, unit, fade, j == 0, m, l2);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.p_full[slot]);
+          tile_parity ^= 1u;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.scale_empty[scales.stage]);
+        scales.next();
+        if (!__all_sync(0xffffffffu, ok)) break;
+      }
+      // ---- the segment's end
+      if (active) {
+        wait_whole_warp(sh, ok, &sh.o_full[slot], segment_parity, limit);
+        __syncwarp();
+        tc_fence_after();
+        segment_parity ^= 1u;
+      }
+    }
+    if (softmax_bar_any(!ok)) return;         // all eight warps meet here whatever failed, and leave together
+    const bool redo = sh.redo[segments.stage] != 0, whole = g.whole;
+    if (tid == 0) sh.redo[(segments.stage + kSegmentRing - 1) % kSegmentRing] = 0;     // the segment before: everybody has read it
+    const Parts parts(total, ctas, g.unit_start, g.unit_tiles);
+    const int r = g.row0 + tid, token = r / a.group;
+    if (active) {
+      const int part = parts.slot(static_cast<int>(blockIdx.x)) * kChunkRows + tid;
+      float l0, l1;
+      f32x2_unpack(l2, l0, l1);
+      const float l = l0 + l1, unscale = __int_as_float((exponent - kUnitShift + 127) << 23);
+      const float f = whole ? (l == 0.0f ? 0.0f : unscale / l) : unscale;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld32(t_o + 32 * c, o);
+        tmem_ld_wait_for(o);
+        if (real && whole && !redo) {
+          uint4* to = reinterpret_cast<uint4*>(a.out + (g.q_first + token) * a.out_stride + (g.head * a.group + r % a.group) * D + 32 * c);
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(o[8 * b + 2 * e]) * f, __uint_as_float(o[8 * b + 2 * e + 1]) * f);
+              w[e] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+            to[b] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        } else if (real && !whole) {
+          float4* to = reinterpret_cast<float4*>(a.partial + static_cast<long long>(part) * D + 32 * c);
+#pragma unroll
+          for (int b = 0; b < 8; ++b)
+            to[b] = make_float4(__uint_as_float(o[4 * b]) * f, __uint_as_float(o[4 * b + 1]) * f, __uint_as_float(o[4 * b + 2]) * f, __uint_as_float(o[4 * b + 3]) * f);
+        }
+      }
+      if (real && !whole)
+        reinterpret_cast<float4*>(a.partial + 2ll * ctas * kChunkRows * D)[part] = make_float4(m, l * 0.0078125f, m, redo ? 1.0f : 0.0f);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.o_empty[slot]);
+    }
+    bool again = whole && redo;               // whether this CTA has to redo the unit row by row
+    if (!whole) {
+      __threadfence();
+      named_bar_sync(1, 256);
+      if (tid == 0) {
+        const bool is_last = atomicAdd(a.tickets + parts.first, 1) == parts.last - parts.first;
+        if (is_last) a.tickets[parts.first] = 0;
+        s_plan.last = is_last;
+      }
+      named_bar_sync(1, 256);
+      if (s_plan.last) {
+        __threadfence();
+        const float4* stats = reinterpret_cast<const float4*>(a.partial + 2ll * ctas * kChunkRows * D);
+        for (int c = parts.first; c <= parts.last; ++c) again |= __ldcg(stats + static_cast<long long>(parts.slot(c)) * kChunkRows).w != 0.0f;
+        if (!again) join_parts<D, kChunkRows, 8>(a, g.q_first, g.row0, g.head, g.rows, ctas, parts, tid, 256);
+      }
+    }
+    if (again) {
+      float* const s_q = reinterpret_cast<float*>(smem + Shape::kRedo) + warp * (D + kKvPage);
+      for (int x = warp; x < g.rows; x += 8) exact_row<D>(a, g.base, g.q_first, g.b, g.head, g.row0 + x, s_q, s_q + D);
+    }
+    if (tid == 0) sh.finished = ++done;
+    i += n;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.segment_empty[segments.stage]);
+    segments.next();
+  }
 }
 
 template <int D>
@@ -164,7 +705,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 attention_chunk_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ AttentionArgs a, int* __restrict__ status,
                        long long wait_limit) {
   using Shape = ChunkShape<D>;
-  using Place = Cursor<kTile, kChunkRows>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   __shared__ ChunkShared sh;
@@ -203,7 +743,11 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
       mbar_init(&sh.o_empty[i], 4);
     }
     mbar_init(&sh.idle, 1);
-    for (int i = 0; i < kFlagRing; ++i) sh.redo[i] = 0;
+    for (int i = 0; i < kSegmentRing; ++i) {
+      mbar_init(&sh.segment_full[i], 1);
+      mbar_init(&sh.segment_empty[i], kSegmentReaders);
+      sh.redo[i] = 0;
+    }
     sh.abort_code = 0;
     sh.finished = 0;
     sh.asked_k = sh.asked_v = sh.asked_scales = 0;
@@ -217,458 +761,21 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh.tmem;                // S of slot s at columns 128 s (P over its first 64), O at 256 + 128 s
-  auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, &sh.abort_code, kStatusChunkTimeout, wait_limit); };
-
-  // 512 threads at 128 registers are all there are: 256 of them at 64 leave 192 for each softmax thread, until the roles are done.
+  // 512 threads at 128 registers are all there are: 256 of them at 56 leave 200 for each softmax thread, until the roles are done.
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
-    // ------------------------------------------------------------------------------------------ softmax, a thread per row
-    const int slot = warp / 4, in_slot = tid % 128;
-    const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
-    const uint32_t t_s = tmem + lanes + slot * 128, t_o = tmem + lanes + 256 + slot * 128;
-    Place at;
-    at.start(plan, s_plan);
-    bool ok = true;
-    int i = 0, tile_no = 0, segment_no = 0;     // of this slot
-    for (int segment = 0; i < count; ++segment) {
-      const int n = min(at.span.tiles - at.tile, count - i), rows = at.rows(a.group);
-      const bool active = slot * 128 < rows, whole = n == at.span.tiles;
-      const Seen seen = seen_by(at, a.group, a.window);
-      const int row = slot * 128 + in_slot, r = at.rt * kChunkRows + row;
-      const bool real = row < rows;
-      const int token = real ? r / a.group : (at.rt * kChunkRows + rows - 1) / a.group;     // (rows beyond the last copy its bounds)
-      const int high = at.s.length - at.s.count + token, low = a.window > 0 ? max(high - a.window + 1, 0) : 0;
-      const __nv_bfloat16* const q = a.q + (at.s.first + token) * a.q_stride + (at.head * a.group + (real ? r % a.group : 0)) * D;
-      float unit = 0.0f;
-      if (active) {
-        // ---- q as two e4m3 terms of q * 2^k, the row's largest at 2^7 .. 2^8
-        uint4 raw[D / 8];
-        unsigned top = 0u;
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-          raw[c] = real ? __ldg(reinterpret_cast<const uint4*>(q) + c) : make_uint4(0u, 0u, 0u, 0u);
-          const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) top = max(top, max(w[e] & 0x7fffu, w[e] >> 16 & 0x7fffu));
-        }
-        const int k = top == 0u ? 0 : min(7 - (static_cast<int>(top >> 7) - 127), 120);
-        const float up = copysignf(__int_as_float((k + 127) << 23), a.scale_log2);
-        // (a scale of zero keeps a factor, so that -infinity stays what it is)
-        unit = top >= 0x7f80u ? __int_as_float(0x7fffffff) : fmaxf(fabsf(a.scale_log2) * __int_as_float((127 - k) << 23), 1e-30f);
-        uint8_t* const hi_tile = smem + Shape::kQ + 2 * slot * Shape::kTileBytes;
-#pragma unroll
-        for (int c = 0; c < D / 16; ++c) {
-          const uint32_t w[8] = {raw[2 * c].x, raw[2 * c].y, raw[2 * c].z, raw[2 * c].w, raw[2 * c + 1].x, raw[2 * c + 1].y, raw[2 * c + 1].z, raw[2 * c + 1].w};
-          uint32_t hi[4], lo[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float x0 = __uint_as_float(w[2 * e] << 16) * up, x1 = __uint_as_float(w[2 * e] & 0xffff0000u) * up;
-            const float x2 = __uint_as_float(w[2 * e + 1] << 16) * up, x3 = __uint_as_float(w[2 * e + 1] & 0xffff0000u) * up;
-            const uint16_t h01 = cvt_e4m3x2(x0, x1), h23 = cvt_e4m3x2(x2, x3);
-            const float2 f01 = e4m3x2_to_float2(h01), f23 = e4m3x2_to_float2(h23);
-            hi[e] = h01 | static_cast<uint32_t>(h23) << 16;
-            lo[e] = cvt_e4m3x2(x0 - f01.x, x1 - f01.y) | static_cast<uint32_t>(cvt_e4m3x2(x2 - f23.x, x3 - f23.y)) << 16;
-          }
-          const int to = swizzled<D>(in_slot, c);
-          *reinterpret_cast<uint4*>(hi_tile + to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          *reinterpret_cast<uint4*>(hi_tile + Shape::kTileBytes + to) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.q_full[slot]);
-      }
-      const int warp_low = __reduce_max_sync(0xffffffffu, low), warp_high = __reduce_min_sync(0xffffffffu, high);   // seen by every row of the warp
-      float m = -INFINITY;
-      uint64_t l2 = 0ull;                       // two halves of the sum
-      int exponent = -100;
-      for (int j = 0; j < n; ++j, ++i) {
-        const int ss = i % kScaleStages, position0 = (at.span.first + at.tile + j) * kTile;
-        mbar_wait_or_clear(ok, &sh.scale_full[ss], i / kScaleStages & 1, &sh.abort_code, kStatusChunkTimeout, wait_limit);
-        mbar_wait_or_clear(ok, &sh.scale_clean[ss], i / kScaleStages & 1, &sh.abort_code, kStatusChunkTimeout, wait_limit);
-        if (active) {
-          const float* const k_scale = reinterpret_cast<const float*>(smem + Shape::kScales) + ss * 2 * kTile;
-          const int there = sh.there[ss];
-          const int e = tile_exponent(k_scale + kTile, there, position0, seen, lane);
-          float fade = 1.0f;
-          if (j == 0) {
-            exponent = e;
-          } else if (e > exponent + kUnitGrowth) {
-            fade = ex2(static_cast<float>(exponent - e));
-            exponent = e;
-          }
-          mbar_wait_or_clear(ok, &sh.s_full[slot], tile_no & 1, &sh.abort_code, kStatusChunkTimeout, wait_limit);
-          __syncwarp();
-          tc_fence_after();
-          uint32_t s[4][32];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld32(t_s + 32 * c, s[c]);
-          tmem_ld_wait_for(s[0]);
-#pragma unroll
-          for (int c = 1; c < 4; ++c) tmem_landed(s[c]);
-          // scores in units of the row's: times the key's scale
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-#pragma unroll
-            for (int e4 = 0; e4 < 8; ++e4) {
-              const float4 ks = *reinterpret_cast<const float4*>(k_scale + 32 * c + 4 * e4);
-              float x0, x1, x2, x3;
-              f32x2_unpack(f32x2_mul(f32x2_pack_bits(s[c][4 * e4], s[c][4 * e4 + 1]), f32x2_pack(ks.x, ks.y)), x0, x1);
-              f32x2_unpack(f32x2_mul(f32x2_pack_bits(s[c][4 * e4 + 2], s[c][4 * e4 + 3]), f32x2_pack(ks.z, ks.w)), x2, x3);
-              s[c][4 * e4] = __float_as_uint(x0);
-              s[c][4 * e4 + 1] = __float_as_uint(x1);
-              s[c][4 * e4 + 2] = __float_as_uint(x2);
-              s[c][4 * e4 + 3] = __float_as_uint(x3);
-            }
-          }
-          if (position0 < warp_low || position0 + kTile - 1 > warp_high || there != 3) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              // bit b: position position0 + 32 c + b is there and seen
-              const int first = low - position0 - 32 * c, last = high - position0 - 32 * c;
-              uint32_t bits = last < 0 || first > 31 || !(there >> (c / 2) & 1) ? 0u : 0xffffffffu;
-              if (last >= 0 && last < 31) bits &= (2u << last) - 1u;
-              if (first > 0 && first <= 31) bits &= 0xffffffffu << first;
-#pragma unroll
-              for (int b = 0; b < 32; ++b)
-                if (!(bits >> b & 1u)) s[c][b] = 0xff800000u;
-            }
-          }
-          float top4[4];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            top4[c] = __uint_as_float(s[c][0]);
-#pragma unroll
-            for (int b = 1; b < 32; ++b) top4[c] = fmaxf(top4[c], __uint_as_float(s[c][b]));
-          }
-          const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * unit;
-          if (top > m + kGrowth) {
-            const float f = ex2(m - top);       // (0 for a row that had seen nothing)
-            fade *= f;
-            float l0, l1;
-            f32x2_unpack(l2, l0, l1);
-            l2 = f32x2_pack(l0 * f, l1 * f);
-            m = top;
-          }
-          if (j > 0 && __any_sync(0xffffffffu, fade != 1.0f)) {
-#pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t o[32];
-              tmem_ld32(t_o + 32 * c, o);
-              tmem_ld_wait_for(o);
-#pragma unroll
-              for (int b = 0; b < 32; ++b) o[b] = __float_as_uint(__uint_as_float(o[b]) * fade);
-              tmem_st32(t_o + 32 * c, o);
-            }
-          }
-          const float shift = kHeadroom - finite_or_zero(m);
-          const uint64_t unit2 = f32x2_pack(unit, unit), shift2 = f32x2_pack(shift, shift);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t p[32];
-#pragma unroll
-            for (int b = 0; b < 32; ++b) {
-              const int c = 2 * h + b / 16, at2 = b % 16 * 2;
-              float x0, x1;
-              f32x2_unpack(f32x2_fma(f32x2_pack_bits(s[c][at2], s[c][at2 + 1]), unit2, shift2), x0, x1);
-              x0 = ex2(x0);
-              x1 = ex2(x1);
-              l2 = f32x2_add(l2, f32x2_pack(x0, x1));
-              p[b] = pack_half2(x0, x1);
-            }
-            tmem_st32(t_s + 32 * h, p);
-          }
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.p_full[slot]);
-          ++tile_no;
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.scale_empty[ss]);
-        if (!__all_sync(0xffffffffu, ok)) break;
-      }
-      // ---- the segment's end
-      if (active) {
-        mbar_wait_or_clear(ok, &sh.o_full[slot], segment_no & 1, &sh.abort_code, kStatusChunkTimeout, wait_limit);
-        __syncwarp();
-        tc_fence_after();
-        ++segment_no;
-      }
-      if (softmax_bar_any(!ok)) break;          // all eight warps meet here whatever failed, and leave together
-      const bool redo = sh.redo[segment % kFlagRing] != 0;
-      if (tid == 0) sh.redo[(segment + kFlagRing - 1) % kFlagRing] = 0;     // the segment before: everybody has read it
-      const long long unit_start = w0 + (i - n) - at.tile;
-      const int slot_no = 2 * static_cast<int>(blockIdx.x) + (w0 >= unit_start ? 0 : 1);
-      const long long part = static_cast<long long>(slot_no) * kChunkRows + row;
-      if (active) {
-        float l0, l1;
-        f32x2_unpack(l2, l0, l1);
-        const float l = l0 + l1, unscale = __int_as_float((exponent - kUnitShift + 127) << 23);
-        const float f = whole ? (l == 0.0f ? 0.0f : unscale / l) : unscale;
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
-          tmem_ld32(t_o + 32 * c, o);
-          tmem_ld_wait_for(o);
-          if (real && whole && !redo) {
-            uint4* to = reinterpret_cast<uint4*>(a.out + (at.s.first + token) * a.out_stride + (at.head * a.group + r % a.group) * D + 32 * c);
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-              uint32_t w[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(o[8 * b + 2 * e]) * f, __uint_as_float(o[8 * b + 2 * e + 1]) * f);
-                w[e] = *reinterpret_cast<const uint32_t*>(&h);
-              }
-              to[b] = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-          } else if (real && !whole) {
-            float4* to = reinterpret_cast<float4*>(a.partial + part * D + 32 * c);
-#pragma unroll
-            for (int b = 0; b < 8; ++b)
-              to[b] = make_float4(__uint_as_float(o[4 * b]) * f, __uint_as_float(o[4 * b + 1]) * f, __uint_as_float(o[4 * b + 2]) * f, __uint_as_float(o[4 * b + 3]) * f);
-          }
-        }
-        if (real && !whole)
-          reinterpret_cast<float4*>(a.partial + 2ll * ctas * kChunkRows * D)[part] = make_float4(m, l * 0.0078125f, m, redo ? 1.0f : 0.0f);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.o_empty[slot]);
-      }
-      float* const s_q = reinterpret_cast<float*>(smem + Shape::kRedo) + warp * (D + kKvPage);
-      if (whole) {
-        if (redo)
-          for (int x = warp; x < rows; x += 8) exact_row<D>(a, at.s, at.b, at.head, at.rt * kChunkRows + x, s_q, s_q + D);
-      } else {
-        const int first = piece_of(total, ctas, unit_start), last = piece_of(total, ctas, unit_start + at.span.tiles - 1);
-        __threadfence();
-        named_bar_sync(1, 256);
-        if (tid == 0) {
-          const bool is_last = atomicAdd(a.tickets + first, 1) == last - first;
-          if (is_last) a.tickets[first] = 0;
-          s_plan.last = is_last;
-        }
-        named_bar_sync(1, 256);
-        if (s_plan.last) {
-          __threadfence();
-          const float4* stats = reinterpret_cast<const float4*>(a.partial + 2ll * ctas * kChunkRows * D);
-          bool any_redo = false;
-          for (int c = first; c <= last; ++c)
-            any_redo |= __ldcg(stats + static_cast<long long>(2 * c + (piece_start(total, ctas, c) >= unit_start ? 0 : 1)) * kChunkRows).w != 0.0f;
-          if (any_redo) {
-            for (int x = warp; x < rows; x += 8) exact_row<D>(a, at.s, at.b, at.head, at.rt * kChunkRows + x, s_q, s_q + D);
-          } else {
-            join_parts<D, kChunkRows>(a, at.s, at.rt, at.head, rows, total, ctas, first, last, unit_start, tid, 256);
-          }
-        }
-      }
-      if (tid == 0) sh.finished = segment + 1;
-      if (i < count) at.next_unit(plan);
-    }
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    softmax_role<D>(a, sh, s_plan, smem, tmem, count, ctas, total, wait_limit);
     asm volatile("setmaxnreg.dec.sync.aligned.u32 128;");
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-  if (warp == 13) {
-    // ------------------------------------------------------------------------------------------ loads
-    if (lane == 0) {
-      const uint64_t keep = l2_policy_evict_normal();      // other row tiles of the sequence read the same pages
-      Place at;
-      at.start(plan, s_plan);
-      int entry[2];
-      Seen seen = seen_by(at, a.group, a.window);
-      auto entries = [&]() {                               // of the tile to ask for next: read one tile ahead
-        const int32_t* table = a.batch.block_table + static_cast<long long>(at.b) * a.batch.max_pages;
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          const int page = 2 * (at.span.first + at.tile) + p;
-          entry[p] = page < a.batch.max_pages && page * kKvPage <= seen.any_high && (page + 1) * kKvPage > seen.any_low ? __ldg(table + page) : -1;
-        }
-      };
-      entries();
-      for (int i = 0; i < count; ++i) {
-        const int ss = i % kScaleStages, ks = i % Shape::kKStages, vs = i % Shape::kVStages;
-        int there = 0;
-#pragma unroll
-        for (int p = 0; p < 2; ++p) there |= (entry[p] >= 0 && entry[p] < a.cache.num_pages) << p;
-        const int pages = (there & 1) + (there >> 1);
-        if (!wait(&sh.scale_empty[ss], (i / kScaleStages & 1) ^ 1)) break;
-        sh.there[ss] = there;
-        mbar_arrive_expect_tx(&sh.scale_full[ss], pages * 2 * kKvPage * 4);
-        float* const scales = reinterpret_cast<float*>(smem + Shape::kScales) + ss * 2 * kTile;
-        const int head = at.head;
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          if (!(there >> p & 1)) continue;
-          bulk_load(scales + p * kKvPage, kv_block<D>(a.cache, entry[p], 0, head) + kKvPage * D, kKvPage * 4, &sh.scale_full[ss], keep);
-          bulk_load(scales + kTile + p * kKvPage, kv_block<D>(a.cache, entry[p], 1, head) + kKvPage * D, kKvPage * 4, &sh.scale_full[ss], keep);
-        }
-        sh.asked_scales = i + 1;
-        if (!wait(&sh.k_empty[ks], (i / Shape::kKStages & 1) ^ 1)) break;
-        mbar_arrive_expect_tx(&sh.k_full[ks], pages * kKvPage * D);
-#pragma unroll
-        for (int p = 0; p < 2; ++p)
-          if (there >> p & 1) tma_load_4d(smem + Shape::kK + ks * Shape::kTileBytes + p * kKvPage * D, &map, &sh.k_full[ks], 0, 0, head, entry[p], keep);
-        sh.asked_k = i + 1;
-        if (!wait(&sh.v_empty[vs], (i / Shape::kVStages & 1) ^ 1)) break;
-        mbar_arrive_expect_tx(&sh.v_full[vs], pages * kKvPage * D);
-#pragma unroll
-        for (int p = 0; p < 2; ++p)
-          if (there >> p & 1) tma_load_4d(smem + Shape::kV + vs * Shape::kTileBytes + p * kKvPage * D, &map, &sh.v_full[vs], 0, 0, a.cache.heads + head, entry[p], keep);
-        sh.asked_v = i + 1;
-        if (i + 1 < count) {
-          if (++at.tile == at.span.tiles) {
-            at.next_unit(plan);
-            seen = seen_by(at, a.group, a.window);
-          }
-          entries();
-        }
-      }
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp < 12) {
+      convert_role<D>(sh, smem, count, wait_limit);
+    } else if (lane == 0) {
+      if (warp == 12) mma_role<D>(sh, smem, tmem, count, wait_limit);
+      if (warp == 13) load_role<D>(map, a, sh, smem, count, wait_limit);
+      if (warp == 14) plan_role(a, plan, s_plan, sh, count, w0, wait_limit);
     }
     __syncwarp();
-  } else if (warp == 12) {
-    // ------------------------------------------------------------------------------------------ MMAs
-    if (lane == 0) {
-      Place at;
-      at.start(plan, s_plan);
-      const uint32_t qk_desc = umma_idesc_e4m3_m128(kTile), pv_desc = umma_idesc_f16_m128_n_major(D);
-      auto operand = [&](int offset) {
-        return D == 128 ? umma_smem_desc_sw128(smem_u32(smem + offset)) : umma_smem_desc_sw64(smem_u32(smem + offset));
-      };
-      auto scores = [&](int slot, int ks) {
-        const uint64_t k = operand(Shape::kK + ks * Shape::kTileBytes);
-#pragma unroll
-        for (int term = 0; term < 2; ++term) {
-          const uint64_t q = operand(Shape::kQ + (2 * slot + term) * Shape::kTileBytes);
-#pragma unroll
-          for (int step = 0; step < D / 32; ++step) umma_f8(tmem + slot * 128, q + 2 * step, k + 2 * step, qk_desc, term + step > 0 ? 1u : 0u);
-        }
-        umma_commit(&sh.s_full[slot]);
-      };
-      auto values = [&](int slot, int hs, bool first) {
-        const uint64_t v = umma_smem_desc_n_major_sw128(smem_u32(smem + Shape::kHalf + hs * Shape::kHalfBytes), kTile * 128);
-#pragma unroll
-        for (int step = 0; step < kTile / 16; ++step)
-          umma_f16_ts(tmem + 256 + slot * 128, tmem + slot * 128 + 8 * step, v + 128 * step, pv_desc, first && step == 0 ? 0u : 1u);
-      };
-      int i = 0, tiles[2] = {0, 0}, segments[2] = {0, 0};  // tiles and segments of each slot so far
-      bool alive = true;
-      while (i < count && alive) {
-        const int n = min(at.span.tiles - at.tile, count - i);
-        const int slots = at.rows(a.group) > 128 ? 2 : 1;
-        for (int s = 0; s < slots && alive; ++s) alive = wait(&sh.q_full[s], segments[s] & 1);
-        alive = alive && wait(&sh.k_full[i % Shape::kKStages], i / Shape::kKStages & 1);
-        if (!alive) break;
-        tc_fence_after();
-        for (int s = 0; s < slots; ++s) scores(s, i % Shape::kKStages);
-        umma_commit(&sh.k_empty[i % Shape::kKStages]);
-        for (int j = 0; j < n && alive; ++j) {
-          const int now = i + j, next = now + 1;
-          const bool more = j + 1 < n;
-          if (more) alive = wait(&sh.k_full[next % Shape::kKStages], next / Shape::kKStages & 1);
-          alive = alive && wait(&sh.half_full[now % 2], now / 2 & 1);
-          for (int s = 0; s < slots && alive; ++s) {
-            if (j == 0) alive = wait(&sh.o_empty[s], (segments[s] & 1) ^ 1);
-            alive = alive && wait(&sh.p_full[s], tiles[s] & 1);
-            if (!alive) break;
-            tc_fence_after();
-            values(s, now % 2, j == 0);
-            ++tiles[s];
-            if (s + 1 == slots) umma_commit(&sh.half_empty[now % 2]);
-            if (more) scores(s, next % Shape::kKStages);
-            else umma_commit(&sh.o_full[s]);
-          }
-          if (alive && more) umma_commit(&sh.k_empty[next % Shape::kKStages]);
-        }
-        for (int s = 0; s < slots; ++s) ++segments[s];
-        i += n;
-        if (i < count) at.next_unit(plan);
-      }
-    }
-    __syncwarp();
-  } else if (warp >= 8 && warp < 12) {
-    // ------------------------------------------------------------------------------------------ values to f16, a thread per position
-    const int t = tid - 8 * 32;
-    Place at;
-    at.start(plan, s_plan);
-    bool ok = true;
-    int segment = 0, unit = -100;
-    bool fresh = true;
-    Seen seen = seen_by(at, a.group, a.window);
-    for (int i = 0; i < count; ++i) {
-      const int ss = i % kScaleStages, vs = i % Shape::kVStages, hs = i % 2;
-      mbar_wait_or_clear(ok, &sh.scale_full[ss], i / kScaleStages & 1, &sh.abort_code, kStatusChunkTimeout, wait_limit);
-      float* const k_scale = reinterpret_cast<float*>(smem + Shape::kScales) + ss * 2 * kTile;
-      const float* const v_scale = k_scale + kTile;
-      const int there = sh.there[ss], position0 = (at.span.first + at.tile) * kTile;
-      const int e = tile_exponent(v_scale, there, position0, seen, lane);
-      if (fresh || e > unit + kUnitGrowth) unit = e;
-      fresh = false;
-      const float scale = v_scale[t];
-      const bool valid = (there >> (t / kKvPage) & 1) && position0 + t >= seen.any_low && position0 + t <= seen.any_high;
-      const bool mixed = position0 < seen.all_low || position0 + kTile - 1 > seen.all_high;     // some rows may see what others do not
-      const float r = scale * __int_as_float((kUnitShift - unit + 127) << 23);
-      // r as two f16 terms, so that the product with a byte's value is rounded once
-      const __half hi = __float2half_rn(r);
-      const __half2 r_hi = __half2half2(hi), r_lo = __half2half2(__float2half_rn(r - __half2float(hi)));
-      mbar_wait_or_clear(ok, &sh.v_full[vs], i / Shape::kVStages & 1, &sh.abort_code, kStatusChunkTimeout, wait_limit);
-      const uint8_t* const from = smem + Shape::kV + vs * Shape::kTileBytes;
-      // Zero times NaN is NaN: where some rows see a value that is not finite and others do not, its bytes become zeros and the NaN
-      // goes by way of its score to the rows that see it.
-      bool bad = false;
-      if (mixed && valid) {
-        uint32_t over = 0u;
-#pragma unroll 4
-        for (int chunk = 0; chunk < D / 16; ++chunk) {
-          const uint4 p = *reinterpret_cast<const uint4*>(from + swizzled<D>(t, chunk));
-          over |= ((p.x & 0x7f7f7f7fu) + 0x01010101u) | ((p.y & 0x7f7f7f7fu) + 0x01010101u) | ((p.z & 0x7f7f7f7fu) + 0x01010101u) | ((p.w & 0x7f7f7f7fu) + 0x01010101u);
-        }
-        bad = (over & 0x80808080u) != 0u || !(fabsf(scale) <= 3.402823466e38f);
-        if (bad) k_scale[t] = __int_as_float(0x7fffffff);
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.scale_clean[ss]);
-      mbar_wait_or_clear(ok, &sh.half_empty[hs], (i / 2 & 1) ^ 1, &sh.abort_code, kStatusChunkTimeout, wait_limit);
-      uint8_t* const to = smem + Shape::kHalf + hs * Shape::kHalfBytes + t * 128;
-      if (valid && !bad) {
-        uint32_t any = 0u;
-#pragma unroll 4
-        for (int chunk = 0; chunk < D / 16; ++chunk) {
-          const uint4 p = *reinterpret_cast<const uint4*>(from + swizzled<D>(t, chunk));
-          const uint32_t w[4] = {p.x, p.y, p.z, p.w};
-          uint32_t h[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const uint32_t bits = e4m3x2_to_half2(w[j / 2] >> (16 * (j % 2)));
-            const __half2 v = *reinterpret_cast<const __half2*>(&bits);
-            const __half2 y = __hfma2(v, r_hi, __hmul2(v, r_lo));
-            h[j] = *reinterpret_cast<const uint32_t*>(&y);
-          }
-          any |= (p.x | p.y | p.z | p.w) & 0x7f7f7f7fu;
-          uint8_t* const row = to + chunk / 4 * (kTile * 128);
-          *reinterpret_cast<uint4*>(row + (((2 * chunk) % 8 ^ (t & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-          *reinterpret_cast<uint4*>(row + (((2 * chunk + 1) % 8 ^ (t & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
-        }
-        if (any != 0u && fabsf(r) < kSmallestUnit) sh.redo[segment % kFlagRing] = 1;
-      } else {
-#pragma unroll 4
-        for (int chunk = 0; chunk < D / 8; ++chunk) *reinterpret_cast<uint4*>(to + chunk / 8 * (kTile * 128) + chunk % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&sh.half_full[hs]);
-        mbar_arrive(&sh.v_empty[vs]);
-        mbar_arrive(&sh.scale_empty[ss]);
-      }
-      if (!__all_sync(0xffffffffu, ok)) break;
-      if (i + 1 < count && ++at.tile == at.span.tiles) {
-        at.next_unit(plan);
-        seen = seen_by(at, a.group, a.window);
-        ++segment;
-        fresh = true;
-      }
-    }
-    }
   }
 
   tc_fence_before();
@@ -690,7 +797,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
     __syncthreads();
     // What is left of the piece becomes NaN, and its units are counted, so that nobody waits for them and the next call finds the
     // counters at zero.
-    Place at;
+    Cursor<kTile, kChunkRows> at;
     at.start(plan, s_plan);
     for (int i = 0, segment = 0; i < count; ++segment) {
       const int n = min(at.span.tiles - at.tile, count - i), rows = at.rows(a.group);
@@ -707,18 +814,18 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
           for (int x = tid; x < rows; x += kChunkThreads)
             reinterpret_cast<float4*>(a.partial + 2ll * ctas * kChunkRows * D)[static_cast<long long>(slot_no) * kChunkRows + x] =
                 make_float4(0.0f, __int_as_float(0x7fffffff), 0.0f, 0.0f);
-          const int first = piece_of(total, ctas, unit_start), last = piece_of(total, ctas, unit_start + at.span.tiles - 1);
+          const Parts parts(total, ctas, unit_start, at.span.tiles);
           __threadfence();
           __syncthreads();
           if (tid == 0) {
-            const bool is_last = atomicAdd(a.tickets + first, 1) == last - first;
-            if (is_last) a.tickets[first] = 0;
+            const bool is_last = atomicAdd(a.tickets + parts.first, 1) == parts.last - parts.first;
+            if (is_last) a.tickets[parts.first] = 0;
             s_plan.last = is_last;
           }
           __syncthreads();
           if (s_plan.last) {
             __threadfence();
-            join_parts<D, kChunkRows>(a, at.s, at.rt, at.head, rows, total, ctas, first, last, unit_start, tid, kChunkThreads);
+            join_parts<D, kChunkRows, 1>(a, at.s.first, at.rt * kChunkRows, at.head, rows, ctas, parts, tid, kChunkThreads);
           }
           __syncthreads();
         }
