@@ -14,7 +14,7 @@ struct AttentionArgs {
   int group, window;
   float scale_log2;
   int* tickets;          // [CTAs] zero between calls
-  float* partial;        // [2 * CTAs][rows][D] sums, then [2 * CTAs][rows] of (m, l, n, redo)
+  float* partial;        // [2 * CTAs][rows][D] sums (the chunk kernel: [2 * CTAs][D / 4][rows][4]), then [2 * CTAs][rows] of (m, l, n, redo)
 };
 
 // paged_attention_chunk.cu.  Bytes of `partial` that a launch on `ctas` CTAs needs, and the launch.
@@ -48,10 +48,11 @@ __device__ __forceinline__ int swizzled(int row, int chunk) {   // byte offset o
   return row * D + ((D == 128 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3)) << 4);
 }
 
-// The parts of a split unit [unit_start, unit_start + tiles) of the line: CTAs first .. last, of which all but perhaps the first have it
-// at the start of their piece.
+// The parts of a split unit whose tiles are the places [unit_start, unit_start + tiles) of the line: CTAs first .. last, of which all but
+// perhaps the first have it at the start of their piece.
 struct Parts {
   int first, last, first_slot;
+  __device__ Parts(int f, int l, int s) : first(f), last(l), first_slot(s) {}
   __device__ Parts(long long total, int ctas, long long unit_start, int tiles)
       : first(piece_of(total, ctas, unit_start)), last(piece_of(total, ctas, unit_start + tiles - 1)),
         first_slot(2 * first + (piece_start(total, ctas, first) < unit_start)) {}

@@ -4,8 +4,9 @@
 // A unit is (sequence, row tile, key head): up to ROWS of the sequence's count * group rows (token major, the query heads of the
 // key head side by side), over the tiles of TILE positions that any of them sees.  All units' tiles, in the order sequence, row
 // tile, head, tile, are one line that is cut into equal pieces, one per CTA; so a piece has at most a unit's end, some whole
-// units and a unit's beginning, whatever the lengths are.  A unit that lies in one piece is finished there.  Else each of its
-// CTAs leaves a partial result, and the one that comes last (a counter per unit) adds them up, in the order of the pieces.
+// units and a unit's beginning, whatever the lengths are.  In front of a unit's tiles the line has EXTRA places that stand for
+// what a unit costs besides its tiles.  A unit that lies in one piece is finished there.  Else each of its CTAs leaves a partial
+// result, and the one that comes last (a counter per unit) adds them up, in the order of the pieces.
 #pragma once
 #include "kv_internal.h"
 
@@ -14,8 +15,8 @@ namespace syfi {
 constexpr int kPlanRound = 128;     // sequences whose tiles are summed at a time
 
 struct PlanShared {
-  long long sum[kPlanRound];        // tiles of each sequence of the round, then their inclusive prefix sums
-  int start_b, start_rt, start_head, start_tile;
+  long long sum[kPlanRound];        // places of each sequence of the round, then their inclusive prefix sums
+  int start_b, start_rt, start_head, start_place;   // place: EXTRA + tile
   int last;                         // the ticket says that this CTA is the unit's last
 };
 
@@ -23,7 +24,7 @@ struct Span {
   int first, tiles;                 // tiles of positions; at least one
 };
 
-template <int TILE, int ROWS>
+template <int TILE, int ROWS, int EXTRA>
 struct Plan {
   const KvBatch& batch;
   int heads, group, window;
@@ -36,10 +37,10 @@ struct Plan {
     const int low = window > 0 ? max(base + row0 / group - window + 1, 0) : 0;
     return high < low ? Span{0, 1} : Span{low / TILE, high / TILE - low / TILE + 1};
   }
-  __device__ long long tiles_of_warp(const KvSequence& s, int lane) const {     // a head's tiles of all row tiles; whole warp
+  __device__ long long tiles_of_warp(const KvSequence& s, int lane) const {     // a head's places of all row tiles; whole warp
     const int n = s.count > 0 ? row_tiles(s) : 0;
     long long sum = 0;
-    for (int rt = lane; rt < n; rt += 32) sum += span(s, rt).tiles;
+    for (int rt = lane; rt < n; rt += 32) sum += EXTRA + span(s, rt).tiles;
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     return sum;
@@ -70,7 +71,7 @@ struct Plan {
     __syncthreads();
   }
 
-  // All units' tiles; whole block.
+  // The line's length; whole block.
   __device__ long long total(PlanShared& sh) const {
     long long sum = 0;
     for (int round = 0; round * kPlanRound < batch.batch; ++round) {
@@ -81,7 +82,7 @@ struct Plan {
     return sum * heads;
   }
 
-  // Where tile `at` of the line lies, into sh.start_*; whole block, ends with a barrier.  Behind total(), whose last round is
+  // Where place `at` of the line lies, into sh.start_*; whole block, ends with a barrier.  Behind total(), whose last round is
   // still in sh.sum.
   __device__ void locate(PlanShared& sh, long long at) const {
     const int rounds = (batch.batch + kPlanRound - 1) / kPlanRound, lane = threadIdx.x % 32;
@@ -104,7 +105,7 @@ struct Plan {
       const KvSequence s = kv_sequence(batch, min(round * kPlanRound + b, batch.batch - 1));
       const int n = row_tiles(s);
       for (int base = 0; base < n; base += 32) {
-        const int mine = base + lane < n ? span(s, base + lane).tiles : 0;
+        const int mine = base + lane < n ? EXTRA + span(s, base + lane).tiles : 0;
         int incl = mine;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -119,7 +120,7 @@ struct Plan {
             sh.start_b = round * kPlanRound + b;
             sh.start_rt = base + lane;
             sh.start_head = o / mine;
-            sh.start_tile = o % mine;
+            sh.start_place = o % mine;
           }
           break;
         }
@@ -130,42 +131,57 @@ struct Plan {
   }
 };
 
-// A place on the line: a unit and a tile of it.  The same in every thread of a block.
-template <int TILE, int ROWS>
+// A walk over the tiles of a piece of the line.  The same in every thread of a block.
+template <int TILE, int ROWS, int EXTRA>
 struct Cursor {
   int b, rt, head, tile;             // tile of the unit, counted from 0
+  int left;                          // places of the piece from this tile on; none: the walk is over
   KvSequence s;
   Span span;
   int row_tiles;
 
-  __device__ void start(const Plan<TILE, ROWS>& plan, const PlanShared& sh) {
+  __device__ void start(const Plan<TILE, ROWS, EXTRA>& plan, const PlanShared& sh, int places) {
     b = sh.start_b;
     rt = sh.start_rt;
     head = sh.start_head;
-    tile = sh.start_tile;
     s = kv_sequence(plan.batch, b);
     row_tiles = plan.row_tiles(s);
     span = plan.span(s, rt);
+    const int skipped = max(EXTRA - sh.start_place, 0);
+    tile = sh.start_place + skipped - EXTRA;
+    left = places - skipped;
   }
-  // To the next unit, if there is one.
-  __device__ void next_unit(const Plan<TILE, ROWS>& plan) {
+  // To the next unit, if the piece has any of its tiles.
+  __device__ void next_unit(const Plan<TILE, ROWS, EXTRA>& plan) {
+    left -= EXTRA;
+    if (left <= 0) return;
     tile = 0;
     if (++head < plan.heads) return;
     head = 0;
     if (++rt >= row_tiles) {
       rt = 0;
       do {
-        if (++b >= plan.batch.batch) return;
+        if (++b >= plan.batch.batch) {
+          left = 0;
+          return;
+        }
         s = kv_sequence(plan.batch, b);
       } while (s.count == 0);
       row_tiles = plan.row_tiles(s);
     }
     span = plan.span(s, rt);
   }
+  // `n` tiles of the unit on; behind its last to the next unit.
+  __device__ void advance(const Plan<TILE, ROWS, EXTRA>& plan, int n) {
+    tile += n;
+    left -= n;
+    if (tile == span.tiles && left > 0) next_unit(plan);
+  }
+  __device__ int tiles_here() const { return min(span.tiles - tile, left); }      // of the unit, in this piece
   __device__ int rows(int group) const { return min(s.count * group - rt * ROWS, ROWS); }
 };
 
-// The pieces of a line of `total` tiles cut among `ctas` CTAs, and the CTAs that share [u0, u1).
+// The pieces of a line of `total` places cut among `ctas` CTAs.
 __device__ __forceinline__ long long piece_start(long long total, int ctas, int c) { return total * c / ctas; }
 __device__ __forceinline__ int piece_of(long long total, int ctas, long long at) {
   int c = static_cast<int>(at * ctas / total);       // piece_start(c) <= at, and at most one too low

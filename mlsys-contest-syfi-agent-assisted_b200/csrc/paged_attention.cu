@@ -42,6 +42,8 @@ __device__ __forceinline__ float quad_sum(float v) {
 //   values: rows x dimensions; a lane's V operand pairs the bytes of two positions (prmt), its 16 dimensions are 16 MMAs' n.
 // Which position an n index of the scores stands for is chosen so that both reads of the swizzled rows are free of bank
 // conflicts: even n is position n, odd n is position (n - 1) ^ 5.
+constexpr int kDecodeExtra = 1;      // what a unit costs besides its pages, in pages
+
 template <int D, int MT>
 struct DecodeShape {
   static constexpr int kRows = 16 * MT;
@@ -67,43 +69,47 @@ __global__ void __launch_bounds__(DecodeShape<D, MT>::kThreads, DecodeShape<D, M
 
   pdl_wait();
   pdl_trigger();
-  const Plan<kKvPage, kRows> plan = {a.batch, a.cache.heads, a.group, a.window};
+  const Plan<kKvPage, kRows, kDecodeExtra> plan = {a.batch, a.cache.heads, a.group, a.window};
   const long long total = plan.total(s_plan);
   const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
   if (static_cast<int>(blockIdx.x) >= ctas) return;
   const long long w0 = piece_start(total, ctas, blockIdx.x), w1 = piece_start(total, ctas, blockIdx.x + 1);
-  const int count = static_cast<int>(w1 - w0);
   plan.locate(s_plan, w0);
 
-  Cursor<kKvPage, kRows> load, use;
-  load.start(plan, s_plan);
+  Cursor<kKvPage, kRows, kDecodeExtra> load, use;
+  load.start(plan, s_plan, static_cast<int>(w1 - w0));
+  if (load.left <= 0) return;
   use = load;
-  int loaded = 0;
-  auto entry_of = [&](const Cursor<kKvPage, kRows>& at) {
+  int stage_in = 0, stage_out = 0;           // of the page to ask for, of the page to work on
+  auto entry_of = [&](const Cursor<kKvPage, kRows, kDecodeExtra>& at) {
     return __ldg(a.batch.block_table + static_cast<long long>(at.b) * a.batch.max_pages + at.span.first + at.tile);
   };
+  const int to_values = a.cache.heads * (kKvPage * (D + 4));
   int entry = entry_of(load);                // of the page to ask for next: read one page ahead
   auto ask = [&]() {
-    if (loaded < count) {
-      const int stage = loaded % kStages;
+    if (load.left > 0) {
+      const int stage = stage_in;
+      stage_in = stage_in + 1 == kStages ? 0 : stage_in + 1;
       const bool there = entry >= 0 && entry < a.cache.num_pages;
       if (there) {
-        const uint32_t dst = smem_u32(smem) + stage * Shape::kStageBytes;
-        const uint8_t* block = kv_block<D>(a.cache, entry, 0, load.head);
-        const long long to_values = static_cast<long long>(a.cache.heads) * (kKvPage * (D + 4));
+        // a thread's chunks lie kThreads apart, a multiple of eight rows: they differ by constants
+        constexpr int kChunks = Shape::kBlockBytes / 16, kEach = (kChunks + Shape::kThreads - 1) / Shape::kThreads;
+        static_assert(Shape::kThreads % (8 * (D / 16)) == 0, "the swizzle repeats every eight rows");
+        const uint32_t base = smem_u32(smem) + stage * Shape::kStageBytes, dst = base + swizzled<D>(tid / (D / 16), tid % (D / 16));
+        const uint8_t* const k_block = kv_block<D>(a.cache, entry, 0, load.head);
+        const uint8_t* const v_block = k_block + to_values;
 #pragma unroll
-        for (int i = 0; i < 2 * Shape::kBlockBytes / 16 / Shape::kThreads; ++i) {
-          const int at = tid + i * Shape::kThreads, kind = at / (Shape::kBlockBytes / 16), chunk = at % (Shape::kBlockBytes / 16);
-          cp_async16(dst + kind * Shape::kBlockBytes + swizzled<D>(chunk / (D / 16), chunk % (D / 16)), block + kind * to_values + chunk * 16);
+        for (int i = 0; i < kEach; ++i) {
+          if (kChunks % Shape::kThreads == 0 || tid + i * Shape::kThreads < kChunks) {
+            cp_async16(dst + i * Shape::kThreads * 16, k_block + (tid + i * Shape::kThreads) * 16);
+            cp_async16(dst + Shape::kBlockBytes + i * Shape::kThreads * 16, v_block + (tid + i * Shape::kThreads) * 16);
+          }
         }
-        if (tid < 32) cp_async16(dst + 2 * Shape::kBlockBytes + tid * 16, block + tid / 16 * to_values + Shape::kBlockBytes + tid % 16 * 16);
+        if (tid < 32) cp_async16(base + 2 * Shape::kBlockBytes + tid * 16, (tid < 16 ? k_block : v_block) + Shape::kBlockBytes + tid % 16 * 16);
       }
       if (tid == 0) s_there[stage] = there;
-      ++loaded;
-      if (loaded < count) {
-        if (++load.tile == load.span.tiles) load.next_unit(plan);
-        entry = entry_of(load);
-      }
+      load.advance(plan, 1);
+      if (load.left > 0) entry = entry_of(load);
     }
     cp_async_commit();
   };
@@ -117,7 +123,7 @@ __global__ void __launch_bounds__(DecodeShape<D, MT>::kThreads, DecodeShape<D, M
   bool fresh = true;
   int begun = use.tile;                      // the segment's first tile
 
-  for (int done = 0; done < count; ++done) {
+  while (use.left > 0) {
     cp_async_wait<kStages - 2>();
     __syncthreads();
     ask();
@@ -166,7 +172,8 @@ __global__ void __launch_bounds__(DecodeShape<D, MT>::kThreads, DecodeShape<D, M
         for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
     }
 
-    const int stage = done % kStages;
+    const int stage = stage_out;
+    stage_out = stage_out + 1 == kStages ? 0 : stage_out + 1;
     uint8_t* const keys = smem + stage * Shape::kStageBytes;
     uint8_t* const values = keys + Shape::kBlockBytes;
     float* const k_scale = reinterpret_cast<float*>(keys + 2 * Shape::kBlockBytes);
@@ -288,7 +295,7 @@ __global__ void __launch_bounds__(DecodeShape<D, MT>::kThreads, DecodeShape<D, M
     }
 
     const bool unit_ends = use.tile + 1 == use.span.tiles;
-    if (unit_ends || done + 1 == count) {
+    if (unit_ends || use.left == 1) {
       // ---- the segment's end: lanes, then the four warps of a row group, then the unit's other pieces
       const int rows = use.rows(a.group);
 #pragma unroll
@@ -341,7 +348,7 @@ __global__ void __launch_bounds__(DecodeShape<D, MT>::kThreads, DecodeShape<D, M
       }
       __syncthreads();
       const bool whole = begun == 0 && unit_ends;
-      const long long unit_start = w0 + done - use.tile;
+      const long long unit_start = w1 - use.left - use.tile;      // the place of its first page
       if (quarter == 0) {
         const float* other = s_merge + (mt * 2 + 1) * 16 * D;
         const int slot = 2 * static_cast<int>(blockIdx.x) + (w0 >= unit_start ? 0 : 1);
@@ -393,10 +400,8 @@ __global__ void __launch_bounds__(DecodeShape<D, MT>::kThreads, DecodeShape<D, M
         }
       }
       fresh = true;
-      if (unit_ends) use.next_unit(plan);
-    } else {
-      ++use.tile;
     }
+    use.advance(plan, 1);
   }
 }
 

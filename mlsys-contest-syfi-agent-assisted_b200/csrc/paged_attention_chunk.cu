@@ -21,8 +21,11 @@ namespace {
 
 constexpr int kTile = 128;             // positions per tile: two pages
 constexpr int kChunkRows = 256;
-constexpr int kChunkThreads = 512;
+constexpr int kChunkThreads = 768;      // 16 softmax warps, 4 converting ones, then MMAs, loads, planning, none
+constexpr int kSoftmaxWarps = 16, kSoftmaxThreads = 512;
+constexpr int kChunkExtra = 3;         // what a unit costs besides its tiles, in tiles
 constexpr int kScaleStages = 4;
+constexpr int kRedoWarps = 4;          // of the softmax warps, redo rows
 constexpr int kStatusChunkTimeout = 301;
 constexpr int kUnitShift = 5;          // the largest value scale becomes 2^4 .. 2^5 when the unit's reference is set, ...
 constexpr int kUnitGrowth = 2;         // ... and may grow to 2^7 (448 * 2^7 < 65504) before the reference follows
@@ -30,8 +33,8 @@ constexpr float kSmallestUnit = 6.103515625e-5f;   // 2^-14: f16's smallest norm
 
 template <int D>
 struct ChunkShape {
-  static constexpr int kKStages = D == 128 ? 3 : 4;
-  static constexpr int kVStages = 2;
+  static constexpr int kKStages = D == 128 ? 2 : 4;
+  static constexpr int kVStages = D == 128 ? 3 : 4;
   static constexpr int kHalfStages = 2;
   static constexpr int kTileBytes = kTile * D;                    // e4m3
   static constexpr int kHalfBytes = 2 * kTileBytes;
@@ -40,39 +43,42 @@ struct ChunkShape {
   static constexpr int kV = kK + kKStages * kTileBytes;
   static constexpr int kHalf = kV + kVStages * kTileBytes;        // [D / 64][128 positions][64] f16 per stage
   static constexpr int kScales = kHalf + kHalfStages * kHalfBytes;  // [K 128 f32][V 128 f32] per stage
-  static constexpr int kRedo = kScales + kScaleStages * 2 * kTile * 4;   // [8 warps][D + 64] f32
-  static constexpr int kSmem = 1024 + kRedo + 8 * (D + kKvPage) * 4;
+  static constexpr int kRedo = kScales + kScaleStages * 2 * kTile * 4;   // [kRedoWarps][D + 64] f32
+  static constexpr int kSmem = 1024 + kRedo + kRedoWarps * (D + kKvPage) * 4;
 };
 
 // A piece of a unit, as the planning warp describes it to the others.
 struct Segment {
-  int tile0, tiles;                    // tiles [tile0, tile0 + tiles) of the sequence's positions
+  int tile0, tiles;                    // tiles [tile0, tile0 + tiles) of the sequence's positions; no tiles: the piece is done
   int rows, row0;                      // rows [row0, row0 + rows) of the sequence's count * group
   int head, b, q_first;                // key head, sequence, its first row of q
   int base;                            // position of the sequence's first query
   int any_low, any_high, all_low, all_high;   // positions that any / all of the rows see
   int whole;                           // the unit lies in this piece alone
-  int unit_tiles;
-  long long unit_start;                // on the line
+  int first_part, last_part, first_slot;   // else: its Parts
 };
+__device__ __forceinline__ Parts parts_of(const Segment& g) { return {g.first_part, g.last_part, g.first_slot}; }
 constexpr int kSegmentRing = 4;
-constexpr int kSegmentReaders = 14;    // arrivals that free an entry: loads, MMAs, 4 converting and 8 softmax warps
+constexpr int kSegmentReaders = 2 + 4 + kSoftmaxWarps;    // arrivals that free an entry: loads, MMAs, converting and softmax warps
 
 struct ChunkShared {
   Segment segment[kSegmentRing];
   uint64_t segment_full[kSegmentRing], segment_empty[kSegmentRing];
-  uint64_t scale_full[kScaleStages], scale_clean[kScaleStages], scale_empty[kScaleStages], k_full[4], k_empty[4], v_full[2], v_empty[2], half_full[2], half_empty[2];
+  uint64_t scale_full[kScaleStages], scale_clean[kScaleStages], scale_empty[kScaleStages], k_full[4], k_empty[4], v_full[4], v_empty[4], half_full[2], half_empty[2];
   uint64_t q_full[2], s_full[2], p_full[2], o_full[2], o_empty[2], idle;
   uint32_t tmem;
   int there[kScaleStages];             // bit p: page p of the tile is there
+  int exponent[kScaleStages];          // the values' reference as of the tile: 2^exponent
+  float top[2][2][2][128];             // [tile parity][slot][half][row]: a row's largest score in half of a tile; at a segment's end, its sum
+  float unit[256];                     // of each row: what a score is worth
   volatile int redo[kSegmentRing];     // of the segment: f16 did not hold a value
   volatile int abort_code;
+  long long wait_limit;                // SM clocks
   int finished;                        // segments of this CTA whose results are written
   int asked_k, asked_v, asked_scales;  // loads that the producer has issued
 };
 
 // The unit's reference after a tile: 2^e above every finite scale of a position that is there and seen by any row; whole warp.
-// Roles that need it follow it by themselves.
 __device__ __forceinline__ int tile_exponent(const float* v_scale, int there, int position0, int any_low, int any_high, int lane) {
   const float4 v = reinterpret_cast<const float4*>(v_scale)[lane];
   const float x[4] = {v.x, v.y, v.z, v.w};
@@ -88,13 +94,57 @@ __device__ __forceinline__ int tile_exponent(const float* v_scale, int there, in
   return max(static_cast<int>(top >> 23) - 126, -100);
 }
 
+// join_parts for partial sums that are kept by dimension: a thread has a row and sixteen of its dimensions.
+template <int D>
+__device__ __forceinline__ void join_columns(const AttentionArgs& a, int q_first, int unit_row0, int head, int rows, int ctas, const Parts& parts, int thread,
+                                             int threads) {
+  const float4* const stats = reinterpret_cast<const float4*>(a.partial + 2ll * ctas * kChunkRows * D);
+  const float4* const sums = reinterpret_cast<const float4*>(a.partial);
+  for (int i = thread; i < kChunkRows * (D / 16); i += threads) {
+    const int row = i % kChunkRows, d16 = i / kChunkRows;
+    if (row >= rows) continue;
+    float m = -INFINITY, l = 0.0f, o[16] = {};
+#pragma unroll 2
+    for (int c = parts.first; c <= parts.last; ++c) {
+      const long long slot = parts.slot(c);
+      const float4 st = __ldcg(stats + slot * kChunkRows + row);
+      float4 p[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) p[k] = __ldcg(sums + (slot * (D / 4) + 4 * d16 + k) * kChunkRows + row);
+      const float m_new = fmaxf(m, st.x), m_ref = finite_or_zero(m_new), f = ex2(m - m_ref), w = ex2(st.x - m_ref);
+      l = l * f + st.y * w;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        o[4 * k] = o[4 * k] * f + p[k].x * w;
+        o[4 * k + 1] = o[4 * k + 1] * f + p[k].y * w;
+        o[4 * k + 2] = o[4 * k + 2] * f + p[k].z * w;
+        o[4 * k + 3] = o[4 * k + 3] * f + p[k].w * w;
+      }
+      m = m_new;
+    }
+    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+    const int r = unit_row0 + row;
+    uint4* const to = reinterpret_cast<uint4*>(a.out + (q_first + r / a.group) * a.out_stride + (head * a.group + r % a.group) * D + 16 * d16);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(o[8 * h + 2 * e] * f, o[8 * h + 2 * e + 1] * f);
+        w[e] = *reinterpret_cast<const uint32_t*>(&b);
+      }
+      to[h] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+
 // A barrier of the softmax warps that tells all of them whether any thread's `p` holds.
 __device__ __forceinline__ bool softmax_bar_any(bool p) {
   uint32_t any;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.u32 p, %1, 0;\n\t"
-      "barrier.cta.red.or.pred q, 1, 256, p;\n\t"
+      "barrier.cta.red.or.pred q, 1, 512, p;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(any)
       : "r"(static_cast<uint32_t>(p))
@@ -104,7 +154,7 @@ __device__ __forceinline__ bool softmax_bar_any(bool p) {
 
 // One row in f32 by one warp, for what the tiles cannot hold: a lane has two of a page's positions, then D / 32 dimensions.
 template <int D>
-__device__ __noinline__ void exact_row(const AttentionArgs& a, int base, int q_first, int b, int head, int r, float* s_q, float* s_p) {
+__device__ __forceinline__ void exact_row(const AttentionArgs& a, int base, int q_first, int b, int head, int r, float* s_q, float* s_p) {
   const int lane = threadIdx.x % 32, t = r / a.group;
   const int position = base + t, low = a.window > 0 ? max(position - a.window + 1, 0) : 0;
   const long long column = static_cast<long long>(head * a.group + r % a.group) * D;
@@ -164,11 +214,50 @@ __device__ __noinline__ void exact_row(const AttentionArgs& a, int base, int q_f
         __floats2bfloat162_rn(acc[2 * i] * inv, acc[2 * i + 1] * inv);
 }
 
-__device__ __forceinline__ bool wait_for(ChunkShared& sh, uint64_t* bar, uint32_t parity, long long limit) {
-  return mbar_wait_bounded(bar, parity, &sh.abort_code, kStatusChunkTimeout, limit);
+// Waits, bounded like the ones in ptx.cuh, that cost the waiting warps few instructions: the barrier is asked with a long suspend
+// hint, up to 64 times in a row, and only then the clock and the abort flag (half of what a tile issued were the waits before).
+__device__ __forceinline__ bool asked_64_times(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\t"
+      "mov.u32 n, 64;\n"
+      "AGAIN_%=:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "@p bra DONE_%=;\n\t"
+      "sub.u32 n, n, 1;\n\t"
+      "setp.ne.u32 q, n, 0;\n\t"
+      "@q bra AGAIN_%=;\n"
+      "DONE_%=:\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
+      : "memory");
+  return ok != 0u;
 }
-__device__ __forceinline__ void wait_whole_warp(ChunkShared& sh, bool& ok, uint64_t* bar, uint32_t parity, long long limit) {
-  mbar_wait_or_clear(ok, bar, parity, &sh.abort_code, kStatusChunkTimeout, limit);
+__device__ __forceinline__ bool wait_for(ChunkShared& sh, uint64_t* bar, uint32_t parity) {
+  if (asked_64_times(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!asked_64_times(bar, parity)) {
+    if (sh.abort_code != 0) return false;
+    if (clock64() - t0 > sh.wait_limit) {
+      sh.abort_code = kStatusChunkTimeout;
+      return false;
+    }
+  }
+  return true;
+}
+// The same for warps that have to stay whole: a lane whose wait ran out clears `ok` and goes on.
+__device__ __forceinline__ void wait_whole_warp(ChunkShared& sh, bool& ok, uint64_t* bar, uint32_t parity) {
+  if (asked_64_times(bar, parity)) return;
+  const long long t0 = clock64();
+  while (ok && !asked_64_times(bar, parity)) {
+    if (sh.abort_code != 0) {
+      ok = false;
+    } else if (clock64() - t0 > sh.wait_limit) {
+      sh.abort_code = kStatusChunkTimeout;
+      ok = false;
+    }
+  }
 }
 
 // A place in a ring of stages: its index, and the parity of its use.
@@ -185,41 +274,46 @@ struct Ring {
 };
 
 // ---------------------------------------------------------------- planning (one thread)
-__device__ __forceinline__ void plan_role(const AttentionArgs& a, const Plan<kTile, kChunkRows>& plan, const PlanShared& s_plan, ChunkShared& sh, int count,
-                                       long long w0, long long limit) {
-  Cursor<kTile, kChunkRows> at;
-  at.start(plan, s_plan);
+__device__ __forceinline__ void plan_role(const AttentionArgs& a, const Plan<kTile, kChunkRows, kChunkExtra>& plan, const PlanShared& s_plan, ChunkShared& sh, int places,
+                                          long long w1, long long total, int ctas) {
+  Cursor<kTile, kChunkRows, kChunkExtra> at;
+  at.start(plan, s_plan, places);
   Ring<kSegmentRing> ring;
-  for (int i = 0; i < count;) {
-    if (!wait_for(sh, &sh.segment_empty[ring.stage], ring.parity ^ 1u, limit)) return;
+  while (true) {
+    if (!wait_for(sh, &sh.segment_empty[ring.stage], ring.parity ^ 1u)) return;
     Segment& g = sh.segment[ring.stage];
-    const int rows = at.rows(a.group), base = at.s.length - at.s.count, row0 = at.rt * kChunkRows;
-    const int first = base + row0 / a.group, last = base + (row0 + rows - 1) / a.group;
-    g.tile0 = at.span.first + at.tile;
-    g.tiles = min(at.span.tiles - at.tile, count - i);
-    g.rows = rows;
-    g.row0 = row0;
-    g.head = at.head;
-    g.b = at.b;
-    g.q_first = at.s.first;
-    g.base = base;
-    g.any_low = a.window > 0 ? max(first - a.window + 1, 0) : 0;
-    g.any_high = last;
-    g.all_low = a.window > 0 ? max(last - a.window + 1, 0) : 0;
-    g.all_high = first;
-    g.whole = g.tiles == at.span.tiles;
-    g.unit_tiles = at.span.tiles;
-    g.unit_start = w0 + i - at.tile;
+    const bool more = at.left > 0;
+    g.tiles = more ? at.tiles_here() : 0;
+    if (more) {
+      const int rows = at.rows(a.group), base = at.s.length - at.s.count, row0 = at.rt * kChunkRows;
+      const int first = base + row0 / a.group, last = base + (row0 + rows - 1) / a.group;
+      g.tile0 = at.span.first + at.tile;
+      g.rows = rows;
+      g.row0 = row0;
+      g.head = at.head;
+      g.b = at.b;
+      g.q_first = at.s.first;
+      g.base = base;
+      g.any_low = a.window > 0 ? max(first - a.window + 1, 0) : 0;
+      g.any_high = last;
+      g.all_low = a.window > 0 ? max(last - a.window + 1, 0) : 0;
+      g.all_high = first;
+      g.whole = g.tiles == at.span.tiles;
+      const Parts parts(total, ctas, w1 - at.left - at.tile, at.span.tiles);
+      g.first_part = parts.first;
+      g.last_part = parts.last;
+      g.first_slot = parts.first_slot;
+    }
     mbar_arrive(&sh.segment_full[ring.stage]);
-    i += g.tiles;
+    if (!more) return;
     ring.next();
-    if (i < count) at.next_unit(plan);
+    at.advance(plan, g.tiles);
   }
 }
 
 // ---------------------------------------------------------------- loads (one thread)
 template <int D>
-__device__ __forceinline__ void load_role(const CUtensorMap& map, const AttentionArgs& a, ChunkShared& sh, uint8_t* smem, int count, long long limit) {
+__device__ __forceinline__ void load_role(const CUtensorMap& map, const AttentionArgs& a, ChunkShared& sh, uint8_t* smem) {
   using Shape = ChunkShape<D>;
   const uint64_t keep = l2_policy_evict_normal();          // other row tiles of the sequence read the same pages
   Ring<kSegmentRing> segments;
@@ -229,13 +323,14 @@ __device__ __forceinline__ void load_role(const CUtensorMap& map, const Attentio
   int head = 0, next_tile = 0, left = 0, any_low = 0, any_high = 0;
   const int32_t* table = nullptr;
   int entry0 = -1, entry1 = -1;
-  // table entries of the tile to ask for next: read one tile ahead
+  // table entries of the tile to ask for next, read one tile ahead; false behind the last
   auto entries = [&]() {
     if (left == 0) {
-      if (!wait_for(sh, &sh.segment_full[segments.stage], segments.parity, limit)) return false;
+      if (!wait_for(sh, &sh.segment_full[segments.stage], segments.parity)) return false;
       const Segment& g = sh.segment[segments.stage];
       next_tile = g.tile0;
       left = g.tiles;
+      if (left == 0) return false;
       any_low = g.any_low;
       any_high = g.any_high;
       head = g.head;
@@ -250,13 +345,13 @@ __device__ __forceinline__ void load_role(const CUtensorMap& map, const Attentio
     --left;
     return true;
   };
-  bool alive = entries();
-  for (int i = 0; i < count && alive; ++i) {
+  bool more = entries();
+  for (int i = 0; more; ++i) {
     const int entry[2] = {entry0, entry1}, h = head;
     const bool here[2] = {entry0 >= 0 && entry0 < a.cache.num_pages, entry1 >= 0 && entry1 < a.cache.num_pages};
     const int pages = here[0] + here[1];
-    if (i + 1 < count && !entries()) return;
-    if (!wait_for(sh, &sh.scale_empty[scales.stage], scales.parity ^ 1u, limit)) return;
+    more = entries();
+    if (!wait_for(sh, &sh.scale_empty[scales.stage], scales.parity ^ 1u)) return;
     sh.there[scales.stage] = here[0] | here[1] << 1;
     mbar_arrive_expect_tx(&sh.scale_full[scales.stage], pages * 2 * kKvPage * 4);
     float* const scale = reinterpret_cast<float*>(smem + Shape::kScales) + scales.stage * 2 * kTile;
@@ -268,14 +363,14 @@ __device__ __forceinline__ void load_role(const CUtensorMap& map, const Attentio
     }
     sh.asked_scales = i + 1;
     scales.next();
-    if (!wait_for(sh, &sh.k_empty[keys.stage], keys.parity ^ 1u, limit)) return;
+    if (!wait_for(sh, &sh.k_empty[keys.stage], keys.parity ^ 1u)) return;
     mbar_arrive_expect_tx(&sh.k_full[keys.stage], pages * kKvPage * D);
 #pragma unroll
     for (int p = 0; p < 2; ++p)
       if (here[p]) tma_load_4d(smem + Shape::kK + keys.stage * Shape::kTileBytes + p * kKvPage * D, &map, &sh.k_full[keys.stage], 0, 0, h, entry[p], keep);
     sh.asked_k = i + 1;
     keys.next();
-    if (!wait_for(sh, &sh.v_empty[values.stage], values.parity ^ 1u, limit)) return;
+    if (!wait_for(sh, &sh.v_empty[values.stage], values.parity ^ 1u)) return;
     mbar_arrive_expect_tx(&sh.v_full[values.stage], pages * kKvPage * D);
 #pragma unroll
     for (int p = 0; p < 2; ++p)
@@ -287,7 +382,7 @@ __device__ __forceinline__ void load_role(const CUtensorMap& map, const Attentio
 
 // ---------------------------------------------------------------- MMAs (one thread)
 template <int D>
-__device__ __forceinline__ void mma_role(ChunkShared& sh, uint8_t* smem, uint32_t tmem, int count, long long limit) {
+__device__ __forceinline__ void mma_role(ChunkShared& sh, uint8_t* smem, uint32_t tmem) {
   using Shape = ChunkShape<D>;
   const uint32_t qk_desc = umma_idesc_e4m3_m128(kTile), pv_desc = umma_idesc_f16_m128_n_major(D);
   const uint64_t q_desc = D == 128 ? umma_smem_desc_sw128(smem_u32(smem + Shape::kQ)) : umma_smem_desc_sw64(smem_u32(smem + Shape::kQ));
@@ -312,26 +407,27 @@ __device__ __forceinline__ void mma_role(ChunkShared& sh, uint8_t* smem, uint32_
   Ring<Shape::kKStages> keys;
   Ring<Shape::kHalfStages> halves;
   uint32_t tile_parity = 0, segment_parity = 0;    // bit s: of slot s
-  for (int i = 0; i < count;) {
-    if (!wait_for(sh, &sh.segment_full[segments.stage], segments.parity, limit)) return;
+  while (true) {
+    if (!wait_for(sh, &sh.segment_full[segments.stage], segments.parity)) return;
     const int n = sh.segment[segments.stage].tiles, slots = sh.segment[segments.stage].rows > 128 ? 2 : 1;
+    if (n == 0) return;
     mbar_arrive(&sh.segment_empty[segments.stage]);
     segments.next();
     for (int s = 0; s < slots; ++s)
-      if (!wait_for(sh, &sh.q_full[s], segment_parity >> s & 1u, limit)) return;
-    if (!wait_for(sh, &sh.k_full[keys.stage], keys.parity, limit)) return;
+      if (!wait_for(sh, &sh.q_full[s], segment_parity >> s & 1u)) return;
+    if (!wait_for(sh, &sh.k_full[keys.stage], keys.parity)) return;
     tc_fence_after();
     for (int s = 0; s < slots; ++s) scores(s, keys.stage);
     umma_commit(&sh.k_empty[keys.stage]);
     keys.next();
     for (int j = 0; j < n; ++j) {
       const bool more = j + 1 < n;
-      if (more && !wait_for(sh, &sh.k_full[keys.stage], keys.parity, limit)) return;
-      if (!wait_for(sh, &sh.half_full[halves.stage], halves.parity, limit)) return;
+      if (more && !wait_for(sh, &sh.k_full[keys.stage], keys.parity)) return;
+      if (!wait_for(sh, &sh.half_full[halves.stage], halves.parity)) return;
 #pragma unroll 1
       for (int s = 0; s < slots; ++s) {
-        if (j == 0 && !wait_for(sh, &sh.o_empty[s], (segment_parity >> s & 1u) ^ 1u, limit)) return;
-        if (!wait_for(sh, &sh.p_full[s], tile_parity >> s & 1u, limit)) return;
+        if (j == 0 && !wait_for(sh, &sh.o_empty[s], (segment_parity >> s & 1u) ^ 1u)) return;
+        if (!wait_for(sh, &sh.p_full[s], tile_parity >> s & 1u)) return;
         tile_parity ^= 1u << s;
         tc_fence_after();
         values(s, halves.stage, j > 0 ? 1u : 0u);
@@ -346,117 +442,164 @@ __device__ __forceinline__ void mma_role(ChunkShared& sh, uint8_t* smem, uint32_
       }
     }
     segment_parity ^= slots == 2 ? 3u : 1u;
-    i += n;
   }
 }
 
 // ---------------------------------------------------------------- values to f16, a thread per position (four warps)
+// The scales of a tile are looked at one tile ahead of its conversion, which has to wait for the MMAs of the tile before the last:
+// the softmax warps wait for the scales.
 template <int D>
-__device__ __forceinline__ void convert_role(ChunkShared& sh, uint8_t* smem, int count, long long limit) {
+__device__ __forceinline__ void convert_role(ChunkShared& sh, uint8_t* smem) {
   using Shape = ChunkShape<D>;
-  const int t = threadIdx.x - 8 * 32, lane = threadIdx.x % 32;
+  const int t = threadIdx.x - kSoftmaxThreads, lane = threadIdx.x % 32;
   Ring<kSegmentRing> segments;
   Ring<kScaleStages> scales;
-  Ring<Shape::kVStages> raw;
+  Ring<Shape::kVStages> ahead, raw;          // of the tile looked at, of the tile converted
   Ring<Shape::kHalfStages> halves;
   bool ok = true;
-  for (int i = 0; i < count;) {
-    wait_whole_warp(sh, ok, &sh.segment_full[segments.stage], segments.parity, limit);
-    if (!__all_sync(0xffffffffu, ok)) return;
-    const Segment& g = sh.segment[segments.stage];
-    const int n = g.tiles;
-    int unit = -100;
-    for (int j = 0; j < n; ++j) {
-      float* const k_scale = reinterpret_cast<float*>(smem + Shape::kScales) + scales.stage * 2 * kTile;
-      wait_whole_warp(sh, ok, &sh.scale_full[scales.stage], scales.parity, limit);
-      const int there = sh.there[scales.stage], position0 = (g.tile0 + j) * kTile, any_low = g.any_low, any_high = g.any_high;
-      const int e = tile_exponent(k_scale + kTile, there, position0, any_low, any_high, lane);
-      if (j == 0 || e > unit + kUnitGrowth) unit = e;
-      const float scale = k_scale[kTile + t];
-      const bool valid = (there >> (t / kKvPage) & 1) && position0 + t >= any_low && position0 + t <= any_high;
-      const bool mixed = position0 < g.all_low || position0 + kTile - 1 > g.all_high;     // some rows may see what others do not
-      const float r = scale * __int_as_float((kUnitShift - unit + 127) << 23);
-      // r as two f16 terms, so that the product with a byte's value is rounded once
-      const __half hi = __float2half_rn(r);
-      const __half2 r_hi = __half2half2(hi), r_lo = __half2half2(__float2half_rn(r - __half2float(hi)));
-      wait_whole_warp(sh, ok, &sh.v_full[raw.stage], raw.parity, limit);
-      const uint8_t* const from = smem + Shape::kV + raw.stage * Shape::kTileBytes;
-      // Zero times NaN is NaN: where some rows see a value that is not finite and others do not, its bytes become zeros and the NaN
-      // goes by way of its score to the rows that see it.
-      bool bad = false;
-      if (mixed && valid) {
+  int left = 0, n = 0, position0 = 0, any_low = 0, any_high = 0, all_low = 0, all_high = 0, unit = -100, entry = 0;
+  // of the tile looked at: what to multiply with (0: no such position), the segment's ring entry, whether the tile is its last
+  float r = 0.0f;
+  bool keep = false, ends = false;
+  auto look = [&]() {                        // false behind the last tile
+    if (left == 0) {
+      wait_whole_warp(sh, ok, &sh.segment_full[segments.stage], segments.parity);
+      __syncwarp();
+      const Segment& g = sh.segment[segments.stage];
+      left = n = __all_sync(0xffffffffu, ok) ? g.tiles : 0;
+      if (n == 0) return false;
+      position0 = g.tile0 * kTile;
+      any_low = g.any_low;
+      any_high = g.any_high;
+      all_low = g.all_low;
+      all_high = g.all_high;
+      entry = segments.stage;
+      segments.next();
+    }
+    float* const k_scale = reinterpret_cast<float*>(smem + Shape::kScales) + scales.stage * 2 * kTile;
+    wait_whole_warp(sh, ok, &sh.scale_full[scales.stage], scales.parity);
+    __syncwarp();
+    const int there = sh.there[scales.stage];
+    const int e = tile_exponent(k_scale + kTile, there, position0, any_low, any_high, lane);
+    if (left == n || e > unit + kUnitGrowth) unit = e;
+    if (t == 0) sh.exponent[scales.stage] = unit;
+    const float scale = k_scale[kTile + t];
+    keep = (there >> (t / kKvPage) & 1) && position0 + t >= any_low && position0 + t <= any_high;
+    r = scale * __int_as_float((kUnitShift - unit + 127) << 23);
+    if (position0 < all_low || position0 + kTile - 1 > all_high) {
+      // Some rows may see what others do not, and zero times NaN is NaN: the bytes of a value that is not finite become zeros, and the
+      // NaN goes by way of its score to the rows that see it.
+      wait_whole_warp(sh, ok, &sh.v_full[ahead.stage], ahead.parity);
+      if (keep) {
+        const uint8_t* const from = smem + Shape::kV + ahead.stage * Shape::kTileBytes;
         uint32_t over = 0u;
-#pragma unroll 2
+#pragma unroll 1
         for (int chunk = 0; chunk < D / 16; ++chunk) {
           const uint4 p = *reinterpret_cast<const uint4*>(from + swizzled<D>(t, chunk));
           over |= ((p.x & 0x7f7f7f7fu) + 0x01010101u) | ((p.y & 0x7f7f7f7fu) + 0x01010101u) | ((p.z & 0x7f7f7f7fu) + 0x01010101u) | ((p.w & 0x7f7f7f7fu) + 0x01010101u);
         }
-        bad = (over & 0x80808080u) != 0u || !(fabsf(scale) <= 3.402823466e38f);
-        if (bad) k_scale[t] = __int_as_float(0x7fffffff);
+        keep = (over & 0x80808080u) == 0u && fabsf(scale) <= 3.402823466e38f;
+        if (!keep) k_scale[t] = __int_as_float(0x7fffffff);
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.scale_clean[scales.stage]);
-      wait_whole_warp(sh, ok, &sh.half_empty[halves.stage], halves.parity ^ 1u, limit);
-      uint8_t* const to = smem + Shape::kHalf + halves.stage * Shape::kHalfBytes + t * 128;
-      if (valid && !bad) {
+      fence_proxy_async_smem();              // in front of the copy that fills these scales next
+    }
+    __syncwarp();
+    if (lane == 0) {
+      mbar_arrive(&sh.scale_clean[scales.stage]);
+      mbar_arrive(&sh.scale_empty[scales.stage]);
+    }
+    scales.next();
+    ahead.next();
+    position0 += kTile;
+    ends = --left == 0;
+    return true;
+  };
+  bool more = look();
+  while (more) {
+    const float scale = r;
+    const bool valid = keep, last = ends;
+    const int segment = entry;
+    wait_whole_warp(sh, ok, &sh.v_full[raw.stage], raw.parity);
+    more = look();
+    wait_whole_warp(sh, ok, &sh.half_empty[halves.stage], halves.parity ^ 1u);
+    __syncwarp();
+    const uint8_t* const from = smem + Shape::kV + raw.stage * Shape::kTileBytes;
+    uint8_t* const to = smem + Shape::kHalf + halves.stage * Shape::kHalfBytes + t * 128;
+    if (valid) {
+      // the factor as two f16 terms, so that the product with a byte's value is rounded once
+      const __half hi = __float2half_rn(scale);
+      const __half2 r_hi = __half2half2(hi), r_lo = __half2half2(__float2half_rn(scale - __half2float(hi)));
+#pragma unroll 1
+      for (int chunk = 0; chunk < D / 16; ++chunk) {
+        const uint4 p = *reinterpret_cast<const uint4*>(from + swizzled<D>(t, chunk));
+        const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+        uint32_t h[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t bits = e4m3x2_to_half2(w[k / 2] >> (16 * (k % 2)));
+          const __half2 v = *reinterpret_cast<const __half2*>(&bits);
+          const __half2 y = __hfma2(v, r_hi, __hmul2(v, r_lo));
+          h[k] = *reinterpret_cast<const uint32_t*>(&y);
+        }
+        uint8_t* const row = to + chunk / 4 * (kTile * 128);
+        *reinterpret_cast<uint4*>(row + (((2 * chunk) % 8 ^ (t & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(row + (((2 * chunk + 1) % 8 ^ (t & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
+      }
+      if (fabsf(scale) < kSmallestUnit) {
         uint32_t any = 0u;
-#pragma unroll 2
         for (int chunk = 0; chunk < D / 16; ++chunk) {
           const uint4 p = *reinterpret_cast<const uint4*>(from + swizzled<D>(t, chunk));
-          const uint32_t w[4] = {p.x, p.y, p.z, p.w};
-          uint32_t h[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const uint32_t bits = e4m3x2_to_half2(w[k / 2] >> (16 * (k % 2)));
-            const __half2 v = *reinterpret_cast<const __half2*>(&bits);
-            const __half2 y = __hfma2(v, r_hi, __hmul2(v, r_lo));
-            h[k] = *reinterpret_cast<const uint32_t*>(&y);
-          }
           any |= (p.x | p.y | p.z | p.w) & 0x7f7f7f7fu;
-          uint8_t* const row = to + chunk / 4 * (kTile * 128);
-          *reinterpret_cast<uint4*>(row + (((2 * chunk) % 8 ^ (t & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-          *reinterpret_cast<uint4*>(row + (((2 * chunk + 1) % 8 ^ (t & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
         }
-        if (any != 0u && fabsf(r) < kSmallestUnit) sh.redo[segments.stage] = 1;
-      } else {
-#pragma unroll 2
-        for (int chunk = 0; chunk < D / 8; ++chunk) *reinterpret_cast<uint4*>(to + chunk / 8 * (kTile * 128) + chunk % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
+        if (any != 0u) sh.redo[segment] = 1;
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&sh.half_full[halves.stage]);
-        mbar_arrive(&sh.v_empty[raw.stage]);
-        mbar_arrive(&sh.scale_empty[scales.stage]);
-      }
-      if (!__all_sync(0xffffffffu, ok)) return;
-      scales.next();
-      raw.next();
-      halves.next();
+    } else {
+#pragma unroll 1
+      for (int chunk = 0; chunk < D / 8; ++chunk) *reinterpret_cast<uint4*>(to + chunk / 8 * (kTile * 128) + chunk % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
     }
-    if (lane == 0) mbar_arrive(&sh.segment_empty[segments.stage]);
-    segments.next();
-    i += n;
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      mbar_arrive(&sh.half_full[halves.stage]);
+      mbar_arrive(&sh.v_empty[raw.stage]);
+      if (last) mbar_arrive(&sh.segment_empty[segment]);
+    }
+    if (!__all_sync(0xffffffffu, ok)) return;
+    raw.next();
+    halves.next();
   }
 }
 
 // ---------------------------------------------------------------- softmax, a thread per row (eight warps, four to a slot)
-// One tile: scores from tensor memory, weights back into it, the row's reference m and sum l2 (in two halves).  `fade`: what the
-// unit's reference has become smaller by.
-__device__ __forceinline__ void softmax_tile(uint32_t t_s, uint32_t t_o, int o_columns, const float* k_scale, bool masked, int low, int high, int there,
-                                             float unit, float fade, bool first, float& m, uint64_t& l2) {
-  uint32_t s[4][32];
-#pragma unroll
-  for (int c = 0; c < 4; ++c) tmem_ld32(t_s + 32 * c, s[c]);
+__device__ __forceinline__ ulonglong2 ld_shared_pairs(uint32_t at) {
+  ulonglong2 v;
+  asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(v.x), "=l"(v.y) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ float ld_shared_f32(uint32_t at) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void st_shared_f32(uint32_t at, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory"); }
+
+// One half of a tile's row: 64 scores from tensor memory, their weights back into it, the row's reference m and this half's sum l.  The partner warp has the other 64; the two agree on the row's largest score through shared memory (`top`: this
+// warp's places, `other`: the partner's), and only behind that barrier, when both have read their scores, write weights over them.
+// `fade`: what the values' reference has become smaller by.  low, high: what the row sees, counted from the first of the 64.
+template <int D>
+__device__ __forceinline__ void softmax_half(uint32_t t_s, uint32_t t_p, uint32_t t_o, uint32_t k_scale, bool masked, int low, int high, bool there,
+                                             float unit, float fade, bool first, uint32_t top, uint32_t other, int barrier, float& m, float& l) {
+  uint32_t s[2][32];
+  tmem_ld32(t_s, s[0]);
+  tmem_ld32(t_s + 32, s[1]);
   tmem_ld_wait_for(s[0]);
+  tmem_landed(s[1]);
+  // times the keys' scales: in units of the row's
 #pragma unroll
-  for (int c = 1; c < 4; ++c) tmem_landed(s[c]);
-  // times the key's scale: scores in units of the row's
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
+  for (int c = 0; c < 2; ++c) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const ulonglong2 ks = *reinterpret_cast<const ulonglong2*>(k_scale + 32 * c + 4 * e);
+      const ulonglong2 ks = ld_shared_pairs(k_scale + 4 * (32 * c + 4 * e));
       float x0, x1, x2, x3;
       f32x2_unpack(f32x2_mul(f32x2_pack_bits(s[c][4 * e], s[c][4 * e + 1]), ks.x), x0, x1);
       f32x2_unpack(f32x2_mul(f32x2_pack_bits(s[c][4 * e + 2], s[c][4 * e + 3]), ks.y), x2, x3);
@@ -468,10 +611,9 @@ __device__ __forceinline__ void softmax_tile(uint32_t t_s, uint32_t t_o, int o_c
   }
   if (masked) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      // bit b: the tile's position 32 c + b is there and seen (low and high count from the tile's first)
+    for (int c = 0; c < 2; ++c) {
       const int first_bit = low - 32 * c, last_bit = high - 32 * c;
-      uint32_t bits = last_bit < 0 || first_bit > 31 || !(there >> (c / 2) & 1) ? 0u : 0xffffffffu;
+      uint32_t bits = last_bit < 0 || first_bit > 31 || !there ? 0u : 0xffffffffu;
       if (last_bit >= 0 && last_bit < 31) bits &= (2u << last_bit) - 1u;
       if (first_bit > 0 && first_bit <= 31) bits &= 0xffffffffu << first_bit;
 #pragma unroll
@@ -479,72 +621,78 @@ __device__ __forceinline__ void softmax_tile(uint32_t t_s, uint32_t t_o, int o_c
         if (!(bits >> b & 1u)) s[c][b] = 0xff800000u;
     }
   }
-  float top4[4];
+  float t0 = __uint_as_float(s[0][0]), t1 = __uint_as_float(s[1][0]);
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    top4[c] = __uint_as_float(s[c][0]);
-#pragma unroll
-    for (int b = 1; b < 32; ++b) top4[c] = fmaxf(top4[c], __uint_as_float(s[c][b]));
+  for (int b = 1; b < 32; ++b) {
+    t0 = fmaxf(t0, __uint_as_float(s[0][b]));
+    t1 = fmaxf(t1, __uint_as_float(s[1][b]));
   }
-  const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * unit;
-  if (top > m + kGrowth) {
-    const float f = ex2(m - top);       // (0 for a row that had seen nothing)
+  t0 = fmaxf(t0, t1);
+  st_shared_f32(top, t0);
+  named_bar_sync(barrier, 64);
+  t0 = fmaxf(t0, ld_shared_f32(other)) * unit;
+  if (t0 > m + kGrowth) {
+    const float f = ex2(m - t0);       // (0 for a row that had seen nothing)
     fade *= f;
-    l2 = f32x2_mul(l2, f32x2_pack(f, f));
-    m = top;
+    l *= f;
+    m = t0;
   }
-  if (!first && __any_sync(0xffffffffu, fade != 1.0f)) {
-    for (int c = 0; c < o_columns; c += 16) {
-      uint32_t o[16];
-      tmem_ld16(t_o + c, o);
+  if (!first && __any_sync(0xffffffffu, fade != 1.0f)) {      // (the partner comes to the same, and has the other dimensions)
+#pragma unroll 1
+    for (int c = 0; c < D / 2; c += 8) {
+      uint32_t o[8];
+      tmem_ld8(t_o + c, o);
       tmem_ld_wait_for(o);
 #pragma unroll
-      for (int b = 0; b < 16; ++b) o[b] = __float_as_uint(__uint_as_float(o[b]) * fade);
-      tmem_st16(t_o + c, o);
+      for (int b = 0; b < 8; ++b) o[b] = __float_as_uint(__uint_as_float(o[b]) * fade);
+      tmem_st8(t_o + c, o);
     }
   }
   const float shift = kHeadroom - finite_or_zero(m);
   const uint64_t unit2 = f32x2_pack(unit, unit), shift2 = f32x2_pack(shift, shift);
-  uint64_t more = 0ull;
+  float more = 0.0f;
 #pragma unroll
   for (int h = 0; h < 4; ++h) {
-    uint32_t p[16];
+    uint32_t p[8];
 #pragma unroll
-    for (int b = 0; b < 16; ++b) {
+    for (int b = 0; b < 8; ++b) {
+      const int at = 16 * (h % 2) + 2 * b;
       float x0, x1;
-      f32x2_unpack(f32x2_fma(f32x2_pack_bits(s[h][2 * b], s[h][2 * b + 1]), unit2, shift2), x0, x1);
+      f32x2_unpack(f32x2_fma(f32x2_pack_bits(s[h / 2][at], s[h / 2][at + 1]), unit2, shift2), x0, x1);
       x0 = ex2(x0);
       x1 = ex2(x1);
-      uint64_t& sum = b & 1 ? more : l2;
-      sum = f32x2_add(sum, f32x2_pack(x0, x1));
+      l += x0;
+      more += x1;
       p[b] = pack_half2(x0, x1);
     }
-    tmem_st16(t_s + 16 * h, p);
+    tmem_st8(t_p + 8 * h, p);
   }
-  l2 = f32x2_add(l2, more);
+  l += more;
   tmem_st_wait();
 }
 
-// The row's part of q as two e4m3 terms of q * 2^k, its largest at 2^7 .. 2^8, into the slot's tiles; returns what a score's unit is.
+// Sixteen rows of q as two e4m3 terms of q * 2^k each, the row's largest at 2^7 .. 2^8, into the slot's tiles (row0: the first of them in
+// the tile; r0: in the sequence; rows: how many there are).  D / 8 lanes read a row.  units: what a score of each row is worth.
 template <int D>
-__device__ __forceinline__ float put_query(const __nv_bfloat16* q, bool real, float scale_log2, uint8_t* hi_tile, int row) {
-  uint4 raw[D / 8];
-  unsigned top = 0u;
-#pragma unroll
-  for (int c = 0; c < D / 8; ++c) {
-    raw[c] = real ? __ldg(reinterpret_cast<const uint4*>(q) + c) : make_uint4(0u, 0u, 0u, 0u);
-    const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+__device__ __forceinline__ void put_queries(const AttentionArgs& a, int q_first, int head, int r0, int rows, uint8_t* hi_tile, int row0, float* units) {
+  constexpr int kLanes = D / 8, kTogether = 32 / kLanes;        // rows at a time
+  const int lane = threadIdx.x % 32, part = lane % kLanes;
+#pragma unroll 2
+  for (int at = 0; at < 16; at += kTogether) {
+    const int row = at + lane / kLanes, r = r0 + row;
+    uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+    if (row < rows) raw = __ldg(reinterpret_cast<const uint4*>(a.q + (q_first + r / a.group) * a.q_stride + (head * a.group + r % a.group) * D) + part);
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    unsigned top = 0u;
 #pragma unroll
     for (int e = 0; e < 4; ++e) top = max(top, max(w[e] & 0x7fffu, w[e] >> 16 & 0x7fffu));
-  }
-  const int k = top == 0u ? 0 : min(7 - (static_cast<int>(top >> 7) - 127), 120);
-  const float up = copysignf(__int_as_float((k + 127) << 23), scale_log2);
 #pragma unroll
-  for (int c = 0; c < D / 16; ++c) {
-    const uint32_t w[8] = {raw[2 * c].x, raw[2 * c].y, raw[2 * c].z, raw[2 * c].w, raw[2 * c + 1].x, raw[2 * c + 1].y, raw[2 * c + 1].z, raw[2 * c + 1].w};
-    uint32_t hi[4], lo[4];
+    for (int d = kLanes / 2; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+    const int k = top == 0u ? 0 : min(7 - (static_cast<int>(top >> 7) - 127), 120);
+    const float up = copysignf(__int_as_float((k + 127) << 23), a.scale_log2);
+    uint32_t hi[2], lo[2];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < 2; ++e) {
       const float x0 = __uint_as_float(w[2 * e] << 16) * up, x1 = __uint_as_float(w[2 * e] & 0xffff0000u) * up;
       const float x2 = __uint_as_float(w[2 * e + 1] << 16) * up, x3 = __uint_as_float(w[2 * e + 1] & 0xffff0000u) * up;
       const uint16_t h01 = cvt_e4m3x2(x0, x1), h23 = cvt_e4m3x2(x2, x3);
@@ -552,66 +700,72 @@ __device__ __forceinline__ float put_query(const __nv_bfloat16* q, bool real, fl
       hi[e] = h01 | static_cast<uint32_t>(h23) << 16;
       lo[e] = cvt_e4m3x2(x0 - f01.x, x1 - f01.y) | static_cast<uint32_t>(cvt_e4m3x2(x2 - f23.x, x3 - f23.y)) << 16;
     }
-    const int to = swizzled<D>(row, c);
-    *reinterpret_cast<uint4*>(hi_tile + to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-    *reinterpret_cast<uint4*>(hi_tile + ChunkShape<D>::kTileBytes + to) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    uint8_t* const to = hi_tile + swizzled<D>(row0 + row, part / 2) + part % 2 * 8;
+    *reinterpret_cast<uint2*>(to) = make_uint2(hi[0], hi[1]);
+    *reinterpret_cast<uint2*>(to + ChunkShape<D>::kTileBytes) = make_uint2(lo[0], lo[1]);
+    // (a scale of zero keeps a factor, so that -infinity stays what it is)
+    if (part == 0) units[row] = top >= 0x7f80u ? __int_as_float(0x7fffffff) : fmaxf(fabsf(a.scale_log2) * __int_as_float((127 - k) << 23), 1e-30f);
   }
-  // (a scale of zero keeps a factor, so that -infinity stays what it is)
-  return top >= 0x7f80u ? __int_as_float(0x7fffffff) : fmaxf(fabsf(scale_log2) * __int_as_float((127 - k) << 23), 1e-30f);
 }
 
 template <int D>
-__device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared& sh, PlanShared& s_plan, uint8_t* smem, uint32_t tmem, int count, int ctas,
-                                             long long total, long long limit) {
+__device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared& sh, PlanShared& s_plan, uint8_t* smem, uint32_t tmem, int ctas) {
   using Shape = ChunkShape<D>;
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, slot = warp / 4;
+  // warps 0-7: slot 0, 8-15: slot 1; of each, the first four have a tile's first 64 positions and the first half of the dimensions
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, slot = warp / 8, half = warp / 4 % 2, in_slot = warp % 4 * 32 + lane;
+  const int row = slot * 128 + in_slot, pair = 2 + slot * 4 + warp % 4;        // named barrier of the two warps of a row
   const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
-  const uint32_t t_s = tmem + lanes + slot * 128, t_o = tmem + lanes + 256 + slot * 128;
+  const uint32_t t_s = tmem + lanes + slot * 128, t_o = tmem + lanes + 256 + slot * 128 + half * (D / 2);
   Ring<kSegmentRing> segments;
   Ring<kScaleStages> scales;
   uint32_t tile_parity = 0, segment_parity = 0;     // of this slot
   bool ok = true;
-  int done = 0;                                     // segments
-  for (int i = 0; i < count;) {
-    wait_whole_warp(sh, ok, &sh.segment_full[segments.stage], segments.parity, limit);
-    __syncwarp();
+  while (true) {
+    wait_whole_warp(sh, ok, &sh.segment_full[segments.stage], segments.parity);
+    if (softmax_bar_any(!ok)) return;         // all sixteen warps meet here whatever failed, and leave together
     const Segment& g = sh.segment[segments.stage];
-    const int n = ok ? g.tiles : 0;
+    const int n = g.tiles;
+    if (n == 0) return;
     const bool active = slot * 128 < g.rows;
-    const bool real = tid < g.rows;
-    float unit = 0.0f, m = -INFINITY;
-    uint64_t l2 = 0ull;
-    int exponent = -100;
-    if (n > 0) {
-      const int r = g.row0 + (real ? tid : g.rows - 1), token = r / a.group;        // (rows beyond the last copy its bounds)
-      const int high = g.base + token, low = a.window > 0 ? max(high - a.window + 1, 0) : 0;
+    float m = -INFINITY;
+    float l = 0.0f;
+    int exponent = 0;
+    {
+      int low, high;
+      {
+        const int token = (g.row0 + min(row, g.rows - 1)) / a.group;        // (rows beyond the last copy its bounds)
+        high = g.base + token;
+        low = a.window > 0 ? max(high - a.window + 1, 0) : 0;
+      }
+      float unit = 0.0f;
       if (active) {
-        unit = put_query<D>(a.q + (g.q_first + token) * a.q_stride + (g.head * a.group + r % a.group) * D, real, a.scale_log2,
-                            smem + Shape::kQ + 2 * slot * Shape::kTileBytes, tid % 128);
+        const int first = slot * 128 + warp % 4 * 32 + half * 16;
+        put_queries<D>(a, g.q_first, g.head, g.row0 + first, g.rows - first, smem + Shape::kQ + 2 * slot * Shape::kTileBytes, first % 128, sh.unit + first);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.q_full[slot]);
+        named_bar_sync(pair, 64);
+        unit = sh.unit[row];
       }
-      const int warp_low = __reduce_max_sync(0xffffffffu, low), warp_high = __reduce_min_sync(0xffffffffu, high);   // seen by every row of the warp
+      // from here on positions count from the first of this warp's half of the segment's first tile
+      const int position0 = g.tile0 * kTile + half * 64;
+      low -= position0;
+      high -= position0;
       for (int j = 0; j < n; ++j) {
-        wait_whole_warp(sh, ok, &sh.scale_full[scales.stage], scales.parity, limit);
-        wait_whole_warp(sh, ok, &sh.scale_clean[scales.stage], scales.parity, limit);
+        wait_whole_warp(sh, ok, &sh.scale_full[scales.stage], scales.parity);
+        wait_whole_warp(sh, ok, &sh.scale_clean[scales.stage], scales.parity);
         if (active) {
-          const float* const k_scale = reinterpret_cast<const float*>(smem + Shape::kScales) + scales.stage * 2 * kTile;
-          const int there = sh.there[scales.stage], position0 = (g.tile0 + j) * kTile;
-          const int e = tile_exponent(k_scale + kTile, there, position0, g.any_low, g.any_high, lane);
-          float fade = 1.0f;
-          if (j == 0) {
-            exponent = e;
-          } else if (e > exponent + kUnitGrowth) {
-            fade = ex2(static_cast<float>(exponent - e));
-            exponent = e;
-          }
-          wait_whole_warp(sh, ok, &sh.s_full[slot], tile_parity, limit);
+          const bool there = sh.there[scales.stage] >> half & 1;
+          const int e = sh.exponent[scales.stage];
+          const float fade = j == 0 ? 1.0f : ex2(static_cast<float>(exponent - e));
+          exponent = e;
+          wait_whole_warp(sh, ok, &sh.s_full[slot], tile_parity);
           __syncwarp();
           tc_fence_after();
-          softmax_tile(t_s, t_o, D, k_scale, position0 < warp_low || position0 + kTile - 1 > warp_high || there != 3, low - position0, high - position0,
-                       there, unit, fade, j == 0, m, l2);
+          const uint32_t top = smem_u32(&sh.top[tile_parity][slot][0][in_slot]);
+          softmax_half<D>(t_s + half * 64, t_s + half * 32, t_o, smem_u32(smem) + Shape::kScales + (scales.stage * 2 * kTile + half * 64) * 4,
+                          !there || __any_sync(0xffffffffu, low > 0 || high < 63), low, high, there, unit, fade, j == 0, top + half * 512,
+                          top + (half ^ 1) * 512, pair, m, l);
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh.p_full[slot]);
@@ -620,80 +774,93 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.scale_empty[scales.stage]);
         scales.next();
-        if (!__all_sync(0xffffffffu, ok)) break;
+        low -= kTile;
+        high -= kTile;
+        // (a warp that failed keeps its partner company at their barrier until the segment's end)
       }
       // ---- the segment's end
       if (active) {
-        wait_whole_warp(sh, ok, &sh.o_full[slot], segment_parity, limit);
+        wait_whole_warp(sh, ok, &sh.o_full[slot], segment_parity);
         __syncwarp();
         tc_fence_after();
         segment_parity ^= 1u;
+        sh.top[tile_parity][slot][half][in_slot] = l;
       }
     }
-    if (softmax_bar_any(!ok)) return;         // all eight warps meet here whatever failed, and leave together
-    const bool redo = sh.redo[segments.stage] != 0, whole = g.whole;
+    if (softmax_bar_any(!ok)) return;
+    const bool redo = sh.redo[segments.stage] != 0, whole = g.whole, real = row < g.rows;
     if (tid == 0) sh.redo[(segments.stage + kSegmentRing - 1) % kSegmentRing] = 0;     // the segment before: everybody has read it
-    const Parts parts(total, ctas, g.unit_start, g.unit_tiles);
-    const int r = g.row0 + tid, token = r / a.group;
     if (active) {
-      const int part = parts.slot(static_cast<int>(blockIdx.x)) * kChunkRows + tid;
-      float l0, l1;
-      f32x2_unpack(l2, l0, l1);
-      const float l = l0 + l1, unscale = __int_as_float((exponent - kUnitShift + 127) << 23);
+      l = sh.top[tile_parity][slot][0][in_slot] + sh.top[tile_parity][slot][1][in_slot];
+      const float unscale = __int_as_float((exponent - kUnitShift + 127) << 23);
       const float f = whole ? (l == 0.0f ? 0.0f : unscale / l) : unscale;
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
-        tmem_ld32(t_o + 32 * c, o);
+      // Rows leave through the slot's q tiles, which nothing reads any more: 32 rows of D bytes per warp (half of the dimensions), swizzled,
+      // then D / 16 lanes write a row's half.  Partial sums are kept by dimension, so that a warp's 32 rows lie side by side.
+      uint8_t* const stage = smem + Shape::kQ + 2 * slot * Shape::kTileBytes + (half * 4 + warp % 4) * (32 * D);
+      float4* const to = reinterpret_cast<float4*>(a.partial);
+      const int part = parts_of(g).slot(static_cast<int>(blockIdx.x));
+#pragma unroll 1
+      for (int c = 0; c < D / 16; ++c) {
+        uint32_t o[8];
+        tmem_ld8(t_o + 8 * c, o);
         tmem_ld_wait_for(o);
-        if (real && whole && !redo) {
-          uint4* to = reinterpret_cast<uint4*>(a.out + (g.q_first + token) * a.out_stride + (g.head * a.group + r % a.group) * D + 32 * c);
+        if (whole) {
+          uint32_t w[4];
 #pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            uint32_t w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(o[8 * b + 2 * e]) * f, __uint_as_float(o[8 * b + 2 * e + 1]) * f);
-              w[e] = *reinterpret_cast<const uint32_t*>(&h);
-            }
-            to[b] = make_uint4(w[0], w[1], w[2], w[3]);
+          for (int e = 0; e < 4; ++e) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(o[2 * e]) * f, __uint_as_float(o[2 * e + 1]) * f);
+            w[e] = *reinterpret_cast<const uint32_t*>(&h);
           }
-        } else if (real && !whole) {
-          float4* to = reinterpret_cast<float4*>(a.partial + static_cast<long long>(part) * D + 32 * c);
+          *reinterpret_cast<uint4*>(stage + lane * D + ((D == 128 ? c ^ (lane & 7) : c ^ (lane >> 1 & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else if (real) {
 #pragma unroll
-          for (int b = 0; b < 8; ++b)
-            to[b] = make_float4(__uint_as_float(o[4 * b]) * f, __uint_as_float(o[4 * b + 1]) * f, __uint_as_float(o[4 * b + 2]) * f, __uint_as_float(o[4 * b + 3]) * f);
+          for (int b = 0; b < 2; ++b)
+            to[(static_cast<long long>(part) * (D / 4) + half * (D / 8) + 2 * c + b) * kChunkRows + row] =
+                make_float4(__uint_as_float(o[4 * b]) * f, __uint_as_float(o[4 * b + 1]) * f, __uint_as_float(o[4 * b + 2]) * f, __uint_as_float(o[4 * b + 3]) * f);
         }
       }
-      if (real && !whole)
-        reinterpret_cast<float4*>(a.partial + 2ll * ctas * kChunkRows * D)[part] = make_float4(m, l * 0.0078125f, m, redo ? 1.0f : 0.0f);
+      if (whole && !redo) {
+        __syncwarp();
+        constexpr int kLanes = D / 16, kTogether = 32 / kLanes;
+#pragma unroll 2
+        for (int at = 0; at < 32; at += kTogether) {
+          const int line = at + lane / kLanes, x = slot * 128 + warp % 4 * 32 + line, r = g.row0 + x;
+          const uint4 p = *reinterpret_cast<const uint4*>(stage + line * D + ((D == 128 ? (lane % kLanes) ^ (line & 7) : (lane % kLanes) ^ (line >> 1 & 3)) << 4));
+          if (x < g.rows)
+            *(reinterpret_cast<uint4*>(a.out + (g.q_first + r / a.group) * a.out_stride + (g.head * a.group + r % a.group) * D + half * (D / 2)) + lane % kLanes) = p;
+        }
+      }
+      if (real && !whole && half == 0)
+        reinterpret_cast<float4*>(a.partial + 2ll * ctas * kChunkRows * D)[static_cast<long long>(part) * kChunkRows + row] = make_float4(m, l, 0.0f, redo ? 1.0f : 0.0f);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.o_empty[slot]);
     }
     bool again = whole && redo;               // whether this CTA has to redo the unit row by row
     if (!whole) {
+      const Parts parts = parts_of(g);
       __threadfence();
-      named_bar_sync(1, 256);
+      named_bar_sync(1, kSoftmaxThreads);
       if (tid == 0) {
         const bool is_last = atomicAdd(a.tickets + parts.first, 1) == parts.last - parts.first;
         if (is_last) a.tickets[parts.first] = 0;
         s_plan.last = is_last;
       }
-      named_bar_sync(1, 256);
+      named_bar_sync(1, kSoftmaxThreads);
       if (s_plan.last) {
         __threadfence();
         const float4* stats = reinterpret_cast<const float4*>(a.partial + 2ll * ctas * kChunkRows * D);
         for (int c = parts.first; c <= parts.last; ++c) again |= __ldcg(stats + static_cast<long long>(parts.slot(c)) * kChunkRows).w != 0.0f;
-        if (!again) join_parts<D, kChunkRows, 8>(a, g.q_first, g.row0, g.head, g.rows, ctas, parts, tid, 256);
+        if (!again) join_columns<D>(a, g.q_first, g.row0, g.head, g.rows, ctas, parts, tid, kSoftmaxThreads);
       }
     }
-    if (again) {
+    if (again && warp < kRedoWarps) {
       float* const s_q = reinterpret_cast<float*>(smem + Shape::kRedo) + warp * (D + kKvPage);
-      for (int x = warp; x < g.rows; x += 8) exact_row<D>(a, g.base, g.q_first, g.b, g.head, g.row0 + x, s_q, s_q + D);
+      for (int x = warp; x < g.rows; x += kRedoWarps) exact_row<D>(a, g.base, g.q_first, g.b, g.head, g.row0 + x, s_q, s_q + D);
     }
-    if (tid == 0) sh.finished = ++done;
-    i += n;
+    if (tid == 0) ++sh.finished;
+    // (the q tiles are written again behind this: by this warp's rows' own stage only when both warps of a row are through)
+    if (active) named_bar_sync(10 + slot, 256);
     __syncwarp();
     if (lane == 0) mbar_arrive(&sh.segment_empty[segments.stage]);
     segments.next();
@@ -713,34 +880,34 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
 
   pdl_wait();
   pdl_trigger();
-  const Plan<kTile, kChunkRows> plan = {a.batch, a.cache.heads, a.group, a.window};
+  const Plan<kTile, kChunkRows, kChunkExtra> plan = {a.batch, a.cache.heads, a.group, a.window};
   const long long total = plan.total(s_plan);
   const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
   if (static_cast<int>(blockIdx.x) >= ctas) return;
   const long long w0 = piece_start(total, ctas, blockIdx.x), w1 = piece_start(total, ctas, blockIdx.x + 1);
-  const int count = static_cast<int>(w1 - w0);
+  const int places = static_cast<int>(w1 - w0);
   plan.locate(s_plan, w0);
 
   if (tid == 0) {
     for (int i = 0; i < kScaleStages; ++i) {
       mbar_init(&sh.scale_full[i], 1);
       mbar_init(&sh.scale_clean[i], 4);         // converting warps
-      mbar_init(&sh.scale_empty[i], 12);        // softmax and converting warps
+      mbar_init(&sh.scale_empty[i], kSoftmaxWarps + 4);   // softmax and converting warps
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&sh.k_full[i], 1);
       mbar_init(&sh.k_empty[i], 1);
-    }
-    for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.v_full[i], 1);
       mbar_init(&sh.v_empty[i], 4);
+    }
+    for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.half_full[i], 4);
       mbar_init(&sh.half_empty[i], 1);
-      mbar_init(&sh.q_full[i], 4);
+      mbar_init(&sh.q_full[i], 8);
       mbar_init(&sh.s_full[i], 1);
-      mbar_init(&sh.p_full[i], 4);
+      mbar_init(&sh.p_full[i], 8);
       mbar_init(&sh.o_full[i], 1);
-      mbar_init(&sh.o_empty[i], 4);
+      mbar_init(&sh.o_empty[i], 8);
     }
     mbar_init(&sh.idle, 1);
     for (int i = 0; i < kSegmentRing; ++i) {
@@ -749,11 +916,12 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
       sh.redo[i] = 0;
     }
     sh.abort_code = 0;
+    sh.wait_limit = wait_limit;
     sh.finished = 0;
     sh.asked_k = sh.asked_v = sh.asked_scales = 0;
     fence_barrier_init();
   }
-  if (warp == 12) {
+  if (warp == 20) {
     tmem_alloc(&sh.tmem, 512);
     tmem_relinquish();
   }
@@ -761,19 +929,19 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh.tmem;                // S of slot s at columns 128 s (P over its first 64), O at 256 + 128 s
-  // 512 threads at 128 registers are all there are: 256 of them at 56 leave 200 for each softmax thread, until the roles are done.
-  if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-    softmax_role<D>(a, sh, s_plan, smem, tmem, count, ctas, total, wait_limit);
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 128;");
+  // 768 threads at 80 registers: 256 of them at 48 leave 96 for each softmax thread, until the roles are done.
+  if (warp < kSoftmaxWarps) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
+    softmax_role<D>(a, sh, s_plan, smem, tmem, ctas);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp < 12) {
-      convert_role<D>(sh, smem, count, wait_limit);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    if (warp < 20) {
+      convert_role<D>(sh, smem);
     } else if (lane == 0) {
-      if (warp == 12) mma_role<D>(sh, smem, tmem, count, wait_limit);
-      if (warp == 13) load_role<D>(map, a, sh, smem, count, wait_limit);
-      if (warp == 14) plan_role(a, plan, s_plan, sh, count, w0, wait_limit);
+      if (warp == 20) mma_role<D>(sh, smem, tmem);
+      if (warp == 21) load_role<D>(map, a, sh, smem);
+      if (warp == 22) plan_role(a, plan, s_plan, sh, places, w1, total, ctas);
     }
     __syncwarp();
   }
@@ -782,27 +950,26 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
   __syncthreads();
   // (Not before every role is done: an idle warp that took its registers back at once could take those that a softmax warp is
   // still to get, and the two would wait for each other.)
-  if (warp >= 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
+  if (warp >= kSoftmaxWarps) asm volatile("setmaxnreg.inc.sync.aligned.u32 80;");
   if (sh.abort_code != 0) {
     // A role gave up: copies and MMAs may still be on their way, which otherwise the roles have waited for.
-    if (tid == 13 * 32) {
+    if (tid == 21 * 32) {
       for (int i = max(sh.asked_scales - kScaleStages, 0); i < sh.asked_scales; ++i) mbar_wait_landed(&sh.scale_full[i % kScaleStages], i / kScaleStages & 1);
       for (int i = max(sh.asked_k - Shape::kKStages, 0); i < sh.asked_k; ++i) mbar_wait_landed(&sh.k_full[i % Shape::kKStages], i / Shape::kKStages & 1);
       for (int i = max(sh.asked_v - Shape::kVStages, 0); i < sh.asked_v; ++i) mbar_wait_landed(&sh.v_full[i % Shape::kVStages], i / Shape::kVStages & 1);
     }
-    if (tid == 12 * 32) {
+    if (tid == 20 * 32) {
       umma_commit(&sh.idle);
       mbar_wait_landed(&sh.idle, 0);
     }
     __syncthreads();
     // What is left of the piece becomes NaN, and its units are counted, so that nobody waits for them and the next call finds the
     // counters at zero.
-    Cursor<kTile, kChunkRows> at;
-    at.start(plan, s_plan);
-    for (int i = 0, segment = 0; i < count; ++segment) {
-      const int n = min(at.span.tiles - at.tile, count - i), rows = at.rows(a.group);
+    Cursor<kTile, kChunkRows, kChunkExtra> at;
+    at.start(plan, s_plan, places);
+    for (int segment = 0; at.left > 0; ++segment) {
+      const int n = at.tiles_here(), rows = at.rows(a.group);
       const bool whole = n == at.span.tiles;
-      const long long unit_start = w0 + i - at.tile;
       if (segment >= sh.finished) {
         if (whole) {
           for (int x = tid; x < rows * D; x += kChunkThreads) {
@@ -810,11 +977,11 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
             a.out[(at.s.first + r / a.group) * a.out_stride + (at.head * a.group + r % a.group) * D + x % D] = __float2bfloat16(__int_as_float(0x7fffffff));
           }
         } else {
-          const int slot_no = 2 * static_cast<int>(blockIdx.x) + (w0 >= unit_start ? 0 : 1);
+          const Parts parts(total, ctas, w1 - at.left - at.tile, at.span.tiles);
+          const int slot_no = parts.slot(static_cast<int>(blockIdx.x));
           for (int x = tid; x < rows; x += kChunkThreads)
             reinterpret_cast<float4*>(a.partial + 2ll * ctas * kChunkRows * D)[static_cast<long long>(slot_no) * kChunkRows + x] =
                 make_float4(0.0f, __int_as_float(0x7fffffff), 0.0f, 0.0f);
-          const Parts parts(total, ctas, unit_start, at.span.tiles);
           __threadfence();
           __syncthreads();
           if (tid == 0) {
@@ -825,18 +992,17 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
           __syncthreads();
           if (s_plan.last) {
             __threadfence();
-            join_parts<D, kChunkRows, 1>(a, at.s.first, at.rt * kChunkRows, at.head, rows, ctas, parts, tid, kChunkThreads);
+            join_columns<D>(a, at.s.first, at.rt * kChunkRows, at.head, rows, ctas, parts, tid, kChunkThreads);
           }
           __syncthreads();
         }
       }
-      i += n;
-      if (i < count) at.next_unit(plan);
+      at.advance(plan, n);
     }
     if (tid == 0) atomicExch(status, sh.abort_code);
   }
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 20) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
