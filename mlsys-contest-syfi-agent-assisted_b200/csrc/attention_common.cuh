@@ -41,6 +41,7 @@ __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY
 
 constexpr float kHeadroom = 7.0f;     // weights are kept times 2^7 in f16 ...
 constexpr float kGrowth = 8.0f;       // ... and may grow to 2^15 before their reference follows
+constexpr float kSumGrowth = 16.0f;   // a sum of weights in f32 lets them grow further
 
 
 template <int D>

@@ -25,44 +25,51 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float quad_max(float v) {
-  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+__device__ __forceinline__ float lg2(float x) {
+  float r;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
-__device__ __forceinline__ float quad_sum(float v) {
-  v += __shfl_xor_sync(0xffffffffu, v, 1);
-  return v + __shfl_xor_sync(0xffffffffu, v, 2);
+// The transpose of an 8 x 8 matrix of f16: lane 4 i + j has elements (i, 2 j) and (i, 2 j + 1) before, (2 j, i) and (2 j + 1, i) after.
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
+
 // ---------------------------------------------------------------- few rows per sequence and key head: decoding
 // A CTA walks its piece of the pages through a ring of stages filled by cp.async.  Four warps share a page, 16 positions each, for
-// every 16 rows (MT row groups of four warps); mma.sync m16n8k16 in f16, whose operands the lanes make from the bytes in
-// registers.  What bounds it is the cache's bytes, so the shape is chosen for loads in flight: three CTAs of three stages per SM.
-//   scores: rows x positions; a lane's K operand is 16 bytes of a position's row, the dimensions of the MMAs' k index being
-//           permuted alike in q;
-//   values: rows x dimensions; a lane's V operand pairs the bytes of two positions (prmt), its 16 dimensions are 16 MMAs' n.
-// Which position an n index of the scores stands for is chosen so that both reads of the swizzled rows are free of bank
-// conflicts: even n is position n, odd n is position (n - 1) ^ 5.
+// every 8 NT rows (MT row groups of four warps); mma.sync m16n8k16 in f16, whose big operand the lanes make from the bytes in
+// registers, so that a row tile is as narrow as an MMA allows:
+//   scores:  positions (M) x rows (N) = K Q^T.  A lane's K operand is 16 bytes of two positions; the MMAs' k index permutes the dimensions,
+//            alike in q.
+//   values:  dimensions (M) x rows (N) = V^T P^T.  A lane's V operand pairs the bytes of two positions (prmt), its 16 dimensions are the m
+//            indices of eight MMAs; the weights come from the scores' layout by an 8 x 8 transpose (movmatrix).
+// Which position an index of the scores stands for is chosen so that both reads of the swizzled rows are free of bank conflicts: even i
+// is position i, odd i is position (i - 1) ^ 5.
+// What bounds it is the cache's bytes, so what counts is loads in flight and few instructions per page.
 constexpr int kDecodeExtra = 1;      // what a unit costs besides its pages, in pages
 
-template <int D, int MT>
+template <int D, int NT, int MT>
 struct DecodeShape {
-  static constexpr int kRows = 16 * MT;
+  static constexpr int kRows = 8 * NT * MT;
   static constexpr int kThreads = 128 * MT;
-  static constexpr int kBlocks = MT == 1 ? 3 : 1;                       // per SM
-  static constexpr int kStages = MT == 1 ? (D == 128 ? 3 : 5) : (D == 128 ? 6 : 10);
+  static constexpr int kBlocks = MT > 1 ? 1 : NT == 1 ? 3 : 2;          // per SM
+  static constexpr int kStages = (MT > 1 ? 6 : NT == 1 ? 3 : 5) * (D == 128 ? 1 : 2) - (D == 128 ? 0 : 1);
   static constexpr int kBlockBytes = kKvPage * D;
   static constexpr int kStageBytes = 2 * kBlockBytes + 2 * kKvPage * 4;
-  static constexpr int kMerge = MT * 2 * 16 * D;                        // floats
+  static constexpr int kMerge = MT * 2 * 8 * NT * D;                    // floats
   static constexpr int kSmem = kStages * kStageBytes + kMerge * 4;
 };
-template <int D, int MT>
-__global__ void __launch_bounds__(DecodeShape<D, MT>::kThreads, DecodeShape<D, MT>::kBlocks) attention_decode_kernel(const __grid_constant__ AttentionArgs a) {
-  using Shape = DecodeShape<D, MT>;
-  constexpr int kRows = Shape::kRows, kStages = Shape::kStages, kSteps = D / 16, kMmas = D / 8;
+
+template <int D, int NT, int MT>
+__global__ void __launch_bounds__(DecodeShape<D, NT, MT>::kThreads, DecodeShape<D, NT, MT>::kBlocks) attention_decode_kernel(const __grid_constant__ AttentionArgs a) {
+  using Shape = DecodeShape<D, NT, MT>;
+  constexpr int kRows = Shape::kRows, kStages = Shape::kStages, kSteps = D / 16, kMmas = D / 16;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ PlanShared s_plan;
   __shared__ int s_there[kStages];
-  __shared__ float4 s_stat[4 * MT][16];
+  __shared__ float4 s_stat[4 * MT][8 * NT];
   float* const s_merge = reinterpret_cast<float*>(smem + kStages * Shape::kStageBytes);
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, c = lane % 4;
   const int mt = warp / 4, quarter = warp % 4;
@@ -116,9 +123,12 @@ __global__ void __launch_bounds__(DecodeShape<D, MT>::kThreads, DecodeShape<D, M
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) ask();
 
-  uint32_t qa[kSteps][4];
-  float unit[2], m[2], l[2], n[2], o[kMmas][4];
-  int low[2], high[2];                       // positions that this lane's two rows see
+  // This lane's positions of a page: t0 and t0 + 8; its rows of the scores: 8 t + 2 c and 8 t + 2 c + 1.
+  const int t0 = quarter * 16 + ((g & 1) ? (g - 1) ^ 5 : g);
+  uint32_t qb[NT][kSteps][2];
+  // Of each row: what a score is worth; the reference of this lane's sum, and the sum; the reference of the values' sum, and 2^(m - n + 7).
+  float unit[NT][2], m[NT][2], l[NT][2], n[NT][2], up[NT][2], o[NT][kMmas][4];
+  int low[NT][2], high[NT][2];               // positions that the rows see
   int all_low = 0, all_high = 0, any_low = 0, any_high = 0;   // positions that all / any of the unit's rows see
   bool fresh = true;
   int begun = use.tile;                      // the segment's first tile
@@ -137,15 +147,10 @@ __global__ void __launch_bounds__(DecodeShape<D, MT>::kThreads, DecodeShape<D, M
       all_high = first;
       any_high = last;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int row = mt * 16 + g + 8 * i, r = r0 + row;
-        const bool real = row < rows;
-        const int position = base + (real ? r / a.group : 0);
-        low[i] = a.window > 0 ? max(position - a.window + 1, 0) : 0;
-        high[i] = real ? position : -1;
-        m[i] = n[i] = -INFINITY;
-        l[i] = 0.0f;
+      for (int t = 0; t < NT; ++t) {
         // 2^k that brings the row's largest magnitude to 2^14 .. 2^15: f16 then holds bf16 values exactly down to 2^-29 of it
+        const int row = (mt * NT + t) * 8 + g, r = r0 + row;
+        const bool real = row < rows;
         const __nv_bfloat16* from = a.q + (use.s.first + (real ? r / a.group : 0)) * a.q_stride + (use.head * a.group + (real ? r % a.group : 0)) * D;
         uint2 raw[kSteps];
         unsigned top = 0u;
@@ -158,18 +163,28 @@ __global__ void __launch_bounds__(DecodeShape<D, MT>::kThreads, DecodeShape<D, M
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const int k = top == 0u ? 0 : min(14 - (static_cast<int>(top >> 7) - 127), 120);
-        const float up = __int_as_float((k + 127) << 23);
-        unit[i] = top >= 0x7f80u ? __int_as_float(0x7fffffff) : a.scale_log2 * __int_as_float((127 - k) << 23);
+        const float factor = __int_as_float((k + 127) << 23);
+        const float worth = top >= 0x7f80u ? __int_as_float(0x7fffffff) : a.scale_log2 * __int_as_float((127 - k) << 23);
 #pragma unroll
         for (int step = 0; step < kSteps; ++step) {
-          qa[step][i] = pack_half2(__uint_as_float(raw[step].x << 16) * up, __uint_as_float(raw[step].x & 0xffff0000u) * up);
-          qa[step][2 + i] = pack_half2(__uint_as_float(raw[step].y << 16) * up, __uint_as_float(raw[step].y & 0xffff0000u) * up);
+          qb[t][step][0] = pack_half2(__uint_as_float(raw[step].x << 16) * factor, __uint_as_float(raw[step].x & 0xffff0000u) * factor);
+          qb[t][step][1] = pack_half2(__uint_as_float(raw[step].y << 16) * factor, __uint_as_float(raw[step].y & 0xffff0000u) * factor);
         }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          unit[t][i] = __shfl_sync(0xffffffffu, worth, 8 * c + 4 * i);
+          const int mine = (mt * NT + t) * 8 + 2 * c + i;
+          const int position = base + (mine < rows ? (r0 + mine) / a.group : 0);
+          low[t][i] = a.window > 0 ? max(position - a.window + 1, 0) : 0;
+          high[t][i] = mine < rows ? position : -1;
+          m[t][i] = n[t][i] = -INFINITY;
+          l[t][i] = up[t][i] = 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < kMmas; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[t][j][e] = 0.0f;
       }
-#pragma unroll
-      for (int j = 0; j < kMmas; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
     }
 
     const int stage = stage_out;
@@ -210,76 +225,118 @@ __global__ void __launch_bounds__(DecodeShape<D, MT>::kThreads, DecodeShape<D, M
         }
         __syncthreads();
       }
-      float x[2][4] = {};
+      float x[NT][4];
+      {
+        float even[NT][4], odd[NT][4];       // two chains of MMAs
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int row = quarter * 16 + 8 * u + ((g & 1) ? (g - 1) ^ 5 : g);
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) even[t][e] = odd[t][e] = 0.0f;
 #pragma unroll
         for (int j = 0; j < D / 64; ++j) {
-          const uint4 p = *reinterpret_cast<const uint4*>(keys + swizzled<D>(row, c + 4 * j));
-          const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+          const uint4 p = *reinterpret_cast<const uint4*>(keys + swizzled<D>(t0, c + 4 * j)), r = *reinterpret_cast<const uint4*>(keys + swizzled<D>(t0 + 8, c + 4 * j));
+          const uint32_t w[4] = {p.x, p.y, p.z, p.w}, v[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) mma_f16(x[u], qa[4 * j + i], e4m3x2_to_half2(w[i]), e4m3x2_to_half2(w[i] >> 16));
-        }
-      }
-      float y[2][4];
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t ka[4] = {e4m3x2_to_half2(w[i]), e4m3x2_to_half2(v[i]), e4m3x2_to_half2(w[i] >> 16), e4m3x2_to_half2(v[i] >> 16)};
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int t = quarter * 16 + 8 * u + (e ? (2 * c) ^ 5 : 2 * c);
-          const float ks = k_scale[t], lv = __log2f(v_scale[t]);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float& v = x[u][2 * i + e];
-            v *= ks * unit[i];
-            if (!plain && (position0 + t < low[i] || position0 + t > high[i])) v = -INFINITY;
-            y[u][2 * i + e] = v == -INFINITY ? -INFINITY : v + lv;
+            for (int t = 0; t < NT; ++t) mma_f16(i & 1 ? odd[t] : even[t], ka, qb[t][4 * j + i][0], qb[t][4 * j + i][1]);
           }
         }
-      }
-      float fade[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        // l by lane, for its own positions; the lanes of a row meet at the unit's end
-        const float top = fmaxf(fmaxf(x[0][2 * i], x[0][2 * i + 1]), fmaxf(x[1][2 * i], x[1][2 * i + 1]));
-        const float m_new = fmaxf(m[i], top), m_ref = finite_or_zero(m_new);
-        l[i] = l[i] * ex2(m[i] - m_ref) + ((ex2(x[0][2 * i] - m_ref) + ex2(x[0][2 * i + 1] - m_ref)) + (ex2(x[1][2 * i] - m_ref) + ex2(x[1][2 * i + 1] - m_ref)));
-        m[i] = m_new;
-        const float y_top = quad_max(fmaxf(fmaxf(y[0][2 * i], y[0][2 * i + 1]), fmaxf(y[1][2 * i], y[1][2 * i + 1])));
-        fade[i] = 1.0f;
-        if (y_top > n[i] + kGrowth) {
-          fade[i] = ex2(n[i] - y_top);
-          n[i] = y_top;
-        }
-        const float shift = kHeadroom - finite_or_zero(n[i]);
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          y[u][2 * i] = ex2(y[u][2 * i] + shift);
-          y[u][2 * i + 1] = ex2(y[u][2 * i + 1] + shift);
+          for (int e = 0; e < 4; ++e) x[t][e] = even[t][e] + odd[t][e];
+      }
+      const float ks[2] = {k_scale[t0], k_scale[t0 + 8]}, vs[2] = {v_scale[t0], v_scale[t0 + 8]};
+      bool grown = false, late = false;
+      // element e: position t0 + 8 (e / 2), row 2 c + e % 2
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[t][e] *= ks[e / 2] * unit[t][e % 2];
+      if (!plain) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int position = position0 + t0 + 8 * (e / 2);
+            if (position < low[t][e % 2] || position > high[t][e % 2]) x[t][e] = -INFINITY;
+          }
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) grown |= fmaxf(x[t][i], x[t][2 + i]) > m[t][i] + kSumGrowth;
+      if (__any_sync(0xffffffffu, grown)) {
+        // a row's sum in this lane follows its scores once they are 2^16 above the reference; the lanes meet at the unit's end
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float top = fmaxf(x[t][i], x[t][2 + i]);
+            if (top > m[t][i] + kSumGrowth) {
+              l[t][i] *= ex2(m[t][i] - top);
+              m[t][i] = top;
+              up[t][i] = n[t][i] == -INFINITY ? 0.0f : ex2(top - n[t][i] + kHeadroom);
+            }
+          }
+      }
+      float p[NT][4];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const float m_ref[2] = {finite_or_zero(m[t][0]), finite_or_zero(m[t][1])};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[t][e] = ex2(x[t][e] - m_ref[e % 2]);
+        l[t][0] += p[t][0] + p[t][2];
+        l[t][1] += p[t][1] + p[t][3];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[t][e] *= vs[e / 2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float top = fmaxf(p[t][i], p[t][2 + i]);
+          late |= top * up[t][i] > 32768.0f || (up[t][i] == 0.0f && top > 0.0f);
         }
       }
-      if (__any_sync(0xffffffffu, fade[0] != 1.0f || fade[1] != 1.0f)) {
+      if (__any_sync(0xffffffffu, late)) {
+        // the reference of the values' sum follows, in all lanes of a row alike
 #pragma unroll
-        for (int j = 0; j < kMmas; ++j) {
-          o[j][0] *= fade[0];
-          o[j][1] *= fade[0];
-          o[j][2] *= fade[1];
-          o[j][3] *= fade[1];
+        for (int t = 0; t < NT; ++t) {
+          float fade[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float top = finite_or_zero(m[t][i]) + lg2(fmaxf(p[t][i], p[t][2 + i]));
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            fade[i] = 1.0f;
+            if (top > n[t][i] + kGrowth) {
+              fade[i] = ex2(n[t][i] - top);
+              n[t][i] = top;
+            }
+            up[t][i] = n[t][i] == -INFINITY || m[t][i] == -INFINITY ? 0.0f : ex2(m[t][i] - n[t][i] + kHeadroom);
+          }
+#pragma unroll
+          for (int j = 0; j < kMmas; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[t][j][e] *= fade[e % 2];
         }
       }
-      const uint32_t pa[4] = {pack_half2(y[0][0], y[0][1]), pack_half2(y[0][2], y[0][3]), pack_half2(y[1][0], y[1][1]), pack_half2(y[1][2], y[1][3])};
+      uint32_t pb[NT][2];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) pb[t][u] = transposed(pack_half2(p[t][2 * u] * up[t][0], p[t][2 * u + 1] * up[t][1]));
       uint32_t even[2][D / 32], odd[2][D / 32];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int t0 = quarter * 16 + 8 * u + 2 * c, t1 = quarter * 16 + 8 * u + ((2 * c) ^ 5);
+        const int v0 = quarter * 16 + 8 * u + 2 * c, v1 = quarter * 16 + 8 * u + ((2 * c) ^ 5);
         if constexpr (D == 128) {
-          const uint4 p = *reinterpret_cast<const uint4*>(values + swizzled<D>(t0, g)), r = *reinterpret_cast<const uint4*>(values + swizzled<D>(t1, g));
-          even[u][0] = p.x; even[u][1] = p.y; even[u][2] = p.z; even[u][3] = p.w;
+          const uint4 w = *reinterpret_cast<const uint4*>(values + swizzled<D>(v0, g)), r = *reinterpret_cast<const uint4*>(values + swizzled<D>(v1, g));
+          even[u][0] = w.x; even[u][1] = w.y; even[u][2] = w.z; even[u][3] = w.w;
           odd[u][0] = r.x; odd[u][1] = r.y; odd[u][2] = r.z; odd[u][3] = r.w;
         } else {
-          const uint2 p = *reinterpret_cast<const uint2*>(values + swizzled<D>(t0, g / 2) + (g & 1) * 8), r = *reinterpret_cast<const uint2*>(values + swizzled<D>(t1, g / 2) + (g & 1) * 8);
-          even[u][0] = p.x; even[u][1] = p.y;
+          const uint2 w = *reinterpret_cast<const uint2*>(values + swizzled<D>(v0, g / 2) + (g & 1) * 8), r = *reinterpret_cast<const uint2*>(values + swizzled<D>(v1, g / 2) + (g & 1) * 8);
+          even[u][0] = w.x; even[u][1] = w.y;
           odd[u][0] = r.x; odd[u][1] = r.y;
         }
       }
@@ -287,9 +344,11 @@ __global__ void __launch_bounds__(DecodeShape<D, MT>::kThreads, DecodeShape<D, M
       for (int w = 0; w < D / 32; ++w) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+          // dimensions 4 w + 2 h and 4 w + 2 h + 1 of this lane's D / 8
           const uint32_t b0 = __byte_perm(even[0][w], odd[0][w], h ? 0x7362 : 0x5140), b1 = __byte_perm(even[1][w], odd[1][w], h ? 0x7362 : 0x5140);
-          mma_f16(o[4 * w + 2 * h], pa, e4m3x2_to_half2(b0), e4m3x2_to_half2(b1));
-          mma_f16(o[4 * w + 2 * h + 1], pa, e4m3x2_to_half2(b0 >> 16), e4m3x2_to_half2(b1 >> 16));
+          const uint32_t va[4] = {e4m3x2_to_half2(b0), e4m3x2_to_half2(b0 >> 16), e4m3x2_to_half2(b1), e4m3x2_to_half2(b1 >> 16)};
+#pragma unroll
+          for (int t = 0; t < NT; ++t) mma_f16(o[t][2 * w + h], va, pb[t][0], pb[t][1]);
         }
       }
     }
@@ -299,90 +358,96 @@ __global__ void __launch_bounds__(DecodeShape<D, MT>::kThreads, DecodeShape<D, M
       // ---- the segment's end: lanes, then the four warps of a row group, then the unit's other pieces
       const int rows = use.rows(a.group);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float top = quad_max(m[i]);
-        l[i] = quad_sum(l[i] * ex2(m[i] - finite_or_zero(top)));
-        m[i] = top;
-        if (c == 0) s_stat[warp][g + 8 * i] = make_float4(m[i], l[i], n[i], 0.0f);
-      }
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float top = m[t][i];
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+          float sum = l[t][i] * ex2(m[t][i] - finite_or_zero(top));
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+          if (g == 0) s_stat[warp][8 * t + 2 * c + i] = make_float4(top, sum, n[t][i], 0.0f);
+        }
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float m_all = -INFINITY, n_all = -INFINITY, l_all = 0.0f;
+      for (int t = 0; t < NT; ++t) {
+        float f[2];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          m_all = fmaxf(m_all, s_stat[mt * 4 + w][g + 8 * i].x);
-          n_all = fmaxf(n_all, s_stat[mt * 4 + w][g + 8 * i].z);
+        for (int i = 0; i < 2; ++i) {
+          float m_all = -INFINITY, n_all = -INFINITY, l_all = 0.0f;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            m_all = fmaxf(m_all, s_stat[mt * 4 + w][8 * t + 2 * c + i].x);
+            n_all = fmaxf(n_all, s_stat[mt * 4 + w][8 * t + 2 * c + i].z);
+          }
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const float4 st = s_stat[mt * 4 + w][8 * t + 2 * c + i];
+            l_all += st.y * ex2(st.x - finite_or_zero(m_all));
+          }
+          f[i] = ex2(n[t][i] - finite_or_zero(n_all));
+          m[t][i] = m_all;
+          n[t][i] = n_all;
+          l[t][i] = l_all;
         }
-#pragma unroll
-        for (int w = 0; w < 4; ++w) l_all += s_stat[mt * 4 + w][g + 8 * i].y * ex2(s_stat[mt * 4 + w][g + 8 * i].x - finite_or_zero(m_all));
-        const float f = ex2(n[i] - finite_or_zero(n_all));
-#pragma unroll
-        for (int j = 0; j < kMmas; ++j) {
-          o[j][2 * i] *= f;
-          o[j][2 * i + 1] *= f;
-        }
-        m[i] = m_all;
-        n[i] = n_all;
-        l[i] = l_all;
-      }
-      float* const mine = s_merge + (mt * 2 + (quarter & 1)) * 16 * D;
-      if (quarter >= 2) {
 #pragma unroll
         for (int j = 0; j < kMmas; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) mine[(j * 4 + e) * 32 + lane] = o[j][e];
+          for (int e = 0; e < 4; ++e) o[t][j][e] *= f[e % 2];
+      }
+      float* const mine = s_merge + (mt * 2 + (quarter & 1)) * 8 * NT * D + lane;
+      if (quarter >= 2) {
+#pragma unroll
+        for (int k = 0; k < NT * kMmas * 4; ++k) mine[k * 32] = o[k / (kMmas * 4)][k / 4 % kMmas][k % 4];
       }
       __syncthreads();
       if (quarter < 2) {
 #pragma unroll
-        for (int j = 0; j < kMmas; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[j][e] += mine[(j * 4 + e) * 32 + lane];
+        for (int k = 0; k < NT * kMmas * 4; ++k) o[k / (kMmas * 4)][k / 4 % kMmas][k % 4] += mine[k * 32];
         if (quarter == 1) {
 #pragma unroll
-          for (int j = 0; j < kMmas; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) mine[(j * 4 + e) * 32 + lane] = o[j][e];
+          for (int k = 0; k < NT * kMmas * 4; ++k) mine[k * 32] = o[k / (kMmas * 4)][k / 4 % kMmas][k % 4];
         }
       }
       __syncthreads();
       const bool whole = begun == 0 && unit_ends;
       const long long unit_start = w1 - use.left - use.tile;      // the place of its first page
       if (quarter == 0) {
-        const float* other = s_merge + (mt * 2 + 1) * 16 * D;
+        const float* other = s_merge + (mt * 2 + 1) * 8 * NT * D + lane;
         const int slot = 2 * static_cast<int>(blockIdx.x) + (w0 >= unit_start ? 0 : 1);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int row = mt * 16 + g + 8 * i, r = use.rt * kRows + row;
-          if (row >= rows) continue;
-          // this lane's dimensions: D / 4 in a row, the MMAs' first columns, then their second ones
-          float v[D / 4];
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
+          for (int i = 0; i < 2; ++i) {
+            const int row = (mt * NT + t) * 8 + 2 * c + i, r = use.rt * kRows + row;
+            if (row >= rows) continue;
+            float v[D / 8];                  // this lane's dimensions of the row, g * D / 8 and on
 #pragma unroll
-            for (int j = 0; j < kMmas; ++j) v[e * kMmas + j] = o[j][2 * i + e] + other[(j * 4 + 2 * i + e) * 32 + lane];
-          if (whole) {
-            const float f = l[i] == 0.0f ? 0.0f : ex2(finite_or_zero(n[i]) - finite_or_zero(m[i]) - kHeadroom) / l[i];
-            uint4* to = reinterpret_cast<uint4*>(a.out + (use.s.first + r / a.group) * a.out_stride + (use.head * a.group + r % a.group) * D + c * (D / 4));
+            for (int j = 0; j < kMmas; ++j)
 #pragma unroll
-            for (int j = 0; j < D / 32; ++j) {
-              uint32_t w[4];
+              for (int e = 0; e < 2; ++e) v[2 * j + e] = o[t][j][2 * e + i] + other[((t * kMmas + j) * 4 + 2 * e + i) * 32];
+            if (whole) {
+              const float f = l[t][i] == 0.0f ? 0.0f : ex2(finite_or_zero(n[t][i]) - finite_or_zero(m[t][i]) - kHeadroom) / l[t][i];
+              uint4* to = reinterpret_cast<uint4*>(a.out + (use.s.first + r / a.group) * a.out_stride + (use.head * a.group + r % a.group) * D + g * (D / 8));
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(v[8 * j + 2 * e] * f, v[8 * j + 2 * e + 1] * f);
-                w[e] = *reinterpret_cast<const uint32_t*>(&h);
+              for (int j = 0; j < D / 64; ++j) {
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const __nv_bfloat162 h = __floats2bfloat162_rn(v[8 * j + 2 * e] * f, v[8 * j + 2 * e + 1] * f);
+                  w[e] = *reinterpret_cast<const uint32_t*>(&h);
+                }
+                to[j] = make_uint4(w[0], w[1], w[2], w[3]);
               }
-              to[j] = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-          } else {
-            const long long at = static_cast<long long>(slot) * kRows + row;
-            float4* to = reinterpret_cast<float4*>(a.partial + at * D + c * (D / 4));
+            } else {
+              const long long at = static_cast<long long>(slot) * kRows + row;
+              float4* to = reinterpret_cast<float4*>(a.partial + at * D + g * (D / 8));
 #pragma unroll
-            for (int j = 0; j < D / 16; ++j) to[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-            if (c == 0) reinterpret_cast<float4*>(a.partial + 2ll * ctas * kRows * D)[at] = make_float4(m[i], l[i], n[i], 0.0f);
+              for (int j = 0; j < D / 32; ++j) to[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+              if (g == 0) reinterpret_cast<float4*>(a.partial + 2ll * ctas * kRows * D)[at] = make_float4(m[t][i], l[t][i], n[t][i], 0.0f);
+            }
           }
-        }
       }
       if (!whole) {
         const Parts parts(total, ctas, unit_start, use.span.tiles);
@@ -415,9 +480,9 @@ constexpr long long kWaitLimit = 1ll << 32;   // SM clocks (about two seconds)
 std::mutex g_mu;
 Device g_devices[64];
 
-template <int D, int MT>
+template <int D, int NT, int MT>
 bool raise_decode() {
-  return cudaFuncSetAttribute(attention_decode_kernel<D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeShape<D, MT>::kSmem) == cudaSuccess;
+  return cudaFuncSetAttribute(attention_decode_kernel<D, NT, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeShape<D, NT, MT>::kSmem) == cudaSuccess;
 }
 
 constexpr size_t kTicketBytes = 4096;      // 1024 CTAs
@@ -430,13 +495,13 @@ bool take_scratch(AttentionArgs& a, Device& d, size_t partial, cudaStream_t st, 
   return true;
 }
 
-template <int D, int MT>
+template <int D, int NT, int MT>
 int launch_decode(AttentionArgs a, Device& d, int sms, cudaStream_t st) {
-  using Shape = DecodeShape<D, MT>;
+  using Shape = DecodeShape<D, NT, MT>;
   const int ctas = sms * Shape::kBlocks;
   int rc = SYFI_KV_OK;
   if (!take_scratch(a, d, 2ull * ctas * Shape::kRows * (D + 4) * sizeof(float), st, &rc)) return rc;
-  return launch_dependent(attention_decode_kernel<D, MT>, dim3(ctas), dim3(Shape::kThreads), Shape::kSmem, st, a) == cudaSuccess
+  return launch_dependent(attention_decode_kernel<D, NT, MT>, dim3(ctas), dim3(Shape::kThreads), Shape::kSmem, st, a) == cudaSuccess
              ? SYFI_KV_OK : kv_fail(SYFI_KV_ERR_CUDA, "attention kernel launch failed");
 }
 
@@ -481,7 +546,8 @@ extern "C" int syfi_paged_attention(const void* q, int64_t q_stride, const void*
   std::lock_guard<std::mutex> lock(g_mu);
   Device& d = g_devices[dev];
   if (!d.status) {
-    if (!raise_decode<128, 1>() || !raise_decode<128, 2>() || !raise_decode<128, 4>() || !raise_decode<64, 1>() || !raise_decode<64, 2>() || !raise_decode<64, 4>() ||
+    if (!raise_decode<128, 1, 1>() || !raise_decode<128, 2, 1>() || !raise_decode<128, 2, 2>() || !raise_decode<128, 2, 4>() ||
+        !raise_decode<64, 1, 1>() || !raise_decode<64, 2, 1>() || !raise_decode<64, 2, 2>() || !raise_decode<64, 2, 4>() ||
         chunk_set_attributes() != cudaSuccess)
       return kv_fail(SYFI_KV_ERR_CUDA, "cannot raise the shared-memory limit of the attention kernels");
     RelaxedCapture relaxed;
@@ -490,7 +556,7 @@ extern "C" int syfi_paged_attention(const void* q, int64_t q_stride, const void*
   const long long wait_limit = d.next_wait_limit > 0 ? d.next_wait_limit : kWaitLimit;
   d.next_wait_limit = 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // Rows per sequence and key head, on average (the lengths themselves are on the device): row tiles of 16, 32 or 64, beyond that
+  // Rows per sequence and key head, on average (the lengths themselves are on the device): row tiles of 8, 16, 32 or 64, beyond that
   // the tensor memory kernel's of 256.
   const int64_t rows = (tokens * a.group + batch - 1) / batch;
   if (rows > 64) {
@@ -499,8 +565,10 @@ extern "C" int syfi_paged_attention(const void* q, int64_t q_stride, const void*
     return launch_chunk(a, head_dim, sms, d.status, wait_limit, st) == cudaSuccess ? SYFI_KV_OK : kv_fail(SYFI_KV_ERR_CUDA, "attention kernel launch failed");
   }
   if (head_dim == 128)
-    return rows <= 16 ? launch_decode<128, 1>(a, d, sms, st) : rows <= 32 ? launch_decode<128, 2>(a, d, sms, st) : launch_decode<128, 4>(a, d, sms, st);
-  return rows <= 16 ? launch_decode<64, 1>(a, d, sms, st) : rows <= 32 ? launch_decode<64, 2>(a, d, sms, st) : launch_decode<64, 4>(a, d, sms, st);
+    return rows <= 8 ? launch_decode<128, 1, 1>(a, d, sms, st) : rows <= 16 ? launch_decode<128, 2, 1>(a, d, sms, st)
+           : rows <= 32 ? launch_decode<128, 2, 2>(a, d, sms, st) : launch_decode<128, 2, 4>(a, d, sms, st);
+  return rows <= 8 ? launch_decode<64, 1, 1>(a, d, sms, st) : rows <= 16 ? launch_decode<64, 2, 1>(a, d, sms, st)
+         : rows <= 32 ? launch_decode<64, 2, 2>(a, d, sms, st) : launch_decode<64, 2, 4>(a, d, sms, st);
 }
 
 // Test hook for the bounded waits, no part of the interface: a wait of the next attention call's kernel on the current device may
