@@ -75,6 +75,12 @@ int syfi_paged_attention(const void* q, int64_t q_stride, const void* cache, int
                          int32_t batch, int64_t tokens, int32_t q_heads, int32_t kv_heads, int32_t head_dim, double scale,
                          int32_t window, void* out, int64_t out_stride, void* stream);
 
+/* The three calls above with their arguments, in their order, in one block of 8-byte words: pointers and integers as int64, doubles as
+ * their bits.  For hosts whose foreign function interface pays for every argument. */
+int syfi_kv_write_block(const int64_t* args);
+int syfi_kv_read_block(const int64_t* args);
+int syfi_paged_attention_block(const int64_t* args);
+
 /* Synchronises `stream` and reports whether an attention kernel gave up on a bounded wait on the current device since the last
  * check (status 301; the rows that it had not finished are NaN). */
 int syfi_kv_check(void* stream);

@@ -1,6 +1,10 @@
 // Writing the quantised paged KV cache and reading rows of it back (include/syfi_kv.h).  Both move bytes: what they read and
 // write once is their floor, so each is one pass with 16-byte accesses and everything in between in registers.
+#include <string.h>
+
 #include <atomic>
+#include <type_traits>
+#include <utility>
 
 #include "kv_internal.h"
 
@@ -9,6 +13,8 @@ namespace syfi {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kWriteHeads = 4, kReadVectors = 4;   // vectors that a group of lanes has under way
+constexpr int kFullGroups = 64;                    // groups per SM that are enough to keep it busy
 
 struct WriteArgs {
   const __nv_bfloat16 *q, *k, *v, *q_weight, *k_weight;
@@ -39,141 +45,163 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// D / 8 lanes have a head vector, eight dimensions each: sum of squares and maximum are shuffles inside the group, the other
-// half of a rotated pair comes from the lane rotary / 16 away.
-template <int D, bool INTERLEAVED>
-__global__ void __launch_bounds__(kThreads) kv_write_kernel(WriteArgs a) {
+// D / 8 lanes have a head vector, eight dimensions each: sum of squares and maximum are shuffles inside the group, the other half of a
+// rotated pair comes from the lane rotary / 16 away.  A group takes up to HEADS neighbouring heads of a token (queries, then keys, then
+// values), so that the token's row of cosines and sines is read once for them and their loads are under way together.
+template <int D, bool INTERLEAVED, int HEADS>
+__global__ void __launch_bounds__(kThreads) kv_write_kernel(const __grid_constant__ WriteArgs a) {
   constexpr int kLanes = D / 8;
-  const int lane = threadIdx.x % kLanes;
-  const int heads = a.q_heads + a.cache.kinds * a.cache.heads;
-  const long long id = static_cast<long long>(blockIdx.x) * (kThreads / kLanes) + threadIdx.x / kLanes;
-  const bool inside = id < static_cast<long long>(a.tokens) * heads;
-  const int t = inside ? static_cast<int>(id / heads) : 0, head = inside ? static_cast<int>(id - static_cast<long long>(t) * heads) : 0;
-  const bool is_q = head < a.q_heads;
-  const int kv = head - a.q_heads, kind = is_q ? 0 : kv / a.cache.heads, kv_head = kv - kind * a.cache.heads;
-  const int slot = is_q ? 0 : a.slots[t];
-  const bool active = inside && (is_q || (slot >= 0 && slot / kKvPage < a.cache.num_pages));
-  float x[8] = {};
-  if (active) {
-    const __nv_bfloat16* from = is_q ? a.q + t * a.q_stride + head * D
-                                     : (kind == 0 ? a.k + t * a.k_stride : a.v + t * a.v_stride) + kv_head * D;
-    unpack8(*reinterpret_cast<const uint4*>(from + lane * 8), x);
-  }
-  if (kind == 0) {       // (the same for all lanes of a group; groups of one warp may differ, so the shuffles name the group)
-    const unsigned mask = (kLanes == 32 ? 0xffffffffu : ((1u << kLanes) - 1u)) << ((threadIdx.x & 31) / kLanes * kLanes);
-    const __nv_bfloat16* weight = is_q ? a.q_weight : a.k_weight;
-    if (weight) {
-      float sum = 0.0f;
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x % kLanes, group0 = (threadIdx.x & 31) / kLanes * kLanes;
+  const unsigned mask = ((1u << kLanes) - 1u) << group0;            // groups of one warp may part, so the shuffles name the group
+  const int kv_heads = a.cache.heads, heads = a.q_heads + a.cache.kinds * kv_heads, runs = (heads + HEADS - 1) / HEADS;
+  const unsigned id = blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
+  const int t = static_cast<int>(id / static_cast<unsigned>(runs)), first = static_cast<int>(id - t * static_cast<unsigned>(runs)) * HEADS;
+  if (t >= a.tokens) return;
+  const int slot = first + HEADS > a.q_heads ? a.slots[t] : -1;
+  const bool kept = slot >= 0 && slot / kKvPage < a.cache.num_pages;
+  uint4 raw[HEADS];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
-#pragma unroll
-      for (int d = kLanes / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(mask, sum, d);
-      const float factor = rsqrtf(sum / D + a.eps);
-      float w[8];
-      unpack8(*reinterpret_cast<const uint4*>(weight + lane * 8), w);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] *= factor * w[i];
-    }
-    if (a.rotary > 0) {
-      const int position = a.positions[t];
-      const bool known = position >= 0 && position < a.max_positions;
-      const float* row = a.cos_sin + (known ? position : 0) * static_cast<long long>(a.rotary);
-      const int half = a.rotary / 16;                    // lanes that hold the first halves of the pairs
-      const bool turned = lane < 2 * half;
-      if constexpr (INTERLEAVED) {
-        if (turned) {
-          const float4 c = *reinterpret_cast<const float4*>(row + lane * 4), s = *reinterpret_cast<const float4*>(row + a.rotary / 2 + lane * 4);
-          const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float u = x[2 * i], v = x[2 * i + 1];
-            x[2 * i] = u * cs[i] - v * sn[i];
-            x[2 * i + 1] = v * cs[i] + u * sn[i];
-          }
-        }
-      } else {
-        const bool second = lane >= half;
-        const int partner = (threadIdx.x & 31) / kLanes * kLanes + (!turned ? lane : second ? lane - half : lane + half);
-        float other[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) other[i] = __shfl_sync(mask, x[i], partner);
-        if (turned) {
-          const int at = (second ? lane - half : lane) * 8;
-#pragma unroll
-          for (int j = 0; j < 8; j += 4) {
-            const float4 c = *reinterpret_cast<const float4*>(row + at + j), s = *reinterpret_cast<const float4*>(row + a.rotary / 2 + at + j);
-            const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[j + i] = x[j + i] * cs[i] + (second ? other[j + i] : -other[j + i]) * sn[i];
-          }
-        }
-      }
-      if (!known) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = __int_as_float(0x7fffffff);
-      }
+  for (int h = 0; h < HEADS; ++h) {
+    const int head = first + h, kv = head - a.q_heads;
+    raw[h] = make_uint4(0u, 0u, 0u, 0u);
+    if (head < heads && (kv < 0 || kept)) {
+      const __nv_bfloat16* from = kv < 0 ? a.q + t * a.q_stride + head * D : kv < kv_heads ? a.k + t * a.k_stride + kv * D : a.v + t * a.v_stride + (kv - kv_heads) * D;
+      raw[h] = *reinterpret_cast<const uint4*>(from + lane * 8);
     }
   }
-  if (is_q) {
-    if (active) *reinterpret_cast<uint4*>(a.q_out + t * a.q_out_stride + head * D + lane * 8) = pack8(x);
-    return;
+  // what the heads share: cosines and sines of this lane's pairs
+  const int half = a.rotary / 16;                      // lanes that hold the first halves of the pairs
+  const bool turned = lane < 2 * half, second = lane >= half;
+  const int partner = group0 + (!turned ? lane : second ? lane - half : lane + half);
+  constexpr int kPairs = INTERLEAVED ? 4 : 8;
+  float cs[kPairs], sn[kPairs];
+  bool known = true;
+  if (turned && first < a.q_heads + kv_heads) {
+    const int position = a.positions[t];
+    known = position >= 0 && position < a.max_positions;
+    const float* row = a.cos_sin + (known ? position : 0) * static_cast<long long>(a.rotary) + (INTERLEAVED ? lane * 4 : (second ? lane - half : lane) * 8);
+#pragma unroll
+    for (int j = 0; j < kPairs; j += 4) {
+      const float4 c = *reinterpret_cast<const float4*>(row + j), s = *reinterpret_cast<const float4*>(row + a.rotary / 2 + j);
+      cs[j] = c.x; cs[j + 1] = c.y; cs[j + 2] = c.z; cs[j + 3] = c.w;
+      sn[j] = s.x; sn[j + 1] = s.y; sn[j + 2] = s.z; sn[j + 3] = s.w;
+    }
   }
-  // Largest magnitude as bits: unlike the largest float it keeps a NaN.
-  unsigned top = 0u;
+  known = (__ballot_sync(mask, !known) & mask) == 0u;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-  const unsigned mask = (kLanes == 32 ? 0xffffffffu : ((1u << kLanes) - 1u)) << ((threadIdx.x & 31) / kLanes * kLanes);
+  for (int h = 0; h < HEADS; ++h) {
+    const int head = first + h, kv = head - a.q_heads;
+    if (head >= heads || (kv >= 0 && !kept)) continue;              // the same for the whole group
+    float x[8];
+    unpack8(raw[h], x);
+    if (kv < kv_heads) {
+      const __nv_bfloat16* weight = kv < 0 ? a.q_weight : a.k_weight;
+      if (weight) {
+        float sum = 0.0f;
 #pragma unroll
-  for (int d = kLanes / 2; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(mask, top, d));
-  const float largest = __uint_as_float(top);
-  const float scale = (largest < 1e-12f ? 1e-12f : largest) / 448.0f;
-  if (!active) return;
-  uint32_t bytes[2];
+        for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-    bytes[i] = cvt_e4m3x2(x[4 * i] / scale, x[4 * i + 1] / scale) | static_cast<uint32_t>(cvt_e4m3x2(x[4 * i + 2] / scale, x[4 * i + 3] / scale)) << 16;
-  uint8_t* block = kv_block<D>(a.cache, slot / kKvPage, kind, kv_head);
-  const int at = slot % kKvPage;
-  *reinterpret_cast<uint2*>(block + at * D + lane * 8) = make_uint2(bytes[0], bytes[1]);
-  if (lane == 0) *reinterpret_cast<float*>(block + kKvPage * D + at * 4) = scale;
+        for (int d = kLanes / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(mask, sum, d);
+        const float factor = rsqrtf(sum / D + a.eps);
+        float w[8];
+        unpack8(*reinterpret_cast<const uint4*>(weight + lane * 8), w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] *= factor * w[i];
+      }
+      if (a.rotary > 0) {
+        if constexpr (INTERLEAVED) {
+          if (turned) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float u = x[2 * i], v = x[2 * i + 1];
+              x[2 * i] = u * cs[i] - v * sn[i];
+              x[2 * i + 1] = v * cs[i] + u * sn[i];
+            }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float other = __shfl_sync(mask, x[i], partner);
+            if (turned) x[i] = x[i] * cs[i] + (second ? other : -other) * sn[i];
+          }
+        }
+        if (!known) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = __int_as_float(0x7fffffff);
+        }
+      }
+    }
+    if (kv < 0) {
+      *reinterpret_cast<uint4*>(a.q_out + t * a.q_out_stride + head * D + lane * 8) = pack8(x);
+      continue;
+    }
+    // Largest magnitude as bits: unlike the largest float it keeps a NaN.
+    unsigned top = 0u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+#pragma unroll
+    for (int d = kLanes / 2; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(mask, top, d));
+    const float largest = __uint_as_float(top);
+    const float scale = (largest < 1e-12f ? 1e-12f : largest) / 448.0f;
+    uint32_t bytes[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      bytes[i] = cvt_e4m3x2(x[4 * i] / scale, x[4 * i + 1] / scale) | static_cast<uint32_t>(cvt_e4m3x2(x[4 * i + 2] / scale, x[4 * i + 3] / scale)) << 16;
+    const int kind = kv >= kv_heads;
+    uint8_t* block = kv_block<D>(a.cache, slot / kKvPage, kind, kv - kind * kv_heads);
+    const int at = slot % kKvPage;
+    *reinterpret_cast<uint2*>(block + at * D + lane * 8) = make_uint2(bytes[0], bytes[1]);
+    if (lane == 0) *reinterpret_cast<float*>(block + kKvPage * D + at * 4) = scale;
+  }
 }
 
-// Sixteen dimensions per lane.
-template <int D, typename Out>
-__global__ void __launch_bounds__(kThreads) kv_read_kernel(KvCache c, const int32_t* __restrict__ slots, long long vectors,
+// D / 8 lanes have a vector, eight dimensions each, and EACH neighbouring ones (heads of keys, then of values) of a row at a time.
+template <int D, typename Out, int EACH>
+__global__ void __launch_bounds__(kThreads) kv_read_kernel(KvCache c, const int32_t* __restrict__ slots, unsigned rows, int first_kind, int kinds,
                                                            Out* __restrict__ k_out, Out* __restrict__ v_out) {
-  constexpr int kLanes = D / 16;
-  const long long id = static_cast<long long>(blockIdx.x) * (kThreads / kLanes) + threadIdx.x / kLanes;
-  const int lane = threadIdx.x % kLanes;
-  if (id >= vectors) return;
-  const int per_row = c.kinds * c.heads;
-  const long long row = id / per_row;
-  const int which = static_cast<int>(id - row * per_row), kind = which / c.heads, head = which - kind * c.heads;
-  Out* out = kind == 0 ? k_out : v_out;
-  if (!out) return;
-  out += (row * c.heads + head) * D + lane * 16;
+  constexpr int kLanes = D / 8;
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x % kLanes, vectors = kinds * c.heads, runs = (vectors + EACH - 1) / EACH;
+  const unsigned id = blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
+  const unsigned row = id / static_cast<unsigned>(runs);
+  const int first = static_cast<int>(id - row * static_cast<unsigned>(runs)) * EACH;
+  if (row >= rows) return;
   const int slot = slots[row];
-  float x[16] = {};
-  if (slot >= 0 && slot / kKvPage < c.num_pages) {
-    const uint8_t* block = kv_block<D>(c, slot / kKvPage, kind, head);
-    const int at = slot % kKvPage;
-    const uint4 p = *reinterpret_cast<const uint4*>(block + at * D + lane * 16);
-    const float scale = *reinterpret_cast<const float*>(block + kKvPage * D + at * 4);
-    const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+  const bool there = slot >= 0 && slot / kKvPage < c.num_pages;
+  uint2 bytes[EACH];
+  float scale[EACH];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float2 f = e4m3x2_to_float2(static_cast<uint16_t>(w[i / 2] >> (16 * (i % 2))));
-      x[2 * i] = f.x * scale;
-      x[2 * i + 1] = f.y * scale;
+  for (int i = 0; i < EACH; ++i) {
+    bytes[i] = make_uint2(0u, 0u);
+    scale[i] = 0.0f;
+    if (there && first + i < vectors) {
+      const int kind = first + i >= c.heads;
+      const uint8_t* block = kv_block<D>(c, slot / kKvPage, first_kind + kind, first + i - kind * c.heads);
+      bytes[i] = *reinterpret_cast<const uint2*>(block + slot % kKvPage * D + lane * 8);
+      scale[i] = *reinterpret_cast<const float*>(block + kKvPage * D + slot % kKvPage * 4);
     }
   }
-  if constexpr (sizeof(Out) == 4) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(out)[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-  } else {
-    const float lo[8] = {x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]}, hi[8] = {x[8], x[9], x[10], x[11], x[12], x[13], x[14], x[15]};
-    reinterpret_cast<uint4*>(out)[0] = pack8(lo);
-    reinterpret_cast<uint4*>(out)[1] = pack8(hi);
+  for (int i = 0; i < EACH; ++i) {
+    if (first + i >= vectors) break;
+    const int kind = first + i >= c.heads;
+    Out* out = (first_kind + kind == 0 ? k_out : v_out) + (static_cast<long long>(row) * c.heads + first + i - kind * c.heads) * D + lane * 8;
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = e4m3x2_to_float2(static_cast<uint16_t>((j < 2 ? bytes[i].x : bytes[i].y) >> (16 * (j % 2))));
+      x[2 * j] = f.x * scale[i];
+      x[2 * j + 1] = f.y * scale[i];
+    }
+    if constexpr (sizeof(Out) == 4) {
+      reinterpret_cast<float4*>(out)[0] = make_float4(x[0], x[1], x[2], x[3]);
+      reinterpret_cast<float4*>(out)[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+      *reinterpret_cast<uint4*>(out) = pack8(x);
+    }
   }
 }
 
@@ -223,7 +251,8 @@ extern "C" int syfi_kv_write(const void* q, const void* k, const void* v, const 
   if (!kv_stride_ok(k_stride, kv_width) || (kinds == 2 && !kv_stride_ok(v_stride, kv_width)) ||
       (q_heads > 0 && (!kv_stride_ok(q_stride, q_width) || !kv_stride_ok(q_out_stride, q_width))))
     return kv_fail(SYFI_KV_ERR_INVALID, "a token stride is smaller than the token's heads or no multiple of 8");
-  if (!kv_device_sms()) return SYFI_KV_ERR_CUDA;
+  const int sms = kv_device_sms();
+  if (!sms) return SYFI_KV_ERR_CUDA;
   WriteArgs a;
   a.q = static_cast<const __nv_bfloat16*>(q);
   a.k = static_cast<const __nv_bfloat16*>(k);
@@ -244,18 +273,18 @@ extern "C" int syfi_kv_write(const void* q, const void* k, const void* v, const 
   a.q_heads = q_heads;
   a.rotary = rotary_dim;
   a.eps = static_cast<float>(eps);
-  const long long vectors = tokens * (q_heads + static_cast<long long>(kinds) * kv_heads);
-  const int per_block = kThreads / (head_dim / 8);
-  const unsigned grid = static_cast<unsigned>((vectors + per_block - 1) / per_block);
+  // One head per group of lanes while that leaves SMs idle, else a run of them.
+  const int heads = q_heads + kinds * kv_heads, per_block = kThreads / (head_dim / 8);
+  const int each = tokens * heads >= static_cast<int64_t>(sms) * kFullGroups * kWriteHeads ? kWriteHeads : 1;
+  const int64_t groups = tokens * ((heads + each - 1) / each);
+  const dim3 grid(static_cast<unsigned>((groups + per_block - 1) / per_block));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (head_dim == 128) {
-    if (interleaved) kv_write_kernel<128, true><<<grid, kThreads, 0, st>>>(a);
-    else kv_write_kernel<128, false><<<grid, kThreads, 0, st>>>(a);
-  } else {
-    if (interleaved) kv_write_kernel<64, true><<<grid, kThreads, 0, st>>>(a);
-    else kv_write_kernel<64, false><<<grid, kThreads, 0, st>>>(a);
-  }
-  return cudaGetLastError() == cudaSuccess ? SYFI_KV_OK : kv_fail(SYFI_KV_ERR_CUDA, "write kernel launch failed");
+  auto run = [&](auto* kernel) { return launch_dependent(kernel, grid, dim3(kThreads), 0, st, a) == cudaSuccess; };
+  const bool ok = head_dim == 128 ? (interleaved ? (each > 1 ? run(kv_write_kernel<128, true, kWriteHeads>) : run(kv_write_kernel<128, true, 1>))
+                                                 : (each > 1 ? run(kv_write_kernel<128, false, kWriteHeads>) : run(kv_write_kernel<128, false, 1>)))
+                                  : (interleaved ? (each > 1 ? run(kv_write_kernel<64, true, kWriteHeads>) : run(kv_write_kernel<64, true, 1>))
+                                                 : (each > 1 ? run(kv_write_kernel<64, false, kWriteHeads>) : run(kv_write_kernel<64, false, 1>)));
+  return ok ? SYFI_KV_OK : kv_fail(SYFI_KV_ERR_CUDA, "write kernel launch failed");
 }
 
 extern "C" int syfi_kv_read(const void* cache, int64_t num_pages, int64_t page_stride, int32_t kinds, int32_t kv_heads,
@@ -266,23 +295,49 @@ extern "C" int syfi_kv_read(const void* cache, int64_t num_pages, int64_t page_s
   if (kinds == 1 && v_out) return kv_fail(SYFI_KV_ERR_INVALID, "this cache holds no values");
   if (rows == 0 || (!k_out && !v_out)) return SYFI_KV_OK;
   if (!kv_table_aligned(slots) || (k_out && !kv_aligned(k_out)) || (v_out && !kv_aligned(v_out))) return kv_fail(SYFI_KV_ERR_INVALID, "a tensor argument is null or not aligned (16 bytes, int32 tables 4)");
-  if (!kv_device_sms()) return SYFI_KV_ERR_CUDA;
+  const int sms = kv_device_sms();
+  if (!sms) return SYFI_KV_ERR_CUDA;
   const KvCache c = {static_cast<uint8_t*>(const_cast<void*>(cache)), page_stride, static_cast<int>(num_pages), kinds, kv_heads};
-  const long long vectors = static_cast<long long>(rows) * kinds * kv_heads;
-  const int per_block = kThreads / (head_dim / 16);
-  const long long blocks = (vectors + per_block - 1) / per_block;
-  if (blocks > 0x7fffffffll) return kv_fail(SYFI_KV_ERR_INVALID, "rows out of range");
-  const unsigned grid = static_cast<unsigned>(blocks);
+  const int first_kind = k_out ? 0 : 1, wanted = (k_out ? 1 : 0) + (v_out ? 1 : 0), per_block = kThreads / (head_dim / 8);
+  const int each = rows * wanted * kv_heads >= static_cast<int64_t>(sms) * kFullGroups * kReadVectors ? kReadVectors : 1;
+  const int64_t groups = rows * ((wanted * kv_heads + each - 1) / each);
+  if (groups > 0x7fffffffll) return kv_fail(SYFI_KV_ERR_INVALID, "rows out of range");
+  const dim3 grid(static_cast<unsigned>((groups + per_block - 1) / per_block));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto run = [&](auto* kernel, auto* typed) {
-    kernel<<<grid, kThreads, 0, st>>>(c, slots, vectors, static_cast<decltype(typed)>(k_out), static_cast<decltype(typed)>(v_out));
+    return launch_dependent(kernel, grid, dim3(kThreads), 0, st, c, slots, static_cast<unsigned>(rows), first_kind, wanted, static_cast<decltype(typed)>(k_out),
+                            static_cast<decltype(typed)>(v_out)) == cudaSuccess;
   };
-  if (out_f32) {
-    if (head_dim == 128) run(kv_read_kernel<128, float>, static_cast<float*>(nullptr));
-    else run(kv_read_kernel<64, float>, static_cast<float*>(nullptr));
-  } else {
-    if (head_dim == 128) run(kv_read_kernel<128, __nv_bfloat16>, static_cast<__nv_bfloat16*>(nullptr));
-    else run(kv_read_kernel<64, __nv_bfloat16>, static_cast<__nv_bfloat16*>(nullptr));
-  }
-  return cudaGetLastError() == cudaSuccess ? SYFI_KV_OK : kv_fail(SYFI_KV_ERR_CUDA, "read kernel launch failed");
+  float* const f32 = nullptr;
+  __nv_bfloat16* const bf16 = nullptr;
+  const bool ok = out_f32 ? (head_dim == 128 ? (each > 1 ? run(kv_read_kernel<128, float, kReadVectors>, f32) : run(kv_read_kernel<128, float, 1>, f32))
+                                             : (each > 1 ? run(kv_read_kernel<64, float, kReadVectors>, f32) : run(kv_read_kernel<64, float, 1>, f32)))
+                          : (head_dim == 128 ? (each > 1 ? run(kv_read_kernel<128, __nv_bfloat16, kReadVectors>, bf16) : run(kv_read_kernel<128, __nv_bfloat16, 1>, bf16))
+                                             : (each > 1 ? run(kv_read_kernel<64, __nv_bfloat16, kReadVectors>, bf16) : run(kv_read_kernel<64, __nv_bfloat16, 1>, bf16)));
+  return ok ? SYFI_KV_OK : kv_fail(SYFI_KV_ERR_CUDA, "read kernel launch failed");
 }
+
+// ---------------------------------------------------------------- the entry points with their arguments in one block
+namespace {
+template <typename T>
+T at(const int64_t* args, int i) {
+  if constexpr (std::is_pointer_v<T>) return reinterpret_cast<T>(args[i]);
+  else if constexpr (std::is_same_v<T, double>) {
+    double v;
+    memcpy(&v, args + i, sizeof(v));
+    return v;
+  } else return static_cast<T>(args[i]);
+}
+template <typename... Args, size_t... I>
+int spread(int (*fn)(Args...), const int64_t* args, std::index_sequence<I...>) {
+  return fn(at<Args>(args, static_cast<int>(I))...);
+}
+template <typename... Args>
+int spread(int (*fn)(Args...), const int64_t* args) {
+  return args ? spread(fn, args, std::index_sequence_for<Args...>()) : kv_fail(SYFI_KV_ERR_INVALID, "no arguments");
+}
+}  // namespace
+
+extern "C" int syfi_kv_write_block(const int64_t* args) { return spread(syfi_kv_write, args); }
+extern "C" int syfi_kv_read_block(const int64_t* args) { return spread(syfi_kv_read, args); }
+extern "C" int syfi_paged_attention_block(const int64_t* args) { return spread(syfi_paged_attention, args); }
