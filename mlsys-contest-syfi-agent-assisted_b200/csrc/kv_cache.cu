@@ -45,96 +45,105 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// D / 8 lanes have a head vector, eight dimensions each: sum of squares and maximum are shuffles inside the group, the other half of a
-// rotated pair comes from the lane rotary / 16 away.  A group takes up to HEADS neighbouring heads of a token (queries, then keys, then
-// values), so that the token's row of cosines and sines is read once for them and their loads are under way together.
+// A warp takes a run of neighbouring heads of one kind (queries, keys or values) of a token, D / 8 lanes per head and HEADS heads one
+// after the other, whose loads are under way together and which share the token's cosines and sines.  A lane has two times four
+// dimensions, chosen so that it holds both of a rotated pair: lanes below rotary / 8 have chunk l and chunk l + rotary / 8, the others two
+// neighbouring chunks of what is not rotated.  Sum of squares and maximum are shuffles inside the head's lanes.
 template <int D, bool INTERLEAVED, int HEADS>
 __global__ void __launch_bounds__(kThreads) kv_write_kernel(const __grid_constant__ WriteArgs a) {
-  constexpr int kLanes = D / 8;
+  constexpr int kLanes = D / 8, kGroups = 32 / kLanes, kRun = kGroups * HEADS;
   pdl_wait();
   pdl_trigger();
-  const int lane = threadIdx.x % kLanes, group0 = (threadIdx.x & 31) / kLanes * kLanes;
-  const unsigned mask = ((1u << kLanes) - 1u) << group0;            // groups of one warp may part, so the shuffles name the group
-  const int kv_heads = a.cache.heads, heads = a.q_heads + a.cache.kinds * kv_heads, runs = (heads + HEADS - 1) / HEADS;
-  const unsigned id = blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
-  const int t = static_cast<int>(id / static_cast<unsigned>(runs)), first = static_cast<int>(id - t * static_cast<unsigned>(runs)) * HEADS;
+  const int lane = threadIdx.x % kLanes, group = (threadIdx.x & 31) / kLanes;
+  const unsigned q_runs = (a.q_heads + kRun - 1) / kRun, kv_runs = (a.cache.heads + kRun - 1) / kRun, runs = q_runs + a.cache.kinds * kv_runs;
+  const unsigned id = blockIdx.x * (kThreads / 32) + threadIdx.x / 32;
+  const int t = static_cast<int>(id / runs);
   if (t >= a.tokens) return;
-  const int slot = first + HEADS > a.q_heads ? a.slots[t] : -1;
-  const bool kept = slot >= 0 && slot / kKvPage < a.cache.num_pages;
-  uint4 raw[HEADS];
+  unsigned run = id - t * runs;
+  const int which = run < q_runs ? 0 : run < q_runs + kv_runs ? 1 : 2;      // queries, keys, values; the same for the warp
+  if (which > 0) run -= q_runs + (which - 1) * kv_runs;
+  const int slot = which > 0 ? a.slots[t] : 0;
+  if (which > 0 && (slot < 0 || slot / kKvPage >= a.cache.num_pages)) return;
+  const int heads = which == 0 ? a.q_heads : a.cache.heads, first = static_cast<int>(run) * kRun + group;
+  const int turning = a.rotary / 8;                                         // lanes that hold rotated pairs
+  const bool turned = lane < turning && which < 2;
+  const bool apart = !INTERLEAVED && lane < turning;
+  const int dims[2] = {apart ? 4 * lane : 8 * lane, apart ? 4 * lane + a.rotary / 2 : 8 * lane + 4};   // (8 lanes' worth of rotary lie in front of the rest)
+  const __nv_bfloat16* const from = which == 0 ? a.q + t * a.q_stride : which == 1 ? a.k + t * a.k_stride : a.v + t * a.v_stride;
+  uint2 raw[HEADS][2];
 #pragma unroll
-  for (int h = 0; h < HEADS; ++h) {
-    const int head = first + h, kv = head - a.q_heads;
-    raw[h] = make_uint4(0u, 0u, 0u, 0u);
-    if (head < heads && (kv < 0 || kept)) {
-      const __nv_bfloat16* from = kv < 0 ? a.q + t * a.q_stride + head * D : kv < kv_heads ? a.k + t * a.k_stride + kv * D : a.v + t * a.v_stride + (kv - kv_heads) * D;
-      raw[h] = *reinterpret_cast<const uint4*>(from + lane * 8);
+  for (int h = 0; h < HEADS; ++h)
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      raw[h][e] = first + h * kGroups < heads ? *reinterpret_cast<const uint2*>(from + (first + h * kGroups) * D + dims[e]) : make_uint2(0u, 0u);
+  // what the heads share: weights, cosines and sines (of pair i: dimensions i of both chunks, or 2 i and 2 i + 1 of both in a row)
+  const __nv_bfloat16* const weight = which == 0 ? a.q_weight : which == 1 ? a.k_weight : nullptr;
+  float w[8], cs[4], sn[4];
+  if (weight) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const uint2 p = *reinterpret_cast<const uint2*>(weight + dims[e]);
+      w[4 * e] = __uint_as_float(p.x << 16);
+      w[4 * e + 1] = __uint_as_float(p.x & 0xffff0000u);
+      w[4 * e + 2] = __uint_as_float(p.y << 16);
+      w[4 * e + 3] = __uint_as_float(p.y & 0xffff0000u);
     }
   }
-  // what the heads share: cosines and sines of this lane's pairs
-  const int half = a.rotary / 16;                      // lanes that hold the first halves of the pairs
-  const bool turned = lane < 2 * half, second = lane >= half;
-  const int partner = group0 + (!turned ? lane : second ? lane - half : lane + half);
-  constexpr int kPairs = INTERLEAVED ? 4 : 8;
-  float cs[kPairs], sn[kPairs];
   bool known = true;
-  if (turned && first < a.q_heads + kv_heads) {
+  if (which < 2 && a.rotary > 0) {
     const int position = a.positions[t];
     known = position >= 0 && position < a.max_positions;
-    const float* row = a.cos_sin + (known ? position : 0) * static_cast<long long>(a.rotary) + (INTERLEAVED ? lane * 4 : (second ? lane - half : lane) * 8);
-#pragma unroll
-    for (int j = 0; j < kPairs; j += 4) {
-      const float4 c = *reinterpret_cast<const float4*>(row + j), s = *reinterpret_cast<const float4*>(row + a.rotary / 2 + j);
-      cs[j] = c.x; cs[j + 1] = c.y; cs[j + 2] = c.z; cs[j + 3] = c.w;
-      sn[j] = s.x; sn[j + 1] = s.y; sn[j + 2] = s.z; sn[j + 3] = s.w;
+    if (turned) {
+      const float* row = a.cos_sin + (known ? position : 0) * static_cast<long long>(a.rotary) + lane * 4;
+      const float4 c = *reinterpret_cast<const float4*>(row), s = *reinterpret_cast<const float4*>(row + a.rotary / 2);
+      cs[0] = c.x; cs[1] = c.y; cs[2] = c.z; cs[3] = c.w;
+      sn[0] = s.x; sn[1] = s.y; sn[2] = s.z; sn[3] = s.w;
     }
   }
-  known = (__ballot_sync(mask, !known) & mask) == 0u;
 #pragma unroll
   for (int h = 0; h < HEADS; ++h) {
-    const int head = first + h, kv = head - a.q_heads;
-    if (head >= heads || (kv >= 0 && !kept)) continue;              // the same for the whole group
+    const int head = first + h * kGroups;
+    const bool real = head < heads;
     float x[8];
-    unpack8(raw[h], x);
-    if (kv < kv_heads) {
-      const __nv_bfloat16* weight = kv < 0 ? a.q_weight : a.k_weight;
-      if (weight) {
-        float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
+    for (int e = 0; e < 2; ++e) {
+      x[4 * e] = __uint_as_float(raw[h][e].x << 16);
+      x[4 * e + 1] = __uint_as_float(raw[h][e].x & 0xffff0000u);
+      x[4 * e + 2] = __uint_as_float(raw[h][e].y << 16);
+      x[4 * e + 3] = __uint_as_float(raw[h][e].y & 0xffff0000u);
+    }
+    if (weight) {
+      float sum = 0.0f;
 #pragma unroll
-        for (int d = kLanes / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(mask, sum, d);
-        const float factor = rsqrtf(sum / D + a.eps);
-        float w[8];
-        unpack8(*reinterpret_cast<const uint4*>(weight + lane * 8), w);
+      for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] *= factor * w[i];
-      }
-      if (a.rotary > 0) {
-        if constexpr (INTERLEAVED) {
-          if (turned) {
+      for (int d = kLanes / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      const float factor = rsqrtf(sum * (1.0f / D) + a.eps);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float u = x[2 * i], v = x[2 * i + 1];
-              x[2 * i] = u * cs[i] - v * sn[i];
-              x[2 * i + 1] = v * cs[i] + u * sn[i];
-            }
-          }
-        } else {
+      for (int i = 0; i < 8; ++i) x[i] *= factor * w[i];
+    }
+    if (turned) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float other = __shfl_sync(mask, x[i], partner);
-            if (turned) x[i] = x[i] * cs[i] + (second ? other : -other) * sn[i];
-          }
-        }
-        if (!known) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = __int_as_float(0x7fffffff);
-        }
+      for (int i = 0; i < 4; ++i) {
+        const int u = INTERLEAVED ? 2 * i : i, v = INTERLEAVED ? 2 * i + 1 : i + 4;
+        const float xu = x[u], xv = x[v];
+        x[u] = xu * cs[i] - xv * sn[i];
+        x[v] = xv * cs[i] + xu * sn[i];
       }
     }
-    if (kv < 0) {
-      *reinterpret_cast<uint4*>(a.q_out + t * a.q_out_stride + head * D + lane * 8) = pack8(x);
+    if (!known) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = __int_as_float(0x7fffffff);
+    }
+    if (which == 0) {
+      if (real) {
+        __nv_bfloat16* const to = a.q_out + t * a.q_out_stride + head * D;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const __nv_bfloat162 lo = __floats2bfloat162_rn(x[4 * e], x[4 * e + 1]), hi = __floats2bfloat162_rn(x[4 * e + 2], x[4 * e + 3]);
+          *reinterpret_cast<uint2*>(to + dims[e]) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+        }
+      }
       continue;
     }
     // Largest magnitude as bits: unlike the largest float it keeps a NaN.
@@ -142,17 +151,16 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const __grid_constan
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
 #pragma unroll
-    for (int d = kLanes / 2; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(mask, top, d));
+    for (int d = kLanes / 2; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
     const float largest = __uint_as_float(top);
     const float scale = (largest < 1e-12f ? 1e-12f : largest) / 448.0f;
-    uint32_t bytes[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      bytes[i] = cvt_e4m3x2(x[4 * i] / scale, x[4 * i + 1] / scale) | static_cast<uint32_t>(cvt_e4m3x2(x[4 * i + 2] / scale, x[4 * i + 3] / scale)) << 16;
-    const int kind = kv >= kv_heads;
-    uint8_t* block = kv_block<D>(a.cache, slot / kKvPage, kind, kv - kind * kv_heads);
+    if (!real) continue;
+    uint8_t* const block = kv_block<D>(a.cache, slot / kKvPage, which - 1, head);
     const int at = slot % kKvPage;
-    *reinterpret_cast<uint2*>(block + at * D + lane * 8) = make_uint2(bytes[0], bytes[1]);
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      *reinterpret_cast<uint32_t*>(block + at * D + dims[e]) =
+          cvt_e4m3x2(x[4 * e] / scale, x[4 * e + 1] / scale) | static_cast<uint32_t>(cvt_e4m3x2(x[4 * e + 2] / scale, x[4 * e + 3] / scale)) << 16;
     if (lane == 0) *reinterpret_cast<float*>(block + kKvPage * D + at * 4) = scale;
   }
 }
@@ -274,9 +282,10 @@ extern "C" int syfi_kv_write(const void* q, const void* k, const void* v, const 
   a.rotary = rotary_dim;
   a.eps = static_cast<float>(eps);
   // One head per group of lanes while that leaves SMs idle, else a run of them.
-  const int heads = q_heads + kinds * kv_heads, per_block = kThreads / (head_dim / 8);
-  const int each = tokens * heads >= static_cast<int64_t>(sms) * kFullGroups * kWriteHeads ? kWriteHeads : 1;
-  const int64_t groups = tokens * ((heads + each - 1) / each);
+  const int heads = q_heads + kinds * kv_heads;
+  const int each = tokens * heads >= static_cast<int64_t>(sms) * kFullGroups * kWriteHeads ? kWriteHeads : 1, run_heads = 32 / (head_dim / 8) * each;
+  const int64_t groups = tokens * ((q_heads + run_heads - 1) / run_heads + static_cast<int64_t>(kinds) * ((kv_heads + run_heads - 1) / run_heads));
+  const int per_block = kThreads / 32;
   const dim3 grid(static_cast<unsigned>((groups + per_block - 1) / per_block));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto run = [&](auto* kernel) { return launch_dependent(kernel, grid, dim3(kThreads), 0, st, a) == cudaSuccess; };
