@@ -50,7 +50,7 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
 // dimensions, chosen so that it holds both of a rotated pair: lanes below rotary / 8 have chunk l and chunk l + rotary / 8, the others two
 // neighbouring chunks of what is not rotated.  Sum of squares and maximum are shuffles inside the head's lanes.
 template <int D, bool INTERLEAVED, int HEADS>
-__global__ void __launch_bounds__(kThreads) kv_write_kernel(const __grid_constant__ WriteArgs a) {
+__global__ void __launch_bounds__(kThreads, HEADS > 1 ? 5 : 1) kv_write_kernel(const __grid_constant__ WriteArgs a) {
   constexpr int kLanes = D / 8, kGroups = 32 / kLanes, kRun = kGroups * HEADS;
   pdl_wait();
   pdl_trigger();
@@ -155,12 +155,20 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const __grid_constan
     const float largest = __uint_as_float(top);
     const float scale = (largest < 1e-12f ? 1e-12f : largest) / 448.0f;
     if (!real) continue;
+    // x / scale for eight x: the product with the reciprocal and one step with its exact remainder (Markstein), which leaves the quotient
+    // correctly rounded, so that a value half way between two e4m3 neighbours goes where the division would send it
+    const float inverse = 1.0f / scale;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float quotient = x[i] * inverse;
+      x[i] = fmaf(fmaf(-quotient, scale, x[i]), inverse, quotient);
+    }
     uint8_t* const block = kv_block<D>(a.cache, slot / kKvPage, which - 1, head);
     const int at = slot % kKvPage;
 #pragma unroll
     for (int e = 0; e < 2; ++e)
       *reinterpret_cast<uint32_t*>(block + at * D + dims[e]) =
-          cvt_e4m3x2(x[4 * e] / scale, x[4 * e + 1] / scale) | static_cast<uint32_t>(cvt_e4m3x2(x[4 * e + 2] / scale, x[4 * e + 3] / scale)) << 16;
+          cvt_e4m3x2(x[4 * e], x[4 * e + 1]) | static_cast<uint32_t>(cvt_e4m3x2(x[4 * e + 2], x[4 * e + 3])) << 16;
     if (lane == 0) *reinterpret_cast<float*>(block + kKvPage * D + at * 4) = scale;
   }
 }

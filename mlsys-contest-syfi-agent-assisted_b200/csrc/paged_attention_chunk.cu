@@ -69,11 +69,12 @@ struct ChunkShared {
   uint32_t tmem;
   int there[kScaleStages];             // bit p: page p of the tile is there
   int exponent[kScaleStages];          // the values' reference as of the tile: 2^exponent
+  float fade[kScaleStages];            // what it has become smaller by since the tile before (1: nothing)
   float top[2][2][2][128];             // [tile parity][slot][half][row]: a row's largest score in half of a tile; at a segment's end, its sum
   float unit[256];                     // of each row: what a score is worth
   volatile int redo[kSegmentRing];     // of the segment: f16 did not hold a value
   volatile int abort_code;
-  long long wait_limit;                // SM clocks
+  volatile uint32_t most_looks;        // at a barrier in one wait
   int finished;                        // segments of this CTA whose results are written
   int asked_k, asked_v, asked_scales;  // loads that the producer has issued
 };
@@ -214,51 +215,18 @@ __device__ __forceinline__ void exact_row(const AttentionArgs& a, int base, int 
         __floats2bfloat162_rn(acc[2 * i] * inv, acc[2 * i + 1] * inv);
 }
 
-// Waits, bounded like the ones in ptx.cuh, that cost the waiting warps few instructions: the barrier is asked with a long suspend
-// hint, up to 64 times in a row, and only then the clock and the abort flag (half of what a tile issued were the waits before).
-__device__ __forceinline__ bool asked_64_times(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\t"
-      "mov.u32 n, 64;\n"
-      "AGAIN_%=:\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-      "@p bra DONE_%=;\n\t"
-      "sub.u32 n, n, 1;\n\t"
-      "setp.ne.u32 q, n, 0;\n\t"
-      "@q bra AGAIN_%=;\n"
-      "DONE_%=:\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
-      : "memory");
-  return ok != 0u;
-}
+// Waits, bounded like the ones in ptx.cuh, in few instructions: this kernel's roles together have more code than the instruction cache
+// of an SM holds, and its warps spend much of their time in these.  So a wait counts its looks at the barrier (each is suspended for a
+// while by the hardware) and leaves the clock alone; a suspend hint turned into a loop of short sleeps.
 __device__ __forceinline__ bool wait_for(ChunkShared& sh, uint64_t* bar, uint32_t parity) {
-  if (asked_64_times(bar, parity)) return true;
-  const long long t0 = clock64();
-  while (!asked_64_times(bar, parity)) {
+  for (uint32_t looks = 0; !mbar_try_wait(bar, parity); ++looks) {
+    if (looks > sh.most_looks) sh.abort_code = kStatusChunkTimeout;
     if (sh.abort_code != 0) return false;
-    if (clock64() - t0 > sh.wait_limit) {
-      sh.abort_code = kStatusChunkTimeout;
-      return false;
-    }
   }
   return true;
 }
-// The same for warps that have to stay whole: a lane whose wait ran out clears `ok` and goes on.
-__device__ __forceinline__ void wait_whole_warp(ChunkShared& sh, bool& ok, uint64_t* bar, uint32_t parity) {
-  if (asked_64_times(bar, parity)) return;
-  const long long t0 = clock64();
-  while (ok && !asked_64_times(bar, parity)) {
-    if (sh.abort_code != 0) {
-      ok = false;
-    } else if (clock64() - t0 > sh.wait_limit) {
-      sh.abort_code = kStatusChunkTimeout;
-      ok = false;
-    }
-  }
-}
+// The same for warps that have to stay whole: a lane whose wait ran out goes on, and the warp asks for the abort code later.
+__device__ __forceinline__ void wait_whole_warp(ChunkShared& sh, uint64_t* bar, uint32_t parity) { wait_for(sh, bar, parity); }
 
 // A place in a ring of stages: its index, and the parity of its use.
 template <int N>
@@ -456,17 +424,16 @@ __device__ __forceinline__ void convert_role(ChunkShared& sh, uint8_t* smem) {
   Ring<kScaleStages> scales;
   Ring<Shape::kVStages> ahead, raw;          // of the tile looked at, of the tile converted
   Ring<Shape::kHalfStages> halves;
-  bool ok = true;
   int left = 0, n = 0, position0 = 0, any_low = 0, any_high = 0, all_low = 0, all_high = 0, unit = -100, entry = 0;
   // of the tile looked at: what to multiply with (0: no such position), the segment's ring entry, whether the tile is its last
   float r = 0.0f;
   bool keep = false, ends = false;
   auto look = [&]() {                        // false behind the last tile
     if (left == 0) {
-      wait_whole_warp(sh, ok, &sh.segment_full[segments.stage], segments.parity);
+      wait_whole_warp(sh, &sh.segment_full[segments.stage], segments.parity);
       __syncwarp();
       const Segment& g = sh.segment[segments.stage];
-      left = n = __all_sync(0xffffffffu, ok) ? g.tiles : 0;
+      left = n = __any_sync(0xffffffffu, sh.abort_code != 0) ? 0 : g.tiles;
       if (n == 0) return false;
       position0 = g.tile0 * kTile;
       any_low = g.any_low;
@@ -477,19 +444,28 @@ __device__ __forceinline__ void convert_role(ChunkShared& sh, uint8_t* smem) {
       segments.next();
     }
     float* const k_scale = reinterpret_cast<float*>(smem + Shape::kScales) + scales.stage * 2 * kTile;
-    wait_whole_warp(sh, ok, &sh.scale_full[scales.stage], scales.parity);
+    wait_whole_warp(sh, &sh.scale_full[scales.stage], scales.parity);
     __syncwarp();
     const int there = sh.there[scales.stage];
     const int e = tile_exponent(k_scale + kTile, there, position0, any_low, any_high, lane);
-    if (left == n || e > unit + kUnitGrowth) unit = e;
-    if (t == 0) sh.exponent[scales.stage] = unit;
+    float fade = 1.0f;
+    if (left == n) {
+      unit = e;
+    } else if (e > unit + kUnitGrowth) {
+      fade = ex2(static_cast<float>(unit - e));
+      unit = e;
+    }
+    if (t == 0) {
+      sh.exponent[scales.stage] = unit;
+      sh.fade[scales.stage] = fade;
+    }
     const float scale = k_scale[kTile + t];
     keep = (there >> (t / kKvPage) & 1) && position0 + t >= any_low && position0 + t <= any_high;
     r = scale * __int_as_float((kUnitShift - unit + 127) << 23);
     if (position0 < all_low || position0 + kTile - 1 > all_high) {
       // Some rows may see what others do not, and zero times NaN is NaN: the bytes of a value that is not finite become zeros, and the
       // NaN goes by way of its score to the rows that see it.
-      wait_whole_warp(sh, ok, &sh.v_full[ahead.stage], ahead.parity);
+      wait_whole_warp(sh, &sh.v_full[ahead.stage], ahead.parity);
       if (keep) {
         const uint8_t* const from = smem + Shape::kV + ahead.stage * Shape::kTileBytes;
         uint32_t over = 0u;
@@ -519,9 +495,9 @@ __device__ __forceinline__ void convert_role(ChunkShared& sh, uint8_t* smem) {
     const float scale = r;
     const bool valid = keep, last = ends;
     const int segment = entry;
-    wait_whole_warp(sh, ok, &sh.v_full[raw.stage], raw.parity);
+    wait_whole_warp(sh, &sh.v_full[raw.stage], raw.parity);
     more = look();
-    wait_whole_warp(sh, ok, &sh.half_empty[halves.stage], halves.parity ^ 1u);
+    wait_whole_warp(sh, &sh.half_empty[halves.stage], halves.parity ^ 1u);
     __syncwarp();
     const uint8_t* const from = smem + Shape::kV + raw.stage * Shape::kTileBytes;
     uint8_t* const to = smem + Shape::kHalf + halves.stage * Shape::kHalfBytes + t * 128;
@@ -564,7 +540,7 @@ __device__ __forceinline__ void convert_role(ChunkShared& sh, uint8_t* smem) {
       mbar_arrive(&sh.v_empty[raw.stage]);
       if (last) mbar_arrive(&sh.segment_empty[segment]);
     }
-    if (!__all_sync(0xffffffffu, ok)) return;
+    if (__any_sync(0xffffffffu, sh.abort_code != 0)) return;
     raw.next();
     halves.next();
   }
@@ -585,13 +561,13 @@ __device__ __forceinline__ void st_shared_f32(uint32_t at, float v) { asm volati
 
 // One half of a tile's row: 64 scores from tensor memory, their weights back into it, the row's reference m and this half's sum l.  The partner warp has the other 64; the two agree on the row's largest score through shared memory (`top`: this
 // warp's places, `other`: the partner's), and only behind that barrier, when both have read their scores, write weights over them.
-// `fade`: what the values' reference has become smaller by.  low, high: what the row sees, counted from the first of the 64.
+// unit_at, fade_at: where the row's unit and what the values' reference has become smaller by lie.  low, high: what the row sees, counted from the first of the 64.
 template <int D>
-__device__ __forceinline__ void softmax_half(uint32_t t_s, uint32_t t_p, uint32_t t_o, uint32_t k_scale, bool masked, int low, int high, bool there,
-                                             float unit, float fade, bool first, uint32_t top, uint32_t other, int barrier, float& m, float& l) {
+__device__ __forceinline__ void softmax_half(uint32_t t_s, uint32_t t_o, int half, uint32_t k_scale, bool masked, int low, int high, bool there,
+                                             uint32_t unit_at, uint32_t fade_at, bool first, uint32_t top, uint32_t other, int barrier, float& m, float& l) {
   uint32_t s[2][32];
-  tmem_ld32(t_s, s[0]);
-  tmem_ld32(t_s + 32, s[1]);
+  tmem_ld32(t_s + half * 64, s[0]);
+  tmem_ld32(t_s + half * 64 + 32, s[1]);
   tmem_ld_wait_for(s[0]);
   tmem_landed(s[1]);
   // times the keys' scales: in units of the row's
@@ -609,7 +585,7 @@ __device__ __forceinline__ void softmax_half(uint32_t t_s, uint32_t t_p, uint32_
       s[c][4 * e + 3] = __float_as_uint(x3);
     }
   }
-  if (masked) {
+  if (__builtin_expect(masked, 0)) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int first_bit = low - 32 * c, last_bit = high - 32 * c;
@@ -630,6 +606,8 @@ __device__ __forceinline__ void softmax_half(uint32_t t_s, uint32_t t_p, uint32_
   t0 = fmaxf(t0, t1);
   st_shared_f32(top, t0);
   named_bar_sync(barrier, 64);
+  const float unit = ld_shared_f32(unit_at);
+  float fade = ld_shared_f32(fade_at);
   t0 = fmaxf(t0, ld_shared_f32(other)) * unit;
   if (t0 > m + kGrowth) {
     const float f = ex2(m - t0);       // (0 for a row that had seen nothing)
@@ -665,46 +643,56 @@ __device__ __forceinline__ void softmax_half(uint32_t t_s, uint32_t t_p, uint32_
       more += x1;
       p[b] = pack_half2(x0, x1);
     }
-    tmem_st8(t_p + 8 * h, p);
+    tmem_st8(t_s + half * 32 + 8 * h, p);
   }
   l += more;
   tmem_st_wait();
 }
 
-// Sixteen rows of q as two e4m3 terms of q * 2^k each, the row's largest at 2^7 .. 2^8, into the slot's tiles (row0: the first of them in
-// the tile; r0: in the sequence; rows: how many there are).  D / 8 lanes read a row.  units: what a score of each row is worth.
+// Sixteen rows of q (rows0 and on of the warp's 32) as two e4m3 terms of q * 2^k each, the row's largest at 2^7 .. 2^8, into the slot's
+// tiles (row0: the warp's first row in the tile; rows: how many it has; mine: where this lane's row begins in q).  D / 8 lanes read a row,
+// all under way together.  units: what a score of each row is worth.
 template <int D>
-__device__ __forceinline__ void put_queries(const AttentionArgs& a, int q_first, int head, int r0, int rows, uint8_t* hi_tile, int row0, float* units) {
-  constexpr int kLanes = D / 8, kTogether = 32 / kLanes;        // rows at a time
+__device__ __forceinline__ void put_queries(const __nv_bfloat16* q, long long mine, float scale_log2, int rows0, int rows, uint8_t* hi_tile, int row0, float* units) {
+  constexpr int kLanes = D / 8, kTogether = 32 / kLanes, kBatch = 16 / kTogether;      // rows at a time
   const int lane = threadIdx.x % 32, part = lane % kLanes;
-#pragma unroll 2
-  for (int at = 0; at < 16; at += kTogether) {
-    const int row = at + lane / kLanes, r = r0 + row;
-    uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-    if (row < rows) raw = __ldg(reinterpret_cast<const uint4*>(a.q + (q_first + r / a.group) * a.q_stride + (head * a.group + r % a.group) * D) + part);
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-    unsigned top = 0u;
+  {
+    const int at = rows0;
+    uint4 raw[kBatch];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) top = max(top, max(w[e] & 0x7fffu, w[e] >> 16 & 0x7fffu));
-#pragma unroll
-    for (int d = kLanes / 2; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
-    const int k = top == 0u ? 0 : min(7 - (static_cast<int>(top >> 7) - 127), 120);
-    const float up = copysignf(__int_as_float((k + 127) << 23), a.scale_log2);
-    uint32_t hi[2], lo[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const float x0 = __uint_as_float(w[2 * e] << 16) * up, x1 = __uint_as_float(w[2 * e] & 0xffff0000u) * up;
-      const float x2 = __uint_as_float(w[2 * e + 1] << 16) * up, x3 = __uint_as_float(w[2 * e + 1] & 0xffff0000u) * up;
-      const uint16_t h01 = cvt_e4m3x2(x0, x1), h23 = cvt_e4m3x2(x2, x3);
-      const float2 f01 = e4m3x2_to_float2(h01), f23 = e4m3x2_to_float2(h23);
-      hi[e] = h01 | static_cast<uint32_t>(h23) << 16;
-      lo[e] = cvt_e4m3x2(x0 - f01.x, x1 - f01.y) | static_cast<uint32_t>(cvt_e4m3x2(x2 - f23.x, x3 - f23.y)) << 16;
+    for (int b = 0; b < kBatch; ++b) {
+      const int row = at + b * kTogether + lane / kLanes;
+      const long long from = __shfl_sync(0xffffffffu, mine, row);
+      raw[b] = make_uint4(0u, 0u, 0u, 0u);
+      if (row < rows) raw[b] = __ldg(reinterpret_cast<const uint4*>(q + from) + part);
     }
-    uint8_t* const to = hi_tile + swizzled<D>(row0 + row, part / 2) + part % 2 * 8;
-    *reinterpret_cast<uint2*>(to) = make_uint2(hi[0], hi[1]);
-    *reinterpret_cast<uint2*>(to + ChunkShape<D>::kTileBytes) = make_uint2(lo[0], lo[1]);
-    // (a scale of zero keeps a factor, so that -infinity stays what it is)
-    if (part == 0) units[row] = top >= 0x7f80u ? __int_as_float(0x7fffffff) : fmaxf(fabsf(a.scale_log2) * __int_as_float((127 - k) << 23), 1e-30f);
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int row = at + b * kTogether + lane / kLanes;
+      const uint32_t w[4] = {raw[b].x, raw[b].y, raw[b].z, raw[b].w};
+      unsigned top = 0u;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = max(top, max(w[e] & 0x7fffu, w[e] >> 16 & 0x7fffu));
+#pragma unroll
+      for (int d = kLanes / 2; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+      const int k = top == 0u ? 0 : min(7 - (static_cast<int>(top >> 7) - 127), 120);
+      const float up = copysignf(__int_as_float((k + 127) << 23), scale_log2);
+      uint32_t hi[2], lo[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float x0 = __uint_as_float(w[2 * e] << 16) * up, x1 = __uint_as_float(w[2 * e] & 0xffff0000u) * up;
+        const float x2 = __uint_as_float(w[2 * e + 1] << 16) * up, x3 = __uint_as_float(w[2 * e + 1] & 0xffff0000u) * up;
+        const uint16_t h01 = cvt_e4m3x2(x0, x1), h23 = cvt_e4m3x2(x2, x3);
+        const float2 f01 = e4m3x2_to_float2(h01), f23 = e4m3x2_to_float2(h23);
+        hi[e] = h01 | static_cast<uint32_t>(h23) << 16;
+        lo[e] = cvt_e4m3x2(x0 - f01.x, x1 - f01.y) | static_cast<uint32_t>(cvt_e4m3x2(x2 - f23.x, x3 - f23.y)) << 16;
+      }
+      uint8_t* const to = hi_tile + swizzled<D>(row0 + row, part / 2) + part % 2 * 8;
+      *reinterpret_cast<uint2*>(to) = make_uint2(hi[0], hi[1]);
+      *reinterpret_cast<uint2*>(to + ChunkShape<D>::kTileBytes) = make_uint2(lo[0], lo[1]);
+      // (a scale of zero keeps a factor, so that -infinity stays what it is)
+      if (part == 0) units[row] = top >= 0x7f80u ? __int_as_float(0x7fffffff) : fmaxf(fabsf(scale_log2) * __int_as_float((127 - k) << 23), 1e-30f);
+    }
   }
 }
 
@@ -715,83 +703,81 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, slot = warp / 8, half = warp / 4 % 2, in_slot = warp % 4 * 32 + lane;
   const int row = slot * 128 + in_slot, pair = 2 + slot * 4 + warp % 4;        // named barrier of the two warps of a row
   const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
-  const uint32_t t_s = tmem + lanes + slot * 128, t_o = tmem + lanes + 256 + slot * 128 + half * (D / 2);
-  Ring<kSegmentRing> segments;
-  Ring<kScaleStages> scales;
-  uint32_t tile_parity = 0, segment_parity = 0;     // of this slot
-  bool ok = true;
+  const uint32_t t_s = tmem + lanes + slot * 128, t_o = t_s + 256 + half * (D / 2), scales0 = smem_u32(smem) + Shape::kScales + half * 256;
+  static_assert(kSegmentRing == 4 && kScaleStages == 4, "stage and parity are bits of a counter");
+  uint32_t segment = 0, tile = 0, own = 0, own_segments = 0;       // segments and tiles so far, and those of this slot
+  int exponent = 0;
   while (true) {
-    wait_whole_warp(sh, ok, &sh.segment_full[segments.stage], segments.parity);
-    if (softmax_bar_any(!ok)) return;         // all sixteen warps meet here whatever failed, and leave together
-    const Segment& g = sh.segment[segments.stage];
-    const int n = g.tiles;
-    if (n == 0) return;
+    wait_whole_warp(sh, &sh.segment_full[segment & 3], segment >> 2 & 1);
+    if (softmax_bar_any(sh.abort_code != 0)) return;      // all sixteen warps meet here whatever failed, and leave together
+    const Segment& g = sh.segment[segment & 3];
+    if (g.tiles == 0) return;
     const bool active = slot * 128 < g.rows;
-    float m = -INFINITY;
-    float l = 0.0f;
-    int exponent = 0;
+    float m = -INFINITY, l = 0.0f;
+    int token_of_row = 0, column_of_row = 0;         // of this thread's row, in q and out
     {
       int low, high;
       {
-        const int token = (g.row0 + min(row, g.rows - 1)) / a.group;        // (rows beyond the last copy its bounds)
+        const int r = g.row0 + min(row, g.rows - 1), token = r / a.group;        // (rows beyond the last copy its bounds)
+        token_of_row = g.q_first + token;
+        column_of_row = (g.head * a.group + r - token * a.group) * D;
         high = g.base + token;
         low = a.window > 0 ? max(high - a.window + 1, 0) : 0;
       }
-      float unit = 0.0f;
       if (active) {
-        const int first = slot * 128 + warp % 4 * 32 + half * 16;
-        put_queries<D>(a, g.q_first, g.head, g.row0 + first, g.rows - first, smem + Shape::kQ + 2 * slot * Shape::kTileBytes, first % 128, sh.unit + first);
+        const int row0 = slot * 128 + warp % 4 * 32;
+        put_queries<D>(a.q, token_of_row * a.q_stride + column_of_row, a.scale_log2, half * 16, g.rows - row0, smem + Shape::kQ + 2 * slot * Shape::kTileBytes,
+                       row0 % 128, sh.unit + row0);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.q_full[slot]);
         named_bar_sync(pair, 64);
-        unit = sh.unit[row];
       }
       // from here on positions count from the first of this warp's half of the segment's first tile
       const int position0 = g.tile0 * kTile + half * 64;
       low -= position0;
       high -= position0;
-      for (int j = 0; j < n; ++j) {
-        wait_whole_warp(sh, ok, &sh.scale_full[scales.stage], scales.parity);
-        wait_whole_warp(sh, ok, &sh.scale_clean[scales.stage], scales.parity);
+      bool first = true;
+      for (int left = g.tiles; left > 0; --left) {
+        const int stage = tile & 3;
+        wait_whole_warp(sh, &sh.scale_full[stage], tile >> 2 & 1);
+        wait_whole_warp(sh, &sh.scale_clean[stage], tile >> 2 & 1);
         if (active) {
-          const bool there = sh.there[scales.stage] >> half & 1;
-          const int e = sh.exponent[scales.stage];
-          const float fade = j == 0 ? 1.0f : ex2(static_cast<float>(exponent - e));
-          exponent = e;
-          wait_whole_warp(sh, ok, &sh.s_full[slot], tile_parity);
+          wait_whole_warp(sh, &sh.s_full[slot], own & 1);
           __syncwarp();
           tc_fence_after();
-          const uint32_t top = smem_u32(&sh.top[tile_parity][slot][0][in_slot]);
-          softmax_half<D>(t_s + half * 64, t_s + half * 32, t_o, smem_u32(smem) + Shape::kScales + (scales.stage * 2 * kTile + half * 64) * 4,
-                          !there || __any_sync(0xffffffffu, low > 0 || high < 63), low, high, there, unit, fade, j == 0, top + half * 512,
-                          top + (half ^ 1) * 512, pair, m, l);
+          const bool there = sh.there[stage] >> half & 1;
+          const uint32_t top = smem_u32(&sh.top[own & 1][slot][0][in_slot]);
+          softmax_half<D>(t_s, t_o, half, scales0 + stage * (2 * kTile * 4), !there || __any_sync(0xffffffffu, low > 0 || high < 63), low, high, there,
+                          smem_u32(&sh.unit[row]), smem_u32(&sh.fade[stage]), first, top + half * 512, top + (half ^ 1) * 512, pair, m, l);
           tc_fence_before();
+          if (left == 1) exponent = sh.exponent[stage];
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh.p_full[slot]);
-          tile_parity ^= 1u;
+          ++own;
+          first = false;
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.scale_empty[scales.stage]);
-        scales.next();
+        if (lane == 0) mbar_arrive(&sh.scale_empty[stage]);
+        ++tile;
         low -= kTile;
         high -= kTile;
         // (a warp that failed keeps its partner company at their barrier until the segment's end)
       }
       // ---- the segment's end
       if (active) {
-        wait_whole_warp(sh, ok, &sh.o_full[slot], segment_parity);
+        wait_whole_warp(sh, &sh.o_full[slot], own_segments & 1);
         __syncwarp();
         tc_fence_after();
-        segment_parity ^= 1u;
-        sh.top[tile_parity][slot][half][in_slot] = l;
+        ++own_segments;
+        sh.top[own & 1][slot][half][in_slot] = l;
       }
     }
-    if (softmax_bar_any(!ok)) return;
-    const bool redo = sh.redo[segments.stage] != 0, whole = g.whole, real = row < g.rows;
-    if (tid == 0) sh.redo[(segments.stage + kSegmentRing - 1) % kSegmentRing] = 0;     // the segment before: everybody has read it
+    if (softmax_bar_any(sh.abort_code != 0)) return;
+    const bool redo = sh.redo[segment & 3] != 0, whole = g.whole, real = row < g.rows;
+    if (tid == 0) sh.redo[(segment + 3) & 3] = 0;     // the segment before: everybody has read it
     if (active) {
-      l = sh.top[tile_parity][slot][0][in_slot] + sh.top[tile_parity][slot][1][in_slot];
+      l = sh.top[own & 1][slot][0][in_slot] + sh.top[own & 1][slot][1][in_slot];
       const float unscale = __int_as_float((exponent - kUnitShift + 127) << 23);
       const float f = whole ? (l == 0.0f ? 0.0f : unscale / l) : unscale;
       // Rows leave through the slot's q tiles, which nothing reads any more: 32 rows of D bytes per warp (half of the dimensions), swizzled,
@@ -800,34 +786,39 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
       float4* const to = reinterpret_cast<float4*>(a.partial);
       const int part = parts_of(g).slot(static_cast<int>(blockIdx.x));
 #pragma unroll 1
-      for (int c = 0; c < D / 16; ++c) {
-        uint32_t o[8];
-        tmem_ld8(t_o + 8 * c, o);
+      for (int c = 0; c < D / 16; c += 2) {
+        uint32_t o[16];
+        tmem_ld16(t_o + 8 * c, o);
         tmem_ld_wait_for(o);
-        if (whole) {
-          uint32_t w[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(o[2 * e]) * f, __uint_as_float(o[2 * e + 1]) * f);
-            w[e] = *reinterpret_cast<const uint32_t*>(&h);
+        for (int b = 0; b < 2; ++b) {
+          if (whole) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(o[8 * b + 2 * e]) * f, __uint_as_float(o[8 * b + 2 * e + 1]) * f);
+              w[e] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+            *reinterpret_cast<uint4*>(stage + lane * D + ((D == 128 ? (c + b) ^ (lane & 7) : (c + b) ^ (lane >> 1 & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          } else if (real) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              to[(static_cast<long long>(part) * (D / 4) + half * (D / 8) + 2 * (c + b) + e) * kChunkRows + row] =
+                  make_float4(__uint_as_float(o[8 * b + 4 * e]) * f, __uint_as_float(o[8 * b + 4 * e + 1]) * f, __uint_as_float(o[8 * b + 4 * e + 2]) * f,
+                              __uint_as_float(o[8 * b + 4 * e + 3]) * f);
           }
-          *reinterpret_cast<uint4*>(stage + lane * D + ((D == 128 ? c ^ (lane & 7) : c ^ (lane >> 1 & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-        } else if (real) {
-#pragma unroll
-          for (int b = 0; b < 2; ++b)
-            to[(static_cast<long long>(part) * (D / 4) + half * (D / 8) + 2 * c + b) * kChunkRows + row] =
-                make_float4(__uint_as_float(o[4 * b]) * f, __uint_as_float(o[4 * b + 1]) * f, __uint_as_float(o[4 * b + 2]) * f, __uint_as_float(o[4 * b + 3]) * f);
         }
       }
       if (whole && !redo) {
         __syncwarp();
         constexpr int kLanes = D / 16, kTogether = 32 / kLanes;
-#pragma unroll 2
+        const long long mine = token_of_row * a.out_stride + column_of_row + half * (D / 2);
+#pragma unroll 4
         for (int at = 0; at < 32; at += kTogether) {
-          const int line = at + lane / kLanes, x = slot * 128 + warp % 4 * 32 + line, r = g.row0 + x;
+          const int line = at + lane / kLanes;
+          const long long begin = __shfl_sync(0xffffffffu, mine, line);
           const uint4 p = *reinterpret_cast<const uint4*>(stage + line * D + ((D == 128 ? (lane % kLanes) ^ (line & 7) : (lane % kLanes) ^ (line >> 1 & 3)) << 4));
-          if (x < g.rows)
-            *(reinterpret_cast<uint4*>(a.out + (g.q_first + r / a.group) * a.out_stride + (g.head * a.group + r % a.group) * D + half * (D / 2)) + lane % kLanes) = p;
+          if (slot * 128 + warp % 4 * 32 + line < g.rows) *(reinterpret_cast<uint4*>(a.out + begin) + lane % kLanes) = p;
         }
       }
       if (real && !whole && half == 0)
@@ -862,8 +853,8 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
     // (the q tiles are written again behind this: by this warp's rows' own stage only when both warps of a row are through)
     if (active) named_bar_sync(10 + slot, 256);
     __syncwarp();
-    if (lane == 0) mbar_arrive(&sh.segment_empty[segments.stage]);
-    segments.next();
+    if (lane == 0) mbar_arrive(&sh.segment_empty[segment & 3]);
+    ++segment;
   }
 }
 
@@ -916,7 +907,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
       sh.redo[i] = 0;
     }
     sh.abort_code = 0;
-    sh.wait_limit = wait_limit;
+    sh.most_looks = static_cast<uint32_t>(min(wait_limit / 64, 0xffffff00ll));
     sh.finished = 0;
     sh.asked_k = sh.asked_v = sh.asked_scales = 0;
     fence_barrier_init();
