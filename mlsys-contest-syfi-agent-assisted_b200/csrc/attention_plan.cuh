@@ -5,7 +5,8 @@
 // key head side by side), over the tiles of TILE positions that any of them sees.  All units' tiles, in the order sequence, row
 // tile, head, tile, are one line that is cut into equal pieces, one per CTA; so a piece has at most a unit's end, some whole
 // units and a unit's beginning, whatever the lengths are.  In front of a unit's tiles the line has EXTRA places that stand for
-// what a unit costs besides its tiles.  A unit that lies in one piece is finished there.  Else each of its CTAs leaves a partial
+// what a unit costs besides its tiles.  Units of at most NARROW rows go through two tiles in the time of one: to the line their tiles
+// are twice as long.  A unit that lies in one piece is finished there.  Else each of its CTAs leaves a partial
 // result, and the one that comes last (a counter per unit) adds them up, in the order of the pieces.
 #pragma once
 #include "kv_internal.h"
@@ -24,7 +25,7 @@ struct Span {
   int first, tiles;                 // tiles of positions; at least one
 };
 
-template <int TILE, int ROWS, int EXTRA>
+template <int TILE, int ROWS, int EXTRA, int NARROW = 0>
 struct Plan {
   const KvBatch& batch;
   int heads, group, window;
@@ -35,7 +36,8 @@ struct Plan {
     const int row0 = rt * ROWS, row1 = min(s.count * group, row0 + ROWS) - 1;
     const int base = s.length - s.count, high = base + row1 / group;
     const int low = window > 0 ? max(base + row0 / group - window + 1, 0) : 0;
-    return high < low ? Span{0, 1} : Span{low / TILE, high / TILE - low / TILE + 1};
+    const int tile = row1 - row0 < NARROW ? 2 * TILE : TILE;
+    return high < low ? Span{0, 1} : Span{low / tile, high / tile - low / tile + 1};
   }
   __device__ long long tiles_of_warp(const KvSequence& s, int lane) const {     // a head's places of all row tiles; whole warp
     const int n = s.count > 0 ? row_tiles(s) : 0;
@@ -132,7 +134,7 @@ struct Plan {
 };
 
 // A walk over the tiles of a piece of the line.  The same in every thread of a block.
-template <int TILE, int ROWS, int EXTRA>
+template <int TILE, int ROWS, int EXTRA, int NARROW = 0>
 struct Cursor {
   int b, rt, head, tile;             // tile of the unit, counted from 0
   int left;                          // places of the piece from this tile on; none: the walk is over
@@ -140,7 +142,7 @@ struct Cursor {
   Span span;
   int row_tiles;
 
-  __device__ void start(const Plan<TILE, ROWS, EXTRA>& plan, const PlanShared& sh, int places) {
+  __device__ void start(const Plan<TILE, ROWS, EXTRA, NARROW>& plan, const PlanShared& sh, int places) {
     b = sh.start_b;
     rt = sh.start_rt;
     head = sh.start_head;
@@ -152,7 +154,7 @@ struct Cursor {
     left = places - skipped;
   }
   // To the next unit, if the piece has any of its tiles.
-  __device__ void next_unit(const Plan<TILE, ROWS, EXTRA>& plan) {
+  __device__ void next_unit(const Plan<TILE, ROWS, EXTRA, NARROW>& plan) {
     left -= EXTRA;
     if (left <= 0) return;
     tile = 0;
@@ -172,7 +174,7 @@ struct Cursor {
     span = plan.span(s, rt);
   }
   // `n` tiles of the unit on; behind its last to the next unit.
-  __device__ void advance(const Plan<TILE, ROWS, EXTRA>& plan, int n) {
+  __device__ void advance(const Plan<TILE, ROWS, EXTRA, NARROW>& plan, int n) {
     tile += n;
     left -= n;
     if (tile == span.tiles && left > 0) next_unit(plan);

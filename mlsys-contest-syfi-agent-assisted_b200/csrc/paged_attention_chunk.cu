@@ -4,14 +4,21 @@
 //   S = Q K^T   tcgen05.mma kind::f8f6f4 straight from the cache's e4m3 bytes as TMA brings them.  A row of q, scaled by a power of two, is
 //               the sum of two e4m3 terms: a bf16 value has 8 significant bits, an e4m3 term 4, so the two hold it exactly as long
 //               as it is not 2^-9 of the row's largest (then to 2^-17 of that).  Both terms add into one accumulator.
-//   P           softmax warps, a thread per row: the weights in f16 (2^-12 of each on average), back into tensor memory over S.
+//   P           softmax warps, a lane per row and a warp per half of the tile's positions: the weights in f16 (2^-12 of each on average),
+//               back into tensor memory over S.
 //   O += P V    kind::f16, P from tensor memory, V as f16 in shared memory.  Four warps make it from the bytes: e4m3 times the position's
 //               scale relative to the unit's (a power of two that follows the largest scale met), rounded once to f16.
-// The slots are out of step by half a tile: while the softmax warps of one work, the tensor core works for the other.
+// The slots are out of step by half a tile: while the softmax warps of one work, the tensor core works for the other.  A unit of at most
+// 128 rows has them in both slots, which take turns at the tiles and add their sums up at the end; with one slot at work the chain of
+// scores, weights and product, 5000 clocks for a tile, stood still in between (24 sequences of 300 .. 30000 positions, 8 rows per key head:
+// 178 us, in turns 141).
 //
 // The sum's reference follows a row's largest score only when that has grown by 2^8 (kGrowth), so O is hardly ever rescaled.
 // What f16 cannot hold is computed again: a unit that meets a value scale below 2^-19 of the largest is redone row by row in f32
 // (exact_row).
+//
+// What bounds it is that chain: a wide tile of 256 rows takes 5200 clocks, of which the tensor core works 2048 and the exponentials 2048
+// (16 per clock).  A prompt of 8192 tokens, 32 heads of 128 over 8: 704 us, 781 TFLOP/s of the causal half.
 #include "attention_common.cuh"
 #include "stream_scratch.h"
 
@@ -21,12 +28,16 @@ namespace {
 
 constexpr int kTile = 128;             // positions per tile: two pages
 constexpr int kChunkRows = 256;
-constexpr int kChunkThreads = 768;      // 16 softmax warps, 4 converting ones, then MMAs, loads, planning, none
+constexpr int kChunkThreads = 768;     // 16 softmax warps, 4 converting ones, then MMAs, loads, planning, scales
 constexpr int kSoftmaxWarps = 16, kSoftmaxThreads = 512;
 constexpr int kChunkExtra = 3;         // what a unit costs besides its tiles, in tiles
+constexpr int kSlotRows = 128;         // units of at most so many rows use one slot for their even tiles and one for their odd ones
+using ChunkPlan = Plan<kTile, kChunkRows, kChunkExtra, kSlotRows>;
+using ChunkCursor = Cursor<kTile, kChunkRows, kChunkExtra, kSlotRows>;
 constexpr int kScaleStages = 4;
 constexpr int kRedoWarps = 4;          // of the softmax warps, redo rows
 constexpr int kStatusChunkTimeout = 301;
+constexpr int kNoValue = 0x7fffffff;   // in a key's scale: a NaN, and its value's bytes are not looked at
 constexpr int kUnitShift = 5;          // the largest value scale becomes 2^4 .. 2^5 when the unit's reference is set, ...
 constexpr int kUnitGrowth = 2;         // ... and may grow to 2^7 (448 * 2^7 < 65504) before the reference follows
 constexpr float kSmallestUnit = 6.103515625e-5f;   // 2^-14: f16's smallest normal number
@@ -55,11 +66,12 @@ struct Segment {
   int base;                            // position of the sequence's first query
   int any_low, any_high, all_low, all_high;   // positions that any / all of the rows see
   int whole;                           // the unit lies in this piece alone
+  int turns;                           // rows 0 .. 127 are in both slots, which take turns at the tiles
   int first_part, last_part, first_slot;   // else: its Parts
 };
 __device__ __forceinline__ Parts parts_of(const Segment& g) { return {g.first_part, g.last_part, g.first_slot}; }
 constexpr int kSegmentRing = 4;
-constexpr int kSegmentReaders = 2 + 4 + kSoftmaxWarps;    // arrivals that free an entry: loads, MMAs, converting and softmax warps
+constexpr int kSegmentReaders = 3 + 4 + kSoftmaxWarps;    // arrivals that free an entry: loads, MMAs, scales, converting and softmax warps
 
 struct ChunkShared {
   Segment segment[kSegmentRing];
@@ -69,8 +81,9 @@ struct ChunkShared {
   uint32_t tmem;
   int there[kScaleStages];             // bit p: page p of the tile is there
   int exponent[kScaleStages];          // the values' reference as of the tile: 2^exponent
-  float fade[kScaleStages];            // what it has become smaller by since the tile before (1: nothing)
-  float top[2][2][2][128];             // [tile parity][slot][half][row]: a row's largest score in half of a tile; at a segment's end, its sum
+  float fade[kScaleStages];            // what it has become smaller by since the slot's tile before (1: nothing)
+  float top[2][2][2][128];             // [tile parity][slot][half][row]: a row's largest score in half of a tile
+  float end[2][3][128];                // [slot][sum of each half, reference][row], at a segment's end
   float unit[256];                     // of each row: what a score is worth
   volatile int redo[kSegmentRing];     // of the segment: f16 did not hold a value
   volatile int abort_code;
@@ -242,31 +255,39 @@ struct Ring {
 };
 
 // ---------------------------------------------------------------- planning (one thread)
-__device__ __forceinline__ void plan_role(const AttentionArgs& a, const Plan<kTile, kChunkRows, kChunkExtra>& plan, const PlanShared& s_plan, ChunkShared& sh, int places,
+__device__ __forceinline__ void plan_role(const AttentionArgs& a, const ChunkPlan& plan, const PlanShared& s_plan, ChunkShared& sh, int places,
                                           long long w1, long long total, int ctas) {
-  Cursor<kTile, kChunkRows, kChunkExtra> at;
+  ChunkCursor at;
   at.start(plan, s_plan, places);
   Ring<kSegmentRing> ring;
   while (true) {
     if (!wait_for(sh, &sh.segment_empty[ring.stage], ring.parity ^ 1u)) return;
     Segment& g = sh.segment[ring.stage];
     const bool more = at.left > 0;
-    g.tiles = more ? at.tiles_here() : 0;
+    const int places = more ? at.tiles_here() : 0;
+    g.tiles = 0;
     if (more) {
       const int rows = at.rows(a.group), base = at.s.length - at.s.count, row0 = at.rt * kChunkRows;
       const int first = base + row0 / a.group, last = base + (row0 + rows - 1) / a.group;
+      g.any_low = a.window > 0 ? max(first - a.window + 1, 0) : 0;
+      g.any_high = last;
       g.tile0 = at.span.first + at.tile;
+      g.tiles = places;
+      if (rows <= kSlotRows) {             // places of two tiles, of which the unit's ends may want one
+        const int end = min(2 * (g.tile0 + places), last / kTile + 1);
+        g.tile0 = max(2 * g.tile0, g.any_low / kTile);
+        g.tiles = max(end - g.tile0, 1);
+      }
+      g.turns = rows <= kSlotRows && g.tiles > 1;
       g.rows = rows;
       g.row0 = row0;
       g.head = at.head;
       g.b = at.b;
       g.q_first = at.s.first;
       g.base = base;
-      g.any_low = a.window > 0 ? max(first - a.window + 1, 0) : 0;
-      g.any_high = last;
       g.all_low = a.window > 0 ? max(last - a.window + 1, 0) : 0;
       g.all_high = first;
-      g.whole = g.tiles == at.span.tiles;
+      g.whole = places == at.span.tiles;
       const Parts parts(total, ctas, w1 - at.left - at.tile, at.span.tiles);
       g.first_part = parts.first;
       g.last_part = parts.last;
@@ -275,7 +296,7 @@ __device__ __forceinline__ void plan_role(const AttentionArgs& a, const Plan<kTi
     mbar_arrive(&sh.segment_full[ring.stage]);
     if (!more) return;
     ring.next();
-    at.advance(plan, g.tiles);
+    at.advance(plan, places);
   }
 }
 
@@ -377,12 +398,45 @@ __device__ __forceinline__ void mma_role(ChunkShared& sh, uint8_t* smem, uint32_
   uint32_t tile_parity = 0, segment_parity = 0;    // bit s: of slot s
   while (true) {
     if (!wait_for(sh, &sh.segment_full[segments.stage], segments.parity)) return;
-    const int n = sh.segment[segments.stage].tiles, slots = sh.segment[segments.stage].rows > 128 ? 2 : 1;
+    const Segment& g = sh.segment[segments.stage];
+    const int n = g.tiles, turns = g.turns, slots = turns || g.rows > kSlotRows ? 2 : 1;
     if (n == 0) return;
     mbar_arrive(&sh.segment_empty[segments.stage]);
     segments.next();
     for (int s = 0; s < slots; ++s)
       if (!wait_for(sh, &sh.q_full[s], segment_parity >> s & 1u)) return;
+    // A slot's scores of its next tile follow its values' product, which reads the weights in their place.
+    if (turns) {                             // tile j in slot j % 2
+      for (int j = 0; j < 2; ++j) {
+        if (!wait_for(sh, &sh.k_full[keys.stage], keys.parity)) return;
+        tc_fence_after();
+        scores(j, keys.stage);
+        umma_commit(&sh.k_empty[keys.stage]);
+        keys.next();
+      }
+      for (int j = 0; j < n; ++j) {
+        const int s = j & 1;
+        const bool more = j + 2 < n;
+        if (j < 2 && !wait_for(sh, &sh.o_empty[s], (segment_parity >> s & 1u) ^ 1u)) return;
+        if (!wait_for(sh, &sh.half_full[halves.stage], halves.parity)) return;
+        if (!wait_for(sh, &sh.p_full[s], tile_parity >> s & 1u)) return;
+        tile_parity ^= 1u << s;
+        tc_fence_after();
+        values(s, halves.stage, j < 2 ? 0u : 1u);
+        umma_commit(&sh.half_empty[halves.stage]);
+        halves.next();
+        if (more) {
+          if (!wait_for(sh, &sh.k_full[keys.stage], keys.parity)) return;
+          scores(s, keys.stage);
+          umma_commit(&sh.k_empty[keys.stage]);
+          keys.next();
+        } else {
+          umma_commit(&sh.o_full[s]);
+        }
+      }
+      segment_parity ^= 3u;
+      continue;
+    }
     if (!wait_for(sh, &sh.k_full[keys.stage], keys.parity)) return;
     tc_fence_after();
     for (int s = 0; s < slots; ++s) scores(s, keys.stage);
@@ -413,140 +467,145 @@ __device__ __forceinline__ void mma_role(ChunkShared& sh, uint8_t* smem, uint32_
   }
 }
 
+// ---------------------------------------------------------------- scales (one warp)
+// Looks at a tile's scales as soon as they are there, ahead of the warps that use them.
+template <int D>
+__device__ __forceinline__ void scale_role(ChunkShared& sh, uint8_t* smem) {
+  using Shape = ChunkShape<D>;
+  const int lane = threadIdx.x % 32;
+  Ring<kSegmentRing> segments;
+  Ring<kScaleStages> scales;
+  Ring<Shape::kVStages> values;
+  int unit = -100, unit_before = -100;
+  while (true) {
+    wait_whole_warp(sh, &sh.segment_full[segments.stage], segments.parity);
+    __syncwarp();
+    const Segment& g = sh.segment[segments.stage];
+    const int n = __any_sync(0xffffffffu, sh.abort_code != 0) ? 0 : g.tiles;
+    if (n == 0) return;
+    int position0 = g.tile0 * kTile;
+    const int any_low = g.any_low, any_high = g.any_high, all_low = g.all_low, all_high = g.all_high, turns = g.turns;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.segment_empty[segments.stage]);
+    segments.next();
+    for (int j = 0; j < n; ++j, position0 += kTile) {
+      float* const k_scale = reinterpret_cast<float*>(smem + Shape::kScales) + scales.stage * 2 * kTile;
+      wait_whole_warp(sh, &sh.scale_full[scales.stage], scales.parity);
+      __syncwarp();
+      const int there = sh.there[scales.stage];
+      const int e = tile_exponent(k_scale + kTile, there, position0, any_low, any_high, lane);
+      const int before = turns ? unit_before : unit;      // as of the tile that the same slot had last
+      unit_before = unit;
+      if (j == 0 || e > unit + kUnitGrowth) unit = e;
+      if (lane == 0) {
+        sh.exponent[scales.stage] = unit;
+        sh.fade[scales.stage] = before == unit ? 1.0f : ex2(static_cast<float>(before - unit));     // (nothing uses a slot's first)
+      }
+      if (position0 < all_low || position0 + kTile - 1 > all_high) {
+        // Some rows may see what others do not, and zero times NaN is NaN: the bytes of a value that is not finite are taken for zeros, and
+        // the NaN goes by way of its score to the rows that see it.
+        wait_whole_warp(sh, &sh.v_full[values.stage], values.parity);
+        const uint8_t* const from = smem + Shape::kV + values.stage * Shape::kTileBytes;
+#pragma unroll 1
+        for (int t = lane; t < kTile; t += 32) {
+          if (!(there >> (t / kKvPage) & 1) || position0 + t < any_low || position0 + t > any_high) continue;
+          uint32_t over = 0u;
+#pragma unroll
+          for (int chunk = 0; chunk < D / 16; ++chunk) {
+            const uint4 p = *reinterpret_cast<const uint4*>(from + swizzled<D>(t, chunk));
+            over |= ((p.x & 0x7f7f7f7fu) + 0x01010101u) | ((p.y & 0x7f7f7f7fu) + 0x01010101u) | ((p.z & 0x7f7f7f7fu) + 0x01010101u) | ((p.w & 0x7f7f7f7fu) + 0x01010101u);
+          }
+          if ((over & 0x80808080u) != 0u || !(fabsf(k_scale[kTile + t]) <= 3.402823466e38f)) k_scale[t] = __int_as_float(kNoValue);
+        }
+        fence_proxy_async_smem();              // in front of the copy that fills these scales next
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.scale_clean[scales.stage]);
+      scales.next();
+      values.next();
+    }
+  }
+}
+
 // ---------------------------------------------------------------- values to f16, a thread per position (four warps)
-// The scales of a tile are looked at one tile ahead of its conversion, which has to wait for the MMAs of the tile before the last:
-// the softmax warps wait for the scales.
 template <int D>
 __device__ __forceinline__ void convert_role(ChunkShared& sh, uint8_t* smem) {
   using Shape = ChunkShape<D>;
   const int t = threadIdx.x - kSoftmaxThreads, lane = threadIdx.x % 32;
   Ring<kSegmentRing> segments;
   Ring<kScaleStages> scales;
-  Ring<Shape::kVStages> ahead, raw;          // of the tile looked at, of the tile converted
+  Ring<Shape::kVStages> raw;
   Ring<Shape::kHalfStages> halves;
-  int left = 0, n = 0, position0 = 0, any_low = 0, any_high = 0, all_low = 0, all_high = 0, unit = -100, entry = 0;
-  // of the tile looked at: what to multiply with (0: no such position), the segment's ring entry, whether the tile is its last
-  float r = 0.0f;
-  bool keep = false, ends = false;
-  auto look = [&]() {                        // false behind the last tile
-    if (left == 0) {
-      wait_whole_warp(sh, &sh.segment_full[segments.stage], segments.parity);
+  while (true) {
+    wait_whole_warp(sh, &sh.segment_full[segments.stage], segments.parity);
+    __syncwarp();
+    const Segment& g = sh.segment[segments.stage];
+    const int n = __any_sync(0xffffffffu, sh.abort_code != 0) ? 0 : g.tiles;
+    if (n == 0) return;
+    int position = g.tile0 * kTile + t;
+    const int any_low = g.any_low, any_high = g.any_high;
+    for (int j = 0; j < n; ++j, position += kTile) {
+      const float* const k_scale = reinterpret_cast<const float*>(smem + Shape::kScales) + scales.stage * 2 * kTile;
+      wait_whole_warp(sh, &sh.scale_clean[scales.stage], scales.parity);
+      // what to multiply with; where there is no such value, zeros
+      const float scale = k_scale[kTile + t] * __int_as_float((kUnitShift - sh.exponent[scales.stage] + 127) << 23);
+      const bool valid = (sh.there[scales.stage] >> (t / kKvPage) & 1) && position >= any_low && position <= any_high && __float_as_int(k_scale[t]) != kNoValue;
       __syncwarp();
-      const Segment& g = sh.segment[segments.stage];
-      left = n = __any_sync(0xffffffffu, sh.abort_code != 0) ? 0 : g.tiles;
-      if (n == 0) return false;
-      position0 = g.tile0 * kTile;
-      any_low = g.any_low;
-      any_high = g.any_high;
-      all_low = g.all_low;
-      all_high = g.all_high;
-      entry = segments.stage;
-      segments.next();
-    }
-    float* const k_scale = reinterpret_cast<float*>(smem + Shape::kScales) + scales.stage * 2 * kTile;
-    wait_whole_warp(sh, &sh.scale_full[scales.stage], scales.parity);
-    __syncwarp();
-    const int there = sh.there[scales.stage];
-    const int e = tile_exponent(k_scale + kTile, there, position0, any_low, any_high, lane);
-    float fade = 1.0f;
-    if (left == n) {
-      unit = e;
-    } else if (e > unit + kUnitGrowth) {
-      fade = ex2(static_cast<float>(unit - e));
-      unit = e;
-    }
-    if (t == 0) {
-      sh.exponent[scales.stage] = unit;
-      sh.fade[scales.stage] = fade;
-    }
-    const float scale = k_scale[kTile + t];
-    keep = (there >> (t / kKvPage) & 1) && position0 + t >= any_low && position0 + t <= any_high;
-    r = scale * __int_as_float((kUnitShift - unit + 127) << 23);
-    if (position0 < all_low || position0 + kTile - 1 > all_high) {
-      // Some rows may see what others do not, and zero times NaN is NaN: the bytes of a value that is not finite become zeros, and the
-      // NaN goes by way of its score to the rows that see it.
-      wait_whole_warp(sh, &sh.v_full[ahead.stage], ahead.parity);
-      if (keep) {
-        const uint8_t* const from = smem + Shape::kV + ahead.stage * Shape::kTileBytes;
-        uint32_t over = 0u;
-#pragma unroll 1
-        for (int chunk = 0; chunk < D / 16; ++chunk) {
-          const uint4 p = *reinterpret_cast<const uint4*>(from + swizzled<D>(t, chunk));
-          over |= ((p.x & 0x7f7f7f7fu) + 0x01010101u) | ((p.y & 0x7f7f7f7fu) + 0x01010101u) | ((p.z & 0x7f7f7f7fu) + 0x01010101u) | ((p.w & 0x7f7f7f7fu) + 0x01010101u);
-        }
-        keep = (over & 0x80808080u) == 0u && fabsf(scale) <= 3.402823466e38f;
-        if (!keep) k_scale[t] = __int_as_float(0x7fffffff);
-      }
-      fence_proxy_async_smem();              // in front of the copy that fills these scales next
-    }
-    __syncwarp();
-    if (lane == 0) {
-      mbar_arrive(&sh.scale_clean[scales.stage]);
-      mbar_arrive(&sh.scale_empty[scales.stage]);
-    }
-    scales.next();
-    ahead.next();
-    position0 += kTile;
-    ends = --left == 0;
-    return true;
-  };
-  bool more = look();
-  while (more) {
-    const float scale = r;
-    const bool valid = keep, last = ends;
-    const int segment = entry;
-    wait_whole_warp(sh, &sh.v_full[raw.stage], raw.parity);
-    more = look();
-    wait_whole_warp(sh, &sh.half_empty[halves.stage], halves.parity ^ 1u);
-    __syncwarp();
-    const uint8_t* const from = smem + Shape::kV + raw.stage * Shape::kTileBytes;
-    uint8_t* const to = smem + Shape::kHalf + halves.stage * Shape::kHalfBytes + t * 128;
-    if (valid) {
-      // the factor as two f16 terms, so that the product with a byte's value is rounded once
-      const __half hi = __float2half_rn(scale);
-      const __half2 r_hi = __half2half2(hi), r_lo = __half2half2(__float2half_rn(scale - __half2float(hi)));
-#pragma unroll 1
-      for (int chunk = 0; chunk < D / 16; ++chunk) {
-        const uint4 p = *reinterpret_cast<const uint4*>(from + swizzled<D>(t, chunk));
-        const uint32_t w[4] = {p.x, p.y, p.z, p.w};
-        uint32_t h[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint32_t bits = e4m3x2_to_half2(w[k / 2] >> (16 * (k % 2)));
-          const __half2 v = *reinterpret_cast<const __half2*>(&bits);
-          const __half2 y = __hfma2(v, r_hi, __hmul2(v, r_lo));
-          h[k] = *reinterpret_cast<const uint32_t*>(&y);
-        }
-        uint8_t* const row = to + chunk / 4 * (kTile * 128);
-        *reinterpret_cast<uint4*>(row + (((2 * chunk) % 8 ^ (t & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-        *reinterpret_cast<uint4*>(row + (((2 * chunk + 1) % 8 ^ (t & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
-      }
-      if (fabsf(scale) < kSmallestUnit) {
+      if (lane == 0) mbar_arrive(&sh.scale_empty[scales.stage]);
+      scales.next();
+      wait_whole_warp(sh, &sh.v_full[raw.stage], raw.parity);
+      wait_whole_warp(sh, &sh.half_empty[halves.stage], halves.parity ^ 1u);
+      __syncwarp();
+      const uint8_t* const from = smem + Shape::kV + raw.stage * Shape::kTileBytes;
+      uint8_t* const to = smem + Shape::kHalf + halves.stage * Shape::kHalfBytes + t * 128;
+      if (valid) {
+        // the factor as two f16 terms, so that the product with a byte's value is rounded once
+        const __half hi = __float2half_rn(scale);
+        const __half2 r_hi = __half2half2(hi), r_lo = __half2half2(__float2half_rn(scale - __half2float(hi)));
         uint32_t any = 0u;
-        for (int chunk = 0; chunk < D / 16; ++chunk) {
-          const uint4 p = *reinterpret_cast<const uint4*>(from + swizzled<D>(t, chunk));
-          any |= (p.x | p.y | p.z | p.w) & 0x7f7f7f7fu;
-        }
-        if (any != 0u) sh.redo[segment] = 1;
-      }
-    } else {
 #pragma unroll 1
-      for (int chunk = 0; chunk < D / 8; ++chunk) *reinterpret_cast<uint4*>(to + chunk / 8 * (kTile * 128) + chunk % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
+        for (int part = 0; part < D / 64; ++part) {
+          uint4 p[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) p[c] = *reinterpret_cast<const uint4*>(from + swizzled<D>(t, 4 * part + c));
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const uint32_t w[4] = {p[c].x, p[c].y, p[c].z, p[c].w};
+            any |= w[0] | w[1] | w[2] | w[3];
+            uint32_t h[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const uint32_t bits = e4m3x2_to_half2(w[k / 2] >> (16 * (k % 2)));
+              const __half2 v = *reinterpret_cast<const __half2*>(&bits);
+              const __half2 y = __hfma2(v, r_hi, __hmul2(v, r_lo));
+              h[k] = *reinterpret_cast<const uint32_t*>(&y);
+            }
+            uint8_t* const row = to + part * (kTile * 128);
+            *reinterpret_cast<uint4*>(row + ((2 * c ^ (t & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4*>(row + ((2 * c + 1 ^ (t & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
+          }
+        }
+        if (fabsf(scale) < kSmallestUnit && (any & 0x7f7f7f7fu) != 0u) sh.redo[segments.stage] = 1;
+      } else {
+#pragma unroll 1
+        for (int chunk = 0; chunk < D / 8; ++chunk) *reinterpret_cast<uint4*>(to + chunk / 8 * (kTile * 128) + chunk % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&sh.half_full[halves.stage]);
+        mbar_arrive(&sh.v_empty[raw.stage]);
+        if (j + 1 == n) mbar_arrive(&sh.segment_empty[segments.stage]);
+      }
+      if (__any_sync(0xffffffffu, sh.abort_code != 0)) return;
+      raw.next();
+      halves.next();
     }
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) {
-      mbar_arrive(&sh.half_full[halves.stage]);
-      mbar_arrive(&sh.v_empty[raw.stage]);
-      if (last) mbar_arrive(&sh.segment_empty[segment]);
-    }
-    if (__any_sync(0xffffffffu, sh.abort_code != 0)) return;
-    raw.next();
-    halves.next();
+    segments.next();
   }
 }
 
-// ---------------------------------------------------------------- softmax, a thread per row (eight warps, four to a slot)
+// ---------------------------------------------------------------- softmax, a lane per row and half of a tile (sixteen warps, eight to a slot)
 __device__ __forceinline__ ulonglong2 ld_shared_pairs(uint32_t at) {
   ulonglong2 v;
   asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(v.x), "=l"(v.y) : "r"(at) : "memory");
@@ -559,9 +618,10 @@ __device__ __forceinline__ float ld_shared_f32(uint32_t at) {
 }
 __device__ __forceinline__ void st_shared_f32(uint32_t at, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory"); }
 
-// One half of a tile's row: 64 scores from tensor memory, their weights back into it, the row's reference m and this half's sum l.  The partner warp has the other 64; the two agree on the row's largest score through shared memory (`top`: this
-// warp's places, `other`: the partner's), and only behind that barrier, when both have read their scores, write weights over them.
-// unit_at, fade_at: where the row's unit and what the values' reference has become smaller by lie.  low, high: what the row sees, counted from the first of the 64.
+// One half of a tile's row: 64 scores from tensor memory, their weights back into it, the row's reference m and this half's sum l.  The
+// partner warp has the other 64; the two agree on the row's largest score through shared memory (`top`: this warp's places, `other`: the
+// partner's), and only behind that barrier, when both have read their scores, write weights over them.  unit_at, fade_at: where the row's
+// unit and what the values' reference has become smaller by lie.  low, high: what the row sees, counted from the first of the 64.
 template <int D>
 __device__ __forceinline__ void softmax_half(uint32_t t_s, uint32_t t_o, int half, uint32_t k_scale, bool masked, int low, int high, bool there,
                                              uint32_t unit_at, uint32_t fade_at, bool first, uint32_t top, uint32_t other, int barrier, float& m, float& l) {
@@ -701,7 +761,8 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
   using Shape = ChunkShape<D>;
   // warps 0-7: slot 0, 8-15: slot 1; of each, the first four have a tile's first 64 positions and the first half of the dimensions
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, slot = warp / 8, half = warp / 4 % 2, in_slot = warp % 4 * 32 + lane;
-  const int row = slot * 128 + in_slot, pair = 2 + slot * 4 + warp % 4;        // named barrier of the two warps of a row
+  const int pair = 2 + slot * 4 + warp % 4;        // named barrier of the two warps of a row
+  const int across = 2 + half * 4 + warp % 4;      // between tiles: of the two slots' warps, for the same rows and dimensions
   const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
   const uint32_t t_s = tmem + lanes + slot * 128, t_o = t_s + 256 + half * (D / 2), scales0 = smem_u32(smem) + Shape::kScales + half * 256;
   static_assert(kSegmentRing == 4 && kScaleStages == 4, "stage and parity are bits of a counter");
@@ -712,22 +773,23 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
     if (softmax_bar_any(sh.abort_code != 0)) return;      // all sixteen warps meet here whatever failed, and leave together
     const Segment& g = sh.segment[segment & 3];
     if (g.tiles == 0) return;
-    const bool active = slot * 128 < g.rows;
+    // whether the next tile is this slot's (bit 0: no), and whether that changes with each (bit 1)
+    unsigned turn = g.turns ? 2u + slot : g.rows <= slot * kSlotRows;
     float m = -INFINITY, l = 0.0f;
     int token_of_row = 0, column_of_row = 0;         // of this thread's row, in q and out
     {
       int low, high;
       {
-        const int r = g.row0 + min(row, g.rows - 1), token = r / a.group;        // (rows beyond the last copy its bounds)
+        const int r = g.row0 + min((g.turns ? 0 : slot * kSlotRows) + in_slot, g.rows - 1), token = r / a.group;        // (rows beyond the last copy its bounds)
         token_of_row = g.q_first + token;
         column_of_row = (g.head * a.group + r - token * a.group) * D;
         high = g.base + token;
         low = a.window > 0 ? max(high - a.window + 1, 0) : 0;
       }
-      if (active) {
-        const int row0 = slot * 128 + warp % 4 * 32;
-        put_queries<D>(a.q, token_of_row * a.q_stride + column_of_row, a.scale_log2, half * 16, g.rows - row0, smem + Shape::kQ + 2 * slot * Shape::kTileBytes,
-                       row0 % 128, sh.unit + row0);
+      if (turn != 1u) {
+        const int in_tile = warp % 4 * 32;
+        put_queries<D>(a.q, token_of_row * a.q_stride + column_of_row, a.scale_log2, half * 16, g.rows - (g.turns ? 0 : slot * kSlotRows) - in_tile,
+                       smem + Shape::kQ + 2 * slot * Shape::kTileBytes, in_tile, sh.unit + slot * 128 + in_tile);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.q_full[slot]);
@@ -740,18 +802,17 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
       bool first = true;
       for (int left = g.tiles; left > 0; --left) {
         const int stage = tile & 3;
-        wait_whole_warp(sh, &sh.scale_full[stage], tile >> 2 & 1);
         wait_whole_warp(sh, &sh.scale_clean[stage], tile >> 2 & 1);
-        if (active) {
+        if (!(turn & 1u)) {
           wait_whole_warp(sh, &sh.s_full[slot], own & 1);
           __syncwarp();
           tc_fence_after();
           const bool there = sh.there[stage] >> half & 1;
           const uint32_t top = smem_u32(&sh.top[own & 1][slot][0][in_slot]);
           softmax_half<D>(t_s, t_o, half, scales0 + stage * (2 * kTile * 4), !there || __any_sync(0xffffffffu, low > 0 || high < 63), low, high, there,
-                          smem_u32(&sh.unit[row]), smem_u32(&sh.fade[stage]), first, top + half * 512, top + (half ^ 1) * 512, pair, m, l);
+                          smem_u32(&sh.unit[slot * 128 + in_slot]), smem_u32(&sh.fade[stage]), first, top + half * 512, top + (half ^ 1) * 512, pair, m, l);
           tc_fence_before();
-          if (left == 1) exponent = sh.exponent[stage];
+          exponent = sh.exponent[stage];
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh.p_full[slot]);
           ++own;
@@ -760,30 +821,42 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.scale_empty[stage]);
         ++tile;
+        turn ^= turn >> 1 & 1u;
         low -= kTile;
         high -= kTile;
         // (a warp that failed keeps its partner company at their barrier until the segment's end)
       }
       // ---- the segment's end
-      if (active) {
+      if (turn != 1u) {
         wait_whole_warp(sh, &sh.o_full[slot], own_segments & 1);
         __syncwarp();
         tc_fence_after();
         ++own_segments;
-        sh.top[own & 1][slot][half][in_slot] = l;
+        sh.end[slot][half][in_slot] = l;
+        if (half == 0) sh.end[slot][2][in_slot] = m;
       }
     }
     if (softmax_bar_any(sh.abort_code != 0)) return;
-    const bool redo = sh.redo[segment & 3] != 0, whole = g.whole, real = row < g.rows;
+    const bool turns = g.turns, active = turn != 1u, redo = sh.redo[segment & 3] != 0, whole = g.whole;
+    const int row = (turns ? 0 : slot * kSlotRows) + in_slot;
+    const bool real = row < g.rows && !(turns && slot == 1);
     if (tid == 0) sh.redo[(segment + 3) & 3] = 0;     // the segment before: everybody has read it
     if (active) {
-      l = sh.top[own & 1][slot][0][in_slot] + sh.top[own & 1][slot][1][in_slot];
-      const float unscale = __int_as_float((exponent - kUnitShift + 127) << 23);
-      const float f = whole ? (l == 0.0f ? 0.0f : unscale / l) : unscale;
+      l = sh.end[slot][0][in_slot] + sh.end[slot][1][in_slot];
+      float f = __int_as_float((exponent - kUnitShift + 127) << 23);
+      if (turns) {                            // to the larger reference of the two slots'
+        const float(&its)[3][128] = sh.end[slot ^ 1];
+        const float its_m = its[2][in_slot], all = fmaxf(m, its_m), ref = finite_or_zero(all), fade = ex2(m - ref);
+        l = l * fade + (its[0][in_slot] + its[1][in_slot]) * ex2(its_m - ref);
+        m = all;
+        f *= fade;
+      }
+      if (whole) f = l == 0.0f ? 0.0f : f / l;
       // Rows leave through the slot's q tiles, which nothing reads any more: 32 rows of D bytes per warp (half of the dimensions), swizzled,
       // then D / 16 lanes write a row's half.  Partial sums are kept by dimension, so that a warp's 32 rows lie side by side.
       uint8_t* const stage = smem + Shape::kQ + 2 * slot * Shape::kTileBytes + (half * 4 + warp % 4) * (32 * D);
       float4* const to = reinterpret_cast<float4*>(a.partial);
+      float4* const its = reinterpret_cast<float4*>(smem + Shape::kQ + 2 * Shape::kTileBytes + (half * 4 + warp % 4) * (32 * D)) + lane;   // of slot 1's q tiles
       const int part = parts_of(g).slot(static_cast<int>(blockIdx.x));
 #pragma unroll 1
       for (int c = 0; c < D / 16; c += 2) {
@@ -791,12 +864,34 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
         tmem_ld16(t_o + 8 * c, o);
         tmem_ld_wait_for(o);
 #pragma unroll
+        for (int b = 0; b < 16; ++b) o[b] = __float_as_uint(__uint_as_float(o[b]) * f);
+        if (turns) {                          // slot 0 adds slot 1's sums to its own
+          if (slot == 1) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+              its[32 * b] = make_float4(__uint_as_float(o[4 * b]), __uint_as_float(o[4 * b + 1]), __uint_as_float(o[4 * b + 2]), __uint_as_float(o[4 * b + 3]));
+          }
+          named_bar_sync(across, 64);
+          if (slot == 0) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+              const float4 x = its[32 * b];
+              o[4 * b] = __float_as_uint(__uint_as_float(o[4 * b]) + x.x);
+              o[4 * b + 1] = __float_as_uint(__uint_as_float(o[4 * b + 1]) + x.y);
+              o[4 * b + 2] = __float_as_uint(__uint_as_float(o[4 * b + 2]) + x.z);
+              o[4 * b + 3] = __float_as_uint(__uint_as_float(o[4 * b + 3]) + x.w);
+            }
+          }
+          named_bar_sync(across, 64);
+          if (slot == 1) continue;
+        }
+#pragma unroll
         for (int b = 0; b < 2; ++b) {
           if (whole) {
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(o[8 * b + 2 * e]) * f, __uint_as_float(o[8 * b + 2 * e + 1]) * f);
+              const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(o[8 * b + 2 * e]), __uint_as_float(o[8 * b + 2 * e + 1]));
               w[e] = *reinterpret_cast<const uint32_t*>(&h);
             }
             *reinterpret_cast<uint4*>(stage + lane * D + ((D == 128 ? (c + b) ^ (lane & 7) : (c + b) ^ (lane >> 1 & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -804,12 +899,12 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
 #pragma unroll
             for (int e = 0; e < 2; ++e)
               to[(static_cast<long long>(part) * (D / 4) + half * (D / 8) + 2 * (c + b) + e) * kChunkRows + row] =
-                  make_float4(__uint_as_float(o[8 * b + 4 * e]) * f, __uint_as_float(o[8 * b + 4 * e + 1]) * f, __uint_as_float(o[8 * b + 4 * e + 2]) * f,
-                              __uint_as_float(o[8 * b + 4 * e + 3]) * f);
+                  make_float4(__uint_as_float(o[8 * b + 4 * e]), __uint_as_float(o[8 * b + 4 * e + 1]), __uint_as_float(o[8 * b + 4 * e + 2]),
+                              __uint_as_float(o[8 * b + 4 * e + 3]));
           }
         }
       }
-      if (whole && !redo) {
+      if (whole && !redo && !(turns && slot == 1)) {
         __syncwarp();
         constexpr int kLanes = D / 16, kTogether = 32 / kLanes;
         const long long mine = token_of_row * a.out_stride + column_of_row + half * (D / 2);
@@ -871,7 +966,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
 
   pdl_wait();
   pdl_trigger();
-  const Plan<kTile, kChunkRows, kChunkExtra> plan = {a.batch, a.cache.heads, a.group, a.window};
+  const ChunkPlan plan = {a.batch, a.cache.heads, a.group, a.window};
   const long long total = plan.total(s_plan);
   const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
   if (static_cast<int>(blockIdx.x) >= ctas) return;
@@ -882,7 +977,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
   if (tid == 0) {
     for (int i = 0; i < kScaleStages; ++i) {
       mbar_init(&sh.scale_full[i], 1);
-      mbar_init(&sh.scale_clean[i], 4);         // converting warps
+      mbar_init(&sh.scale_clean[i], 1);
       mbar_init(&sh.scale_empty[i], kSoftmaxWarps + 4);   // softmax and converting warps
     }
     for (int i = 0; i < 4; ++i) {
@@ -929,6 +1024,8 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
     asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
     if (warp < 20) {
       convert_role<D>(sh, smem);
+    } else if (warp == 23) {
+      scale_role<D>(sh, smem);
     } else if (lane == 0) {
       if (warp == 20) mma_role<D>(sh, smem, tmem);
       if (warp == 21) load_role<D>(map, a, sh, smem);
@@ -956,7 +1053,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
     __syncthreads();
     // What is left of the piece becomes NaN, and its units are counted, so that nobody waits for them and the next call finds the
     // counters at zero.
-    Cursor<kTile, kChunkRows, kChunkExtra> at;
+    ChunkCursor at;
     at.start(plan, s_plan, places);
     for (int segment = 0; at.left > 0; ++segment) {
       const int n = at.tiles_here(), rows = at.rows(a.group);
