@@ -39,8 +39,8 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {
 
 // ---------------------------------------------------------------- few rows per sequence and key head: decoding
 // A CTA walks its piece of the pages through a ring of stages filled by cp.async.  Four warps share a page, 16 positions each, for
-// every 8 NT rows (MT row groups of four warps); mma.sync m16n8k16 in f16, whose big operand the lanes make from the bytes in
-// registers, so that a row tile is as narrow as an MMA allows:
+// 8 NT rows; mma.sync m16n8k16 in f16, whose big operand the lanes make from the bytes in registers, so that a row tile is as narrow
+// as an MMA allows:
 //   scores:  positions (M) x rows (N) = K Q^T.  A lane's K operand is 16 bytes of two positions; the MMAs' k index permutes the dimensions,
 //            alike in q.
 //   values:  dimensions (M) x rows (N) = V^T P^T.  A lane's V operand pairs the bytes of two positions (prmt), its 16 dimensions are the m
@@ -50,29 +50,28 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {
 // What bounds it is the cache's bytes, so what counts is loads in flight and few instructions per page.
 constexpr int kDecodeExtra = 1;      // what a unit costs besides its pages, in pages
 
-template <int D, int NT, int MT>
+template <int D, int NT>
 struct DecodeShape {
-  static constexpr int kRows = 8 * NT * MT;
-  static constexpr int kThreads = 128 * MT;
-  static constexpr int kBlocks = MT > 1 ? 1 : NT == 1 ? 3 : 2;          // per SM
-  static constexpr int kStages = (MT > 1 ? 6 : NT == 1 ? 3 : 5) * (D == 128 ? 1 : 2) - (D == 128 ? 0 : 1);
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kThreads = 128;
+  static constexpr int kBlocks = NT == 1 ? 3 : 2;          // per SM
+  static constexpr int kStages = D == 128 ? (NT == 1 ? 3 : 5) : (NT == 1 ? 5 : 9);
   static constexpr int kBlockBytes = kKvPage * D;
   static constexpr int kStageBytes = 2 * kBlockBytes + 2 * kKvPage * 4;
-  static constexpr int kMerge = MT * 2 * 8 * NT * D;                    // floats
+  static constexpr int kMerge = 2 * 8 * NT * D;                         // floats
   static constexpr int kSmem = kStages * kStageBytes + kMerge * 4;
 };
 
-template <int D, int NT, int MT>
-__global__ void __launch_bounds__(DecodeShape<D, NT, MT>::kThreads, DecodeShape<D, NT, MT>::kBlocks) attention_decode_kernel(const __grid_constant__ AttentionArgs a) {
-  using Shape = DecodeShape<D, NT, MT>;
+template <int D, int NT>
+__global__ void __launch_bounds__(DecodeShape<D, NT>::kThreads, DecodeShape<D, NT>::kBlocks) attention_decode_kernel(const __grid_constant__ AttentionArgs a) {
+  using Shape = DecodeShape<D, NT>;
   constexpr int kRows = Shape::kRows, kStages = Shape::kStages, kSteps = D / 16, kMmas = D / 16;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ PlanShared s_plan;
   __shared__ int s_there[kStages];
-  __shared__ float4 s_stat[4 * MT][8 * NT];
+  __shared__ float4 s_stat[4][8 * NT];
   float* const s_merge = reinterpret_cast<float*>(smem + kStages * Shape::kStageBytes);
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, c = lane % 4;
-  const int mt = warp / 4, quarter = warp % 4;
 
   pdl_wait();
   pdl_trigger();
@@ -124,7 +123,7 @@ __global__ void __launch_bounds__(DecodeShape<D, NT, MT>::kThreads, DecodeShape<
   for (int i = 0; i < kStages - 1; ++i) ask();
 
   // This lane's positions of a page: t0 and t0 + 8; its rows of the scores: 8 t + 2 c and 8 t + 2 c + 1.
-  const int t0 = quarter * 16 + ((g & 1) ? (g - 1) ^ 5 : g);
+  const int t0 = warp * 16 + ((g & 1) ? (g - 1) ^ 5 : g);
   uint32_t qb[NT][kSteps][2];
   // Of each row: what a score is worth; the reference of this lane's sum, and the sum; the reference of the values' sum, and 2^(m - n + 7).
   float unit[NT][2], m[NT][2], l[NT][2], n[NT][2], up[NT][2], o[NT][kMmas][4];
@@ -149,7 +148,7 @@ __global__ void __launch_bounds__(DecodeShape<D, NT, MT>::kThreads, DecodeShape<
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         // 2^k that brings the row's largest magnitude to 2^14 .. 2^15: f16 then holds bf16 values exactly down to 2^-29 of it
-        const int row = (mt * NT + t) * 8 + g, r = r0 + row;
+        const int row = t * 8 + g, r = r0 + row;
         const bool real = row < rows;
         const __nv_bfloat16* from = a.q + (use.s.first + (real ? r / a.group : 0)) * a.q_stride + (use.head * a.group + (real ? r % a.group : 0)) * D;
         uint2 raw[kSteps];
@@ -173,7 +172,7 @@ __global__ void __launch_bounds__(DecodeShape<D, NT, MT>::kThreads, DecodeShape<
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           unit[t][i] = __shfl_sync(0xffffffffu, worth, 8 * c + 4 * i);
-          const int mine = (mt * NT + t) * 8 + 2 * c + i;
+          const int mine = t * 8 + 2 * c + i;
           const int position = base + (mine < rows ? (r0 + mine) / a.group : 0);
           low[t][i] = a.window > 0 ? max(position - a.window + 1, 0) : 0;
           high[t][i] = mine < rows ? position : -1;
@@ -329,7 +328,7 @@ __global__ void __launch_bounds__(DecodeShape<D, NT, MT>::kThreads, DecodeShape<
       uint32_t even[2][D / 32], odd[2][D / 32];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int v0 = quarter * 16 + 8 * u + 2 * c, v1 = quarter * 16 + 8 * u + ((2 * c) ^ 5);
+        const int v0 = warp * 16 + 8 * u + 2 * c, v1 = warp * 16 + 8 * u + ((2 * c) ^ 5);
         if constexpr (D == 128) {
           const uint4 w = *reinterpret_cast<const uint4*>(values + swizzled<D>(v0, g)), r = *reinterpret_cast<const uint4*>(values + swizzled<D>(v1, g));
           even[u][0] = w.x; even[u][1] = w.y; even[u][2] = w.z; even[u][3] = w.w;
@@ -378,12 +377,12 @@ __global__ void __launch_bounds__(DecodeShape<D, NT, MT>::kThreads, DecodeShape<
           float m_all = -INFINITY, n_all = -INFINITY, l_all = 0.0f;
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
-            m_all = fmaxf(m_all, s_stat[mt * 4 + w][8 * t + 2 * c + i].x);
-            n_all = fmaxf(n_all, s_stat[mt * 4 + w][8 * t + 2 * c + i].z);
+            m_all = fmaxf(m_all, s_stat[w][8 * t + 2 * c + i].x);
+            n_all = fmaxf(n_all, s_stat[w][8 * t + 2 * c + i].z);
           }
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
-            const float4 st = s_stat[mt * 4 + w][8 * t + 2 * c + i];
+            const float4 st = s_stat[w][8 * t + 2 * c + i];
             l_all += st.y * ex2(st.x - finite_or_zero(m_all));
           }
           f[i] = ex2(n[t][i] - finite_or_zero(n_all));
@@ -396,16 +395,16 @@ __global__ void __launch_bounds__(DecodeShape<D, NT, MT>::kThreads, DecodeShape<
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[t][j][e] *= f[e % 2];
       }
-      float* const mine = s_merge + (mt * 2 + (quarter & 1)) * 8 * NT * D + lane;
-      if (quarter >= 2) {
+      float* const mine = s_merge + (warp & 1) * 8 * NT * D + lane;
+      if (warp >= 2) {
 #pragma unroll
         for (int k = 0; k < NT * kMmas * 4; ++k) mine[k * 32] = o[k / (kMmas * 4)][k / 4 % kMmas][k % 4];
       }
       __syncthreads();
-      if (quarter < 2) {
+      if (warp < 2) {
 #pragma unroll
         for (int k = 0; k < NT * kMmas * 4; ++k) o[k / (kMmas * 4)][k / 4 % kMmas][k % 4] += mine[k * 32];
-        if (quarter == 1) {
+        if (warp == 1) {
 #pragma unroll
           for (int k = 0; k < NT * kMmas * 4; ++k) mine[k * 32] = o[k / (kMmas * 4)][k / 4 % kMmas][k % 4];
         }
@@ -413,14 +412,14 @@ __global__ void __launch_bounds__(DecodeShape<D, NT, MT>::kThreads, DecodeShape<
       __syncthreads();
       const bool whole = begun == 0 && unit_ends;
       const long long unit_start = w1 - use.left - use.tile;      // the place of its first page
-      if (quarter == 0) {
-        const float* other = s_merge + (mt * 2 + 1) * 8 * NT * D + lane;
+      if (warp == 0) {
+        const float* other = s_merge + 8 * NT * D + lane;
         const int slot = 2 * static_cast<int>(blockIdx.x) + (w0 >= unit_start ? 0 : 1);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const int row = (mt * NT + t) * 8 + 2 * c + i, r = use.rt * kRows + row;
+            const int row = t * 8 + 2 * c + i, r = use.rt * kRows + row;
             if (row >= rows) continue;
             float v[D / 8];                  // this lane's dimensions of the row, g * D / 8 and on
 #pragma unroll
@@ -449,6 +448,21 @@ __global__ void __launch_bounds__(DecodeShape<D, NT, MT>::kThreads, DecodeShape<
             }
           }
       }
+      // (what the next segment sets anyway: not kept in registers across the join, whose own made the loop above spill)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+#pragma unroll
+        for (int step = 0; step < kSteps; ++step) qb[t][step][0] = qb[t][step][1] = 0u;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          unit[t][i] = m[t][i] = l[t][i] = n[t][i] = up[t][i] = 0.0f;
+          low[t][i] = high[t][i] = 0;
+        }
+#pragma unroll
+        for (int j = 0; j < kMmas; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[t][j][e] = 0.0f;
+      }
       if (!whole) {
         const Parts parts(total, ctas, unit_start, use.span.tiles);
         __threadfence();
@@ -461,7 +475,7 @@ __global__ void __launch_bounds__(DecodeShape<D, NT, MT>::kThreads, DecodeShape<
         __syncthreads();
         if (s_plan.last) {
           __threadfence();
-          join_parts<D, kRows, 1>(a, use.s.first, use.rt * kRows, use.head, rows, ctas, parts, tid, Shape::kThreads);
+          join_parts<D, kRows>(a, use.s.first, use.rt * kRows, use.head, rows, ctas, parts, warp, 4);
         }
       }
       fresh = true;
@@ -480,9 +494,9 @@ constexpr long long kWaitLimit = 1ll << 32;   // SM clocks (about two seconds)
 std::mutex g_mu;
 Device g_devices[64];
 
-template <int D, int NT, int MT>
+template <int D, int NT>
 bool raise_decode() {
-  return cudaFuncSetAttribute(attention_decode_kernel<D, NT, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeShape<D, NT, MT>::kSmem) == cudaSuccess;
+  return cudaFuncSetAttribute(attention_decode_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeShape<D, NT>::kSmem) == cudaSuccess;
 }
 
 constexpr size_t kTicketBytes = 4096;      // 1024 CTAs
@@ -495,13 +509,13 @@ bool take_scratch(AttentionArgs& a, Device& d, size_t partial, cudaStream_t st, 
   return true;
 }
 
-template <int D, int NT, int MT>
+template <int D, int NT>
 int launch_decode(AttentionArgs a, Device& d, int sms, cudaStream_t st) {
-  using Shape = DecodeShape<D, NT, MT>;
+  using Shape = DecodeShape<D, NT>;
   const int ctas = sms * Shape::kBlocks;
   int rc = SYFI_KV_OK;
   if (!take_scratch(a, d, 2ull * ctas * Shape::kRows * (D + 4) * sizeof(float), st, &rc)) return rc;
-  return launch_dependent(attention_decode_kernel<D, NT, MT>, dim3(ctas), dim3(Shape::kThreads), Shape::kSmem, st, a) == cudaSuccess
+  return launch_dependent(attention_decode_kernel<D, NT>, dim3(ctas), dim3(Shape::kThreads), Shape::kSmem, st, a) == cudaSuccess
              ? SYFI_KV_OK : kv_fail(SYFI_KV_ERR_CUDA, "attention kernel launch failed");
 }
 
@@ -546,8 +560,7 @@ extern "C" int syfi_paged_attention(const void* q, int64_t q_stride, const void*
   std::lock_guard<std::mutex> lock(g_mu);
   Device& d = g_devices[dev];
   if (!d.status) {
-    if (!raise_decode<128, 1, 1>() || !raise_decode<128, 2, 1>() || !raise_decode<128, 2, 2>() || !raise_decode<128, 2, 4>() ||
-        !raise_decode<64, 1, 1>() || !raise_decode<64, 2, 1>() || !raise_decode<64, 2, 2>() || !raise_decode<64, 2, 4>() ||
+    if (!raise_decode<128, 1>() || !raise_decode<128, 2>() || !raise_decode<64, 1>() || !raise_decode<64, 2>() ||
         chunk_set_attributes() != cudaSuccess)
       return kv_fail(SYFI_KV_ERR_CUDA, "cannot raise the shared-memory limit of the attention kernels");
     RelaxedCapture relaxed;
@@ -556,19 +569,17 @@ extern "C" int syfi_paged_attention(const void* q, int64_t q_stride, const void*
   const long long wait_limit = d.next_wait_limit > 0 ? d.next_wait_limit : kWaitLimit;
   d.next_wait_limit = 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // Rows per sequence and key head, on average (the lengths themselves are on the device): row tiles of 8, 16, 32 or 64, beyond that
-  // the tensor memory kernel's of 256.
+  // Rows per sequence and key head, on average (the lengths themselves are on the device): row tiles of 8 or 16, beyond that the tensor
+  // memory kernel's.  24 sequences of 300 .. 30000 positions, 8 key heads of 128, us for 8 | 16 | 32 rows each: tiles of 8 79 | 134 | 249,
+  // tiles of 16 121 | 135 | 259, the tensor memory kernel 141 | 141 | 142.
   const int64_t rows = (tokens * a.group + batch - 1) / batch;
-  if (rows > 64) {
+  if (rows > 16) {
     int rc = SYFI_KV_OK;
     if (!take_scratch(a, d, chunk_partial_bytes(head_dim, sms), st, &rc)) return rc;
     return launch_chunk(a, head_dim, sms, d.status, wait_limit, st) == cudaSuccess ? SYFI_KV_OK : kv_fail(SYFI_KV_ERR_CUDA, "attention kernel launch failed");
   }
-  if (head_dim == 128)
-    return rows <= 8 ? launch_decode<128, 1, 1>(a, d, sms, st) : rows <= 16 ? launch_decode<128, 2, 1>(a, d, sms, st)
-           : rows <= 32 ? launch_decode<128, 2, 2>(a, d, sms, st) : launch_decode<128, 2, 4>(a, d, sms, st);
-  return rows <= 8 ? launch_decode<64, 1, 1>(a, d, sms, st) : rows <= 16 ? launch_decode<64, 2, 1>(a, d, sms, st)
-         : rows <= 32 ? launch_decode<64, 2, 2>(a, d, sms, st) : launch_decode<64, 2, 4>(a, d, sms, st);
+  if (head_dim == 128) return rows <= 8 ? launch_decode<128, 1>(a, d, sms, st) : launch_decode<128, 2>(a, d, sms, st);
+  return rows <= 8 ? launch_decode<64, 1>(a, d, sms, st) : launch_decode<64, 2>(a, d, sms, st);
 }
 
 // Test hook for the bounded waits, no part of the interface: a wait of the next attention call's kernel on the current device may

@@ -30,7 +30,7 @@ constexpr int kTile = 128;             // positions per tile: two pages
 constexpr int kChunkRows = 256;
 constexpr int kChunkThreads = 768;     // 16 softmax warps, 4 converting ones, then MMAs, loads, planning, scales
 constexpr int kSoftmaxWarps = 16, kSoftmaxThreads = 512;
-constexpr int kChunkExtra = 3;         // what a unit costs besides its tiles, in tiles
+constexpr int kChunkExtra = 4;         // what a unit costs besides its tiles, in tiles (8192-token prompt with 3, 4, 5, 6: 704, 656, 662, 672 us)
 constexpr int kSlotRows = 128;         // units of at most so many rows use one slot for their even tiles and one for their odd ones
 using ChunkPlan = Plan<kTile, kChunkRows, kChunkExtra, kSlotRows>;
 using ChunkCursor = Cursor<kTile, kChunkRows, kChunkExtra, kSlotRows>;
