@@ -571,7 +571,7 @@ extern "C" int syfi_paged_attention(const void* q, int64_t q_stride, const void*
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // Rows per sequence and key head, on average (the lengths themselves are on the device): row tiles of 8 or 16, beyond that the tensor
   // memory kernel's.  24 sequences of 300 .. 30000 positions, 8 key heads of 128, us for 8 | 16 | 32 rows each: tiles of 8 79 | 134 | 249,
-  // tiles of 16 121 | 135 | 259, the tensor memory kernel 141 | 141 | 142.
+  // tiles of 16 121 | 129 | 259, the tensor memory kernel 141 | 143 | 145.
   const int64_t rows = (tokens * a.group + batch - 1) / batch;
   if (rows > 16) {
     int rc = SYFI_KV_OK;

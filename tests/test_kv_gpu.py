@@ -4,6 +4,7 @@ Tolerances follow from the number formats: a result in bf16 is off by half a uni
 of the cache by half an e4m3 step (2^-4 of its value, 2^-10 scales near zero), f32 arithmetic on a head's up to 128 dimensions by
 a few 1e-6 of the vector's largest; attention weights may be rounded to f16 (2^-11 of each), twice that is allowed, in units of
 the average of |value| under the weights."""
+import ctypes
 import importlib
 
 import pytest
@@ -337,6 +338,57 @@ def test_one_large_weight_and_a_long_tail(q_len, spike, pkg, kv):
     scales[int(table[0, at // 64]), 0, 0, at % 64] = 17.0 * 0.6931471805599453 * 128 ** 0.5
     inputs = (q, cache, table, lens, starts)
     _check_attention(_attend(pkg, inputs), *kv.attention(*inputs))
+
+
+@pytest.mark.parametrize("HQ,HK,D", [(8, 1, 128), (4, 1, 64), (16, 1, 128), (14, 1, 64)])
+def test_a_long_sequence_in_more_parts_than_a_warp_has_lanes(HQ, HK, D, pkg, kv):
+    inputs = _attention_inputs(kv, [1], [60000], HQ, HK, D, seed=6)
+    _check_attention(_attend(pkg, inputs), *kv.attention(*inputs))
+
+
+@pytest.mark.parametrize("q_len", [31, 32, 33, 64, 65])
+@pytest.mark.parametrize("kv_len", [120, 128, 129, 257, 400, 6000])
+@pytest.mark.parametrize("D", [64, 128])
+def test_rows_around_a_tile_and_references_that_move(q_len, kv_len, D, pkg, kv):
+    """128 rows of a key head and one token more or less, over even and odd numbers of tiles.  Along the sequence scores and the
+    values' scales grow, so that references follow, or fall, or jump up and down."""
+    inputs = _attention_inputs(kv, [q_len, 3], [kv_len, 3000], 8, 2, D, seed=7)
+    q, cache, table, lens, starts = inputs
+    _, scales = kv.views(cache)
+    kept = scales.clone()
+    j = torch.arange(kv_len, device=DEV)
+    page, at = table[0, j // 64].long(), j % 64
+    wave = torch.where(j // 128 % 3 == 1, 5.0, -5.0)
+    for window in (0, 333):
+        for octaves in (12.0 * j / kv_len - 6, 6 - 12.0 * j / kv_len, wave):
+            scales.copy_(kept)
+            scales[page, 1, :, at] *= torch.exp2(octaves)[:, None]
+            scales[page, 0, :, at] *= torch.exp2(octaves / 4)[:, None]
+            _check_attention(_attend(pkg, inputs, window=window), *kv.attention(*inputs, window=window))
+
+
+@pytest.mark.parametrize("q_lens,kv_lens,D", [([300, 5], [3000, 9000], 128), ([6] * 9, [4000] * 9, 64)])
+def test_bounded_waits_run_out(q_lens, kv_lens, D, pkg, kv):
+    """A wait that runs out ends its call with a status; rows that were not computed are NaN, all others are what they are, and
+    the next call is undisturbed."""
+    inputs = _attention_inputs(kv, q_lens, kv_lens, 8, 2, D, seed=8)
+    clean = _attend(pkg, inputs)
+    lib = pkg.load_library()
+    failed = 0
+    for limit in (1, 1, 64, 200, 1000, 5000):
+        assert lib.syfi_kv_debug_wait_limit(ctypes.c_int64(limit)) == 0
+        out = _attend(pkg, inputs)
+        try:
+            pkg.kv_check()
+            assert torch.equal(out, clean)
+        except pkg.MoeError as err:
+            assert "status 301" in str(err), str(err)
+            failed += 1
+            done = ~out.isnan().any(-1)
+            assert torch.equal(out[done], clean[done]) and not bool(done.all())
+        assert torch.equal(_attend(pkg, inputs), clean), limit
+        pkg.kv_check()
+    assert failed >= 1, failed
 
 
 @pytest.mark.parametrize("q_lens,kv_lens", [([1] * 5, [900, 20000, 3, 64, 7000]), ([400, 3], [5000, 6000])])
