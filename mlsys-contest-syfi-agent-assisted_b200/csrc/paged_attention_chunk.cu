@@ -502,10 +502,11 @@ __device__ __forceinline__ void scale_role(ChunkShared& sh, uint8_t* smem) {
         sh.exponent[scales.stage] = unit;
         sh.fade[scales.stage] = before == unit ? 1.0f : ex2(static_cast<float>(before - unit));     // (nothing uses a slot's first)
       }
+      // (in every tile: a wait by parity is one for this use of the stage only where the use before it is known to be over)
+      wait_whole_warp(sh, &sh.v_full[values.stage], values.parity);
       if (position0 < all_low || position0 + kTile - 1 > all_high) {
         // Some rows may see what others do not, and zero times NaN is NaN: the bytes of a value that is not finite are taken for zeros, and
         // the NaN goes by way of its score to the rows that see it.
-        wait_whole_warp(sh, &sh.v_full[values.stage], values.parity);
         const uint8_t* const from = smem + Shape::kV + values.stage * Shape::kTileBytes;
 #pragma unroll 1
         for (int t = lane; t < kTile; t += 32) {
