@@ -90,6 +90,7 @@ struct Plan {
     const int rounds = (batch.batch + kPlanRound - 1) / kPlanRound, lane = threadIdx.x % 32;
     long long before = 0;            // tiles of the rounds in front
     int round = 0;
+    if (rounds > 1) __syncthreads(); // every thread has read total()'s last sum
     while (true) {
       if (rounds > 1) sum_round(sh, round);
       const long long in_round = sh.sum[kPlanRound - 1] * heads;

@@ -250,6 +250,21 @@ def test_chunks_match_the_definition(q_lens, kv_lens, window, HQ, HK, D, pkg, kv
     _check_attention(_attend(pkg, inputs, window=window), *kv.attention(*inputs, window=window))
 
 
+@pytest.mark.parametrize("batch", [128, 129, 300, 1000])
+@pytest.mark.parametrize("new_tokens", ["one", "few", "chunk"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_batches_of_many_sequences(batch, new_tokens, D, pkg, kv):
+    """Ragged batches around and beyond 128 sequences, some without a new token; by the average of the rows per sequence that is either
+    kernel's work."""
+    pick = lambda b, n: (b * 7919 + 13) % n  # noqa: E731
+    q_lens = [0 if pick(b, 11) == 0 else 1 if new_tokens == "one" else 1 + pick(b, 3) for b in range(batch)]
+    if new_tokens == "chunk":
+        q_lens[batch // 2], q_lens[-1] = 300, 7 * batch
+    kv_lens = [n + pick(b, 2000 if b % 16 == 0 else 130) for b, n in enumerate(q_lens)]
+    inputs = _attention_inputs(kv, q_lens, kv_lens, 8, 2, D, seed=9)
+    _check_attention(_attend(pkg, inputs), *kv.attention(*inputs))
+
+
 @pytest.mark.parametrize("q_lens,kv_lens", [([1, 1, 1], [500, 130, 64]), ([40, 200], [600, 200])])
 @pytest.mark.parametrize("D", [64, 128])
 def test_what_is_not_seen_does_not_matter(q_lens, kv_lens, D, pkg, kv):
