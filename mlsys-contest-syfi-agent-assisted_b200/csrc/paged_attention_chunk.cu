@@ -335,13 +335,15 @@ __device__ __forceinline__ void load_role(const CUtensorMap& map, const Attentio
     --left;
     return true;
   };
+  // A role that gave up still arrives at barriers, which may free a stage whose copy is on its way: no copy is asked for behind that.
+  auto free_stage = [&](uint64_t* bar, uint32_t parity) { return wait_for(sh, bar, parity) && sh.abort_code == 0; };
   bool more = entries();
   for (int i = 0; more; ++i) {
     const int entry[2] = {entry0, entry1}, h = head;
     const bool here[2] = {entry0 >= 0 && entry0 < a.cache.num_pages, entry1 >= 0 && entry1 < a.cache.num_pages};
     const int pages = here[0] + here[1];
     more = entries();
-    if (!wait_for(sh, &sh.scale_empty[scales.stage], scales.parity ^ 1u)) return;
+    if (!free_stage(&sh.scale_empty[scales.stage], scales.parity ^ 1u)) return;
     sh.there[scales.stage] = here[0] | here[1] << 1;
     mbar_arrive_expect_tx(&sh.scale_full[scales.stage], pages * 2 * kKvPage * 4);
     float* const scale = reinterpret_cast<float*>(smem + Shape::kScales) + scales.stage * 2 * kTile;
@@ -353,14 +355,14 @@ __device__ __forceinline__ void load_role(const CUtensorMap& map, const Attentio
     }
     sh.asked_scales = i + 1;
     scales.next();
-    if (!wait_for(sh, &sh.k_empty[keys.stage], keys.parity ^ 1u)) return;
+    if (!free_stage(&sh.k_empty[keys.stage], keys.parity ^ 1u)) return;
     mbar_arrive_expect_tx(&sh.k_full[keys.stage], pages * kKvPage * D);
 #pragma unroll
     for (int p = 0; p < 2; ++p)
       if (here[p]) tma_load_4d(smem + Shape::kK + keys.stage * Shape::kTileBytes + p * kKvPage * D, &map, &sh.k_full[keys.stage], 0, 0, h, entry[p], keep);
     sh.asked_k = i + 1;
     keys.next();
-    if (!wait_for(sh, &sh.v_empty[values.stage], values.parity ^ 1u)) return;
+    if (!free_stage(&sh.v_empty[values.stage], values.parity ^ 1u)) return;
     mbar_arrive_expect_tx(&sh.v_full[values.stage], pages * kKvPage * D);
 #pragma unroll
     for (int p = 0; p < 2; ++p)

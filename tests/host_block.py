@@ -123,3 +123,33 @@ def build(folder, text):
     done = subprocess.run(["g++", "-std=c++17", "-O1", "-w", "-o", str(out), str(path)], capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr[-3000:]
     return str(out)
+
+
+# What the chunk kernel's roles need around them: types, casts, and barriers in memory whose word counts the phases that are over.
+ROLE_SHIM = r"""
+struct float4 { float x, y, z, w; };
+struct uint4 { uint32_t x, y, z, w; };
+static float __int_as_float(int i) { float f; memcpy(&f, &i, 4); return f; }
+static int __float_as_int(float f) { int i; memcpy(&i, &f, 4); return i; }
+static unsigned __float_as_uint(float f) { return static_cast<unsigned>(__float_as_int(f)); }
+static float ex2(float x) { return exp2f(x); }
+static void fence_proxy_async_smem() {}
+static void mbar_arrive(uint64_t* bar);
+static bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
+  if ((*bar & 1) != parity) return true;
+  stop(AT_LOOK);                               // (the hardware waits a while, too)
+  return (*bar & 1) != parity;
+}
+constexpr int kKvPage = 64;
+"""
+
+
+def role(name):
+    """The chunk kernel's shared memory and the function `name`, as C++ for the host."""
+    chunk, common = source("paged_attention_chunk.cu"), source("attention_common.cuh")
+    constants = [line for line in piece(chunk, "constexpr int kTile = 128;", "template <int D>").splitlines() if line.startswith("constexpr")]
+    return "\n".join([
+        piece(common, "template <int D>\n__device__ __forceinline__ int swizzled", "\n}\n"), *constants, piece(chunk, "template <int D>\nstruct ChunkShape", "\n};\n"),
+        piece(chunk, "struct Segment {", "\n};\n"), piece(chunk, "constexpr int kSegmentRing", "\n\n"), piece(chunk, "struct ChunkShared {", "\n};\n"),
+        piece(chunk, "__device__ __forceinline__ int tile_exponent", "\n}\n"), piece(chunk, "__device__ __forceinline__ bool wait_for", "// ------"),
+        piece(chunk, "template <int D>\n__device__ __forceinline__ void %s(" % name, "\n}\n")])

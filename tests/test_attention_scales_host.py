@@ -5,7 +5,7 @@ import subprocess
 
 import pytest
 
-from host_block import EMULATOR, build, piece, source
+from host_block import EMULATOR, ROLE_SHIM, build, role
 
 HARNESS = r"""
 template <int D>
@@ -69,38 +69,11 @@ int main(int, char** argv) {
 }
 """
 
-SHIM = r"""
-struct float4 { float x, y, z, w; };
-struct uint4 { uint32_t x, y, z, w; };
-static float __int_as_float(int i) { float f; memcpy(&f, &i, 4); return f; }
-static int __float_as_int(float f) { int i; memcpy(&i, &f, 4); return i; }
-static unsigned __float_as_uint(float f) { return static_cast<unsigned>(__float_as_int(f)); }
-static float ex2(float x) { return exp2f(x); }
-static void fence_proxy_async_smem() {}
-static void mbar_arrive(uint64_t* bar);
-// a barrier's word counts its phases that are over
-static bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
-  if ((*bar & 1) != parity) return true;
-  stop(AT_LOOK);
-  return false;
-}
-constexpr int kKvPage = 64;
-"""
-
-
 @pytest.fixture(scope="module")
 def program(tmp_path_factory):
     if shutil.which("g++") is None:
         pytest.skip("no g++")
-    chunk, common = source("paged_attention_chunk.cu"), source("attention_common.cuh")
-    constants = [line for line in piece(chunk, "constexpr int kTile = 128;", "template <int D>").splitlines() if line.startswith("constexpr")]
-    pieces = [piece(common, "template <int D>\n__device__ __forceinline__ int swizzled", "\n}\n"), "\n".join(constants),
-              piece(chunk, "template <int D>\nstruct ChunkShape", "\n};\n"), piece(chunk, "struct Segment {", "\n};\n"),
-              piece(chunk, "constexpr int kSegmentRing", "\n\n"), piece(chunk, "struct ChunkShared {", "\n};\n"),
-              piece(chunk, "__device__ __forceinline__ int tile_exponent", "\n}\n"),
-              piece(chunk, "__device__ __forceinline__ bool wait_for", "// ------"),
-              piece(chunk, "template <int D>\n__device__ __forceinline__ void scale_role", "\n}\n")]
-    return build(tmp_path_factory.mktemp("scales"), EMULATOR + SHIM + "\n".join(pieces) + HARNESS)
+    return build(tmp_path_factory.mktemp("scales"), EMULATOR + ROLE_SHIM + role("scale_role") + HARNESS)
 
 
 @pytest.mark.parametrize("masked_from", range(13))
