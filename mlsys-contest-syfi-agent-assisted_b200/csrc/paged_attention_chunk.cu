@@ -751,11 +751,13 @@ __device__ __forceinline__ void put_queries(const __nv_bfloat16* q, long long mi
         hi[e] = h01 | static_cast<uint32_t>(h23) << 16;
         lo[e] = cvt_e4m3x2(x0 - f01.x, x1 - f01.y) | static_cast<uint32_t>(cvt_e4m3x2(x2 - f23.x, x3 - f23.y)) << 16;
       }
+      // (a row that is not finite is NaN throughout, so that the mask takes its scores out like any other's)
+      if (top >= 0x7f80u) hi[0] = hi[1] = lo[0] = lo[1] = 0x7f7f7f7fu;
       uint8_t* const to = hi_tile + swizzled<D>(row0 + row, part / 2) + part % 2 * 8;
       *reinterpret_cast<uint2*>(to) = make_uint2(hi[0], hi[1]);
       *reinterpret_cast<uint2*>(to + ChunkShape<D>::kTileBytes) = make_uint2(lo[0], lo[1]);
       // (a scale of zero keeps a factor, so that -infinity stays what it is)
-      if (part == 0) units[row] = top >= 0x7f80u ? __int_as_float(0x7fffffff) : fmaxf(fabsf(scale_log2) * __int_as_float((127 - k) << 23), 1e-30f);
+      if (part == 0) units[row] = fmaxf(fabsf(scale_log2) * __int_as_float((127 - k) << 23), 1e-30f);
     }
   }
 }

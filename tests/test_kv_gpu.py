@@ -313,6 +313,30 @@ def test_absent_pages_and_rows_that_see_nothing(q_lens, kv_lens, HQ, HK, D, pkg,
     assert (out[starts[2]] == 0).all()
 
 
+@pytest.mark.parametrize("q_lens,kv_lens", [([1, 1, 2], [100, 64, 1]), ([300, 64, 100], [1000, 64, 60])])
+@pytest.mark.parametrize("HQ,HK,D", [(16, 4, 128), (8, 1, 64)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_a_query_that_is_not_finite_and_sees_nothing(q_lens, kv_lens, HQ, HK, D, bad, pkg, kv):
+    """It gets zeros like any other; where it sees something its head is NaN; no other row is touched."""
+    inputs = _attention_inputs(kv, q_lens, kv_lens, HQ, HK, D, seed=12)
+    q, cache, table, lens, starts = inputs
+    table[1, :] = -1
+    clean = _attend(pkg, inputs)
+    rows = [0, q_lens[0], q_lens[0] + q_lens[1] - 1, q_lens[0] + q_lens[1], sum(q_lens) - 1]
+    for row in rows:
+        q[row, 1, 7] = bad
+    out = _attend(pkg, inputs)
+    blind = torch.zeros(q.shape[:2], dtype=torch.bool, device=DEV)
+    blind[starts[1]:starts[2]] = True
+    blind[starts[2]:starts[2] + max(q_lens[2] - kv_lens[2], 0)] = True
+    hit = torch.zeros_like(blind)
+    hit[rows, 1] = True
+    hit &= ~blind
+    assert (out[blind] == 0).all()
+    assert out[hit].isnan().all()
+    assert torch.equal(out[~hit], clean[~hit])
+
+
 @pytest.mark.parametrize("q_len,kv_len", [(1, 3000), (300, 3000)])
 def test_strides_scale_and_extremes(q_len, kv_len, pkg, kv):
     """Slices of fused rows and of a cache of several layers, another scale; scores far apart, one weight of nearly 1 and a long
