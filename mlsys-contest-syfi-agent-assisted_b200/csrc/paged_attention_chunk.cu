@@ -756,8 +756,8 @@ __device__ __forceinline__ void put_queries(const __nv_bfloat16* q, long long mi
       uint8_t* const to = hi_tile + swizzled<D>(row0 + row, part / 2) + part % 2 * 8;
       *reinterpret_cast<uint2*>(to) = make_uint2(hi[0], hi[1]);
       *reinterpret_cast<uint2*>(to + ChunkShape<D>::kTileBytes) = make_uint2(lo[0], lo[1]);
-      // (a scale of zero keeps a factor, so that -infinity stays what it is)
-      if (part == 0) units[row] = fmaxf(fabsf(scale_log2) * __int_as_float((127 - k) << 23), 1e-30f);
+      // (a scale of zero keeps a factor, f32's smallest normal number, so that -infinity stays what it is)
+      if (part == 0) units[row] = fmaxf(fabsf(scale_log2) * __int_as_float((127 - k) << 23), 1.17549435e-38f);
     }
   }
 }

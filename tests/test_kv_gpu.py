@@ -364,6 +364,17 @@ def test_strides_scale_and_extremes(q_len, kv_len, pkg, kv):
 
 
 @pytest.mark.parametrize("q_len", [1, 200])
+@pytest.mark.parametrize("q_factor,key_factor,scale", [(1e-32, 1e32, None), (1e-36, 1e20, 1e15), (1.0, 1e28, 1e-29), (1e25, 1e-25, None), (1.0, 1.0, 0.0)])
+def test_queries_keys_and_scales_of_any_size(q_len, q_factor, key_factor, scale, pkg, kv):
+    """Scores of ordinary size from factors that are not."""
+    q, cache, table, lens, starts = _attention_inputs(kv, [q_len], [700], 8, 2, 128, seed=13)
+    q *= q_factor
+    kv.views(cache)[1][:, 0] *= key_factor
+    inputs = (q, cache, table, lens, starts)
+    _check_attention(_attend(pkg, inputs, scale=scale), *kv.attention(*inputs, scale=scale))
+
+
+@pytest.mark.parametrize("q_len", [1, 200])
 @pytest.mark.parametrize("spike", [0, 1000, 29999])
 def test_one_large_weight_and_a_long_tail(q_len, spike, pkg, kv):
     """All positions but one have the same score, 17 octaves below the one: the tail's weights together are a quarter of it."""
