@@ -492,7 +492,7 @@ struct Device {
   int* status = nullptr;
   long long next_wait_limit = 0;   // syfi_kv_debug_wait_limit: applies to the next call, then clears itself
 };
-constexpr long long kWaitLimit = 1ll << 32;   // SM clocks (about two seconds)
+constexpr long long kWaitLimit = 1ll << 32;   // SM clocks without a finished tile (about two seconds)
 std::mutex g_mu;
 Device g_devices[64];
 
@@ -584,8 +584,8 @@ extern "C" int syfi_paged_attention(const void* q, int64_t q_stride, const void*
   return rows <= 8 ? launch_decode<64, 1>(a, d, sms, st) : launch_decode<64, 2>(a, d, sms, st);
 }
 
-// Test hook for the bounded waits, no part of the interface: a wait of the next attention call's kernel on the current device may
-// take this many SM clocks (0: the normal limit).
+// Test hook for the bounded waits, no part of the interface: a CTA of the next attention call's kernel on the current device may
+// go without finishing a tile for this many SM clocks (0: the normal limit).
 extern "C" int syfi_kv_debug_wait_limit(int64_t clocks) {
   if (clocks < 0) return kv_fail(SYFI_KV_ERR_INVALID, "a wait limit must not be negative");
   int dev = 0;

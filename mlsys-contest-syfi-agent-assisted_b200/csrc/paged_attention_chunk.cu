@@ -88,7 +88,8 @@ struct ChunkShared {
   float unit[256];                     // of each row: what a score is worth
   volatile int redo[kSegmentRing];     // of the segment: f16 did not hold a value
   volatile int abort_code;
-  volatile uint32_t most_looks;        // at a barrier in one wait
+  volatile uint32_t tiles_done;        // or what else shows that the CTA goes on
+  volatile int done;                   // every segment is
   int finished;                        // segments of this CTA whose results are written
   int asked_k, asked_v, asked_scales;  // loads that the producer has issued
 };
@@ -229,14 +230,13 @@ __device__ __forceinline__ void exact_row(const AttentionArgs& a, int base, int 
         __floats2bfloat162_rn(acc[2 * i] * inv, acc[2 * i + 1] * inv);
 }
 
-// Waits, bounded like the ones in ptx.cuh, in few instructions: this kernel's roles together have more code than the instruction cache
-// of an SM holds, and its warps spend much of their time in these.  So a wait counts its looks at the barrier (each is suspended for a
-// while by the hardware) and leaves the clock alone; a suspend hint turned into a loop of short sleeps.
+// Waits in few instructions: this kernel's roles together have more code than the instruction cache of an SM holds, and its warps spend
+// much of their time in these.  So a wait only asks whether somebody gave up, and the clock is the planning thread's, which has time: it
+// gives up when no tile was finished for the limit (the clock in every wait: a batch of 4 to 92 rows a unit 75.2 us instead of 68.4).  (A
+// suspend hint turned into a loop of short sleeps.)
 __device__ __forceinline__ bool wait_for(ChunkShared& sh, uint64_t* bar, uint32_t parity) {
-  for (uint32_t looks = 0; !mbar_try_wait(bar, parity); ++looks) {
-    if (looks > sh.most_looks) sh.abort_code = kStatusChunkTimeout;
+  while (!mbar_try_wait(bar, parity))
     if (sh.abort_code != 0) return false;
-  }
   return true;
 }
 // The same for warps that have to stay whole: a lane whose wait ran out goes on, and the warp asks for the abort code later.
@@ -255,14 +255,31 @@ struct Ring {
   }
 };
 
-// ---------------------------------------------------------------- planning (one thread)
+// ---------------------------------------------------------------- planning, and the clock (one thread)
+struct Watch {
+  long long limit, since;
+  uint32_t seen;
+  __device__ bool over(ChunkShared& sh) {
+    const long long now = clock64();
+    if (sh.tiles_done != seen) {
+      seen = sh.tiles_done;
+      since = now;
+    } else if (now - since > limit) {
+      sh.abort_code = kStatusChunkTimeout;
+    }
+    return sh.abort_code != 0;
+  }
+};
+
 __device__ __forceinline__ void plan_role(const AttentionArgs& a, const ChunkPlan& plan, const PlanShared& s_plan, ChunkShared& sh, int places,
-                                          long long w1, long long total, int ctas) {
+                                          long long w1, long long total, int ctas, long long wait_limit) {
+  Watch watch = {wait_limit, clock64(), 0u};
   ChunkCursor at;
   at.start(plan, s_plan, places);
   Ring<kSegmentRing> ring;
   while (true) {
-    if (!wait_for(sh, &sh.segment_empty[ring.stage], ring.parity ^ 1u)) return;
+    while (!mbar_try_wait(&sh.segment_empty[ring.stage], ring.parity ^ 1u))
+      if (watch.over(sh)) return;
     Segment& g = sh.segment[ring.stage];
     const bool more = at.left > 0;
     const int places = more ? at.tiles_here() : 0;
@@ -295,10 +312,11 @@ __device__ __forceinline__ void plan_role(const AttentionArgs& a, const ChunkPla
       g.first_slot = parts.first_slot;
     }
     mbar_arrive(&sh.segment_full[ring.stage]);
-    if (!more) return;
+    if (!more) break;
     ring.next();
     at.advance(plan, places);
   }
+  while (sh.done == 0 && !watch.over(sh)) __nanosleep(200);
 }
 
 // ---------------------------------------------------------------- loads (one thread)
@@ -778,7 +796,10 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
     wait_whole_warp(sh, &sh.segment_full[segment & 3], segment >> 2 & 1);
     if (softmax_bar_any(sh.abort_code != 0)) return;      // all sixteen warps meet here whatever failed, and leave together
     const Segment& g = sh.segment[segment & 3];
-    if (g.tiles == 0) return;
+    if (g.tiles == 0) {
+      if (tid == 0) sh.done = 1;
+      return;
+    }
     // whether the next tile is this slot's (bit 0: no), and whether that changes with each (bit 1)
     unsigned turn = g.turns ? 2u + slot : g.rows <= slot * kSlotRows;
     float m = -INFINITY, l = 0.0f;
@@ -827,6 +848,7 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.scale_empty[stage]);
         ++tile;
+        if (tid == 0) sh.tiles_done = tile;
         turn ^= turn >> 1 & 1u;
         low -= kTile;
         high -= kTile;
@@ -1008,7 +1030,8 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
       sh.redo[i] = 0;
     }
     sh.abort_code = 0;
-    sh.most_looks = static_cast<uint32_t>(min(wait_limit / 64, 0xffffff00ll));
+    sh.tiles_done = 0u;
+    sh.done = 0;
     sh.finished = 0;
     sh.asked_k = sh.asked_v = sh.asked_scales = 0;
     fence_barrier_init();
@@ -1035,7 +1058,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
     } else if (lane == 0) {
       if (warp == 20) mma_role<D>(sh, smem, tmem);
       if (warp == 21) load_role<D>(map, a, sh, smem);
-      if (warp == 22) plan_role(a, plan, s_plan, sh, places, w1, total, ctas);
+      if (warp == 22) plan_role(a, plan, s_plan, sh, places, w1, total, ctas, wait_limit);
     }
     __syncwarp();
   }
@@ -1061,10 +1084,12 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
     // counters at zero.
     ChunkCursor at;
     at.start(plan, s_plan, places);
+    bool unfinished = false;                  // (the last tile's time may run out when all that is left is to leave)
     for (int segment = 0; at.left > 0; ++segment) {
       const int n = at.tiles_here(), rows = at.rows(a.group);
       const bool whole = n == at.span.tiles;
       if (segment >= sh.finished) {
+        unfinished = true;
         if (whole) {
           for (int x = tid; x < rows * D; x += kChunkThreads) {
             const int r = at.rt * kChunkRows + x / D;
@@ -1093,7 +1118,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
       }
       at.advance(plan, n);
     }
-    if (tid == 0) atomicExch(status, sh.abort_code);
+    if (tid == 0 && unfinished) atomicExch(status, sh.abort_code);
   }
   __syncthreads();
   if (warp == 20) {

@@ -135,8 +135,12 @@ static unsigned __float_as_uint(float f) { return static_cast<unsigned>(__float_
 static float ex2(float x) { return exp2f(x); }
 static void fence_proxy_async_smem() {}
 static void mbar_arrive(uint64_t* bar);
+static long long clocks, look_clocks;           // now, and what a look takes that finds a barrier closed
+static long long clock64() { return clocks; }
+static void __nanosleep(unsigned n) { clocks += 2 * n; stop(AT_LOOK); }
 static bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
   if ((*bar & 1) != parity) return true;
+  clocks += look_clocks;
   stop(AT_LOOK);                               // (the hardware waits a while, too)
   return (*bar & 1) != parity;
 }
@@ -144,12 +148,12 @@ constexpr int kKvPage = 64;
 """
 
 
-def role(name):
-    """The chunk kernel's shared memory and the function `name`, as C++ for the host."""
+def role(*names):
+    """The chunk kernel's shared memory, its waits and the functions `names`, as C++ for the host."""
     chunk, common = source("paged_attention_chunk.cu"), source("attention_common.cuh")
     constants = [line for line in piece(chunk, "constexpr int kTile = 128;", "template <int D>").splitlines() if line.startswith("constexpr")]
     return "\n".join([
         piece(common, "template <int D>\n__device__ __forceinline__ int swizzled", "\n}\n"), *constants, piece(chunk, "template <int D>\nstruct ChunkShape", "\n};\n"),
         piece(chunk, "struct Segment {", "\n};\n"), piece(chunk, "constexpr int kSegmentRing", "\n\n"), piece(chunk, "struct ChunkShared {", "\n};\n"),
         piece(chunk, "__device__ __forceinline__ int tile_exponent", "\n}\n"), piece(chunk, "__device__ __forceinline__ bool wait_for", "// ------"),
-        piece(chunk, "template <int D>\n__device__ __forceinline__ void %s(" % name, "\n}\n")])
+        *(piece(chunk, "template <int D>\n__device__ __forceinline__ void %s(" % name, "\n}\n") for name in names)])

@@ -48,7 +48,6 @@ struct World {
   }
   static int run(int n) {
     fail_after = n;
-    sh.most_looks = 1u << 30;
     a.cache = {smem, 1 << 16, 64, 2, 1};
     a.batch = {table, nullptr, nullptr, 1, 64, 1};
     run_block(32, [] { if (threadIdx.x == 0) load_role<D>(CUtensorMap(), a, sh, smem); }, 0, step);

@@ -49,7 +49,6 @@ struct World {
   static int run() {
     memset(smem, 0x7f, sizeof(smem));
     sh = ChunkShared{};
-    sh.most_looks = 1u << 30;
     run_block(32, [] { scale_role<D>(sh, smem); }, 0, step);
     if (cleaned != kTiles) { printf("%d tiles\n", cleaned); ++bad; }
     return bad != 0;
@@ -73,7 +72,7 @@ int main(int, char** argv) {
 def program(tmp_path_factory):
     if shutil.which("g++") is None:
         pytest.skip("no g++")
-    return build(tmp_path_factory.mktemp("scales"), EMULATOR + ROLE_SHIM + role("scale_role") + HARNESS)
+    return build(tmp_path_factory.mktemp("scales"), EMULATOR + ROLE_SHIM + role("scale_role") + "\n" + HARNESS)
 
 
 @pytest.mark.parametrize("masked_from", range(13))
