@@ -14,7 +14,7 @@ struct AttentionArgs {
   int group, window;
   float scale_log2;
   int* tickets;          // [CTAs] zero between calls
-  float* partial;        // [2 * CTAs][rows][D] sums (the chunk kernel: [2 * CTAs][D / 4][rows][4]), then [2 * CTAs][rows] of (m, l, n, redo)
+  float* partial;        // [2 * CTAs][rows][D] sums (the chunk kernel: [2 * CTAs][D / 4][rows][4]), then [2 * CTAs][rows] of (m, l, n, doubt)
 };
 
 // paged_attention_chunk.cu.  Bytes of `partial` that a launch on `ctas` CTAs needs, and the launch.

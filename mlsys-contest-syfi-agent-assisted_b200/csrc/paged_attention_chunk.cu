@@ -14,8 +14,9 @@
 // 178 us, in turns 141).
 //
 // The sum's reference follows a row's largest score only when that has grown by 2^8 (kGrowth), so O is hardly ever rescaled.
-// What f16 cannot hold is computed again: a unit that meets a value scale below 2^-19 of the largest is redone row by row in f32
-// (exact_row).
+// What f16 cannot hold is computed again: where a unit meets a value scale below 2^-19 of the largest, the rows whose sums are so small
+// that its rounding could show are redone one by one in f32 (kDoubt, exact_row).  The 8192-token prompt with one such value in every key head:
+// 1.4 ms instead of 0.7; all rows of the units that meet it 797 ms.
 //
 // What bounds it is that chain: a wide tile of 256 rows takes 5200 clocks, of which the tensor core works 2048 and the exponentials 2048
 // (16 per clock).  A prompt of 8192 tokens, 32 heads of 128 over 8: 654 us (841 TFLOP/s of what is visible)
@@ -36,12 +37,14 @@ constexpr int kSlotRows = 128;         // units of at most so many rows use one 
 using ChunkPlan = Plan<kTile, kChunkRows, kChunkExtra, kSlotRows>;
 using ChunkCursor = Cursor<kTile, kChunkRows, kChunkExtra, kSlotRows>;
 constexpr int kScaleStages = 4;
-constexpr int kRedoWarps = 4;          // of the softmax warps, redo rows
 constexpr int kStatusChunkTimeout = 301;
 constexpr int kNoValue = 0x7fffffff;   // in a key's scale: a NaN, and its value's bytes are not looked at
 constexpr int kUnitShift = 5;          // the largest value scale becomes 2^4 .. 2^5 when the unit's reference is set, ...
 constexpr int kUnitGrowth = 2;         // ... and may grow to 2^7 (448 * 2^7 < 65504) before the reference follows
 constexpr float kSmallestUnit = 6.103515625e-5f;   // 2^-14: f16's smallest normal number
+// A value below that is off by up to 2^-25, so a row's sum by 2^-25 of its weights' sum; where a sum is smaller than 2^-14 of it, which would
+// be an error of more than 2^-11, the row is computed again.
+constexpr float kDoubt = 6.103515625e-5f;
 
 template <int D>
 struct ChunkShape {
@@ -55,8 +58,7 @@ struct ChunkShape {
   static constexpr int kV = kK + kKStages * kTileBytes;
   static constexpr int kHalf = kV + kVStages * kTileBytes;        // [D / 64][128 positions][64] f16 per stage
   static constexpr int kScales = kHalf + kHalfStages * kHalfBytes;  // [K 128 f32][V 128 f32] per stage
-  static constexpr int kRedo = kScales + kScaleStages * 2 * kTile * 4;   // [kRedoWarps][D + 64] f32
-  static constexpr int kSmem = 1024 + kRedo + kRedoWarps * (D + kKvPage) * 4;
+  static constexpr int kSmem = 1024 + kScales + kScaleStages * 2 * kTile * 4;
 };
 
 // A piece of a unit, as the planning warp describes it to the others.
@@ -84,9 +86,10 @@ struct ChunkShared {
   int exponent[kScaleStages];          // the values' reference as of the tile: 2^exponent
   float fade[kScaleStages];            // what it has become smaller by since the slot's tile before (1: nothing)
   float top[2][2][2][128];             // [tile parity][slot][half][row]: a row's largest score in half of a tile
-  float end[2][3][128];                // [slot][sum of each half, reference][row], at a segment's end
+  float end[2][4][128];                // [slot][sum of each half, reference, values' reference][row], at a segment's end
   float unit[256];                     // of each row: what a score is worth
   volatile int redo[kSegmentRing];     // of the segment: f16 did not hold a value
+  uint32_t again[kChunkRows / 32];     // bit by row: the unit's rows whose result that touched
   volatile int abort_code;
   volatile uint32_t tiles_done;        // or what else shows that the CTA goes on
   volatile int done;                   // every segment is
@@ -110,16 +113,17 @@ __device__ __forceinline__ int tile_exponent(const float* v_scale, int there, in
   return max(static_cast<int>(top >> 23) - 126, -100);
 }
 
-// join_parts for partial sums that are kept by dimension: a thread has a row and sixteen of its dimensions.
+// join_parts for partial sums that are kept by dimension: a thread has a row and sixteen of its dimensions.  Rows that have to be computed
+// again (kDoubt) are noted in `again`.
 template <int D>
-__device__ __forceinline__ void join_columns(const AttentionArgs& a, int q_first, int unit_row0, int head, int rows, int ctas, const Parts& parts, int thread,
-                                             int threads) {
+__device__ __forceinline__ void join_columns(const AttentionArgs& a, int q_first, int unit_row0, int head, int rows, int ctas, const Parts& parts, uint32_t* again,
+                                             int thread, int threads) {
   const float4* const stats = reinterpret_cast<const float4*>(a.partial + 2ll * ctas * kChunkRows * D);
   const float4* const sums = reinterpret_cast<const float4*>(a.partial);
   for (int i = thread; i < kChunkRows * (D / 16); i += threads) {
     const int row = i % kChunkRows, d16 = i / kChunkRows;
     if (row >= rows) continue;
-    float m = -INFINITY, l = 0.0f, o[16] = {};
+    float m = -INFINITY, l = 0.0f, doubt = 0.0f, o[16] = {};
 #pragma unroll 2
     for (int c = parts.first; c <= parts.last; ++c) {
       const long long slot = parts.slot(c);
@@ -129,6 +133,7 @@ __device__ __forceinline__ void join_columns(const AttentionArgs& a, int q_first
       for (int k = 0; k < 4; ++k) p[k] = __ldcg(sums + (slot * (D / 4) + 4 * d16 + k) * kChunkRows + row);
       const float m_new = fmaxf(m, st.x), m_ref = finite_or_zero(m_new), f = ex2(m - m_ref), w = ex2(st.x - m_ref);
       l = l * f + st.y * w;
+      doubt = doubt * f + st.w * w;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         o[4 * k] = o[4 * k] * f + p[k].x * w;
@@ -138,6 +143,10 @@ __device__ __forceinline__ void join_columns(const AttentionArgs& a, int q_first
       }
       m = m_new;
     }
+    bool small = false;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) small |= fabsf(o[k]) < doubt;
+    if (small) atomicOr(again + row / 32, 1u << (row % 32));
     const float f = l == 0.0f ? 0.0f : 1.0f / l;
     const int r = unit_row0 + row;
     uint4* const to = reinterpret_cast<uint4*>(a.out + (q_first + r / a.group) * a.out_stride + (head * a.group + r % a.group) * D + 16 * d16);
@@ -171,29 +180,39 @@ __device__ __forceinline__ bool softmax_bar_any(bool p) {
 // One row in f32 by one warp, for what the tiles cannot hold: a lane has two of a page's positions, then D / 32 dimensions.
 template <int D>
 __device__ __forceinline__ void exact_row(const AttentionArgs& a, int base, int q_first, int b, int head, int r, float* s_q, float* s_p) {
+  constexpr int kMine = D / 32;
   const int lane = threadIdx.x % 32, t = r / a.group;
   const int position = base + t, low = a.window > 0 ? max(position - a.window + 1, 0) : 0;
   const long long column = static_cast<long long>(head * a.group + r % a.group) * D;
   const __nv_bfloat16* q = a.q + (q_first + t) * a.q_stride + column;
   for (int d = lane; d < D; d += 32) s_q[d] = __bfloat162float(q[d]);
   __syncwarp();
-  float m = -INFINITY, l = 0.0f, acc[D / 32] = {};
+  float m = -INFINITY, l = 0.0f, acc[kMine] = {};
   for (int page = low / kKvPage; page * kKvPage <= position; ++page) {
     const int at = a.batch.block_table[static_cast<long long>(b) * a.batch.max_pages + page];
     if (at < 0 || at >= a.cache.num_pages) continue;
     const uint8_t* keys = kv_block<D>(a.cache, at, 0, head);
     const uint8_t* values = kv_block<D>(a.cache, at, 1, head);
     float x[2];
+#pragma unroll 1
     for (int i = 0; i < 2; ++i) {
       const int token = lane + 32 * i, j = page * kKvPage + token;
       x[i] = -INFINITY;
       if (j >= low && j <= position) {
-        float sum = 0.0f;
-        for (int d = 0; d < D; d += 2) {
-          const float2 f = e4m3x2_to_float2(*reinterpret_cast<const uint16_t*>(keys + token * D + d));
-          sum = fmaf(s_q[d], f.x, fmaf(s_q[d + 1], f.y, sum));
+        float sum[2] = {};
+#pragma unroll 2
+        for (int c = 0; c < D; c += 16) {
+          const uint4 p = *reinterpret_cast<const uint4*>(keys + token * D + c);
+          const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float4 y = *reinterpret_cast<const float4*>(s_q + c + 4 * k);
+            const float2 f = e4m3x2_to_float2(static_cast<uint16_t>(w[k])), g = e4m3x2_to_float2(static_cast<uint16_t>(w[k] >> 16));
+            sum[0] = fmaf(y.x, f.x, fmaf(y.y, f.y, sum[0]));
+            sum[1] = fmaf(y.z, g.x, fmaf(y.w, g.y, sum[1]));
+          }
         }
-        x[i] = sum * *reinterpret_cast<const float*>(keys + kKvPage * D + token * 4) * a.scale_log2;
+        x[i] = (sum[0] + sum[1]) * *reinterpret_cast<const float*>(keys + kKvPage * D + token * 4) * a.scale_log2;
       }
     }
     float top = fmaxf(x[0], x[1]);
@@ -201,8 +220,10 @@ __device__ __forceinline__ void exact_row(const AttentionArgs& a, int base, int 
     for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
     const float m_new = fmaxf(m, top), fade = ex2(m - finite_or_zero(m_new));
     l *= fade;
-    for (int i = 0; i < D / 32; ++i) acc[i] *= fade;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) acc[i] *= fade;
     m = m_new;
+#pragma unroll
     for (int i = 0; i < 2; ++i) {
       const float p = ex2(x[i] - finite_or_zero(m));
       l += p;
@@ -210,13 +231,14 @@ __device__ __forceinline__ void exact_row(const AttentionArgs& a, int base, int 
     }
     __syncwarp();
     const int first = max(low - page * kKvPage, 0), last = min(position - page * kKvPage, kKvPage - 1);
+#pragma unroll 4
     for (int token = first; token <= last; ++token) {
       const float p = s_p[token] * *reinterpret_cast<const float*>(values + kKvPage * D + token * 4);
 #pragma unroll
-      for (int i = 0; i < D / 64; ++i) {
-        const float2 f = e4m3x2_to_float2(*reinterpret_cast<const uint16_t*>(values + token * D + i * 64 + lane * 2));
-        acc[2 * i] = fmaf(p, f.x, acc[2 * i]);
-        acc[2 * i + 1] = fmaf(p, f.y, acc[2 * i + 1]);
+      for (int i = 0; i < kMine; i += 2) {
+        const float2 f = e4m3x2_to_float2(*reinterpret_cast<const uint16_t*>(values + token * D + lane * kMine + i));
+        acc[i] = fmaf(p, f.x, acc[i]);
+        acc[i + 1] = fmaf(p, f.y, acc[i + 1]);
       }
     }
     __syncwarp();
@@ -225,9 +247,8 @@ __device__ __forceinline__ void exact_row(const AttentionArgs& a, int base, int 
   for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-  for (int i = 0; i < D / 64; ++i)
-    *reinterpret_cast<__nv_bfloat162*>(a.out + (q_first + t) * a.out_stride + column + i * 64 + lane * 2) =
-        __floats2bfloat162_rn(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+  for (int i = 0; i < kMine; i += 2)
+    *reinterpret_cast<__nv_bfloat162*>(a.out + (q_first + t) * a.out_stride + column + lane * kMine + i) = __floats2bfloat162_rn(acc[i] * inv, acc[i + 1] * inv);
 }
 
 // Waits in few instructions: this kernel's roles together have more code than the instruction cache of an SM holds, and its warps spend
@@ -795,6 +816,7 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
   while (true) {
     wait_whole_warp(sh, &sh.segment_full[segment & 3], segment >> 2 & 1);
     if (softmax_bar_any(sh.abort_code != 0)) return;      // all sixteen warps meet here whatever failed, and leave together
+    if (tid < kChunkRows / 32) sh.again[tid] = 0u;        // (the segment before is over, and what this one notes comes behind the next such barrier)
     const Segment& g = sh.segment[segment & 3];
     if (g.tiles == 0) {
       if (tid == 0) sh.done = 1;
@@ -861,7 +883,10 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
         tc_fence_after();
         ++own_segments;
         sh.end[slot][half][in_slot] = l;
-        if (half == 0) sh.end[slot][2][in_slot] = m;
+        if (half == 0) {
+          sh.end[slot][2][in_slot] = m;
+          sh.end[slot][3][in_slot] = __int_as_float((exponent - kUnitShift + 127) << 23);
+        }
       }
     }
     if (softmax_bar_any(sh.abort_code != 0)) return;
@@ -871,15 +896,21 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
     if (tid == 0) sh.redo[(segment + 3) & 3] = 0;     // the segment before: everybody has read it
     if (active) {
       l = sh.end[slot][0][in_slot] + sh.end[slot][1][in_slot];
-      float f = __int_as_float((exponent - kUnitShift + 127) << 23);
+      float f = __int_as_float((exponent - kUnitShift + 127) << 23), doubt = redo ? kDoubt * l * f : 0.0f;
       if (turns) {                            // to the larger reference of the two slots'
-        const float(&its)[3][128] = sh.end[slot ^ 1];
-        const float its_m = its[2][in_slot], all = fmaxf(m, its_m), ref = finite_or_zero(all), fade = ex2(m - ref);
-        l = l * fade + (its[0][in_slot] + its[1][in_slot]) * ex2(its_m - ref);
+        const float(&its)[4][128] = sh.end[slot ^ 1];
+        const float its_m = its[2][in_slot], all = fmaxf(m, its_m), ref = finite_or_zero(all), fade = ex2(m - ref), its_l = (its[0][in_slot] + its[1][in_slot]) * ex2(its_m - ref);
+        l = l * fade + its_l;
+        doubt = redo ? doubt * fade + kDoubt * its_l * its[3][in_slot] : 0.0f;
         m = all;
         f *= fade;
       }
-      if (whole) f = l == 0.0f ? 0.0f : f / l;
+      if (whole) {
+        const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+        f = l == 0.0f ? 0.0f : f / l;
+        doubt *= inverse;
+      }
+      bool small = false;
       // Rows leave through the slot's q tiles, which nothing reads any more: 32 rows of D bytes per warp (half of the dimensions), swizzled,
       // then D / 16 lanes write a row's half.  Partial sums are kept by dimension, so that a warp's 32 rows lie side by side.
       uint8_t* const stage = smem + Shape::kQ + 2 * slot * Shape::kTileBytes + (half * 4 + warp % 4) * (32 * D);
@@ -913,6 +944,10 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
           named_bar_sync(across, 64);
           if (slot == 1) continue;
         }
+        if (redo) {
+#pragma unroll
+          for (int b = 0; b < 16; ++b) small |= fabsf(__uint_as_float(o[b])) < doubt;
+        }
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           if (whole) {
@@ -932,7 +967,8 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
           }
         }
       }
-      if (whole && !redo && !(turns && slot == 1)) {
+      if (whole && real && small) atomicOr(&sh.again[row / 32], 1u << (row % 32));
+      if (whole && !(turns && slot == 1)) {
         __syncwarp();
         constexpr int kLanes = D / 16, kTogether = 32 / kLanes;
         const long long mine = token_of_row * a.out_stride + column_of_row + half * (D / 2);
@@ -945,12 +981,12 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
         }
       }
       if (real && !whole && half == 0)
-        reinterpret_cast<float4*>(a.partial + 2ll * ctas * kChunkRows * D)[static_cast<long long>(part) * kChunkRows + row] = make_float4(m, l, 0.0f, redo ? 1.0f : 0.0f);
+        reinterpret_cast<float4*>(a.partial + 2ll * ctas * kChunkRows * D)[static_cast<long long>(part) * kChunkRows + row] = make_float4(m, l, 0.0f, doubt);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.o_empty[slot]);
     }
-    bool again = whole && redo;               // whether this CTA has to redo the unit row by row
+    bool again = whole && redo;               // whether this CTA has to look for rows to compute again
     if (!whole) {
       const Parts parts = parts_of(g);
       __threadfence();
@@ -963,14 +999,16 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
       named_bar_sync(1, kSoftmaxThreads);
       if (s_plan.last) {
         __threadfence();
-        const float4* stats = reinterpret_cast<const float4*>(a.partial + 2ll * ctas * kChunkRows * D);
-        for (int c = parts.first; c <= parts.last; ++c) again |= __ldcg(stats + static_cast<long long>(parts.slot(c)) * kChunkRows).w != 0.0f;
-        if (!again) join_columns<D>(a, g.q_first, g.row0, g.head, g.rows, ctas, parts, tid, kSoftmaxThreads);
+        join_columns<D>(a, g.q_first, g.row0, g.head, g.rows, ctas, parts, sh.again, tid, kSoftmaxThreads);
+        again = true;
       }
     }
-    if (again && warp < kRedoWarps) {
-      float* const s_q = reinterpret_cast<float*>(smem + Shape::kRedo) + warp * (D + kKvPage);
-      for (int x = warp; x < g.rows; x += kRedoWarps) exact_row<D>(a, g.base, g.q_first, g.b, g.head, g.row0 + x, s_q, s_q + D);
+    if (again) {
+      named_bar_sync(1, kSoftmaxThreads);     // all rows are written, all notes made
+      float* const s_q = reinterpret_cast<float*>(smem + Shape::kQ) + warp * (D + kKvPage);      // (nothing reads the q tiles any more)
+      const bool any = __any_sync(0xffffffffu, lane < kChunkRows / 32 && sh.again[lane] != 0u);
+      for (int x = warp; any && x < g.rows; x += kSoftmaxWarps)
+        if (sh.again[x / 32] >> (x % 32) & 1u) exact_row<D>(a, g.base, g.q_first, g.b, g.head, g.row0 + x, s_q, s_q + D);
     }
     if (tid == 0) ++sh.finished;
     // (the q tiles are written again behind this: by this warp's rows' own stage only when both warps of a row are through)
@@ -1111,7 +1149,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap map, const __grid_con
           __syncthreads();
           if (s_plan.last) {
             __threadfence();
-            join_columns<D>(a, at.s.first, at.rt * kChunkRows, at.head, rows, ctas, parts, tid, kChunkThreads);
+            join_columns<D>(a, at.s.first, at.rt * kChunkRows, at.head, rows, ctas, parts, sh.again, tid, kChunkThreads);
           }
           __syncthreads();
         }

@@ -441,6 +441,52 @@ def test_bounded_waits_run_out(q_lens, kv_lens, D, pkg, kv):
     assert failed >= 1, failed
 
 
+def _ms(f, calls=5):
+    times = []
+    for _ in range(calls + 1):
+        begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        begin.record()
+        f()
+        end.record()
+        torch.cuda.synchronize()
+        times.append(begin.elapsed_time(end))
+    return min(times[1:])
+
+
+@pytest.mark.parametrize("q_lens,kv_lens,D", [([3000], [3000], 128), ([300], [20000], 64), ([1, 80, 1, 200], [400, 3000, 9000, 5000], 128)])
+def test_one_tiny_value_is_right_and_does_not_cost_much(q_lens, kv_lens, D, pkg, kv):
+    """A value scale far below the others, which f16 does not hold beside them: only rows that it decides are computed again.  All rows of a
+    unit were, and a call took 200 to 1000 times as long."""
+    inputs = _attention_inputs(kv, q_lens, kv_lens, 32, 8, D, seed=15)
+    q, cache, table, lens, starts = inputs
+    plain = _ms(lambda: _attend(pkg, inputs))
+    for b in range(len(kv_lens)):
+        for position in (0, kv_lens[b] // 2):
+            kv.views(cache)[1][int(table[b, position // 64]), 1, :, position % 64] *= 2.0 ** -30
+    tiny = _ms(lambda: _attend(pkg, inputs))
+    _check_attention(_attend(pkg, inputs), *kv.attention(*inputs))
+    assert tiny < 20.0 * plain, (tiny, plain)
+
+
+@pytest.mark.parametrize("q_len,kv_len", [(300, 300), (300, 2000), (40, 2500), (2, 6000)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_rows_that_tiny_values_decide(q_len, kv_len, D, pkg, kv):
+    """Value scales 30 octaves apart, position by position, and queries of every other head that look away from the large ones."""
+    inputs = _attention_inputs(kv, [q_len, 30], [kv_len, 700], 16, 2, D, seed=16)
+    q, cache, table, lens, starts = inputs
+    _, scales = kv.views(cache)
+    values, _ = kv.views(cache)
+    large = torch.arange(64, device=DEV) % 7 == 3
+    scales[:, 1, :, ~large] *= 2.0 ** -30
+    values.view(torch.uint8)[:, 0, :, large] = 0
+    values.view(torch.uint8)[:, 0, :, large, 0] = 0xb8       # -1
+    scales[:, 0, :, large] = 60.0 * D ** 0.5            # a score of -60 for those heads
+    q[:, :, 0] = 0.0
+    q[:, ::2, 0] = 1.0
+    _check_attention(_attend(pkg, inputs), *kv.attention(*inputs))
+    assert not _attend(pkg, inputs).isnan().any()
+
+
 @pytest.mark.parametrize("q_lens,kv_lens", [([1] * 5, [900, 20000, 3, 64, 7000]), ([400, 3], [5000, 6000])])
 def test_attention_is_repeatable_on_several_streams_and_in_graphs(q_lens, kv_lens, pkg, kv):
     """The same bits in a row of calls, on side streams at once, and in a replayed graph whose inputs change."""
