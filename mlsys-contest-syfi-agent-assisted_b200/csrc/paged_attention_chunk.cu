@@ -91,7 +91,7 @@ struct ChunkShared {
   volatile int redo[kSegmentRing];     // of the segment: f16 did not hold a value
   uint32_t again[kChunkRows / 32];     // bit by row: the unit's rows whose result that touched
   volatile int abort_code;
-  volatile uint32_t tiles_done;        // or what else shows that the CTA goes on
+  volatile uint32_t tiles_done;        // and pages of rows that are computed again: it changes while the CTA goes on
   volatile int done;                   // every segment is
   int finished;                        // segments of this CTA whose results are written
   int asked_k, asked_v, asked_scales;  // loads that the producer has issued
@@ -179,7 +179,8 @@ __device__ __forceinline__ bool softmax_bar_any(bool p) {
 
 // One row in f32 by one warp, for what the tiles cannot hold: a lane has two of a page's positions, then D / 32 dimensions.
 template <int D>
-__device__ __forceinline__ void exact_row(const AttentionArgs& a, int base, int q_first, int b, int head, int r, float* s_q, float* s_p) {
+__device__ __forceinline__ void exact_row(const AttentionArgs& a, int base, int q_first, int b, int head, int r, float* s_q, float* s_p,
+                                          volatile uint32_t* going) {
   constexpr int kMine = D / 32;
   const int lane = threadIdx.x % 32, t = r / a.group;
   const int position = base + t, low = a.window > 0 ? max(position - a.window + 1, 0) : 0;
@@ -189,6 +190,7 @@ __device__ __forceinline__ void exact_row(const AttentionArgs& a, int base, int 
   __syncwarp();
   float m = -INFINITY, l = 0.0f, acc[kMine] = {};
   for (int page = low / kKvPage; page * kKvPage <= position; ++page) {
+    if (lane == 0) *going = *going + 1u;       // (whatever the other warps make of it: it changes)
     const int at = a.batch.block_table[static_cast<long long>(b) * a.batch.max_pages + page];
     if (at < 0 || at >= a.cache.num_pages) continue;
     const uint8_t* keys = kv_block<D>(a.cache, at, 0, head);
@@ -253,8 +255,8 @@ __device__ __forceinline__ void exact_row(const AttentionArgs& a, int base, int 
 
 // Waits in few instructions: this kernel's roles together have more code than the instruction cache of an SM holds, and its warps spend
 // much of their time in these.  So a wait only asks whether somebody gave up, and the clock is the planning thread's, which has time: it
-// gives up when no tile was finished for the limit (the clock in every wait: a batch of 4 to 92 rows a unit 75.2 us instead of 68.4).  (A
-// suspend hint turned into a loop of short sleeps.)
+// gives up when no tile, and no page of a row that is computed again, was finished for the limit.  (The clock in every wait: a batch of
+// units of 4 to 92 rows 75.2 us instead of 68.4.  A suspend hint turned into a loop of short sleeps.)
 __device__ __forceinline__ bool wait_for(ChunkShared& sh, uint64_t* bar, uint32_t parity) {
   while (!mbar_try_wait(bar, parity))
     if (sh.abort_code != 0) return false;
@@ -870,7 +872,7 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.scale_empty[stage]);
         ++tile;
-        if (tid == 0) sh.tiles_done = tile;
+        if (tid == 0) sh.tiles_done = sh.tiles_done + 1u;
         turn ^= turn >> 1 & 1u;
         low -= kTile;
         high -= kTile;
@@ -1008,7 +1010,7 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
       float* const s_q = reinterpret_cast<float*>(smem + Shape::kQ) + warp * (D + kKvPage);      // (nothing reads the q tiles any more)
       const bool any = __any_sync(0xffffffffu, lane < kChunkRows / 32 && sh.again[lane] != 0u);
       for (int x = warp; any && x < g.rows; x += kSoftmaxWarps)
-        if (sh.again[x / 32] >> (x % 32) & 1u) exact_row<D>(a, g.base, g.q_first, g.b, g.head, g.row0 + x, s_q, s_q + D);
+        if (sh.again[x / 32] >> (x % 32) & 1u) exact_row<D>(a, g.base, g.q_first, g.b, g.head, g.row0 + x, s_q, s_q + D, &sh.tiles_done);
     }
     if (tid == 0) ++sh.finished;
     // (the q tiles are written again behind this: by this warp's rows' own stage only when both warps of a row are through)

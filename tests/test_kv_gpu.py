@@ -487,6 +487,31 @@ def test_rows_that_tiny_values_decide(q_len, kv_len, D, pkg, kv):
     assert not _attend(pkg, inputs).isnan().any()
 
 
+@pytest.mark.parametrize("q_lens,kv_lens,D", [([2500, 200], [2500, 3000], 128), ([3000], [5000], 64)])
+def test_rows_that_are_computed_again_do_not_run_into_the_wait_limit(q_lens, kv_lens, D, pkg, kv):
+    """All queries look away from the one large value, so that every row of every unit is computed again.  That is no reason to give up,
+    though no tile is finished meanwhile: the limit is 2^18 clocks, a seventh of a millisecond."""
+    inputs = _attention_inputs(kv, q_lens, kv_lens, 32, 8, D, seed=14)
+    q, cache, table, lens, starts = inputs
+    values, scales = kv.views(cache)
+    first = table[:, 0].long()
+    scales[:, 1] *= 2.0 ** -30
+    scales[first, 1, :, 0] *= 2.0 ** 30
+    values.view(torch.uint8)[first, 0, :, 0] = 0
+    values.view(torch.uint8)[first, 0, :, 0, 0] = 0xb8       # -1
+    scales[first, 0, :, 0] = 60.0 * D ** 0.5                 # a score of -60
+    q[:, :, 0] = 1.0
+    out = torch.full_like(q, 7.0)
+    begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    assert pkg.load_library().syfi_kv_debug_wait_limit(ctypes.c_int64(1 << 18)) == 0
+    begin.record()
+    pkg.run_paged_attention(*inputs, out)
+    end.record()
+    pkg.kv_check()
+    assert begin.elapsed_time(end) > 1.0             # (else this tests nothing)
+    _check_attention(out, *kv.attention(*inputs))
+
+
 @pytest.mark.parametrize("q_lens,kv_lens", [([1] * 5, [900, 20000, 3, 64, 7000]), ([400, 3], [5000, 6000])])
 def test_attention_is_repeatable_on_several_streams_and_in_graphs(q_lens, kv_lens, pkg, kv):
     """The same bits in a row of calls, on side streams at once, and in a replayed graph whose inputs change."""
