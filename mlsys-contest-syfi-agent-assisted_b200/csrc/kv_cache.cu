@@ -349,8 +349,11 @@ T at(const int64_t* args, int i) {
     return v;
   } else return static_cast<T>(args[i]);
 }
+template <typename T>
+bool fits(int64_t word) { return !std::is_same_v<T, int32_t> || word == static_cast<int32_t>(word); }
 template <typename... Args, size_t... I>
 int spread(int (*fn)(Args...), const int64_t* args, std::index_sequence<I...>) {
+  if (!(fits<Args>(args[I]) && ...)) return kv_fail(SYFI_KV_ERR_INVALID, "an argument does not fit in 32 bits");
   return fn(at<Args>(args, static_cast<int>(I))...);
 }
 template <typename... Args>

@@ -138,6 +138,14 @@ def _plain_cache(t):
     return None
 
 
+def _window_of(window):
+    """As 32 bits: a window of 2^31 - 1 positions is as wide as any."""
+    window = int(window)
+    if window < 0:
+        raise ValueError("window must not be negative")
+    return window if window < 2 ** 31 else 2 ** 31 - 1
+
+
 def _stream_of(stream, device):
     return _raw_stream(device) if stream is None and _raw_stream is not None else _stream_ptr(stream, device)
 
@@ -295,7 +303,7 @@ def run_paged_attention(q, kv_cache, block_table, seq_lens, q_starts, out, *, sc
         _call(_lib().syfi_paged_attention_block, device,
               _pack_attention(q.data_ptr(), q_stride, kv_cache.data_ptr(), pages, page_stride, block_table.data_ptr(), max_pages,
                               seq_lens.data_ptr(), q_starts.data_ptr(), batch, tokens, q_heads, heads, dim,
-                              1.0 / math.sqrt(dim) if scale is None else float(scale), int(window), out.data_ptr(), out_stride, _stream_of(stream, device)))
+                              1.0 / math.sqrt(dim) if scale is None else float(scale), _window_of(window), out.data_ptr(), out_stride, _stream_of(stream, device)))
         return out
     pages, page_stride, kinds, heads, dim = _cache_of(kv_cache)
     dev = kv_cache.device
@@ -314,12 +322,11 @@ def run_paged_attention(q, kv_cache, block_table, seq_lens, q_starts, out, *, sc
     table_ptr = _expect(block_table, "block_table", _int, (batch, max_pages), dev)
     lens_ptr = _expect(seq_lens, "seq_lens", _int, (batch,), dev)
     starts_ptr = _expect(q_starts, "q_starts", _int, (batch + 1,), dev)
-    if window < 0:
-        raise ValueError("window must not be negative")
+    window = _window_of(window)
     if tokens and batch:
         _call(_lib().syfi_paged_attention_block, dev.index,
               _pack_attention(q.data_ptr(), q_stride, kv_cache.data_ptr(), pages, page_stride, table_ptr, max_pages, lens_ptr, starts_ptr, batch,
-                              tokens, q_heads, heads, dim, 1.0 / math.sqrt(dim) if scale is None else float(scale), int(window), out.data_ptr(),
+                              tokens, q_heads, heads, dim, 1.0 / math.sqrt(dim) if scale is None else float(scale), window, out.data_ptr(),
                               out_stride, _stream_ptr(stream, dev.index)))
     return out
 

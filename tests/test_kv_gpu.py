@@ -364,6 +364,13 @@ def test_strides_scale_and_extremes(q_len, kv_len, pkg, kv):
 
 
 @pytest.mark.parametrize("q_len", [1, 200])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 32 + 100, 2 ** 40 + 1])
+def test_windows_wider_than_any_sequence(q_len, window, pkg, kv):
+    inputs = _attention_inputs(kv, [q_len], [700], 8, 2, 128, seed=17)
+    assert torch.equal(_attend(pkg, inputs, window=window), _attend(pkg, inputs))
+
+
+@pytest.mark.parametrize("q_len", [1, 200])
 @pytest.mark.parametrize("q_factor,key_factor,scale", [(1e-32, 1e32, None), (1e-36, 1e20, 1e15), (1.0, 1e28, 1e-29), (1e25, 1e-25, None), (1.0, 1.0, 0.0)])
 def test_queries_keys_and_scales_of_any_size(q_len, q_factor, key_factor, scale, pkg, kv):
     """Scores of ordinary size from factors that are not."""

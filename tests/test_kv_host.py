@@ -101,3 +101,20 @@ def test_oracle_against_a_dense_computation():
     x = torch.randn(3, 2, 64, generator=g)
     turned = kv.head_vectors(x, None, torch.tensor([[0.0] * 32 + [1.0] * 32]), torch.zeros(3), interleaved=False)
     assert torch.allclose(turned[..., :32], -x[..., 32:].double()) and torch.allclose(turned[..., 32:], x[..., :32].double())
+
+
+@pytest.mark.parametrize("name,index", [("syfi_paged_attention", 15), ("syfi_paged_attention", 11), ("syfi_paged_attention", 6), ("syfi_kv_write", 9), ("syfi_kv_read", 4)])
+@pytest.mark.parametrize("value", [2 ** 32 + 1, 2 ** 31, -2 ** 32 + 1])
+def test_a_block_refuses_what_does_not_fit_in_32_bits(name, index, value, pkg):
+    """A block's words are 64 bits wide, some of the arguments they stand for 32: no word is cut.  (No call here has any work.)"""
+    p = 4096
+    blocks = {"syfi_paged_attention": [p, 256, p, 9, 4 * 8448, p, 3, p, p, 0, 0, 2, 2, 128, 1.0, 0, p, 256, 0],
+              "syfi_kv_write": [p, p, p, p, p, p, p, p, 0, 2, 1, 128, 128, 0, 9, 256, 128, 128, 256, 1e-6, p, 2, 2 * 8448, 2, p, 0],
+              "syfi_kv_read": [p, 2, 2 * 8448, 2, 1, 128, p, 0, 0, p, p, 0]}
+    module = import_module(pkg.__name__ + ".kv")
+    call = _fn(pkg, name + "_block")
+    assert call(module._block(name)(*blocks[name])) == 0
+    args = list(blocks[name])
+    args[index] = value
+    assert call(module._block(name)(*args)) == 1
+    assert "32 bits" in pkg.load_library().syfi_moe_last_error().decode()
