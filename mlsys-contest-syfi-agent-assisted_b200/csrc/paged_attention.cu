@@ -555,7 +555,7 @@ extern "C" int syfi_paged_attention(const void* q, int64_t q_stride, const void*
   a.cache = {static_cast<uint8_t*>(const_cast<void*>(cache)), page_stride, static_cast<int>(num_pages), 2, kv_heads};
   a.batch = {block_table, seq_lens, q_starts, batch, max_pages, static_cast<int>(tokens)};
   a.group = q_heads / kv_heads;
-  a.window = window;
+  a.window = window < max_pages * kKvPage ? window : 0;      // (one as wide as any sequence is none; position - window stays in 32 bits)
   a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
   int dev = 0;
   cudaGetDevice(&dev);

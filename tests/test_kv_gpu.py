@@ -370,6 +370,15 @@ def test_windows_wider_than_any_sequence(q_len, window, pkg, kv):
     assert torch.equal(_attend(pkg, inputs, window=window), _attend(pkg, inputs))
 
 
+@pytest.mark.parametrize("q_len", [5, 200])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 100, 2 ** 20])
+def test_wide_windows_over_sequences_shorter_than_their_new_tokens(q_len, window, pkg, kv):
+    """The first queries' positions are negative."""
+    inputs = _attention_inputs(kv, [q_len, 1], [q_len, 100], 8, 2, 128, seed=18)
+    inputs[3][0] = q_len // 2
+    _check_attention(_attend(pkg, inputs, window=window), *kv.attention(*inputs, window=window))
+
+
 @pytest.mark.parametrize("q_len", [1, 200])
 @pytest.mark.parametrize("q_factor,key_factor,scale", [(1e-32, 1e32, None), (1e-36, 1e20, 1e15), (1.0, 1e28, 1e-29), (1e25, 1e-25, None), (1.0, 1.0, 0.0)])
 def test_queries_keys_and_scales_of_any_size(q_len, q_factor, key_factor, scale, pkg, kv):
