@@ -67,9 +67,8 @@ int syfi_kv_read(const void* cache, int64_t num_pages, int64_t page_stride, int3
  * Positions that a query does not see do not touch its result, whatever the cache holds there.  Scales are not negative.
  * Calls on different streams may run at the same time: every stream has a scratch buffer of its own (up to 45 MB), which
  * grows on demand (that waits for the device).  Up to eight streams of a device hold one; a ninth waits for the device and takes
- * over the least recently used.  A captured graph keeps using the buffer that its stream had then: do not replay two graphs
- * captured on one stream at the same time, nor beside calls on that stream; and where more than eight streams call, capture
- * after a call of the same kind, and replay beside no other call. */
+ * over the least recently used.  A captured graph has buffers of its own, one for each stream that was captured into it, until it is
+ * destroyed: it may be replayed beside anything but itself. */
 int syfi_paged_attention(const void* q, int64_t q_stride, const void* cache, int64_t num_pages, int64_t page_stride,
                          const int32_t* block_table, int32_t max_pages, const int32_t* seq_lens, const int32_t* q_starts,
                          int32_t batch, int64_t tokens, int32_t q_heads, int32_t kv_heads, int32_t head_dim, double scale,

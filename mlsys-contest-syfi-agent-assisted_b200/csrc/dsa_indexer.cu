@@ -679,7 +679,7 @@ extern "C" int syfi_dsa_topk_indexer(const void* q_index_fp8, const void* k_inde
   const size_t n_scores = static_cast<size_t>(batch) * max_ls;
   const size_t need = n_scores + 2 * static_cast<size_t>(batch) * ((max_ls + kTokTile - 1) / kTokTile);
   int rc = SYFI_DSA_OK;
-  Scratch* const s = d.scratch.get(st, need * sizeof(float), 0, SYFI_DSA_ERR_CUDA, &rc);
+  ScratchBuffer* const s = d.scratch.get(st, need * sizeof(float), 0, SYFI_DSA_ERR_CUDA, &rc);
   if (!s) return rc;
   if (!d.status) {
     if (cudaMalloc(&d.status, 16) != cudaSuccess) return fail(SYFI_DSA_ERR_CUDA, "out of device memory");

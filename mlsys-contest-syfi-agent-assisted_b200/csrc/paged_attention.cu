@@ -504,7 +504,7 @@ bool raise_decode() {
 constexpr size_t kTicketBytes = 4096;      // 1024 CTAs
 
 bool take_scratch(AttentionArgs& a, Device& d, size_t partial, cudaStream_t st, int* rc) {
-  Scratch* const s = d.scratch.get(st, kTicketBytes + partial, kTicketBytes, SYFI_KV_ERR_CUDA, rc);
+  ScratchBuffer* const s = d.scratch.get(st, kTicketBytes + partial, kTicketBytes, SYFI_KV_ERR_CUDA, rc);
   if (!s) return false;
   a.tickets = static_cast<int*>(s->memory);
   a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(s->memory) + kTicketBytes);

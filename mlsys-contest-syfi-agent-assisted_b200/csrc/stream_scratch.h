@@ -1,11 +1,14 @@
 // Scratch memory of the operators that have no context of their own: one buffer per stream, so that calls on one stream follow
-// each other in theirs and calls on two streams never meet; and the driver functions they need without a link to libcuda.
+// each other in theirs and calls on two streams never meet, and buffers of their own for captured graphs; and the driver functions
+// they need without a link to libcuda.
 #pragma once
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <mutex>
+#include <new>
 
 #include "moe_internal.h"
 
@@ -52,26 +55,39 @@ struct RelaxedCapture {
   ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
 };
 
-// A stream is known by its id, which is never given out twice (a handle may be, after the stream was destroyed); a stream
-// that is being captured cannot be asked for it and is known by its handle.
-struct Scratch {
-  cudaStream_t handle = nullptr;
-  unsigned long long id = 0; // 0: not known yet
-  uint64_t last_use = 0;     // 0: free
+struct ScratchBuffer {
   void* memory = nullptr;
   size_t bytes = 0;
-  bool captured = false;     // a graph may use it
+};
+
+// A stream is known by its id, which is never given out twice (a handle may be, after the stream was destroyed).
+struct Scratch : ScratchBuffer {
+  unsigned long long id = 0;
+  uint64_t last_use = 0;     // 0: free
 };
 constexpr int kMaxScratch = 8;   // streams of a device that hold one at a time; the next one takes over the least recently used
+
+// A captured graph uses its buffer whenever it is replayed, so that buffer is no stream's, is never freed, and is another graph's only when
+// the graph is gone, which a user object of the graph tells.  Branches of a graph that may run at the same time are captured on
+// different streams and have one each.
+struct GraphScratch : ScratchBuffer {
+  unsigned long long capture = 0;
+  cudaStream_t stream = nullptr;
+  std::atomic<bool> taken{false};
+  GraphScratch* next = nullptr;
+  static void CUDART_CB release(void* self) { static_cast<GraphScratch*>(self)->taken.store(false, std::memory_order_release); }
+};
 
 // One operator's buffers of one device.  The caller holds a lock.
 struct ScratchPool {
   Scratch scratch[kMaxScratch];
   uint64_t calls = 0;
+  GraphScratch* graphs = nullptr;
 
-  // The stream's buffer of at least `need` bytes; null with the error code in *rc when there is none.  The first `zeroed` bytes
-  // of a new buffer are zero.
-  Scratch* get(cudaStream_t st, size_t need, size_t zeroed, int error, int* rc);
+  // The stream's buffer of at least `need` bytes, or that of the graph that it captures; null with the error code in *rc when there is
+  // none.  The first `zeroed` bytes of a new buffer are zero.
+  ScratchBuffer* get(cudaStream_t st, size_t need, size_t zeroed, int error, int* rc);
+  ScratchBuffer* get_for_graph(cudaStream_t st, size_t need, size_t zeroed, int error, int* rc);
 };
 
 inline bool zero_now(void* p, size_t bytes) {     // on a stream of its own: the caller's may be capturing
@@ -83,71 +99,99 @@ inline bool zero_now(void* p, size_t bytes) {     // on a stream of its own: the
   return ok;
 }
 
-inline Scratch* ScratchPool::get(cudaStream_t st, size_t need, size_t zeroed, int error, int* rc) {
+// Null memory when there is none to be had.
+inline ScratchBuffer new_buffer(size_t bytes, size_t zeroed) {
+  ScratchBuffer b;
+  RelaxedCapture relaxed;
+  if (cudaMalloc(&b.memory, bytes) != cudaSuccess) return {};
+  if (!zero_now(b.memory, zeroed)) {
+    cudaFree(b.memory);
+    return {};
+  }
+  b.bytes = bytes;
+  return b;
+}
+
+inline ScratchBuffer* ScratchPool::get_for_graph(cudaStream_t st, size_t need, size_t zeroed, int error, int* rc) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long capture = 0;
+  cudaGraph_t graph = nullptr;
+  if (cudaStreamGetCaptureInfo_v2(st, &status, &capture, &graph, nullptr, nullptr) != cudaSuccess || status != cudaStreamCaptureStatusActive) {
+    *rc = set_last_error(error, "the stream's capture is not in order");
+    return nullptr;
+  }
+  GraphScratch* g = nullptr;
+  for (GraphScratch* c = graphs; c; c = c->next) {
+    if (c->bytes < need) continue;
+    const bool taken = c->taken.load(std::memory_order_acquire);
+    if (taken && c->capture == capture && c->stream == st) return c;      // of an earlier call in this capture
+    if (!taken && (!g || c->bytes < g->bytes)) g = c;
+  }
+  const bool fresh = !g;
+  if (fresh) {
+    const ScratchBuffer b = new_buffer(need, zeroed);
+    g = b.memory ? new (std::nothrow) GraphScratch : nullptr;
+    if (!g) {
+      if (b.memory) cudaFree(b.memory);
+      *rc = set_last_error(error, "out of memory for a graph's scratch buffer");
+      return nullptr;
+    }
+    static_cast<ScratchBuffer&>(*g) = b;
+    g->next = graphs;
+    graphs = g;
+  }
+  g->capture = capture;
+  g->stream = st;
+  cudaUserObject_t object;
+  g->taken.store(true, std::memory_order_relaxed);
+  if (cudaUserObjectCreate(&object, g, GraphScratch::release, 1, cudaUserObjectNoDestructorSync) != cudaSuccess) {
+    g->taken.store(false, std::memory_order_relaxed);
+    *rc = set_last_error(error, "cannot tie a scratch buffer to the graph");
+    return nullptr;
+  }
+  if (cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove) != cudaSuccess) {
+    cudaUserObjectRelease(object, 1);
+    *rc = set_last_error(error, "cannot tie a scratch buffer to the graph");
+    return nullptr;
+  }
+  return g;
+}
+
+inline ScratchBuffer* ScratchPool::get(cudaStream_t st, size_t need, size_t zeroed, int error, int* rc) {
   const Driver& drv = driver();
   CUstreamCaptureStatus capture = CU_STREAM_CAPTURE_STATUS_NONE;
   unsigned long long id = 0;
   bool known = drv.is_capturing && drv.stream_id;
   if (known && drv.is_capturing(st, &capture) != CUDA_SUCCESS) capture = CU_STREAM_CAPTURE_STATUS_NONE;   // the default stream beside a capture: the launch will say so
-  const bool capturing = capture != CU_STREAM_CAPTURE_STATUS_NONE;
-  if (known && !capturing) known = drv.stream_id(st, &id) == CUDA_SUCCESS;
-  if (!known) {
+  if (known && capture != CU_STREAM_CAPTURE_STATUS_NONE) return get_for_graph(st, need, zeroed, error, rc);
+  if (!known || drv.stream_id(st, &id) != CUDA_SUCCESS) {
     *rc = set_last_error(error, "not a stream of the current device");
     return nullptr;
   }
-  // The stream's own; of two (below) the larger.
-  Scratch *s = nullptr, *spare = nullptr;
+  Scratch *s = nullptr, *oldest = &scratch[0];
   for (Scratch& c : scratch) {
-    if (c.last_use == 0) spare = &c;
-    else if ((capturing || c.id == 0 ? c.handle == st : c.id == id) && (!s || c.bytes > s->bytes)) s = &c;
+    if (c.last_use != 0 && c.id == id) s = &c;
+    if (c.last_use < oldest->last_use) oldest = &c;
   }
-  if (s && s->bytes < need && (capturing || s->captured) && spare) s = nullptr;   // a graph keeps the small one
-  if (capturing && !spare && (!s || s->bytes < need)) {
-    // Nothing may wait now, so nothing can be freed: whichever is large enough, as if the two streams were one.
-    s = nullptr;
-    for (Scratch& c : scratch)
-      if (c.bytes >= need && (!s || c.last_use < s->last_use)) s = &c;
-    if (!s) *rc = set_last_error(error, "no scratch buffer is large enough, and none can be had during a capture");
-    else s->captured = true;
-    return s;
-  }
-  if (!s) {
-    s = spare;
-    if (!s) {   // the one that was not used for longest, of those that no graph needs, if there is one
-      for (Scratch& c : scratch)
-        if (!s || (c.captured != s->captured ? s->captured : c.last_use < s->last_use)) s = &c;
-      if (cudaDeviceSynchronize() != cudaSuccess) {
-        *rc = set_last_error(error, "device synchronisation failed");
-        return nullptr;
-      }
+  const bool other = !s && oldest->last_use != 0;      // takes over another stream's
+  if (!s) s = oldest;
+  if (other || (s->memory && s->bytes < need)) {
+    if (cudaDeviceSynchronize() != cudaSuccess) {
+      *rc = set_last_error(error, "device synchronisation failed");
+      return nullptr;
     }
-    s->handle = st;
-    s->id = 0;
-    s->captured = false;
   }
-  if (need > s->bytes) {
-    if (s->memory) {
-      if (cudaDeviceSynchronize() != cudaSuccess) {
-        *rc = set_last_error(error, "device synchronisation failed");
-        return nullptr;
-      }
-      cudaFree(s->memory);
-    }
-    s->memory = nullptr;
-    s->bytes = 0;
-    RelaxedCapture relaxed;
-    if (cudaMalloc(&s->memory, need) != cudaSuccess || !zero_now(s->memory, zeroed)) {
-      if (s->memory) cudaFree(s->memory);
-      s->memory = nullptr;
+  s->id = id;
+  s->last_use = ++calls;
+  if (s->bytes < need) {
+    if (s->memory) cudaFree(s->memory);
+    static_cast<ScratchBuffer&>(*s) = new_buffer(need, zeroed);
+    if (!s->memory) {
       s->last_use = 0;
       *rc = set_last_error(error, "out of device memory for the scratch buffer");
       return nullptr;
     }
-    s->bytes = need;
   }
-  if (id != 0) s->id = id;
-  if (capturing) s->captured = true;
-  s->last_use = ++calls;
   return s;
 }
 
