@@ -259,7 +259,7 @@ extern "C" int syfi_kv_write(const void* q, const void* k, const void* v, const 
                              double eps, void* cache, int64_t num_pages, int64_t page_stride, int32_t kinds, void* q_out,
                              void* stream) {
   if (const char* wrong = kv_cache_error(cache, num_pages, page_stride, kinds, kv_heads, head_dim)) return kv_fail(SYFI_KV_ERR_INVALID, wrong);
-  if (tokens < 0 || q_heads < 0 || q_heads > 4096 || tokens * (q_heads + 2ll * kv_heads) > 0x7fffffffll) return kv_fail(SYFI_KV_ERR_INVALID, "tokens or q_heads out of range");
+  if (tokens < 0 || q_heads < 0 || q_heads > 4096 || tokens > 0x7fffffffll / (q_heads + 2ll * kv_heads)) return kv_fail(SYFI_KV_ERR_INVALID, "tokens or q_heads out of range");
   if (rotary_dim < 0 || rotary_dim > head_dim || rotary_dim % 16 != 0) return kv_fail(SYFI_KV_ERR_INVALID, "rotary_dim must be a multiple of 16 up to head_dim");
   if (rotary_dim > 0 && max_positions < 1) return kv_fail(SYFI_KV_ERR_INVALID, "cos_sin has no row");
   if (!(eps >= 0.0 && eps <= 1e30)) return kv_fail(SYFI_KV_ERR_INVALID, "eps must not be negative");

@@ -118,3 +118,10 @@ def test_a_block_refuses_what_does_not_fit_in_32_bits(name, index, value, pkg):
     args[index] = value
     assert call(module._block(name)(*args)) == 1
     assert "32 bits" in pkg.load_library().syfi_moe_last_error().decode()
+
+
+@pytest.mark.parametrize("tokens", [2 ** 61 + 1, 2 ** 62, 2 ** 63 - 1, (2 ** 31 - 1) // 8 + 1])
+def test_write_refuses_tokens_whose_product_does_not_fit(tokens, pkg):
+    p = 4096
+    assert _fn(pkg, "syfi_kv_write")(p, p, p, None, None, None, None, p, tokens, 6, 1, 128, 0, 0, 0, 768, 128, 128, 768, 1e-6, p, 2, 2 * 8448, 2, p, None) == 1
+    assert "tokens" in pkg.load_library().syfi_moe_last_error().decode()
