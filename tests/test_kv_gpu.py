@@ -84,6 +84,40 @@ def test_write_matches_the_definition(T, HQ, HK, D, rotary, interleaved, norm, l
     _check_written(kv, cache, before, slots, 1, v.double())
 
 
+@pytest.mark.parametrize("T,HQ,HK,D,rotary,interleaved", [
+    (3000, 40, 5, 64, 48, False), (3000, 40, 5, 64, 64, True), (3000, 24, 9, 128, 128, True), (2600, 35, 7, 128, 96, False), (5000, 16, 16, 64, 16, True)])
+def test_write_of_many_tokens_matches_the_definition(T, HQ, HK, D, rotary, interleaved, pkg, kv):
+    """Enough vectors that a group of lanes takes a run of four heads; numbers of heads that leave a rest of a run."""
+    q, k, v, qw, kw, turn, positions, slots, cache, q_out = _write_inputs(kv, T, HQ, HK, D, rotary, True, seed=5)
+    before = cache.clone()
+    pkg.run_kv_write(q, k, v, qw, kw, turn, positions, slots, cache, q_out, interleaved=interleaved)
+    want = kv.head_vectors(q, qw, turn, positions, interleaved=interleaved)
+    assert ((q_out.double() - want).abs() <= want.abs() * 2.0 ** -8 * 1.001 + 4e-6 * want.abs().amax(-1, keepdim=True)).all()
+    _check_written(kv, cache, before, slots, 0, kv.head_vectors(k, kw, turn, positions, interleaved=interleaved))
+    _check_written(kv, cache, before, slots, 1, v.double())
+
+
+@pytest.mark.parametrize("T,HK,D", [(70, 3, 128), (1, 8, 64), (4000, 8, 128), (9000, 5, 64)])
+def test_written_bytes_are_the_rounded_quotients(T, HK, D, pkg, kv):
+    """Without norm and rotation: the scale is the division by 448 rounded once, the bytes are the division by the scale, rounded to f32
+    and then to e4m3.  (A quotient of f32 numbers rounded to 53 bits and then to 24 is the one rounded at once.)"""
+    g = torch.Generator(device=DEV).manual_seed(T)
+    k, v = ((torch.randn(T, HK, D, generator=g, device=DEV) * torch.exp2(torch.randint(-40, 40, (T, HK, 1), generator=g, device=DEV).float())).to(torch.bfloat16) for _ in range(2))
+    steps = torch.arange(D, device=DEV)                     # half way between two e4m3 numbers, for a scale of 1
+    k[0, 0] = torch.where(steps == 0, 448.0, (17.0 + 2.0 * (steps % 8)) * torch.exp2((steps % 11).float() - 8.0)).to(torch.bfloat16)
+    v[0, 0] = 0.0
+    cache = kv.random_cache(T // 64 + 1, 2, HK, D, 3, DEV)
+    slots = torch.randperm(cache.shape[0] * 64, generator=g, device=DEV)[:T].to(torch.int32)
+    pkg.run_kv_write(None, k, v, None, None, None, None, slots, cache, None)
+    values, scales = kv.views(cache)
+    page, at = slots.long() // 64, slots.long() % 64
+    for kind, x in enumerate((k.double(), v.double())):
+        scale = (x.abs().amax(-1).clamp(min=float(torch.tensor(1e-12))) / 448.0).float()
+        assert torch.equal(scales[page, kind, :, at], scale)
+        want = (x / scale.double()[..., None]).float().to(F8).view(torch.uint8)
+        assert torch.equal(values.view(torch.uint8)[page, kind, :, at], want)
+
+
 @pytest.mark.parametrize("T,HK,rotary", [(1, 1, 64), (300, 1, 64), (70, 3, 128)])
 def test_write_of_keys_only(T, HK, rotary, pkg, kv):
     _, k, _, _, kw, turn, positions, slots, cache, _ = _write_inputs(kv, T, 0, HK, 128, rotary, True, kinds=1)
@@ -171,6 +205,20 @@ def test_read_matches_the_definition(rows, H, D, dtype, layers, pkg, kv):
     alone = torch.empty_like(v)
     pkg.run_kv_read(cache, slots, None, alone)
     assert torch.equal(alone, v)
+
+
+@pytest.mark.parametrize("rows,H,D,dtype", [(8000, 3, 64, torch.bfloat16), (8000, 5, 128, torch.float32), (8001, 5, 64, torch.float32), (13000, 3, 128, torch.bfloat16)])
+def test_read_of_many_rows_matches_the_definition(rows, H, D, dtype, pkg, kv):
+    """Enough vectors that a group of lanes takes four; odd numbers of heads, so that a run of four has keys and values."""
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    cache = kv.random_cache(rows // 64 + 2, 2, H, D, 4, DEV)
+    slots = torch.randint(-20, cache.shape[0] * 64 + 20, (rows,), generator=g, device=DEV, dtype=torch.int32)
+    k, v = (torch.full((rows, H, D), 7.0, dtype=dtype, device=DEV) for _ in range(2))
+    pkg.run_kv_read(cache, slots, k, v)
+    alone = torch.empty_like(v)
+    pkg.run_kv_read(cache, slots, None, alone)
+    for got, kind in ((k, 0), (v, 1), (alone, 1)):
+        assert torch.equal(got, kv.rows(cache, slots, kind).float().to(dtype))
 
 
 def test_cache_beyond_four_gigabytes(pkg, kv):
