@@ -136,7 +136,7 @@ __device__ __forceinline__ void join_parts(const AttentionArgs& a, int q_first, 
       }
       const int row = row0 + b * warps, r = unit_row0 + row;
       if (row >= rows || sub != 0) continue;
-      const float f = l[b] == 0.0f ? 0.0f : ex2(finite_or_zero(n[b]) - finite_or_zero(m[b]) - kHeadroom) / l[b];
+      const float f = l[b] == 0.0f || n[b] == -INFINITY ? 0.0f : ex2(n[b] - finite_or_zero(m[b]) - kHeadroom) / l[b];
       __nv_bfloat16* to = a.out + (q_first + r / a.group) * a.out_stride + (head * a.group + r % a.group) * D + d;
       const __nv_bfloat162 lo = __floats2bfloat162_rn(o[b].x * f, o[b].y * f), hi = __floats2bfloat162_rn(o[b].z * f, o[b].w * f);
       *reinterpret_cast<uint2*>(to) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));

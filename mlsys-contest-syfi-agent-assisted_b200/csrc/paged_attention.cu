@@ -51,6 +51,7 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {
 // 4 key heads of 128, 8 rows each: 346 us, 6.4 TB/s.  Short or few sequences: the chain of planning, a page's latency, and the join of
 // parts (one sequence of 700 positions 13 us).
 constexpr int kDecodeExtra = 1;      // what a unit costs besides its pages, in pages
+constexpr float kFarBehind = 1.2676506e30f;   // 2^100 between the references of the two sums: the values' follows
 
 template <int D, int NT>
 struct DecodeShape {
@@ -280,6 +281,7 @@ __global__ void __launch_bounds__(DecodeShape<D, NT>::kThreads, DecodeShape<D, N
               l[t][i] *= ex2(m[t][i] - top);
               m[t][i] = top;
               up[t][i] = n[t][i] == -INFINITY ? 0.0f : ex2(top - n[t][i] + kHeadroom);
+              late |= up[t][i] > kFarBehind;
             }
           }
       }
@@ -306,7 +308,7 @@ __global__ void __launch_bounds__(DecodeShape<D, NT>::kThreads, DecodeShape<D, N
           float fade[2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            float top = finite_or_zero(m[t][i]) + lg2(fmaxf(p[t][i], p[t][2 + i]));
+            float top = m[t][i] + fmaxf(lg2(fmaxf(p[t][i], p[t][2 + i])), -90.0f);      // (never further behind: a value may be zero)
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
             fade[i] = 1.0f;
@@ -429,7 +431,7 @@ __global__ void __launch_bounds__(DecodeShape<D, NT>::kThreads, DecodeShape<D, N
 #pragma unroll
               for (int e = 0; e < 2; ++e) v[2 * j + e] = o[t][j][2 * e + i] + other[((t * kMmas + j) * 4 + 2 * e + i) * 32];
             if (whole) {
-              const float f = l[t][i] == 0.0f ? 0.0f : ex2(finite_or_zero(n[t][i]) - finite_or_zero(m[t][i]) - kHeadroom) / l[t][i];
+              const float f = l[t][i] == 0.0f || n[t][i] == -INFINITY ? 0.0f : ex2(n[t][i] - finite_or_zero(m[t][i]) - kHeadroom) / l[t][i];
               uint4* to = reinterpret_cast<uint4*>(a.out + (use.s.first + r / a.group) * a.out_stride + (use.head * a.group + r % a.group) * D + g * (D / 8));
 #pragma unroll
               for (int j = 0; j < D / 64; ++j) {

@@ -454,6 +454,30 @@ def test_one_large_weight_and_a_long_tail(q_len, spike, pkg, kv):
     _check_attention(_attend(pkg, inputs), *kv.attention(*inputs))
 
 
+@pytest.mark.parametrize("q_len", [1, 2, 200])
+@pytest.mark.parametrize("kv_len", [300, 9000])
+@pytest.mark.parametrize("octaves", [60, 110, 150, 400])
+def test_a_zero_value_far_above_the_others(q_len, kv_len, octaves, pkg, kv):
+    """Positions with a value scale of zero whose scores lie far above all others, first, last or in between: next to nothing is left of
+    the others, and no NaN.  Then scores far below zero with nothing but such values."""
+    for spike in (0, kv_len // 2, kv_len - q_len):
+        inputs = _attention_inputs(kv, [q_len], [kv_len], 8, 1, 128, seed=19)
+        q, cache, table, lens, starts = inputs
+        values, scales = kv.views(cache)
+        page, at = int(table[0, spike // 64]), spike % 64
+        values.view(torch.uint8)[page, 0, 0, at] = 0
+        values.view(torch.uint8)[page, 0, 0, at, 0] = 0x38      # 1
+        q[:, :, 0] = 1.0
+        scales[page, 0, 0, at] = octaves * 0.6931471805599453 * 128 ** 0.5
+        scales[page, 1, 0, at] = 0.0
+        _check_attention(_attend(pkg, inputs), *kv.attention(*inputs))
+    values.view(torch.uint8)[:, 0] = 0
+    values.view(torch.uint8)[:, 0, :, :, 0] = 0xb8              # -1
+    scales[:, 0] = octaves * 0.6931471805599453 * 128 ** 0.5
+    scales[:, 1] = 0.0
+    assert (_attend(pkg, inputs) == 0).all()
+
+
 @pytest.mark.parametrize("HQ,HK,D", [(8, 1, 128), (4, 1, 64), (16, 1, 128), (14, 1, 64)])
 def test_a_long_sequence_in_more_parts_than_a_warp_has_lanes(HQ, HK, D, pkg, kv):
     inputs = _attention_inputs(kv, [1], [60000], HQ, HK, D, seed=6)
