@@ -32,14 +32,15 @@ extern "C" {
 /* New tokens' queries, keys and values: head norms, rotation, quantisation and the scatter into the cache in one pass.
  *   q [tokens, q_heads, head_dim], k and v [tokens, kv_heads, head_dim]: bf16.  q (with q_out) may be null with q_heads = 0,
  *       v is null where kinds = 1.
- *   q_weight, k_weight: bf16 [head_dim] or null; y = x / sqrt(mean(x^2) + eps) * weight over the dimensions of a head.
+ *   q_weight, k_weight: bf16 [head_dim] or null; y = x / sqrt(mean(x^2) + eps) * weight over the dimensions of a head, in f32
+ *       (a head whose sum of squares is beyond that becomes zeros).
  *   cos_sin: f32 [max_positions, rotary_dim] (rotary_dim / 2 cosines, then as many sines) or null with rotary_dim = 0;
  *       rotary_dim is a multiple of 16 up to head_dim.  The first rotary_dim dimensions of q and k are turned by the row of
  *       the token's position: (a, b) -> (a cos - b sin, b cos + a sin), pair i being the dimensions (i, i + rotary_dim / 2),
  *       or (2 i, 2 i + 1) where `interleaved` is not 0.  A position outside the table gives NaN.
  *   positions: int32 [tokens] (may be null with rotary_dim = 0).
- *   slots: int32 [tokens]: where a token's keys and values go; a slot outside the cache (-1: padding) is not written.  Two
- *       tokens with one slot leave either's.
+ *   slots: int32 [tokens]: where a token's keys and values go; a slot outside the cache (-1: padding) is not written.  No two
+ *       tokens of a call may have one slot: its scale may then be one's and its bytes the other's.
  *   q_out: bf16 [tokens, q_heads, head_dim], may be q itself.
  * A written head vector z (rounded to bf16 nowhere on its way) has the scale max(max|z|, 1e-12) / 448 and the bytes
  * e4m3(z / scale), rounded to nearest; one with a NaN or an infinity is read back as NaN. */
@@ -64,7 +65,11 @@ int syfi_kv_read(const void* cache, int64_t num_pages, int64_t page_stride, int3
  *       Rows of no sequence are left alone.
  * The query at position p sees the positions j <= p that are there, with window > 0 only those with j > p - window:
  *   out = sum_j softmax_j(scale * q . key_j) * value_j;  a query that sees nothing gets zeros.
- * Positions that a query does not see do not touch its result, whatever the cache holds there.  Scales are not negative.
+ * Positions that a query does not see do not touch its result, whatever the cache holds there.  Scales are not negative.  A
+ * query or a seen position that is not finite makes its heads' results NaN (a NaN in some dimensions of a value: those, or all).
+ * Sums are in f32.  A weight is rounded to f16 (2^-12 of it on average); one 2^-32 below the row's largest may not be added, nor,
+ * with few rows, one whose value is 2^-32 below the row's largest.  With more than 16 rows per sequence and key head on average
+ * q is held to 2^-17 of its row's largest dimension.
  * Calls on different streams may run at the same time: every stream has a scratch buffer of its own (up to 45 MB), which
  * grows on demand (that waits for the device).  Up to eight streams of a device hold one; a ninth waits for the device and takes
  * over the least recently used.  A captured graph has buffers of its own, one for each stream that was captured into it, until it is

@@ -1,5 +1,6 @@
 // Writing the quantised paged KV cache and reading rows of it back (include/syfi_kv.h).  Both move bytes: what they read and
-// write once is their floor, so each is one pass with 16-byte accesses and everything in between in registers.
+// write once is their floor, so each is one pass with everything in between in registers.  A lane of the write loads 8 bytes at a time and
+// stores 8 or 4 (both dimensions of a rotated pair are one lane's), one of the read loads 8 and stores 16.
 #include <string.h>
 
 #include <atomic>
@@ -14,7 +15,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWriteHeads = 4, kReadVectors = 4;   // vectors that a group of lanes has under way
-constexpr int kFullGroups = 64;                    // groups per SM that are enough to keep it busy
+// Groups per SM that are enough to keep it busy: with 16, 64, 256 a write of 600 tokens of 32 + 2 x 8 heads 11.3, 12.4, 12.5 us, of 3000 26.7,
+// 26.6, 33.8; a read of 2048 rows of 2 x 8 heads 9.1, 10.2, 9.2, of 9000 15.4, 15.4, 21.4 (other memory touched in between).
+constexpr int kFullGroups = 64;
 
 struct WriteArgs {
   const __nv_bfloat16 *q, *k, *v, *q_weight, *k_weight;
@@ -27,14 +30,6 @@ struct WriteArgs {
   float eps;
 };
 
-__device__ __forceinline__ void unpack8(const uint4& p, float (&x)[8]) {
-  const uint32_t w[4] = {p.x, p.y, p.z, p.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = __uint_as_float(w[i] << 16);
-    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-  }
-}
 __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
   uint32_t w[4];
 #pragma unroll
@@ -50,8 +45,9 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
 // dimensions, chosen so that it holds both of a rotated pair: lanes below rotary / 8 have chunk l and chunk l + rotary / 8, the others two
 // neighbouring chunks of what is not rotated.  Sum of squares and maximum are shuffles inside the head's lanes.
 // What bounds it at many tokens is the instructions of norm, rotation and rounding beside the bytes: 8192 tokens of 64 + 2 x 8 heads of 128,
-// 75 us, 4.3 TB/s.  One division per head: the eight quotients take its reciprocal and one residual each, correctly rounded as a
-// division's.  Few tokens: the call itself.
+// 74 us, 4.4 TB/s.  One division per head: the eight quotients take its reciprocal and one residual each, correctly rounded as a
+// division's.  Few tokens: the call itself.  Five CTAs an SM (48 registers, 36 bytes of them spilled) 79.0 us, four (63, none) 81.9, six (40, 64
+// bytes) 84.0, with a flushed L2.
 template <int D, bool INTERLEAVED, int HEADS>
 __global__ void __launch_bounds__(kThreads, HEADS > 1 ? 5 : 1) kv_write_kernel(const __grid_constant__ WriteArgs a) {
   constexpr int kLanes = D / 8, kGroups = 32 / kLanes, kRun = kGroups * HEADS;
@@ -177,7 +173,7 @@ __global__ void __launch_bounds__(kThreads, HEADS > 1 ? 5 : 1) kv_write_kernel(c
 }
 
 // D / 8 lanes have a vector, eight dimensions each, and EACH neighbouring ones (heads of keys, then of values) of a row at a time.
-// What bounds it is the bytes: 40000 rows of 2 x 8 heads of 128, 43 us, 5.8 TB/s.
+// What bounds it is the bytes: 40000 rows of 2 x 8 heads of 128, 43 us, 5.8 TB/s to bf16 (91 us, 4.5 TB/s to f32).
 template <int D, typename Out, int EACH>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(KvCache c, const int32_t* __restrict__ slots, unsigned rows, int first_kind, int kinds,
                                                            Out* __restrict__ k_out, Out* __restrict__ v_out) {

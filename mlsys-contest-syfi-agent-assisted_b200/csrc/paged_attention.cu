@@ -48,9 +48,11 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {
 // Which position an index of the scores stands for is chosen so that both reads of the swizzled rows are free of bank conflicts: even i
 // is position i, odd i is position (i - 1) ^ 5.
 // What bounds it is the cache's bytes, so what counts is loads in flight and few instructions per page: 32 sequences of 65536 positions,
-// 4 key heads of 128, 8 rows each: 346 us, 6.4 TB/s.  Short or few sequences: the chain of planning, a page's latency, and the join of
+// 4 key heads of 128, 8 rows each: 347 us, 6.4 TB/s back to back, 374 to 403 us with other memory touched in between.  Short or few sequences: the chain of planning, a page's latency, and the join of
 // parts (one sequence of 700 positions 13 us).
-constexpr int kDecodeExtra = 1;      // what a unit costs besides its pages, in pages
+// What a unit costs besides its pages, in pages.  With 0, 1, 2, 4 (us, a flushed L2): 24 sequences of 300 .. 30000 positions, 8 rows 95, 94, 87,
+// 87; 128 of 100 .. 3000 115, 91, 84, 81; 128 of 300 57, 55, 55, 55; 32 of 65536 360, 362, 362, 361.
+constexpr int kDecodeExtra = 1;
 constexpr float kFarBehind = 1.2676506e30f;   // 2^100 between the references of the two sums: the values' follows
 
 template <int D, int NT>
@@ -575,7 +577,9 @@ extern "C" int syfi_paged_attention(const void* q, int64_t q_stride, const void*
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // Rows per sequence and key head, on average (the lengths themselves are on the device): row tiles of 8 or 16, beyond that the tensor
   // memory kernel's.  24 sequences of 300 .. 30000 positions, 8 key heads of 128, us for 8 | 16 | 32 rows each: tiles of 8 79 | 134 | 249,
-  // tiles of 16 121 | 129 | 259, the tensor memory kernel 141 | 143 | 145.
+  // tiles of 16 121 | 129 | 259, the tensor memory kernel 141 | 143 | 145.  Unequal rows, a chunk of 512 tokens behind 4000 positions beside
+  // 24 | 100 | 256 | 500 sequences of 2000 with one token, 4 rows a token: row tiles 293 | 381 | 592 | 903, the tensor memory kernel
+  // 117 | 271 | 536 | 1079 (each half alone in its own kernel: the chunk 70, 256 sequences 257).
   const int64_t rows = (tokens * a.group + batch - 1) / batch;
   if (rows > 16) {
     int rc = SYFI_KV_OK;

@@ -5,7 +5,8 @@
 //               the sum of two e4m3 terms: a bf16 value has 8 significant bits, an e4m3 term 4, so the two hold it exactly as long
 //               as it is not 2^-9 of the row's largest (then to 2^-17 of that).  Both terms add into one accumulator.
 //   P           softmax warps, a lane per row and a warp per half of the tile's positions: the weights in f16 (2^-12 of each on average),
-//               back into tensor memory over S.
+//               back into tensor memory over S.  Below 2^-21 of the row's largest they lose bits, below 2^-32 they are lost: that shows
+//               only in a row whose heavier positions all have values a thousand times smaller.
 //   O += P V    kind::f16, P from tensor memory, V as f16 in shared memory.  Four warps make it from the bytes: e4m3 times the position's
 //               scale relative to the unit's (a power of two that follows the largest scale met), rounded once to f16.
 // The slots are out of step by half a tile: while the softmax warps of one work, the tensor core works for the other.  A unit of at most
@@ -19,8 +20,8 @@
 // 1.4 ms instead of 0.7; all rows of the units that meet it 797 ms.
 //
 // What bounds it is that chain: a wide tile of 256 rows takes 5200 clocks, of which the tensor core works 2048 and the exponentials 2048
-// (16 per clock).  A prompt of 8192 tokens, 32 heads of 128 over 8: 654 us (841 TFLOP/s of what is visible)
-// back to back, 704 us with other memory touched in between.
+// (16 per clock).  A prompt of 8192 tokens, 32 heads of 128 over 8: 649 us (848 TFLOP/s of what is visible)
+// back to back, 707 to 722 us with other memory touched in between.
 #include "attention_common.cuh"
 #include "stream_scratch.h"
 
@@ -32,7 +33,9 @@ constexpr int kTile = 128;             // positions per tile: two pages
 constexpr int kChunkRows = 256;
 constexpr int kChunkThreads = 768;     // 16 softmax warps, 4 converting ones, then MMAs, loads, planning, scales
 constexpr int kSoftmaxWarps = 16, kSoftmaxThreads = 512;
-constexpr int kChunkExtra = 4;         // what a unit costs besides its tiles, in tiles (8192-token prompt with 3, 4, 5, 6: 704, 656, 662, 672 us)
+// What a unit costs besides its tiles, in tiles.  With 2, 3, 4, 6 (us, a flushed L2): 8192-token prompt 855, 717, 660, 674; two chunks with a window
+// of 1024 141, 143, 141, 143; 8 sequences of 4 to 1000 rows 68, 68, 70, 73; a chunk of 512 behind 40000 positions 325, 324, 324, 327.
+constexpr int kChunkExtra = 4;
 constexpr int kSlotRows = 128;         // units of at most so many rows use one slot for their even tiles and one for their odd ones
 using ChunkPlan = Plan<kTile, kChunkRows, kChunkExtra, kSlotRows>;
 using ChunkCursor = Cursor<kTile, kChunkRows, kChunkExtra, kSlotRows>;
