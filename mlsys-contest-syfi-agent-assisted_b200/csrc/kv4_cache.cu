@@ -1,0 +1,320 @@
+// Writing the paged KV cache in 4 bits and reading rows of it back (include/syfi_kv4.h).  Both move bytes: what they read and write once
+// is their floor, so each is one pass with everything in between in registers.
+#include "kv4_internal.h"
+
+namespace syfi {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWriteHeads = 4, kReadVectors = 4;   // vectors that a group of lanes has under way
+constexpr int kFullGroups = 64;                    // groups per SM that are enough to keep it busy
+
+struct Write4Args {
+  const __nv_bfloat16 *q, *k, *v, *q_weight, *k_weight;
+  const float* cos_sin;
+  const int32_t *positions, *slots;
+  __nv_bfloat16* q_out;
+  long long q_stride, k_stride, v_stride, q_out_stride, max_positions;
+  KvCache cache;
+  int tokens, q_heads, rotary;
+  float eps;
+};
+
+__device__ __forceinline__ uint4 bf16x8(const float (&x)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void floats8(uint4 p, float (&x)[8]) {
+  const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+// x / y given RN(1 / y): the product and one step with its exact remainder (Markstein), which leaves the quotient correctly rounded, so
+// that a value half way between two codes goes where the division would send it.
+__device__ __forceinline__ float quotient(float x, float y, float inverse) {
+  const float q = x * inverse;
+  return fmaf(fmaf(-q, y, x), inverse, q);
+}
+
+// A warp takes a run of neighbouring heads of one kind (queries, keys or values) of a token, D / 8 lanes per head and HEADS heads one
+// after the other, whose loads are under way together and which share the token's cosines and sines.  A lane has eight neighbouring
+// dimensions: a word of codes, half a group.  Its partner's in a rotation of halves come by shuffles (rotary / 2 is a multiple of eight).
+template <int D, bool INTERLEAVED, int HEADS>
+__global__ void __launch_bounds__(kThreads) kv4_write_kernel(const __grid_constant__ Write4Args a) {
+  constexpr int kLanes = D / 8, kGroups = 32 / kLanes, kRun = kGroups * HEADS;
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x % kLanes, group = (threadIdx.x & 31) / kLanes;
+  const unsigned q_runs = (a.q_heads + kRun - 1) / kRun, kv_runs = (a.cache.heads + kRun - 1) / kRun, runs = q_runs + 2 * kv_runs;
+  const unsigned id = blockIdx.x * (kThreads / 32) + threadIdx.x / 32;
+  const int t = static_cast<int>(id / runs);
+  if (t >= a.tokens) return;
+  unsigned run = id - t * runs;
+  const int which = run < q_runs ? 0 : run < q_runs + kv_runs ? 1 : 2;      // queries, keys, values; the same for the warp
+  if (which > 0) run -= q_runs + (which - 1) * kv_runs;
+  const int slot = which > 0 ? a.slots[t] : 0;
+  if (which > 0 && (slot < 0 || slot / kKvPage >= a.cache.num_pages)) return;
+  const int heads = which == 0 ? a.q_heads : a.cache.heads, first = static_cast<int>(run) * kRun + group;
+  const __nv_bfloat16* const from = (which == 0 ? a.q + t * a.q_stride : which == 1 ? a.k + t * a.k_stride : a.v + t * a.v_stride) + lane * 8;
+  uint4 raw[HEADS];
+#pragma unroll
+  for (int h = 0; h < HEADS; ++h)
+    raw[h] = first + h * kGroups < heads ? *reinterpret_cast<const uint4*>(from + (first + h * kGroups) * D) : make_uint4(0u, 0u, 0u, 0u);
+  // what the heads share: weights, cosines and sines
+  const __nv_bfloat16* const weight = which == 0 ? a.q_weight : which == 1 ? a.k_weight : nullptr;
+  float w[8];
+  if (weight) floats8(*reinterpret_cast<const uint4*>(weight + lane * 8), w);
+  const bool rotates = which < 2 && a.rotary > 0, turned = rotates && lane < a.rotary / 8;
+  const int half = a.rotary / 16;               // lanes of half of the rotated dimensions
+  const int partner = (threadIdx.x & 31) + (lane < half ? half : -half);
+  constexpr int kTurns = INTERLEAVED ? 4 : 8;
+  float cs[kTurns], sn[kTurns];
+#pragma unroll
+  for (int i = 0; i < kTurns; ++i) {
+    cs[i] = 1.0f;
+    sn[i] = 0.0f;
+  }
+  bool known = true;
+  if (rotates) {
+    const int position = a.positions[t];
+    known = position >= 0 && position < a.max_positions;
+    if (turned) {
+      const float* row = a.cos_sin + (known ? position : 0) * static_cast<long long>(a.rotary) + (INTERLEAVED ? lane * 4 : (lane < half ? lane : lane - half) * 8);
+#pragma unroll
+      for (int i = 0; i < kTurns; i += 4) {
+        const float4 c = *reinterpret_cast<const float4*>(row + i), s = *reinterpret_cast<const float4*>(row + a.rotary / 2 + i);
+        cs[i] = c.x; cs[i + 1] = c.y; cs[i + 2] = c.z; cs[i + 3] = c.w;
+        sn[i] = s.x; sn[i + 1] = s.y; sn[i + 2] = s.z; sn[i + 3] = s.w;
+      }
+      if (!INTERLEAVED && lane < half) {
+#pragma unroll
+        for (int i = 0; i < kTurns; ++i) sn[i] = -sn[i];
+      }
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < HEADS; ++h) {
+    const int head = first + h * kGroups;
+    const bool real = head < heads;
+    float x[8];
+    floats8(raw[h], x);
+    if (weight) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
+#pragma unroll
+      for (int d = kLanes / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      const float factor = rsqrtf(sum * (1.0f / D) + a.eps);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] *= factor * w[i];
+    }
+    if (rotates) {
+      if constexpr (INTERLEAVED) {
+        if (turned) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float u = x[2 * i], v = x[2 * i + 1];
+            x[2 * i] = u * cs[i] - v * sn[i];
+            x[2 * i + 1] = v * cs[i] + u * sn[i];
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float other = __shfl_sync(0xffffffffu, x[i], partner);
+          if (turned) x[i] = x[i] * cs[i] + other * sn[i];
+        }
+      }
+    }
+    if (!known) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = __int_as_float(0x7fffffff);
+    }
+    if (which == 0) {
+      if (real) *reinterpret_cast<uint4*>(a.q_out + t * a.q_out_stride + head * D + lane * 8) = bf16x8(x);
+      continue;
+    }
+    // Largest magnitudes as bits: unlike the largest float they keep a NaN.
+    unsigned top = 0u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    const float group_top = __uint_as_float(top);
+#pragma unroll
+    for (int d = 2; d < kLanes; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+    if (!real) continue;
+    const float largest = __uint_as_float(top);
+    float scale = quotient(largest < 1e-12f ? 1e-12f : largest, 2688.0f, 1.0f / 2688.0f);
+    const float six = 6.0f * scale;
+    uint32_t group_byte = cvt_e4m3x2(quotient(group_top, six, 1.0f / six), 0.0f) & 0x7fu;
+    const float unit = e4m3x2_to_float2(static_cast<uint16_t>(group_byte)).x * scale, inverse = 1.0f / unit;
+    uint32_t codes = 0u;
+    if (top >= 0x7f800000u) {                 // not finite: read back as NaN
+      scale = __int_as_float(0x7fffffff);
+      group_byte = 0u;
+    } else if (group_byte != 0u) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = quotient(x[i], unit, inverse);
+      codes = cvt_e2m1x8(x);
+    }
+    uint8_t* const block = kv4_block<D>(a.cache, slot / kKvPage, which - 1, head);
+    const int at = slot % kKvPage;
+    *reinterpret_cast<uint32_t*>(block + lane / 8 * kKv4Plane + at * 32 + lane % 8 * 4) = codes;
+    if (lane % 2 == 0) block[Kv4Block<D>::kGroups + at * (D / kKv4Group) + lane / 2] = static_cast<uint8_t>(group_byte);
+    if (lane == 0) *reinterpret_cast<float*>(block + Kv4Block<D>::kScales + at * 4) = scale;
+  }
+}
+
+// D / 8 lanes have a vector, eight dimensions each, and EACH neighbouring ones (heads of keys, then of values) of a row at a time.
+template <int D, typename Out, int EACH>
+__global__ void __launch_bounds__(kThreads) kv4_read_kernel(KvCache c, const int32_t* __restrict__ slots, unsigned rows, int first_kind, int kinds,
+                                                            Out* __restrict__ k_out, Out* __restrict__ v_out) {
+  constexpr int kLanes = D / 8;
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x % kLanes, vectors = kinds * c.heads, runs = (vectors + EACH - 1) / EACH;
+  const unsigned id = blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
+  const unsigned row = id / static_cast<unsigned>(runs);
+  const int first = static_cast<int>(id - row * static_cast<unsigned>(runs)) * EACH;
+  if (row >= rows) return;
+  const int slot = slots[row];
+  const bool there = slot >= 0 && slot / kKvPage < c.num_pages;
+  const int at = slot % kKvPage;
+  uint32_t codes[EACH], group[EACH];
+  float scale[EACH];
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    codes[i] = group[i] = 0u;
+    scale[i] = 0.0f;
+    if (there && first + i < vectors) {
+      const int kind = first + i >= c.heads;
+      const uint8_t* block = kv4_block<D>(c, slot / kKvPage, first_kind + kind, first + i - kind * c.heads);
+      codes[i] = *reinterpret_cast<const uint32_t*>(block + lane / 8 * kKv4Plane + at * 32 + lane % 8 * 4);
+      group[i] = block[Kv4Block<D>::kGroups + at * (D / kKv4Group) + lane / 2];
+      scale[i] = *reinterpret_cast<const float*>(block + Kv4Block<D>::kScales + at * 4);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    if (first + i >= vectors) break;
+    const int kind = first + i >= c.heads;
+    Out* out = (first_kind + kind == 0 ? k_out : v_out) + (static_cast<long long>(row) * c.heads + first + i - kind * c.heads) * D + lane * 8;
+    const uint32_t h[4] = {e2m1x2_to_half2<0>(codes[i]), e2m1x2_to_half2<1>(codes[i]), e2m1x2_to_half2<2>(codes[i]), e2m1x2_to_half2<3>(codes[i])};
+    const float g = e4m3x2_to_float2(static_cast<uint16_t>(group[i])).x;
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+      x[2 * j] = f.x * g * scale[i];          // (the first product is exact)
+      x[2 * j + 1] = f.y * g * scale[i];
+    }
+    if constexpr (sizeof(Out) == 4) {
+      reinterpret_cast<float4*>(out)[0] = make_float4(x[0], x[1], x[2], x[3]);
+      reinterpret_cast<float4*>(out)[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+      *reinterpret_cast<uint4*>(out) = bf16x8(x);
+    }
+  }
+}
+
+}  // namespace
+
+}  // namespace syfi
+
+using namespace syfi;
+
+extern "C" int syfi_kv4_write(const void* q, const void* k, const void* v, const void* q_weight, const void* k_weight,
+                              const float* cos_sin, const int32_t* positions, const int32_t* slots, int64_t tokens,
+                              int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t rotary_dim, int32_t interleaved,
+                              int64_t max_positions, int64_t q_stride, int64_t k_stride, int64_t v_stride, int64_t q_out_stride,
+                              double eps, void* cache, int64_t num_pages, int64_t page_stride, void* q_out, void* stream) {
+  if (const char* wrong = kv4_cache_error(cache, num_pages, page_stride, kv_heads, head_dim)) return kv_fail(SYFI_KV4_ERR_INVALID, wrong);
+  if (tokens < 0 || q_heads < 0 || q_heads > 4096 || tokens > 0x7fffffffll / (q_heads + 2ll * kv_heads)) return kv_fail(SYFI_KV4_ERR_INVALID, "tokens or q_heads out of range");
+  if (rotary_dim < 0 || rotary_dim > head_dim || rotary_dim % 16 != 0) return kv_fail(SYFI_KV4_ERR_INVALID, "rotary_dim must be a multiple of 16 up to head_dim");
+  if (rotary_dim > 0 && max_positions < 1) return kv_fail(SYFI_KV4_ERR_INVALID, "cos_sin has no row");
+  if (!(eps >= 0.0 && eps <= 1e30)) return kv_fail(SYFI_KV4_ERR_INVALID, "eps must not be negative");
+  if (tokens == 0) return SYFI_KV4_OK;
+  const int64_t kv_width = static_cast<int64_t>(kv_heads) * head_dim, q_width = static_cast<int64_t>(q_heads) * head_dim;
+  if (!kv_aligned(k) || !kv_aligned(v) || !kv_table_aligned(slots) || (q_heads > 0 && (!kv_aligned(q) || !kv_aligned(q_out))) ||
+      (rotary_dim > 0 && (!kv_aligned(cos_sin) || !kv_table_aligned(positions))) || (q_weight && !kv_aligned(q_weight)) || (k_weight && !kv_aligned(k_weight)))
+    return kv_fail(SYFI_KV4_ERR_INVALID, "a tensor argument is null or not aligned (16 bytes, int32 tables 4)");
+  if (!kv_stride_ok(k_stride, kv_width) || !kv_stride_ok(v_stride, kv_width) ||
+      (q_heads > 0 && (!kv_stride_ok(q_stride, q_width) || !kv_stride_ok(q_out_stride, q_width))))
+    return kv_fail(SYFI_KV4_ERR_INVALID, "a token stride is smaller than the token's heads or no multiple of 8");
+  const int sms = kv_device_sms();
+  if (!sms) return SYFI_KV4_ERR_CUDA;
+  Write4Args a;
+  a.q = static_cast<const __nv_bfloat16*>(q);
+  a.k = static_cast<const __nv_bfloat16*>(k);
+  a.v = static_cast<const __nv_bfloat16*>(v);
+  a.q_weight = static_cast<const __nv_bfloat16*>(q_weight);
+  a.k_weight = static_cast<const __nv_bfloat16*>(k_weight);
+  a.cos_sin = cos_sin;
+  a.positions = positions;
+  a.slots = slots;
+  a.q_out = static_cast<__nv_bfloat16*>(q_out);
+  a.q_stride = q_stride;
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.q_out_stride = q_out_stride;
+  a.max_positions = max_positions;
+  a.cache = {static_cast<uint8_t*>(cache), page_stride, static_cast<int>(num_pages), 2, kv_heads};
+  a.tokens = static_cast<int>(tokens);
+  a.q_heads = q_heads;
+  a.rotary = rotary_dim;
+  a.eps = static_cast<float>(eps);
+  // One head per group of lanes while that leaves SMs idle, else a run of them.
+  const int heads = q_heads + 2 * kv_heads;
+  const int each = tokens * heads >= static_cast<int64_t>(sms) * kFullGroups * kWriteHeads ? kWriteHeads : 1, run_heads = 32 / (head_dim / 8) * each;
+  const int64_t groups = tokens * ((q_heads + run_heads - 1) / run_heads + 2ll * ((kv_heads + run_heads - 1) / run_heads));
+  const int per_block = kThreads / 32;
+  const dim3 grid(static_cast<unsigned>((groups + per_block - 1) / per_block));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto run = [&](auto* kernel) { return launch_dependent(kernel, grid, dim3(kThreads), 0, st, a) == cudaSuccess; };
+  const bool ok = head_dim == 128 ? (interleaved ? (each > 1 ? run(kv4_write_kernel<128, true, kWriteHeads>) : run(kv4_write_kernel<128, true, 1>))
+                                                 : (each > 1 ? run(kv4_write_kernel<128, false, kWriteHeads>) : run(kv4_write_kernel<128, false, 1>)))
+                                  : (interleaved ? (each > 1 ? run(kv4_write_kernel<64, true, kWriteHeads>) : run(kv4_write_kernel<64, true, 1>))
+                                                 : (each > 1 ? run(kv4_write_kernel<64, false, kWriteHeads>) : run(kv4_write_kernel<64, false, 1>)));
+  return ok ? SYFI_KV4_OK : kv_fail(SYFI_KV4_ERR_CUDA, "write kernel launch failed");
+}
+
+extern "C" int syfi_kv4_read(const void* cache, int64_t num_pages, int64_t page_stride, int32_t kv_heads, int32_t head_dim,
+                             const int32_t* slots, int64_t rows, int32_t out_f32, void* k_out, void* v_out, void* stream) {
+  if (const char* wrong = kv4_cache_error(cache, num_pages, page_stride, kv_heads, head_dim)) return kv_fail(SYFI_KV4_ERR_INVALID, wrong);
+  if (rows < 0 || rows > 0x7fffffffll / 16) return kv_fail(SYFI_KV4_ERR_INVALID, "rows out of range");
+  if (rows == 0 || (!k_out && !v_out)) return SYFI_KV4_OK;
+  if (!kv_table_aligned(slots) || (k_out && !kv_aligned(k_out)) || (v_out && !kv_aligned(v_out))) return kv_fail(SYFI_KV4_ERR_INVALID, "a tensor argument is null or not aligned (16 bytes, int32 tables 4)");
+  const int sms = kv_device_sms();
+  if (!sms) return SYFI_KV4_ERR_CUDA;
+  const KvCache c = {static_cast<uint8_t*>(const_cast<void*>(cache)), page_stride, static_cast<int>(num_pages), 2, kv_heads};
+  const int first_kind = k_out ? 0 : 1, wanted = (k_out ? 1 : 0) + (v_out ? 1 : 0), per_block = kThreads / (head_dim / 8);
+  const int each = rows * wanted * kv_heads >= static_cast<int64_t>(sms) * kFullGroups * kReadVectors ? kReadVectors : 1;
+  const int64_t groups = rows * ((wanted * kv_heads + each - 1) / each);
+  if (groups > 0x7fffffffll) return kv_fail(SYFI_KV4_ERR_INVALID, "rows out of range");
+  const dim3 grid(static_cast<unsigned>((groups + per_block - 1) / per_block));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto run = [&](auto* kernel, auto* typed) {
+    return launch_dependent(kernel, grid, dim3(kThreads), 0, st, c, slots, static_cast<unsigned>(rows), first_kind, wanted, static_cast<decltype(typed)>(k_out),
+                            static_cast<decltype(typed)>(v_out)) == cudaSuccess;
+  };
+  float* const f32 = nullptr;
+  __nv_bfloat16* const bf16 = nullptr;
+  const bool ok = out_f32 ? (head_dim == 128 ? (each > 1 ? run(kv4_read_kernel<128, float, kReadVectors>, f32) : run(kv4_read_kernel<128, float, 1>, f32))
+                                             : (each > 1 ? run(kv4_read_kernel<64, float, kReadVectors>, f32) : run(kv4_read_kernel<64, float, 1>, f32)))
+                          : (head_dim == 128 ? (each > 1 ? run(kv4_read_kernel<128, __nv_bfloat16, kReadVectors>, bf16) : run(kv4_read_kernel<128, __nv_bfloat16, 1>, bf16))
+                                             : (each > 1 ? run(kv4_read_kernel<64, __nv_bfloat16, kReadVectors>, bf16) : run(kv4_read_kernel<64, __nv_bfloat16, 1>, bf16)));
+  return ok ? SYFI_KV4_OK : kv_fail(SYFI_KV4_ERR_CUDA, "read kernel launch failed");
+}
+
+extern "C" int syfi_kv4_write_block(const int64_t* args) { return kv_spread(syfi_kv4_write, args); }
+extern "C" int syfi_kv4_read_block(const int64_t* args) { return kv_spread(syfi_kv4_read, args); }
+extern "C" int syfi_kv4_attention_block(const int64_t* args) { return kv_spread(syfi_kv4_attention, args); }

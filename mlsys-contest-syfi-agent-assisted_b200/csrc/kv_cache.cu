@@ -1,11 +1,7 @@
 // Writing the quantised paged KV cache and reading rows of it back (include/syfi_kv.h).  Both move bytes: what they read and
 // write once is their floor, so each is one pass with everything in between in registers.  A lane of the write loads 8 bytes at a time and
 // stores 8 or 4 (both dimensions of a rotated pair are one lane's), one of the read loads 8 and stores 16.
-#include <string.h>
-
 #include <atomic>
-#include <type_traits>
-#include <utility>
 
 #include "kv_internal.h"
 
@@ -335,29 +331,6 @@ extern "C" int syfi_kv_read(const void* cache, int64_t num_pages, int64_t page_s
 }
 
 // ---------------------------------------------------------------- the entry points with their arguments in one block
-namespace {
-template <typename T>
-T at(const int64_t* args, int i) {
-  if constexpr (std::is_pointer_v<T>) return reinterpret_cast<T>(args[i]);
-  else if constexpr (std::is_same_v<T, double>) {
-    double v;
-    memcpy(&v, args + i, sizeof(v));
-    return v;
-  } else return static_cast<T>(args[i]);
-}
-template <typename T>
-bool fits(int64_t word) { return !std::is_same_v<T, int32_t> || word == static_cast<int32_t>(word); }
-template <typename... Args, size_t... I>
-int spread(int (*fn)(Args...), const int64_t* args, std::index_sequence<I...>) {
-  if (!(fits<Args>(args[I]) && ...)) return kv_fail(SYFI_KV_ERR_INVALID, "an argument does not fit in 32 bits");
-  return fn(at<Args>(args, static_cast<int>(I))...);
-}
-template <typename... Args>
-int spread(int (*fn)(Args...), const int64_t* args) {
-  return args ? spread(fn, args, std::index_sequence_for<Args...>()) : kv_fail(SYFI_KV_ERR_INVALID, "no arguments");
-}
-}  // namespace
-
-extern "C" int syfi_kv_write_block(const int64_t* args) { return spread(syfi_kv_write, args); }
-extern "C" int syfi_kv_read_block(const int64_t* args) { return spread(syfi_kv_read, args); }
-extern "C" int syfi_paged_attention_block(const int64_t* args) { return spread(syfi_paged_attention, args); }
+extern "C" int syfi_kv_write_block(const int64_t* args) { return kv_spread(syfi_kv_write, args); }
+extern "C" int syfi_kv_read_block(const int64_t* args) { return kv_spread(syfi_kv_read, args); }
+extern "C" int syfi_paged_attention_block(const int64_t* args) { return kv_spread(syfi_paged_attention, args); }

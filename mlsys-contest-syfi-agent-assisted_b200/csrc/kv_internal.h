@@ -3,6 +3,10 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <string.h>
+
+#include <type_traits>
+#include <utility>
 
 #include "../../include/syfi_kv.h"
 #include "moe_internal.h"
@@ -65,5 +69,27 @@ inline bool kv_stride_ok(int64_t stride, int64_t least) { return stride >= least
 int kv_device_sms();
 
 inline int kv_fail(int code, const char* msg) { return set_last_error(code, msg); }
+
+// An entry point with its arguments in one block of 8-byte words.
+template <typename T>
+T kv_word(const int64_t* args, int i) {
+  if constexpr (std::is_pointer_v<T>) return reinterpret_cast<T>(args[i]);
+  else if constexpr (std::is_same_v<T, double>) {
+    double v;
+    memcpy(&v, args + i, sizeof(v));
+    return v;
+  } else return static_cast<T>(args[i]);
+}
+template <typename T>
+bool kv_fits(int64_t word) { return !std::is_same_v<T, int32_t> || word == static_cast<int32_t>(word); }
+template <typename... Args, size_t... I>
+int kv_spread(int (*fn)(Args...), const int64_t* args, std::index_sequence<I...>) {
+  if (!(kv_fits<Args>(args[I]) && ...)) return kv_fail(SYFI_KV_ERR_INVALID, "an argument does not fit in 32 bits");
+  return fn(kv_word<Args>(args, static_cast<int>(I))...);
+}
+template <typename... Args>
+int kv_spread(int (*fn)(Args...), const int64_t* args) {
+  return args ? kv_spread(fn, args, std::index_sequence_for<Args...>()) : kv_fail(SYFI_KV_ERR_INVALID, "no arguments");
+}
 
 }  // namespace syfi
