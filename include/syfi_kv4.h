@@ -26,6 +26,7 @@ extern "C" {
 #define SYFI_KV4_OK 0
 #define SYFI_KV4_ERR_INVALID 1   /* bad argument */
 #define SYFI_KV4_ERR_CUDA 2      /* a CUDA call failed, no CUDA device, or not an sm_100 device */
+#define SYFI_KV4_ERR_DEVICE 3    /* a kernel gave up on a bounded wait (syfi_kv4_check) */
 #define SYFI_KV4_PAGE 64
 
 /* New tokens' queries, keys and values: head norms, rotation, quantisation and the scatter into the cache in one pass.  Arguments as
@@ -64,6 +65,10 @@ int syfi_kv4_attention(const void* q, int64_t q_stride, const void* cache, int64
 int syfi_kv4_write_block(const int64_t* args);
 int syfi_kv4_read_block(const int64_t* args);
 int syfi_kv4_attention_block(const int64_t* args);
+
+/* Synchronises `stream` and reports whether an attention kernel gave up on a bounded wait on the current device since the last
+ * check (status 401; the rows that it had not finished are NaN). */
+int syfi_kv4_check(void* stream);
 
 #ifdef __cplusplus
 }

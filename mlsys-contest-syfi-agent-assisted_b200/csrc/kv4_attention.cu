@@ -4,9 +4,10 @@
 // in one pass over the cache, k and v being code * group scale, which f16 holds exactly (at most 6 * 448, two bits times four).  With x in
 // units of log2 and references m (of the sum l) and n (of the sum o) that follow the largest terms,
 //   l = sum 2^(x_j - m),   o_d = sum 2^(x_j + log2 vscale_j - n) v_jd,   out_d = o_d 2^(n - m) / l.
+#include <cstdio>
 #include <mutex>
 
-#include "kv4_internal.h"
+#include "kv4_chunk.cuh"
 #include "stream_scratch.h"
 
 namespace syfi {
@@ -23,11 +24,6 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ float lg2(float x) {
-  float r;
-  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
 }
 // The transpose of an 8 x 8 matrix of f16: lane 4 i + j has elements (i, 2 j) and (i, 2 j + 1) before, (2 j, i) and (2 j + 1, i) after.
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {
@@ -508,8 +504,10 @@ __global__ void __launch_bounds__(Decode4Shape<D, NT>::kThreads, Decode4Shape<D,
 // ---------------------------------------------------------------- host
 struct Device {
   ScratchPool scratch;
-  bool ready = false;
+  int* status = nullptr;
+  long long next_wait_limit = 0;   // syfi_kv4_debug_wait_limit: applies to the next call, then clears itself
 };
+constexpr long long kWaitLimit = 1ll << 32;   // SM clocks without a finished tile (about two seconds)
 std::mutex g_mu;
 Device g_devices[64];
 
@@ -578,14 +576,58 @@ extern "C" int syfi_kv4_attention(const void* q, int64_t q_stride, const void* c
   cudaGetDevice(&dev);
   std::lock_guard<std::mutex> lock(g_mu);
   Device& d = g_devices[dev];
-  if (!d.ready) {
-    if (!raise_decode<128, 1>() || !raise_decode<128, 2>() || !raise_decode<64, 1>() || !raise_decode<64, 2>())
+  if (!d.status) {
+    if (!raise_decode<128, 1>() || !raise_decode<128, 2>() || !raise_decode<64, 1>() || !raise_decode<64, 2>() ||
+        kv4_chunk_set_attributes() != cudaSuccess)
       return kv_fail(SYFI_KV4_ERR_CUDA, "cannot raise the shared-memory limit of the attention kernels");
-    d.ready = true;
+    RelaxedCapture relaxed;
+    int* fresh = nullptr;
+    if (cudaMalloc(&fresh, 16) != cudaSuccess) return kv_fail(SYFI_KV4_ERR_CUDA, "out of device memory");
+    if (!zero_now(fresh, 16)) {
+      cudaFree(fresh);
+      return kv_fail(SYFI_KV4_ERR_CUDA, "cannot clear the status word");
+    }
+    d.status = fresh;
   }
+  const long long wait_limit = d.next_wait_limit > 0 ? d.next_wait_limit : kWaitLimit;
+  d.next_wait_limit = 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // Rows per sequence and key head, on average (the lengths themselves are on the device).
   const int64_t rows = (tokens * a.group + batch - 1) / batch;
+  if (rows > 16) {
+    int rc = SYFI_KV4_OK;
+    if (!take_scratch(a, d, kv4_chunk_partial_bytes(head_dim, sms), st, &rc)) return rc;
+    return launch_kv4_chunk(a, head_dim, sms, d.status, wait_limit, st) == cudaSuccess ? SYFI_KV4_OK : kv_fail(SYFI_KV4_ERR_CUDA, "attention kernel launch failed");
+  }
   if (head_dim == 128) return rows <= 8 ? launch_decode<128, 1>(a, d, sms, st) : launch_decode<128, 2>(a, d, sms, st);
   return rows <= 8 ? launch_decode<64, 1>(a, d, sms, st) : launch_decode<64, 2>(a, d, sms, st);
+}
+
+// Test hook for the bounded waits, no part of the interface: a CTA of the next attention call's kernel on the current device may
+// go without finishing a tile for this many SM clocks (0: the normal limit).
+extern "C" int syfi_kv4_debug_wait_limit(int64_t clocks) {
+  if (clocks < 0) return kv_fail(SYFI_KV4_ERR_INVALID, "a wait limit must not be negative");
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return kv_fail(SYFI_KV4_ERR_CUDA, "no current CUDA device");
+  std::lock_guard<std::mutex> lock(g_mu);
+  g_devices[dev].next_wait_limit = clocks;
+  return SYFI_KV4_OK;
+}
+
+extern "C" int syfi_kv4_check(void* stream) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return kv_fail(SYFI_KV4_ERR_CUDA, "no current CUDA device");
+  if (cudaStreamSynchronize(static_cast<cudaStream_t>(stream)) != cudaSuccess) return kv_fail(SYFI_KV4_ERR_CUDA, "stream synchronisation failed");
+  std::lock_guard<std::mutex> lock(g_mu);
+  Device& d = g_devices[dev];
+  if (!d.status) return SYFI_KV4_OK;
+  int status = 0;
+  if (cudaMemcpy(&status, d.status, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess) return kv_fail(SYFI_KV4_ERR_CUDA, "cannot read the status word");
+  if (status != 0) {
+    cudaMemset(d.status, 0, sizeof(int));
+    char msg[128];
+    snprintf(msg, sizeof(msg), "a kernel reported status %d (401: a bounded wait of the attention ran out; its rows are NaN)", status);
+    return kv_fail(SYFI_KV4_ERR_DEVICE, msg);
+  }
+  return SYFI_KV4_OK;
 }

@@ -1,0 +1,1012 @@
+// Attention of many rows per sequence and key head over the 4-bit cache: chunks of prompts and whole prompts, on the tensor cores.
+//
+// A CTA (one per SM) walks its piece of the line of 128-position tiles.  A unit's up to 256 rows are two slots of 128, the M of an MMA:
+//   S = Q K^T   tcgen05.mma kind::f16.  Keys are code * group scale, which f16 holds exactly; a row of q, scaled by a power of two, too (down
+//               to 2^-29 of its largest).
+//   P           softmax warps, a thread per row.  With x in units of log2 and references m (of the sum l) and n (of O) that follow the
+//               row's largest terms, l = sum 2^(x - m) and P = 2^(x - n + 10) * vscale, rounded to f16, back into tensor memory over S.
+//   O += P V    kind::f16, P from tensor memory, values as code * group scale in shared memory, exact again.
+// Eight converting warps, a thread per position of keys or of values, keep a row's codes in registers while the stage in front is in use,
+// so nothing but f16 tiles lies in shared memory.  The slots are out of step by half a tile: while the softmax warps of one work, the tensor
+// core works for the other.  A unit of at most 128 rows takes turns: its even tiles are slot 0's, its odd ones slot 1's, and the sums are
+// added up at the end.
+//
+// n comes from a bound, the row's largest score of the tile times the tile's largest value scale.  That is near enough while the tile's
+// scales are within a factor of 8 (the largest P is then 2^7 at least, and what f16 drops 2^-32 of it at most); a tile whose scales are
+// further apart, or a row whose tile lies far below n, takes the products' own largest, as decoding does.
+#include "kv4_chunk.cuh"
+#include "stream_scratch.h"
+
+namespace syfi {
+
+namespace {
+
+constexpr int kTile = 128;             // positions per tile: two pages
+constexpr int kChunkRows = 256;
+constexpr int kChunkThreads = 640;     // 8 softmax warps, 4 for keys, 4 for values, then MMAs, planning, two idle ones
+constexpr int kSoftmaxWarps = 8, kSoftmaxThreads = 256;
+constexpr int kChunkExtra = 4;         // what a unit costs besides its tiles, in tiles
+constexpr int kSlotRows = 128;         // units of at most so many rows use one slot for their even tiles and one for their odd ones
+using ChunkPlan = Plan<kTile, kChunkRows, kChunkExtra, kSlotRows>;
+using ChunkCursor = Cursor<kTile, kChunkRows, kChunkExtra, kSlotRows>;
+constexpr int kScaleStages = 4;
+constexpr int kStatusTimeout = 401;
+
+constexpr float kProductHeadroom = 10.0f;   // P is kept times 2^10, ...
+constexpr float kProductGrowth = 4.0f;      // ... may grow by 2^4 before the reference follows, ...
+constexpr float kNear = 0.125f;             // ... and its bound is this near, or the products themselves are asked
+constexpr float kFarBelow = 70.0f;          // a tile whose bound lies so many octaves below n is summed up with its own reference
+
+template <int D>
+struct ChunkShape {
+  static constexpr int kStages = D == 128 ? 2 : 4;
+  static constexpr int kTileBytes = kTile * D * 2;                // f16: [D / 64][128 rows][64], rows of 128 bytes, swizzled
+  static constexpr int kQ = 0;                                    // [2 slots]
+  static constexpr int kK = kQ + 2 * kTileBytes;
+  static constexpr int kV = kK + kStages * kTileBytes;
+  static constexpr int kScales = kV + kStages * kTileBytes;       // [K 128 f32][V 128 f32] per stage
+  static constexpr int kSmem = 1024 + kScales + kScaleStages * 2 * kTile * 4;
+};
+
+// A piece of a unit, as the planning warp describes it to the others.
+struct Segment {
+  int tile0, tiles;                    // tiles [tile0, tile0 + tiles) of the sequence's positions; no tiles: the piece is done
+  int rows, row0;                      // rows [row0, row0 + rows) of the sequence's count * group
+  int head, b, q_first;                // key head, sequence, its first row of q
+  int base;                            // position of the sequence's first query
+  int any_low, any_high, all_low, all_high;   // positions that any / all of the rows see
+  int whole;                           // the unit lies in this piece alone
+  int turns;                           // both slots work on rows 0 .. 127 and take turns at the tiles
+  int first_part, last_part, first_slot;   // else: its Parts
+};
+__device__ __forceinline__ Parts parts_of(const Segment& g) { return {g.first_part, g.last_part, g.first_slot}; }
+constexpr int kSegmentRing = 4;
+constexpr int kSegmentReaders = 1 + 8 + kSoftmaxWarps;    // arrivals that free an entry: MMAs, converting and softmax warps
+
+struct ChunkShared {
+  Segment segment[kSegmentRing];
+  uint64_t segment_full[kSegmentRing], segment_empty[kSegmentRing];
+  uint64_t scale_full[kScaleStages], scale_empty[kScaleStages], k_full[4], k_empty[4], v_full[4], v_empty[4];
+  uint64_t q_full[2], s_full[2], p_half[2], p_full[2], o_full[2], o_empty[2], idle;
+  uint32_t tmem;
+  int there[kScaleStages][2];          // page p of the tile is there
+  alignas(16) float largest[kScaleStages][4];    // value scales of 32 positions each that any row sees, ...
+  alignas(16) float smallest[kScaleStages][4];   // ... read four at a time
+  float end[2][3][128];                // [slot][m, l, n][row], at a segment's end
+  float unit[256];                     // of each row: what a score is worth
+  volatile int abort_code;
+  volatile uint32_t tiles_done;
+  volatile int done;                   // every segment is
+  int finished;                        // segments of this CTA whose results are written
+};
+
+// Waits ask only whether somebody gave up; the clock is the planning thread's, which has time.
+__device__ __forceinline__ bool wait_for(ChunkShared& sh, uint64_t* bar, uint32_t parity) {
+  while (!mbar_try_wait(bar, parity))
+    if (sh.abort_code != 0) return false;
+  return true;
+}
+// The same for warps that have to stay whole: a lane whose wait ran out goes on, and the warp asks for the abort code later.
+__device__ __forceinline__ void wait_whole_warp(ChunkShared& sh, uint64_t* bar, uint32_t parity) { wait_for(sh, bar, parity); }
+
+// A place in a ring of stages: its index, and the parity of its use.
+template <int N>
+struct Ring {
+  int stage = 0;
+  uint32_t parity = 0;
+  __device__ void next() {
+    if (++stage == N) {
+      stage = 0;
+      parity ^= 1u;
+    }
+  }
+};
+
+// ---------------------------------------------------------------- planning, and the clock (one thread)
+struct Watch {
+  long long limit, since;
+  uint32_t seen;
+  __device__ bool over(ChunkShared& sh) {
+    const long long now = clock64();
+    if (sh.tiles_done != seen) {
+      seen = sh.tiles_done;
+      since = now;
+    } else if (now - since > limit) {
+      sh.abort_code = kStatusTimeout;
+    }
+    return sh.abort_code != 0;
+  }
+};
+
+__device__ __forceinline__ void plan_role(const AttentionArgs& a, const ChunkPlan& plan, const PlanShared& s_plan, ChunkShared& sh, int places,
+                                          long long w1, long long total, int ctas, long long wait_limit) {
+  Watch watch = {wait_limit, clock64(), 0u};
+  ChunkCursor at;
+  at.start(plan, s_plan, places);
+  Ring<kSegmentRing> ring;
+  while (true) {
+    while (!mbar_try_wait(&sh.segment_empty[ring.stage], ring.parity ^ 1u))
+      if (watch.over(sh)) return;
+    Segment& g = sh.segment[ring.stage];
+    const bool more = at.left > 0;
+    const int here = more ? at.tiles_here() : 0;
+    g.tiles = 0;
+    if (more) {
+      const int rows = at.rows(a.group), base = at.s.length - at.s.count, row0 = at.rt * kChunkRows;
+      const int first = base + row0 / a.group, last = base + (row0 + rows - 1) / a.group;
+      g.any_low = a.window > 0 ? max(first - a.window + 1, 0) : 0;
+      g.any_high = last;
+      g.tile0 = at.span.first + at.tile;
+      g.tiles = here;
+      if (rows <= kSlotRows) {             // places of two tiles, of which the unit's ends may want one
+        const int end = min(2 * (g.tile0 + here), last / kTile + 1);
+        g.tile0 = max(2 * g.tile0, g.any_low / kTile);
+        g.tiles = max(end - g.tile0, 1);
+      }
+      g.turns = rows <= kSlotRows && g.tiles > 1;
+      g.rows = rows;
+      g.row0 = row0;
+      g.head = at.head;
+      g.b = at.b;
+      g.q_first = at.s.first;
+      g.base = base;
+      g.all_low = a.window > 0 ? max(last - a.window + 1, 0) : 0;
+      g.all_high = first;
+      g.whole = here == at.span.tiles;
+      const Parts parts(total, ctas, w1 - at.left - at.tile, at.span.tiles);
+      g.first_part = parts.first;
+      g.last_part = parts.last;
+      g.first_slot = parts.first_slot;
+    }
+    mbar_arrive(&sh.segment_full[ring.stage]);
+    if (!more) break;
+    ring.next();
+    at.advance(plan, here);
+  }
+  while (sh.done == 0 && !watch.over(sh)) __nanosleep(200);
+}
+
+// ---------------------------------------------------------------- MMAs (one thread)
+template <int D>
+__device__ __forceinline__ void mma_role(ChunkShared& sh, uint8_t* smem, uint32_t tmem) {
+  using Shape = ChunkShape<D>;
+  constexpr int kStages = Shape::kStages;
+  const uint32_t qk_desc = umma_idesc_f16_m128(kTile), pv_desc = umma_idesc_f16_m128_n_major(D);
+  const uint64_t q_desc = umma_smem_desc_sw128(smem_u32(smem + Shape::kQ));
+  const uint64_t v_desc = umma_smem_desc_n_major_sw128(smem_u32(smem + Shape::kV), kTile * 128);
+  const uint32_t q0 = static_cast<uint32_t>(q_desc), k0 = q0 + (Shape::kK - Shape::kQ) / 16, qk_hi = static_cast<uint32_t>(q_desc >> 32);
+  const uint32_t v0 = static_cast<uint32_t>(v_desc), v_hi = static_cast<uint32_t>(v_desc >> 32);
+  auto scores = [&](int slot, int q_slot, int stage) {
+    const uint32_t k = k0 + stage * (Shape::kTileBytes / 16), q = q0 + q_slot * (Shape::kTileBytes / 16), to = tmem + slot * 128;
+#pragma unroll
+    for (int step = 0; step < D / 16; ++step) {
+      const uint32_t at = step / 4 * (kTile * 128 / 16) + step % 4 * 2;
+      umma_f16_words(to, q + at, k + at, qk_hi, qk_desc, step > 0 ? 1u : 0u);
+    }
+    umma_commit(&sh.s_full[slot]);
+  };
+  auto values = [&](int slot, int stage, int half, uint32_t add) {
+    const uint32_t v = v0 + stage * (Shape::kTileBytes / 16), p = tmem + slot * 128;
+#pragma unroll
+    for (int i = 0; i < kTile / 32; ++i) {
+      const int step = half * (kTile / 32) + i;
+      umma_f16_ts_words(p + 256, p + 8 * step, v + 128 * step, v_hi, pv_desc, step == 0 ? add : 1u);
+    }
+  };
+  Ring<kSegmentRing> segments;
+  Ring<kStages> keys, vals;
+  uint32_t tile_parity = 0, segment_parity = 0;    // bit s: of slot s
+  // P of the slot's tile, in two halves, times its values
+  auto product = [&](int s, int stage, uint32_t add) {
+    const uint32_t parity = tile_parity >> s & 1u;
+    tile_parity ^= 1u << s;
+    if (!wait_for(sh, &sh.p_half[s], parity)) return false;
+    tc_fence_after();
+    values(s, stage, 0, add);
+    if (!wait_for(sh, &sh.p_full[s], parity)) return false;
+    tc_fence_after();
+    values(s, stage, 1, 1u);
+    return true;
+  };
+  while (true) {
+    if (!wait_for(sh, &sh.segment_full[segments.stage], segments.parity)) return;
+    const Segment& g = sh.segment[segments.stage];
+    const int n = g.tiles, turns = g.turns, slots = turns || g.rows > kSlotRows ? 2 : 1;
+    if (n == 0) return;
+    mbar_arrive(&sh.segment_empty[segments.stage]);
+    segments.next();
+    for (int s = 0; s < slots; ++s)
+      if (!wait_for(sh, &sh.q_full[s], segment_parity >> s & 1u)) return;
+    // A slot's scores of its next tile follow its values' product, which reads the weights in their place.
+    if (turns) {                             // tile j in slot j % 2
+      for (int j = 0; j < 2; ++j) {
+        if (!wait_for(sh, &sh.k_full[keys.stage], keys.parity)) return;
+        tc_fence_after();
+        scores(j, 0, keys.stage);
+        umma_commit(&sh.k_empty[keys.stage]);
+        keys.next();
+      }
+      for (int j = 0; j < n; ++j) {
+        const int s = j & 1;
+        const bool more = j + 2 < n;
+        if (j < 2 && !wait_for(sh, &sh.o_empty[s], (segment_parity >> s & 1u) ^ 1u)) return;
+        if (!wait_for(sh, &sh.v_full[vals.stage], vals.parity)) return;
+        if (!product(s, vals.stage, j < 2 ? 0u : 1u)) return;
+        umma_commit(&sh.v_empty[vals.stage]);
+        vals.next();
+        if (more) {
+          if (!wait_for(sh, &sh.k_full[keys.stage], keys.parity)) return;
+          tc_fence_after();
+          scores(s, 0, keys.stage);
+          umma_commit(&sh.k_empty[keys.stage]);
+          keys.next();
+        } else {
+          umma_commit(&sh.o_full[s]);
+        }
+      }
+      segment_parity ^= 3u;
+      continue;
+    }
+    if (!wait_for(sh, &sh.k_full[keys.stage], keys.parity)) return;
+    tc_fence_after();
+    for (int s = 0; s < slots; ++s) scores(s, s, keys.stage);
+    umma_commit(&sh.k_empty[keys.stage]);
+    keys.next();
+    for (int j = 0; j < n; ++j) {
+      const bool more = j + 1 < n;
+      if (more && !wait_for(sh, &sh.k_full[keys.stage], keys.parity)) return;
+      if (!wait_for(sh, &sh.v_full[vals.stage], vals.parity)) return;
+#pragma unroll 1
+      for (int s = 0; s < slots; ++s) {
+        if (j == 0 && !wait_for(sh, &sh.o_empty[s], (segment_parity >> s & 1u) ^ 1u)) return;
+        if (!product(s, vals.stage, j > 0 ? 1u : 0u)) return;
+        if (s + 1 == slots) umma_commit(&sh.v_empty[vals.stage]);
+        if (more) scores(s, s, keys.stage);
+        else umma_commit(&sh.o_full[s]);
+      }
+      vals.next();
+      if (more) {
+        umma_commit(&sh.k_empty[keys.stage]);
+        keys.next();
+      }
+    }
+    segment_parity ^= slots == 2 ? 3u : 1u;
+  }
+}
+
+// ---------------------------------------------------------------- codes to f16, a thread per position (four warps for keys, four for values)
+// A row of codes and its scales on their way from the cache.
+template <int D>
+struct RawRow {
+  uint4 codes[D / 32];
+  uint32_t groups[D / 64];
+  float k_scale, v_scale;              // (values' threads only)
+};
+
+template <int D, bool VALUES>
+__device__ __forceinline__ void convert_role(const AttentionArgs& a, ChunkShared& sh, uint8_t* smem) {
+  using Shape = ChunkShape<D>;
+  constexpr int kStages = Shape::kStages;
+  const int t = threadIdx.x % 128, lane = threadIdx.x % 32, warp = t / 32, page_of = t / kKvPage, at = t % kKvPage;
+  uint64_t* const full = VALUES ? sh.v_full : sh.k_full;
+  uint64_t* const empty = VALUES ? sh.v_empty : sh.k_empty;
+  Ring<kSegmentRing> segments;           // of the tile to ask for
+  Ring<kScaleStages> scales;
+  Ring<kStages> tiles;
+  // The walk of the loads: a tile's row is asked for when the tile in front is converted, its table entry one tile earlier.
+  int next_tile = 0, left = 0, any_low = 0, any_high = 0, all_low = 0, all_high = 0, head = 0;
+  const int32_t* table = nullptr;
+  int entry = -1, position = 0;          // of the tile to ask for
+  int entry_low = 0, entry_high = 0, entry_all_low = 0, entry_all_high = 0, entry_head = 0;
+  auto next_entry = [&]() -> bool {      // whole warp; false behind the last tile
+    if (left == 0) {
+      wait_whole_warp(sh, &sh.segment_full[segments.stage], segments.parity);
+      __syncwarp();
+      const Segment& g = sh.segment[segments.stage];
+      left = __any_sync(0xffffffffu, sh.abort_code != 0) ? 0 : g.tiles;
+      if (left == 0) return false;
+      next_tile = g.tile0;
+      any_low = g.any_low;
+      any_high = g.any_high;
+      all_low = g.all_low;
+      all_high = g.all_high;
+      head = g.head;
+      table = a.batch.block_table + static_cast<long long>(g.b) * a.batch.max_pages;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.segment_empty[segments.stage]);
+      segments.next();
+    }
+    const int page = 2 * next_tile + page_of;
+    position = next_tile * kTile + t;
+    entry = page < a.batch.max_pages && page * kKvPage <= any_high && (page + 1) * kKvPage > any_low ? __ldg(table + page) : -1;
+    entry_low = any_low;
+    entry_high = any_high;
+    entry_all_low = all_low;
+    entry_all_high = all_high;
+    entry_head = head;
+    ++next_tile;
+    --left;
+    return true;
+  };
+  RawRow<D> row;
+  bool there = false, plain = false, seen = false;     // of the row in registers
+  auto ask = [&]() {
+    there = entry >= 0 && entry < a.cache.num_pages;
+    seen = position >= entry_low && position <= entry_high;
+    const int first = position - t;
+    plain = first >= entry_all_low && first + kTile - 1 <= entry_all_high;
+    if (there) {
+      const uint8_t* const keys = kv4_block<D>(a.cache, entry, 0, entry_head);
+      const uint8_t* const block = VALUES ? keys + static_cast<long long>(a.cache.heads) * Kv4Block<D>::kBytes : keys;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) row.codes[i] = __ldg(reinterpret_cast<const uint4*>(block + i / 2 * kKv4Plane + at * 32) + i % 2);
+      const uint32_t* const groups = reinterpret_cast<const uint32_t*>(block + Kv4Block<D>::kGroups + at * (D / kKv4Group));
+      if constexpr (D == 128) {
+        const uint2 g = __ldg(reinterpret_cast<const uint2*>(groups));
+        row.groups[0] = g.x;
+        row.groups[1] = g.y;
+      } else {
+        row.groups[0] = __ldg(groups);
+      }
+      if constexpr (VALUES) {
+        row.k_scale = __ldg(reinterpret_cast<const float*>(keys + Kv4Block<D>::kScales) + at);
+        row.v_scale = __ldg(reinterpret_cast<const float*>(block + Kv4Block<D>::kScales) + at);
+      }
+    }
+  };
+  bool more = next_entry();
+  if (more) ask();
+  while (more) {
+    more = next_entry();                 // (of the tile behind the one in registers)
+    bool valid = there;
+    if constexpr (VALUES) {
+      // What a row does not see must not reach its sums, and zero times NaN is NaN: values of positions that no row sees become zeros, and
+      // where some rows see a value that is not finite, the NaN goes by way of its score to those rows alone.
+      float ks = there ? row.k_scale : 0.0f, vs = there ? row.v_scale : 1.0f;
+      bool bad = !(fabsf(vs) <= 3.402823466e38f);
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) bad |= there && (((row.groups[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0u;
+      valid = there && seen && (plain || !bad);
+      if (bad || !(fabsf(ks) <= 3.402823466e38f)) ks = __int_as_float(0x7fffffff);
+      if (!valid) vs = 1.0f;
+      const unsigned bits = __float_as_uint(vs);
+      const bool counts = valid && bits < 0x7f800000u;
+      const unsigned high = __reduce_max_sync(0xffffffffu, counts ? bits : 0u), low = __reduce_min_sync(0xffffffffu, counts ? bits : 0x7f800000u);
+      wait_whole_warp(sh, &sh.scale_empty[scales.stage], scales.parity ^ 1u);
+      __syncwarp();
+      float* const to = reinterpret_cast<float*>(smem + Shape::kScales) + scales.stage * 2 * kTile;
+      to[t] = ks;
+      to[kTile + t] = vs;
+      if (lane == 0) {
+        sh.largest[scales.stage][warp] = __uint_as_float(high);
+        sh.smallest[scales.stage][warp] = __uint_as_float(low);
+        if (warp % 2 == 0) sh.there[scales.stage][page_of] = there;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.scale_full[scales.stage]);
+      scales.next();
+    }
+    wait_whole_warp(sh, &empty[tiles.stage], tiles.parity ^ 1u);
+    __syncwarp();
+    uint8_t* const to = smem + (VALUES ? Shape::kV : Shape::kK) + tiles.stage * Shape::kTileBytes + t * 128;
+    if (valid) {
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        const uint32_t w[4] = {row.codes[i].x, row.codes[i].y, row.codes[i].z, row.codes[i].w};
+        // two groups of 16 dimensions, 8 in a word
+        const uint32_t both = e4m3x2_to_half2(row.groups[i / 2] >> (16 * (i % 2)));
+        const uint32_t scale[2] = {__byte_perm(both, both, 0x1010), __byte_perm(both, both, 0x3232)};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int chunk = i % 2 * 4 + k;
+          *reinterpret_cast<uint4*>(to + i / 2 * (kTile * 128) + ((chunk ^ (t & 7)) << 4)) =
+              make_uint4(hmul2_bits(e2m1x2_to_half2<0>(w[k]), scale[k / 2]), hmul2_bits(e2m1x2_to_half2<1>(w[k]), scale[k / 2]),
+                         hmul2_bits(e2m1x2_to_half2<2>(w[k]), scale[k / 2]), hmul2_bits(e2m1x2_to_half2<3>(w[k]), scale[k / 2]));
+        }
+      }
+    } else if (VALUES) {
+#pragma unroll 1
+      for (int chunk = 0; chunk < D / 8; ++chunk) *reinterpret_cast<uint4*>(to + chunk / 8 * (kTile * 128) + chunk % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&full[tiles.stage]);
+    tiles.next();
+    if (more) ask();
+    if (__any_sync(0xffffffffu, sh.abort_code != 0)) return;
+  }
+}
+
+// ---------------------------------------------------------------- softmax, a thread per row (eight warps, four to a slot)
+__device__ __forceinline__ ulonglong2 ld_shared_pairs(uint32_t at) {
+  ulonglong2 v;
+  asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(v.x), "=l"(v.y) : "r"(at) : "memory");
+  return v;
+}
+
+// A tile's row: 128 scores from tensor memory, their weights back into it; the row's references m and n and its sum l.  unit: what a score
+// is worth.  low, high: what the row sees, counted from the tile's first position; there0, there1: the tile's pages.
+template <int D>
+__device__ __forceinline__ void softmax_tile(ChunkShared& sh, int slot, int stage, uint32_t t_s, uint32_t t_o, uint32_t scales, bool masked, int low, int high,
+                                             float unit, bool first, float& m, float& n, float& l) {
+  uint32_t s[4][32];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) tmem_ld32(t_s + 32 * c, s[c]);
+  tmem_ld_wait_for(s[0]);
+#pragma unroll
+  for (int c = 1; c < 4; ++c) tmem_landed(s[c]);
+  // times the keys' scales: in units of the row's
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const ulonglong2 ks = ld_shared_pairs(scales + 4 * (32 * c + 4 * e));
+      float x0, x1, x2, x3;
+      f32x2_unpack(f32x2_mul(f32x2_pack_bits(s[c][4 * e], s[c][4 * e + 1]), ks.x), x0, x1);
+      f32x2_unpack(f32x2_mul(f32x2_pack_bits(s[c][4 * e + 2], s[c][4 * e + 3]), ks.y), x2, x3);
+      s[c][4 * e] = __float_as_uint(x0);
+      s[c][4 * e + 1] = __float_as_uint(x1);
+      s[c][4 * e + 2] = __float_as_uint(x2);
+      s[c][4 * e + 3] = __float_as_uint(x3);
+    }
+  }
+  if (__builtin_expect(masked, 0)) {
+    const bool there[2] = {sh.there[stage][0] != 0, sh.there[stage][1] != 0};
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int first_bit = low - 32 * c, last_bit = high - 32 * c;
+      uint32_t bits = last_bit < 0 || first_bit > 31 || !there[c / 2] ? 0u : 0xffffffffu;
+      if (last_bit >= 0 && last_bit < 31) bits &= (2u << last_bit) - 1u;
+      if (first_bit > 0 && first_bit <= 31) bits &= 0xffffffffu << first_bit;
+#pragma unroll
+      for (int b = 0; b < 32; ++b)
+        if (!(bits >> b & 1u)) s[c][b] = 0xff800000u;
+    }
+  }
+  float tops[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    tops[c] = fmaxf(__uint_as_float(s[c][0]), __uint_as_float(s[c][1]));
+#pragma unroll
+    for (int b = 2; b < 32; b += 2) tops[c] = fmaxf(tops[c], fmaxf(__uint_as_float(s[c][b]), __uint_as_float(s[c][b + 1])));
+  }
+  const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * unit;
+  const float4 v_high = *reinterpret_cast<const float4*>(sh.largest[stage]), v_low = *reinterpret_cast<const float4*>(sh.smallest[stage]);
+  const float largest = fmaxf(fmaxf(v_high.x, v_high.y), fmaxf(v_high.z, v_high.w)), smallest = fminf(fminf(v_low.x, v_low.y), fminf(v_low.z, v_low.w));
+  if (top > m + kSumGrowth) {
+    l *= ex2(m - top);                 // (0 for a row that had seen nothing)
+    m = top;
+  }
+  float bound = top + lg2(largest);
+  const bool near = smallest >= kNear * largest && largest >= 1e-18f && largest <= 1e18f;     // (no scale of zero among them)
+  const uint64_t unit2 = f32x2_pack(unit, unit);
+  const bool slow = !near || __any_sync(0xffffffffu, bound < n - kFarBelow && top != -INFINITY);      // (not for a row that is not finite)
+  const uint32_t v_scales = scales + kTile * 4;
+  if (__builtin_expect(slow, 0)) {
+    // the products themselves: weights in units of m, then times the values' scales
+    const float shift = -finite_or_zero(m);
+    float sum = 0.0f, most = 0.0f;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+#pragma unroll
+      for (int e = 0; e < 32; e += 4) {
+        const ulonglong2 vs = ld_shared_pairs(v_scales + 4 * (32 * c + e));
+        float v[4];
+        f32x2_unpack(vs.x, v[0], v[1]);
+        f32x2_unpack(vs.y, v[2], v[3]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float p = ex2(fmaf(__uint_as_float(s[c][e + k]), unit, shift));
+          sum += p;
+          const float y = p * v[k];
+          most = fmaxf(most, y);
+          s[c][e + k] = __float_as_uint(y);
+        }
+      }
+    }
+    l += sum;
+    bound = m + fmaxf(lg2(most), -90.0f);      // (never further behind: a value may be zero)
+  }
+  float fade = 1.0f;
+  if (bound > n + kProductGrowth) {
+    fade = ex2(n - bound);
+    n = bound;
+  }
+  if (!first && __any_sync(0xffffffffu, fade != 1.0f)) {
+#pragma unroll 1
+    for (int c = 0; c < D; c += 8) {
+      uint32_t o[8];
+      tmem_ld8(t_o + c, o);
+      tmem_ld_wait_for(o);
+#pragma unroll
+      for (int b = 0; b < 8; ++b) o[b] = __float_as_uint(__uint_as_float(o[b]) * fade);
+      tmem_st8(t_o + c, o);
+    }
+  }
+  const int lane = threadIdx.x % 32;
+  if (__builtin_expect(slow, 0)) {
+    const float f = m == -INFINITY || n == -INFINITY ? 0.0f : ex2(m - n + kProductHeadroom);
+#pragma unroll
+    for (int h = 0; h < 8; ++h) {
+      uint32_t p[8];
+#pragma unroll
+      for (int b = 0; b < 8; ++b) p[b] = pack_half2(__uint_as_float(s[h / 2][16 * (h % 2) + 2 * b]) * f, __uint_as_float(s[h / 2][16 * (h % 2) + 2 * b + 1]) * f);
+      tmem_st8(t_s + 8 * h, p);
+    }
+    tmem_st_wait();
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) {
+      mbar_arrive(&sh.p_half[slot]);
+      mbar_arrive(&sh.p_full[slot]);
+    }
+    return;
+  }
+  const float shift = kProductHeadroom - finite_or_zero(n);
+  const uint64_t shift2 = f32x2_pack(shift, shift);
+  uint64_t sums[2] = {0ull, 0ull};
+#pragma unroll
+  for (int h = 0; h < 8; ++h) {
+    uint32_t p[8];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const int at = 16 * (h % 2) + 4 * b;
+      const ulonglong2 vs = ld_shared_pairs(v_scales + 4 * (16 * h + 4 * b));
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float x0, x1;
+        f32x2_unpack(f32x2_fma(f32x2_pack_bits(s[h / 2][at + 2 * k], s[h / 2][at + 2 * k + 1]), unit2, shift2), x0, x1);
+        const uint64_t w = f32x2_pack(ex2(x0), ex2(x1));
+        sums[k] = f32x2_add(sums[k], w);
+        f32x2_unpack(f32x2_mul(w, k ? vs.y : vs.x), x0, x1);
+        p[2 * b + k] = pack_half2(x0, x1);
+      }
+    }
+    tmem_st8(t_s + 8 * h, p);
+    if (h % 4 == 3) {
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(h == 3 ? &sh.p_half[slot] : &sh.p_full[slot]);
+    }
+  }
+  float a0, a1;
+  f32x2_unpack(f32x2_add(sums[0], sums[1]), a0, a1);
+  l += (a0 + a1) * ex2(-shift - finite_or_zero(m));
+}
+
+// The warp's 32 rows of q (of which `rows` are there; mine: where this lane's row begins in q) as f16 times 2^k each, the row's largest at
+// 2^14 .. 2^15, into rows row0 and on of a tile.  D / 8 lanes read a row.  units: what a score of each row is worth.
+template <int D>
+__device__ __forceinline__ void put_queries(const __nv_bfloat16* q, long long mine, float scale_log2, int rows, uint8_t* tile, int row0, float* units) {
+  constexpr int kLanes = D / 8, kTogether = 32 / kLanes, kBatch = 4;      // rows at a time, loads under way
+  const int lane = threadIdx.x % 32, part = lane % kLanes;
+#pragma unroll 1
+  for (int at = 0; at < 32; at += kTogether * kBatch) {
+    uint4 raw[kBatch];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int row = at + b * kTogether + lane / kLanes;
+      const long long from = __shfl_sync(0xffffffffu, mine, row);
+      raw[b] = make_uint4(0u, 0u, 0u, 0u);
+      if (row < rows) raw[b] = __ldg(reinterpret_cast<const uint4*>(q + from) + part);
+    }
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int row = at + b * kTogether + lane / kLanes;
+      const uint32_t w[4] = {raw[b].x, raw[b].y, raw[b].z, raw[b].w};
+      unsigned top = 0u;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = max(top, max(w[e] & 0x7fffu, w[e] >> 16 & 0x7fffu));
+#pragma unroll
+      for (int d = kLanes / 2; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+      const int k = top == 0u ? 0 : min(14 - (static_cast<int>(top >> 7) - 127), 120);
+      const float up = copysignf(__int_as_float((k + 127) << 23), scale_log2);
+      uint32_t h[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) h[e] = pack_half2(__uint_as_float(w[e] << 16) * up, __uint_as_float(w[e] & 0xffff0000u) * up);
+      // (a row that is not finite is NaN throughout, so that the mask takes its scores out like any other's)
+      if (top >= 0x7f80u) h[0] = h[1] = h[2] = h[3] = 0x7fff7fffu;
+      *reinterpret_cast<uint4*>(tile + part / 8 * (kTile * 128) + (row0 + row) * 128 + ((part % 8 ^ ((row0 + row) & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+      // (a scale of zero keeps a factor, f32's smallest normal number, so that -infinity stays what it is)
+      if (part == 0) units[row] = fmaxf(fabsf(scale_log2) * __int_as_float((127 - k) << 23), 1.17549435e-38f);
+    }
+  }
+}
+
+// A barrier of the softmax warps that tells all of them whether any thread's `p` holds.
+__device__ __forceinline__ bool softmax_bar_any(bool p) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, 1, 256, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any)
+      : "r"(static_cast<uint32_t>(p))
+      : "memory");
+  return any != 0u;
+}
+
+// Adds up a split unit's parts, kept by dimension ([part][D / 4][rows][4], then [part][rows] of (m, l, n, -)): a thread has a row and sixteen of
+// its dimensions.
+template <int D>
+__device__ __forceinline__ void join_columns(const AttentionArgs& a, int q_first, int unit_row0, int head, int rows, int ctas, const Parts& parts, int thread, int threads) {
+  const float4* const stats = reinterpret_cast<const float4*>(a.partial + 2ll * ctas * kChunkRows * D);
+  const float4* const sums = reinterpret_cast<const float4*>(a.partial);
+  for (int i = thread; i < kChunkRows * (D / 16); i += threads) {
+    const int row = i % kChunkRows, d16 = i / kChunkRows;
+    if (row >= rows) continue;
+    float m = -INFINITY, n = -INFINITY, l = 0.0f, o[16] = {};
+#pragma unroll 2
+    for (int c = parts.first; c <= parts.last; ++c) {
+      const long long slot = parts.slot(c);
+      const float4 st = __ldcg(stats + slot * kChunkRows + row);
+      float4 p[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) p[k] = __ldcg(sums + (slot * (D / 4) + 4 * d16 + k) * kChunkRows + row);
+      const float m_new = fmaxf(m, st.x), m_ref = finite_or_zero(m_new), n_new = fmaxf(n, st.z), n_ref = finite_or_zero(n_new);
+      l = l * ex2(m - m_ref) + st.y * ex2(st.x - m_ref);
+      const float f = ex2(n - n_ref), w = ex2(st.z - n_ref);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        o[4 * k] = o[4 * k] * f + p[k].x * w;
+        o[4 * k + 1] = o[4 * k + 1] * f + p[k].y * w;
+        o[4 * k + 2] = o[4 * k + 2] * f + p[k].z * w;
+        o[4 * k + 3] = o[4 * k + 3] * f + p[k].w * w;
+      }
+      m = m_new;
+      n = n_new;
+    }
+    const float f = l == 0.0f || n == -INFINITY ? 0.0f : ex2(n - finite_or_zero(m) - kProductHeadroom) / l;
+    const int r = unit_row0 + row;
+    uint4* const to = reinterpret_cast<uint4*>(a.out + (q_first + r / a.group) * a.out_stride + (head * a.group + r % a.group) * D + 16 * d16);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(o[8 * h + 2 * e] * f, o[8 * h + 2 * e + 1] * f);
+        w[e] = *reinterpret_cast<const uint32_t*>(&b);
+      }
+      to[h] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared& sh, PlanShared& s_plan, uint8_t* smem, uint32_t tmem, int ctas) {
+  using Shape = ChunkShape<D>;
+  // warps 0-3: slot 0, 4-7: slot 1
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, slot = warp / 4, in_slot = warp % 4 * 32 + lane;
+  const int across = 2 + warp % 4;                 // named barrier of the two slots' warps for the same rows
+  const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
+  const uint32_t t_s = tmem + lanes + slot * 128, t_o = tmem + lanes + 256 + slot * 128, scales0 = smem_u32(smem) + Shape::kScales;
+  static_assert(kSegmentRing == 4 && kScaleStages == 4, "stage and parity are bits of a counter");
+  uint32_t segment = 0, tile = 0, own = 0, own_segments = 0;       // segments and tiles so far, and those of this slot
+  while (true) {
+    wait_whole_warp(sh, &sh.segment_full[segment & 3], segment >> 2 & 1);
+    if (softmax_bar_any(sh.abort_code != 0)) return;      // all eight warps meet here whatever failed, and leave together
+    const Segment& g = sh.segment[segment & 3];
+    if (g.tiles == 0) {
+      if (tid == 0) sh.done = 1;
+      return;
+    }
+    const bool turns = g.turns;
+    // whether the next tile is this slot's (bit 0: no), and whether that changes with each (bit 1)
+    unsigned turn = turns ? 2u + slot : g.rows <= slot * kSlotRows;
+    const bool active = turn != 1u;
+    const int row = (turns ? 0 : slot * kSlotRows) + in_slot;
+    float m = -INFINITY, n = -INFINITY, l = 0.0f;
+    int token_of_row = 0, column_of_row = 0;         // of this thread's row, in q and out
+    {
+      int low, high;
+      {
+        const int r = g.row0 + min(row, g.rows - 1), token = r / a.group;        // (rows beyond the last copy its bounds)
+        token_of_row = g.q_first + token;
+        column_of_row = (g.head * a.group + r - token * a.group) * D;
+        high = g.base + token;
+        low = a.window > 0 ? max(high - a.window + 1, 0) : 0;
+      }
+      const int q_slot = turns ? 0 : slot;
+      if (active && q_slot == slot) {
+        const int in_tile = warp % 4 * 32;
+        put_queries<D>(a.q, token_of_row * a.q_stride + column_of_row, a.scale_log2, g.rows - slot * kSlotRows - in_tile,
+                       smem + Shape::kQ + slot * Shape::kTileBytes, in_tile, sh.unit + slot * 128 + in_tile);
+        fence_proxy_async_smem();
+      }
+      __syncwarp();
+      if (active && lane == 0) mbar_arrive(&sh.q_full[slot]);
+      if (turns) named_bar_sync(1, kSoftmaxThreads);       // slot 1 reads slot 0's units
+      const float unit = sh.unit[q_slot * 128 + in_slot];
+      // from here on positions count from the segment's first tile
+      low -= g.tile0 * kTile;
+      high -= g.tile0 * kTile;
+      bool first = true;
+      for (int left = g.tiles; left > 0; --left) {
+        const int stage = tile & 3;
+        wait_whole_warp(sh, &sh.scale_full[stage], tile >> 2 & 1);
+        if (!(turn & 1u)) {
+          wait_whole_warp(sh, &sh.s_full[slot], own & 1);
+          __syncwarp();
+          tc_fence_after();
+          const bool masked = sh.there[stage][0] == 0 || sh.there[stage][1] == 0 || __any_sync(0xffffffffu, low > 0 || high < kTile - 1);
+          softmax_tile<D>(sh, slot, stage, t_s, t_o, scales0 + stage * (2 * kTile * 4), masked, low, high, unit, first, m, n, l);
+          ++own;
+          first = false;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.scale_empty[stage]);
+        ++tile;
+        if (tid == 0) sh.tiles_done = sh.tiles_done + 1u;
+        turn ^= turn >> 1 & 1u;
+        low -= kTile;
+        high -= kTile;
+      }
+    }
+    // ---- the segment's end
+    if (active) {
+      wait_whole_warp(sh, &sh.o_full[slot], own_segments & 1);
+      __syncwarp();
+      tc_fence_after();
+      ++own_segments;
+      sh.end[slot][0][in_slot] = m;
+      sh.end[slot][1][in_slot] = l;
+      sh.end[slot][2][in_slot] = n;
+    }
+    if (softmax_bar_any(sh.abort_code != 0)) return;
+    const bool whole = g.whole, real = row < g.rows && !(turns && slot == 1);
+    if (active) {
+      float f = 1.0f;
+      if (turns) {                            // to the larger references of the two slots'
+        const float(&its)[3][128] = sh.end[slot ^ 1];
+        const float m_all = fmaxf(m, its[0][in_slot]), m_ref = finite_or_zero(m_all), n_all = fmaxf(n, its[2][in_slot]);
+        l = l * ex2(m - m_ref) + its[1][in_slot] * ex2(its[0][in_slot] - m_ref);
+        f = ex2(n - finite_or_zero(n_all));
+        m = m_all;
+        n = n_all;
+      }
+      const float inverse = l == 0.0f || n == -INFINITY ? 0.0f : ex2(n - finite_or_zero(m) - kProductHeadroom) / l;
+      if (whole) f *= inverse;
+      // Rows leave through the warp's own rows of the slot's q tile, which nothing reads any more.  Partial sums are kept by dimension, so that
+      // a warp's 32 rows lie side by side.
+      uint8_t* const own_rows = smem + Shape::kQ + slot * Shape::kTileBytes + warp % 4 * (32 * 128);
+      float4* const its = reinterpret_cast<float4*>(smem + Shape::kQ + Shape::kTileBytes + warp % 4 * (32 * 128)) + lane;   // of slot 1's q tile
+      float4* const to = reinterpret_cast<float4*>(a.partial);
+      const int part = parts_of(g).slot(static_cast<int>(blockIdx.x));
+#pragma unroll 1
+      for (int c = 0; c < D; c += 16) {
+        uint32_t o[16];
+        tmem_ld16(t_o + c, o);
+        tmem_ld_wait_for(o);
+#pragma unroll
+        for (int b = 0; b < 16; ++b) o[b] = __float_as_uint(__uint_as_float(o[b]) * f);
+        if (turns) {                          // slot 0 adds slot 1's sums to its own
+          if (slot == 1) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+              its[32 * b] = make_float4(__uint_as_float(o[4 * b]), __uint_as_float(o[4 * b + 1]), __uint_as_float(o[4 * b + 2]), __uint_as_float(o[4 * b + 3]));
+          }
+          named_bar_sync(across, 64);
+          if (slot == 0) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+              const float4 x = its[32 * b];
+              o[4 * b] = __float_as_uint(__uint_as_float(o[4 * b]) + x.x);
+              o[4 * b + 1] = __float_as_uint(__uint_as_float(o[4 * b + 1]) + x.y);
+              o[4 * b + 2] = __float_as_uint(__uint_as_float(o[4 * b + 2]) + x.z);
+              o[4 * b + 3] = __float_as_uint(__uint_as_float(o[4 * b + 3]) + x.w);
+            }
+          }
+          named_bar_sync(across, 64);
+          if (slot == 1) continue;
+        }
+        if (whole) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(o[8 * h + 2 * e]), __uint_as_float(o[8 * h + 2 * e + 1]));
+              w[e] = *reinterpret_cast<const uint32_t*>(&b);
+            }
+            const int chunk = c / 8 + h;
+            *reinterpret_cast<uint4*>(own_rows + chunk / 8 * (kTile * 128) + lane * 128 + ((chunk % 8 ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        } else if (real) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            to[(static_cast<long long>(part) * (D / 4) + c / 4 + e) * kChunkRows + row] =
+                make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
+        }
+      }
+      if (whole && !(turns && slot == 1)) {
+        __syncwarp();
+        constexpr int kLanes = D / 8, kTogether = 32 / kLanes;
+        const long long mine = token_of_row * a.out_stride + column_of_row;
+        const int first_row = (turns ? 0 : slot * kSlotRows) + warp % 4 * 32, chunk = lane % kLanes;
+#pragma unroll 4
+        for (int at = 0; at < 32; at += kTogether) {
+          const int line = at + lane / kLanes;
+          const long long begin = __shfl_sync(0xffffffffu, mine, line);
+          const uint4 p = *reinterpret_cast<const uint4*>(own_rows + chunk / 8 * (kTile * 128) + line * 128 + ((chunk % 8 ^ (line & 7)) << 4));
+          if (first_row + line < g.rows) *(reinterpret_cast<uint4*>(a.out + begin) + chunk) = p;
+        }
+      }
+      if (real && !whole) reinterpret_cast<float4*>(a.partial + 2ll * ctas * kChunkRows * D)[static_cast<long long>(part) * kChunkRows + row] = make_float4(m, l, n, 0.0f);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.o_empty[slot]);
+    }
+    if (!whole) {
+      const Parts parts = parts_of(g);
+      __threadfence();
+      named_bar_sync(1, kSoftmaxThreads);
+      if (tid == 0) {
+        const bool is_last = atomicAdd(a.tickets + parts.first, 1) == parts.last - parts.first;
+        if (is_last) a.tickets[parts.first] = 0;
+        s_plan.last = is_last;
+      }
+      named_bar_sync(1, kSoftmaxThreads);
+      if (s_plan.last) {
+        __threadfence();
+        join_columns<D>(a, g.q_first, g.row0, g.head, g.rows, ctas, parts, tid, kSoftmaxThreads);
+      }
+    }
+    if (tid == 0) ++sh.finished;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.segment_empty[segment & 3]);
+    ++segment;
+  }
+}
+
+template <int D>
+__global__ void __launch_bounds__(kChunkThreads, 1)
+kv4_chunk_kernel(const __grid_constant__ AttentionArgs a, int* __restrict__ status, long long wait_limit) {
+  using Shape = ChunkShape<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  __shared__ ChunkShared sh;
+  __shared__ PlanShared s_plan;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+
+  pdl_wait();
+  pdl_trigger();
+  const ChunkPlan plan = {a.batch, a.cache.heads, a.group, a.window};
+  const long long total = plan.total(s_plan);
+  const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
+  if (static_cast<int>(blockIdx.x) >= ctas) return;
+  const long long w0 = piece_start(total, ctas, blockIdx.x), w1 = piece_start(total, ctas, blockIdx.x + 1);
+  const int places = static_cast<int>(w1 - w0);
+  plan.locate(s_plan, w0);
+
+  if (tid == 0) {
+    for (int i = 0; i < kScaleStages; ++i) {
+      mbar_init(&sh.scale_full[i], 4);
+      mbar_init(&sh.scale_empty[i], kSoftmaxWarps);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&sh.k_full[i], 4);
+      mbar_init(&sh.k_empty[i], 1);
+      mbar_init(&sh.v_full[i], 4);
+      mbar_init(&sh.v_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.q_full[i], 4);
+      mbar_init(&sh.s_full[i], 1);
+      mbar_init(&sh.p_half[i], 4);
+      mbar_init(&sh.p_full[i], 4);
+      mbar_init(&sh.o_full[i], 1);
+      mbar_init(&sh.o_empty[i], 4);
+    }
+    mbar_init(&sh.idle, 1);
+    for (int i = 0; i < kSegmentRing; ++i) {
+      mbar_init(&sh.segment_full[i], 1);
+      mbar_init(&sh.segment_empty[i], kSegmentReaders);
+    }
+    sh.abort_code = 0;
+    sh.tiles_done = 0u;
+    sh.done = 0;
+    sh.finished = 0;
+    fence_barrier_init();
+  }
+  if (warp == 16) {
+    tmem_alloc(&sh.tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;                // S of slot s at columns 128 s (P over its first 64), O at 256 + 128 s
+  // 640 threads at 96 registers: 256 softmax threads at 160, 256 converting ones at 56 and 128 at 40 make 60416 of the 61440.
+  if (warp < kSoftmaxWarps) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
+    softmax_role<D>(a, sh, s_plan, smem, tmem, ctas);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+  } else if (warp < 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp < 12) convert_role<D, false>(a, sh, smem);
+    else convert_role<D, true>(a, sh, smem);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (lane == 0) {
+      if (warp == 16) mma_role<D>(sh, smem, tmem);
+      if (warp == 17) plan_role(a, plan, s_plan, sh, places, w1, total, ctas, wait_limit);
+    }
+    __syncwarp();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  // (Not before every role is done: an idle warp that took its registers back at once could take those that a softmax warp is
+  // still to get, and the two would wait for each other.)
+  if (warp >= kSoftmaxWarps) asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
+  if (sh.abort_code != 0) {
+    // A role gave up: MMAs may still be on their way, which otherwise the roles have waited for.
+    if (tid == 16 * 32) {
+      umma_commit(&sh.idle);
+      mbar_wait_landed(&sh.idle, 0);
+    }
+    __syncthreads();
+    // What is left of the piece becomes NaN, and its units are counted, so that nobody waits for them and the next call finds the
+    // counters at zero.
+    ChunkCursor at;
+    at.start(plan, s_plan, places);
+    bool unfinished = false;                  // (the last tile's time may run out when all that is left is to leave)
+    for (int segment = 0; at.left > 0; ++segment) {
+      const int n = at.tiles_here(), rows = at.rows(a.group);
+      const bool whole = n == at.span.tiles;
+      if (segment >= sh.finished) {
+        unfinished = true;
+        if (whole) {
+          for (int x = tid; x < rows * D; x += kChunkThreads) {
+            const int r = at.rt * kChunkRows + x / D;
+            a.out[(at.s.first + r / a.group) * a.out_stride + (at.head * a.group + r % a.group) * D + x % D] = __float2bfloat16(__int_as_float(0x7fffffff));
+          }
+        } else {
+          const Parts parts(total, ctas, w1 - at.left - at.tile, at.span.tiles);
+          const int slot_no = parts.slot(static_cast<int>(blockIdx.x));
+          for (int x = tid; x < rows; x += kChunkThreads)
+            reinterpret_cast<float4*>(a.partial + 2ll * ctas * kChunkRows * D)[static_cast<long long>(slot_no) * kChunkRows + x] =
+                make_float4(0.0f, __int_as_float(0x7fffffff), 0.0f, 0.0f);
+          __threadfence();
+          __syncthreads();
+          if (tid == 0) {
+            const bool is_last = atomicAdd(a.tickets + parts.first, 1) == parts.last - parts.first;
+            if (is_last) a.tickets[parts.first] = 0;
+            s_plan.last = is_last;
+          }
+          __syncthreads();
+          if (s_plan.last) {
+            __threadfence();
+            join_columns<D>(a, at.s.first, at.rt * kChunkRows, at.head, rows, ctas, parts, tid, kChunkThreads);
+          }
+          __syncthreads();
+        }
+      }
+      at.advance(plan, n);
+    }
+    if (tid == 0 && unfinished) atomicExch(status, sh.abort_code);
+  }
+  __syncthreads();
+  if (warp == 16) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace
+
+size_t kv4_chunk_partial_bytes(int head_dim, int ctas) { return 2ull * ctas * kChunkRows * (head_dim + 4) * sizeof(float); }
+
+cudaError_t kv4_chunk_set_attributes() {
+  const cudaError_t e = cudaFuncSetAttribute(kv4_chunk_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, ChunkShape<128>::kSmem);
+  return e != cudaSuccess ? e : cudaFuncSetAttribute(kv4_chunk_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, ChunkShape<64>::kSmem);
+}
+
+cudaError_t launch_kv4_chunk(const AttentionArgs& a, int head_dim, int ctas, int* status, long long wait_limit, cudaStream_t st) {
+  return head_dim == 128 ? launch_dependent(kv4_chunk_kernel<128>, dim3(ctas), dim3(kChunkThreads), ChunkShape<128>::kSmem, st, a, status, wait_limit)
+                         : launch_dependent(kv4_chunk_kernel<64>, dim3(ctas), dim3(kChunkThreads), ChunkShape<64>::kSmem, st, a, status, wait_limit);
+}
+
+}  // namespace syfi

@@ -17,7 +17,7 @@ import struct
 import torch
 
 from .kv import _call, _expect, _stream_of, _tokens_of, _window_of
-from .moe import load_library
+from .moe import _check, _stream_ptr, load_library
 
 PAGE, GROUP = 64, 16
 _vp, _i32, _i64, _f64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_double
@@ -30,6 +30,7 @@ ABI = {
     "syfi_kv4_write_block": (ctypes.c_int, [ctypes.c_char_p]),
     "syfi_kv4_read_block": (ctypes.c_int, [ctypes.c_char_p]),
     "syfi_kv4_attention_block": (ctypes.c_int, [ctypes.c_char_p]),
+    "syfi_kv4_check": (ctypes.c_int, [_vp]),
 }
 
 
@@ -262,4 +263,11 @@ def run_kv4_attention(q, kv4_cache, block_table, seq_lens, q_starts, out, *, sca
     return out
 
 
-__all__ = ["kv4_cache_shape", "run_kv4_attention", "run_kv4_read", "run_kv4_write"]
+def kv4_check(device=None, stream=None):
+    """Synchronise and raise :class:`MoeError` if an attention kernel gave up on a bounded wait."""
+    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    with torch.cuda.device(dev):
+        _check(_lib().syfi_kv4_check(_stream_ptr(stream, dev.index)))
+
+
+__all__ = ["kv4_cache_shape", "kv4_check", "run_kv4_attention", "run_kv4_read", "run_kv4_write"]

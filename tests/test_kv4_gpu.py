@@ -4,6 +4,7 @@ Tolerances follow from the number formats: a result in bf16 is off by half a uni
 scale by half an e4m3 step (2^-4 of it, 2^-10 near zero), a code by half the distance to its neighbour (a quarter up to 2, a half up to 4, 1
 up to 6, what lies above 6 by that), f32 arithmetic on a head's up to 128 dimensions by a few 1e-6 of the vector's largest; attention
 weights may be rounded to f16 (2^-11 of each), twice that is allowed, in units of the average of |value| under the weights."""
+import ctypes
 import importlib
 
 import pytest
@@ -554,6 +555,30 @@ def test_rows_that_tiny_values_decide(q_len, kv_len, octaves, D, pkg, kv4):
     q[:, ::2, 0] = 1.0
     _check_attention(_attend(pkg, inputs), *kv4.attention(*inputs))
     assert not _attend(pkg, inputs).isnan().any()
+
+
+@pytest.mark.parametrize("q_lens,kv_lens,D", [([300, 5], [3000, 9000], 128), ([6] * 9, [4000] * 9, 64)])
+def test_bounded_waits_run_out(q_lens, kv_lens, D, pkg, kv4):
+    """A wait that runs out ends its call with a status; rows that were not computed are NaN, all others are what they are, and
+    the next call is undisturbed."""
+    inputs = _attention_inputs(kv4, q_lens, kv_lens, 8, 2, D, seed=8)
+    clean = _attend(pkg, inputs)
+    lib = pkg.load_library()
+    failed = 0
+    for limit in (1, 1, 64, 200, 1000, 5000):
+        assert lib.syfi_kv4_debug_wait_limit(ctypes.c_int64(limit)) == 0
+        out = _attend(pkg, inputs)
+        try:
+            pkg.kv4_check()
+            assert torch.equal(out, clean)
+        except pkg.MoeError as err:
+            assert "status 401" in str(err), str(err)
+            failed += 1
+            done = ~out.isnan().any(-1)
+            assert torch.equal(out[done], clean[done]) and not bool(done.all())
+        assert torch.equal(_attend(pkg, inputs), clean), limit
+        pkg.kv4_check()
+    assert failed >= 1, failed
 
 
 @pytest.mark.parametrize("q_lens,kv_lens", [([1] * 5, [900, 20000, 3, 64, 7000]), ([400, 3], [5000, 6000])])
