@@ -3,17 +3,17 @@
 // A CTA (one per SM) walks its piece of the line of 128-position tiles.  A unit's up to 256 rows are two slots of 128, the M of an MMA:
 //   S = Q K^T   tcgen05.mma kind::f16.  Keys are code * group scale, which f16 holds exactly; a row of q, scaled by a power of two, too (down
 //               to 2^-29 of its largest).
-//   P           softmax warps, a thread per row.  With x in units of log2 and references m (of the sum l) and n (of O) that follow the
-//               row's largest terms, l = sum 2^(x - m) and P = 2^(x - n + 10) * vscale, rounded to f16, back into tensor memory over S.
+//   P           softmax warps, four rows to a lane.  With x in units of log2 and references m (of the sum l) and n (of O) that follow the
+//               row's largest terms, l = sum 2^(x - m) and P = 2^(x - n + 5) * vscale, rounded to f16, back into tensor memory over S.
 //   O += P V    kind::f16, P from tensor memory, values as code * group scale in shared memory, exact again.
-// Eight converting warps, a thread per position of keys or of values, keep a row's codes in registers while the stage in front is in use,
-// so nothing but f16 tiles lies in shared memory.  The slots are out of step by half a tile: while the softmax warps of one work, the tensor
+// Four converting warps, a thread per position, keep its key's and value's codes in registers while the stages in front are in use, so
+// nothing but f16 tiles lies in shared memory.  The slots are out of step by half a tile: while the softmax warps of one work, the tensor
 // core works for the other.  A unit of at most 128 rows takes turns: its even tiles are slot 0's, its odd ones slot 1's, and the sums are
 // added up at the end.
 //
-// n comes from a bound, the row's largest score of the tile times the tile's largest value scale.  That is near enough while the tile's
-// scales are within a factor of 8 (the largest P is then 2^7 at least, and what f16 drops 2^-32 of it at most); a tile whose scales are
-// further apart, or a row whose tile lies far below n, takes the products' own largest, as decoding does.
+// n comes from a bound, the row's largest score of the first tile times that tile's largest value scale.  That is near enough while the tile's
+// scales are within a factor of 4 (the largest P is then 2^3 at least, and what f16 drops 2^-28 of it at most); a tile whose scales are
+// further apart takes the products' own largest, as decoding does.
 #include "kv4_chunk.cuh"
 #include "stream_scratch.h"
 
@@ -23,7 +23,7 @@ namespace {
 
 constexpr int kTile = 128;             // positions per tile: two pages
 constexpr int kChunkRows = 256;
-constexpr int kChunkThreads = 640;     // 8 softmax warps, 4 for keys, 4 for values, then MMAs, planning, two idle ones
+constexpr int kChunkThreads = 512;     // 8 softmax warps, 4 converting ones, then MMAs, planning, two idle ones
 constexpr int kSoftmaxWarps = 8, kSoftmaxThreads = 256;
 constexpr int kChunkExtra = 4;         // what a unit costs besides its tiles, in tiles
 constexpr int kSlotRows = 128;         // units of at most so many rows use one slot for their even tiles and one for their odd ones
@@ -32,10 +32,13 @@ using ChunkCursor = Cursor<kTile, kChunkRows, kChunkExtra, kSlotRows>;
 constexpr int kScaleStages = 4;
 constexpr int kStatusTimeout = 401;
 
-constexpr float kProductHeadroom = 10.0f;   // P is kept times 2^10, ...
-constexpr float kProductGrowth = 4.0f;      // ... may grow by 2^4 before the reference follows, ...
-constexpr float kNear = 0.125f;             // ... and its bound is this near, or the products themselves are asked
-constexpr float kFarBelow = 70.0f;          // a tile whose bound lies so many octaves below n is summed up with its own reference
+// P is kept times 2^5 and may grow to 2^15 before the reference follows: a step of a row's reference stops its whole slot while O fades, and of
+// 256 rows one or another took such a step in every other tile when P might grow by 2^5 only (512 tokens behind 40000 positions, scores of
+// standard deviation 1.5: 618 us).
+constexpr float kProductHeadroom = 5.0f;
+constexpr float kProductGrowth = 9.0f;      // (where the reference is set from a bound that may be twice too low)
+constexpr float kNear = 0.25f;              // a tile's value scales are so near one another, or the products themselves are asked
+constexpr float kFarAbove = 60.0f;          // a row whose n lies so many octaves above m, because of a huge value, keeps its weights in units of m
 
 template <int D>
 struct ChunkShape {
@@ -61,23 +64,30 @@ struct Segment {
 };
 __device__ __forceinline__ Parts parts_of(const Segment& g) { return {g.first_part, g.last_part, g.first_slot}; }
 constexpr int kSegmentRing = 4;
-constexpr int kSegmentReaders = 1 + 8 + kSoftmaxWarps;    // arrivals that free an entry: MMAs, converting and softmax warps
+constexpr int kSegmentReaders = 1 + 4 + kSoftmaxWarps;    // arrivals that free an entry: MMAs, converting and softmax warps
 
 struct ChunkShared {
   Segment segment[kSegmentRing];
   uint64_t segment_full[kSegmentRing], segment_empty[kSegmentRing];
   uint64_t scale_full[kScaleStages], scale_empty[kScaleStages], k_full[4], k_empty[4], v_full[4], v_empty[4];
-  uint64_t q_full[2], s_full[2], p_half[2], p_full[2], o_full[2], o_empty[2], idle;
+  uint64_t q_full[2], s_full[2], p_half[2], half_done[2], p_full[2], o_full[2], o_empty[2], idle;
   uint32_t tmem;
   int there[kScaleStages][2];          // page p of the tile is there
   alignas(16) float largest[kScaleStages][4];    // value scales of 32 positions each that any row sees, ...
   alignas(16) float smallest[kScaleStages][4];   // ... read four at a time
   float end[2][3][128];                // [slot][m, l, n][row], at a segment's end
   float unit[256];                     // of each row: what a score is worth
+  int2 bounds[2][128];                 // [slot][row]: the positions that it sees, counted from the segment's first tile
   volatile int abort_code;
   volatile uint32_t tiles_done;
   volatile int done;                   // every segment is
   int finished;                        // segments of this CTA whose results are written
+};
+
+// The CTA's piece of the line.
+struct Piece {
+  long long total, w1;
+  int ctas, places;
 };
 
 // Waits ask only whether somebody gave up; the clock is the planning thread's, which has time.
@@ -118,11 +128,10 @@ struct Watch {
   }
 };
 
-__device__ __forceinline__ void plan_role(const AttentionArgs& a, const ChunkPlan& plan, const PlanShared& s_plan, ChunkShared& sh, int places,
-                                          long long w1, long long total, int ctas, long long wait_limit) {
+__device__ __forceinline__ void plan_role(const AttentionArgs& a, const ChunkPlan& plan, const PlanShared& s_plan, ChunkShared& sh, const Piece& piece, long long wait_limit) {
   Watch watch = {wait_limit, clock64(), 0u};
   ChunkCursor at;
-  at.start(plan, s_plan, places);
+  at.start(plan, s_plan, piece.places);
   Ring<kSegmentRing> ring;
   while (true) {
     while (!mbar_try_wait(&sh.segment_empty[ring.stage], ring.parity ^ 1u))
@@ -153,7 +162,7 @@ __device__ __forceinline__ void plan_role(const AttentionArgs& a, const ChunkPla
       g.all_low = a.window > 0 ? max(last - a.window + 1, 0) : 0;
       g.all_high = first;
       g.whole = here == at.span.tiles;
-      const Parts parts(total, ctas, w1 - at.left - at.tile, at.span.tiles);
+      const Parts parts(piece.total, piece.ctas, piece.w1 - at.left - at.tile, at.span.tiles);
       g.first_part = parts.first;
       g.last_part = parts.last;
       g.first_slot = parts.first_slot;
@@ -203,6 +212,7 @@ __device__ __forceinline__ void mma_role(ChunkShared& sh, uint8_t* smem, uint32_
     if (!wait_for(sh, &sh.p_half[s], parity)) return false;
     tc_fence_after();
     values(s, stage, 0, add);
+    umma_commit(&sh.half_done[s]);
     if (!wait_for(sh, &sh.p_full[s], parity)) return false;
     tc_fence_after();
     values(s, stage, 1, 1u);
@@ -274,30 +284,63 @@ __device__ __forceinline__ void mma_role(ChunkShared& sh, uint8_t* smem, uint32_
   }
 }
 
-// ---------------------------------------------------------------- codes to f16, a thread per position (four warps for keys, four for values)
+// ---------------------------------------------------------------- codes to f16, a thread per position (four warps)
+// 32 bytes that are read once
+__device__ __forceinline__ void ld_global_32(const void* p, uint4& a, uint4& b) {
+  asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w) : "l"(p));
+}
 // A row of codes and its scales on their way from the cache.
 template <int D>
 struct RawRow {
   uint4 codes[D / 32];
   uint32_t groups[D / 64];
-  float k_scale, v_scale;              // (values' threads only)
+  float scale;
+  __device__ __forceinline__ void ask(const uint8_t* block, int at) {
+#pragma unroll
+    for (int p = 0; p < D / 64; ++p) ld_global_32(block + p * kKv4Plane + at * 32, codes[2 * p], codes[2 * p + 1]);
+    const uint32_t* const from = reinterpret_cast<const uint32_t*>(block + Kv4Block<D>::kGroups + at * (D / kKv4Group));
+    if constexpr (D == 128) {
+      const uint2 g = __ldg(reinterpret_cast<const uint2*>(from));
+      groups[0] = g.x;
+      groups[1] = g.y;
+    } else {
+      groups[0] = __ldg(from);
+    }
+    scale = __ldg(reinterpret_cast<const float*>(block + Kv4Block<D>::kScales) + at);
+  }
+  // code * group scale as f16 into row t of a tile (`to`: the row in its first 64 dimensions)
+  __device__ __forceinline__ void put(uint8_t* to, int t) const {
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      const uint32_t w[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
+      // two groups of 16 dimensions, 8 in a word
+      const uint32_t both = e4m3x2_to_half2(groups[i / 2] >> (16 * (i % 2)));
+      const uint32_t scale[2] = {__byte_perm(both, both, 0x1010), __byte_perm(both, both, 0x3232)};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int chunk = i % 2 * 4 + k;
+        *reinterpret_cast<uint4*>(to + i / 2 * (kTile * 128) + ((chunk ^ (t & 7)) << 4)) =
+            make_uint4(hmul2_bits(e2m1x2_to_half2<0>(w[k]), scale[k / 2]), hmul2_bits(e2m1x2_to_half2<1>(w[k]), scale[k / 2]),
+                       hmul2_bits(e2m1x2_to_half2<2>(w[k]), scale[k / 2]), hmul2_bits(e2m1x2_to_half2<3>(w[k]), scale[k / 2]));
+      }
+    }
+  }
 };
 
-template <int D, bool VALUES>
+template <int D>
 __device__ __forceinline__ void convert_role(const AttentionArgs& a, ChunkShared& sh, uint8_t* smem) {
   using Shape = ChunkShape<D>;
   constexpr int kStages = Shape::kStages;
   const int t = threadIdx.x % 128, lane = threadIdx.x % 32, warp = t / 32, page_of = t / kKvPage, at = t % kKvPage;
-  uint64_t* const full = VALUES ? sh.v_full : sh.k_full;
-  uint64_t* const empty = VALUES ? sh.v_empty : sh.k_empty;
   Ring<kSegmentRing> segments;           // of the tile to ask for
   Ring<kScaleStages> scales;
   Ring<kStages> tiles;
-  // The walk of the loads: a tile's row is asked for when the tile in front is converted, its table entry one tile earlier.
+  // The walk of the loads: a tile's rows are asked for when the tile in front is converted, its table entry one tile earlier.
   int next_tile = 0, left = 0, any_low = 0, any_high = 0, all_low = 0, all_high = 0, head = 0;
   const int32_t* table = nullptr;
-  int entry = -1, position = 0;          // of the tile to ask for
-  int entry_low = 0, entry_high = 0, entry_all_low = 0, entry_all_high = 0, entry_head = 0;
+  int entry = -1, entry_head = 0;        // of the tile to ask for
+  bool entry_seen = false, entry_plain = false;
   auto next_entry = [&]() -> bool {      // whole warp; false behind the last tile
     if (left == 0) {
       wait_whole_warp(sh, &sh.segment_full[segments.stage], segments.parity);
@@ -316,263 +359,335 @@ __device__ __forceinline__ void convert_role(const AttentionArgs& a, ChunkShared
       if (lane == 0) mbar_arrive(&sh.segment_empty[segments.stage]);
       segments.next();
     }
-    const int page = 2 * next_tile + page_of;
-    position = next_tile * kTile + t;
+    const int page = 2 * next_tile + page_of, first = next_tile * kTile;
     entry = page < a.batch.max_pages && page * kKvPage <= any_high && (page + 1) * kKvPage > any_low ? __ldg(table + page) : -1;
-    entry_low = any_low;
-    entry_high = any_high;
-    entry_all_low = all_low;
-    entry_all_high = all_high;
     entry_head = head;
+    entry_seen = first + t >= any_low && first + t <= any_high;
+    entry_plain = first >= all_low && first + kTile - 1 <= all_high;
     ++next_tile;
     --left;
     return true;
   };
-  RawRow<D> row;
-  bool there = false, plain = false, seen = false;     // of the row in registers
+  RawRow<D> key, value;
+  bool there = false, plain = false, seen = false;     // of the rows in registers
   auto ask = [&]() {
     there = entry >= 0 && entry < a.cache.num_pages;
-    seen = position >= entry_low && position <= entry_high;
-    const int first = position - t;
-    plain = first >= entry_all_low && first + kTile - 1 <= entry_all_high;
+    seen = entry_seen;
+    plain = entry_plain;
     if (there) {
-      const uint8_t* const keys = kv4_block<D>(a.cache, entry, 0, entry_head);
-      const uint8_t* const block = VALUES ? keys + static_cast<long long>(a.cache.heads) * Kv4Block<D>::kBytes : keys;
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) row.codes[i] = __ldg(reinterpret_cast<const uint4*>(block + i / 2 * kKv4Plane + at * 32) + i % 2);
-      const uint32_t* const groups = reinterpret_cast<const uint32_t*>(block + Kv4Block<D>::kGroups + at * (D / kKv4Group));
-      if constexpr (D == 128) {
-        const uint2 g = __ldg(reinterpret_cast<const uint2*>(groups));
-        row.groups[0] = g.x;
-        row.groups[1] = g.y;
-      } else {
-        row.groups[0] = __ldg(groups);
-      }
-      if constexpr (VALUES) {
-        row.k_scale = __ldg(reinterpret_cast<const float*>(keys + Kv4Block<D>::kScales) + at);
-        row.v_scale = __ldg(reinterpret_cast<const float*>(block + Kv4Block<D>::kScales) + at);
-      }
+      const uint8_t* const block = kv4_block<D>(a.cache, entry, 0, entry_head);
+      key.ask(block, at);
+      value.ask(block + static_cast<long long>(a.cache.heads) * Kv4Block<D>::kBytes, at);
     }
   };
   bool more = next_entry();
   if (more) ask();
   while (more) {
     more = next_entry();                 // (of the tile behind the one in registers)
-    bool valid = there;
-    if constexpr (VALUES) {
-      // What a row does not see must not reach its sums, and zero times NaN is NaN: values of positions that no row sees become zeros, and
-      // where some rows see a value that is not finite, the NaN goes by way of its score to those rows alone.
-      float ks = there ? row.k_scale : 0.0f, vs = there ? row.v_scale : 1.0f;
-      bool bad = !(fabsf(vs) <= 3.402823466e38f);
-#pragma unroll
-      for (int i = 0; i < D / 64; ++i) bad |= there && (((row.groups[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0u;
-      valid = there && seen && (plain || !bad);
-      if (bad || !(fabsf(ks) <= 3.402823466e38f)) ks = __int_as_float(0x7fffffff);
-      if (!valid) vs = 1.0f;
-      const unsigned bits = __float_as_uint(vs);
-      const bool counts = valid && bits < 0x7f800000u;
-      const unsigned high = __reduce_max_sync(0xffffffffu, counts ? bits : 0u), low = __reduce_min_sync(0xffffffffu, counts ? bits : 0x7f800000u);
-      wait_whole_warp(sh, &sh.scale_empty[scales.stage], scales.parity ^ 1u);
-      __syncwarp();
-      float* const to = reinterpret_cast<float*>(smem + Shape::kScales) + scales.stage * 2 * kTile;
-      to[t] = ks;
-      to[kTile + t] = vs;
-      if (lane == 0) {
-        sh.largest[scales.stage][warp] = __uint_as_float(high);
-        sh.smallest[scales.stage][warp] = __uint_as_float(low);
-        if (warp % 2 == 0) sh.there[scales.stage][page_of] = there;
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.scale_full[scales.stage]);
-      scales.next();
-    }
-    wait_whole_warp(sh, &empty[tiles.stage], tiles.parity ^ 1u);
+    wait_whole_warp(sh, &sh.k_empty[tiles.stage], tiles.parity ^ 1u);
     __syncwarp();
-    uint8_t* const to = smem + (VALUES ? Shape::kV : Shape::kK) + tiles.stage * Shape::kTileBytes + t * 128;
+    if (there) key.put(smem + Shape::kK + tiles.stage * Shape::kTileBytes + t * 128, t);
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.k_full[tiles.stage]);
+    // What a row does not see must not reach its sums, and zero times NaN is NaN: values of positions that no row sees become zeros, and
+    // where some rows see a value that is not finite, the NaN goes by way of its score to those rows alone.
+    float ks = there ? key.scale : 0.0f, vs = there ? value.scale : 1.0f;
+    bool bad = !(fabsf(vs) <= 3.402823466e38f);
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) bad |= there && (((value.groups[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0u;
+    const bool valid = there && seen && (plain || !bad);
+    if (bad || !(fabsf(ks) <= 3.402823466e38f)) ks = __int_as_float(0x7fffffff);
+    if (!valid) vs = 1.0f;
+    const unsigned bits = __float_as_uint(vs);
+    const bool counts = valid && bits < 0x7f800000u;
+    const unsigned high = __reduce_max_sync(0xffffffffu, counts ? bits : 0u), low = __reduce_min_sync(0xffffffffu, counts ? bits : 0x7f800000u);
+    wait_whole_warp(sh, &sh.scale_empty[scales.stage], scales.parity ^ 1u);
+    __syncwarp();
+    float* const to = reinterpret_cast<float*>(smem + Shape::kScales) + scales.stage * 2 * kTile;
+    to[t] = ks;
+    to[kTile + t] = vs;
+    if (lane == 0) {
+      sh.largest[scales.stage][warp] = __uint_as_float(high);
+      sh.smallest[scales.stage][warp] = __uint_as_float(low);
+      if (warp % 2 == 0) sh.there[scales.stage][page_of] = there;
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.scale_full[scales.stage]);
+    scales.next();
+    wait_whole_warp(sh, &sh.v_empty[tiles.stage], tiles.parity ^ 1u);
+    __syncwarp();
+    uint8_t* const row = smem + Shape::kV + tiles.stage * Shape::kTileBytes + t * 128;
     if (valid) {
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        const uint32_t w[4] = {row.codes[i].x, row.codes[i].y, row.codes[i].z, row.codes[i].w};
-        // two groups of 16 dimensions, 8 in a word
-        const uint32_t both = e4m3x2_to_half2(row.groups[i / 2] >> (16 * (i % 2)));
-        const uint32_t scale[2] = {__byte_perm(both, both, 0x1010), __byte_perm(both, both, 0x3232)};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int chunk = i % 2 * 4 + k;
-          *reinterpret_cast<uint4*>(to + i / 2 * (kTile * 128) + ((chunk ^ (t & 7)) << 4)) =
-              make_uint4(hmul2_bits(e2m1x2_to_half2<0>(w[k]), scale[k / 2]), hmul2_bits(e2m1x2_to_half2<1>(w[k]), scale[k / 2]),
-                         hmul2_bits(e2m1x2_to_half2<2>(w[k]), scale[k / 2]), hmul2_bits(e2m1x2_to_half2<3>(w[k]), scale[k / 2]));
-        }
-      }
-    } else if (VALUES) {
+      value.put(row, t);
+    } else {
 #pragma unroll 1
-      for (int chunk = 0; chunk < D / 8; ++chunk) *reinterpret_cast<uint4*>(to + chunk / 8 * (kTile * 128) + chunk % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
+      for (int chunk = 0; chunk < D / 8; ++chunk) *reinterpret_cast<uint4*>(row + chunk / 8 * (kTile * 128) + chunk % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
     }
     fence_proxy_async_smem();
     __syncwarp();
-    if (lane == 0) mbar_arrive(&full[tiles.stage]);
+    if (lane == 0) mbar_arrive(&sh.v_full[tiles.stage]);
     tiles.next();
     if (more) ask();
     if (__any_sync(0xffffffffu, sh.abort_code != 0)) return;
   }
 }
 
-// ---------------------------------------------------------------- softmax, a thread per row (eight warps, four to a slot)
-__device__ __forceinline__ ulonglong2 ld_shared_pairs(uint32_t at) {
-  ulonglong2 v;
-  asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(v.x), "=l"(v.y) : "r"(at) : "memory");
+// ---------------------------------------------------------------- softmax (eight warps, four to a slot, 32 rows each)
+// A lane has four rows, 8 i + lane / 4, and of every eight positions two, 2 (lane % 4) and the next: the accumulator's layout of an m16n8 MMA,
+// which tensor memory's 16x256b loads give.  So a scale that is read serves four rows; with a row to a lane, the scales' 64 reads of 16 bytes a
+// tile and warp alone took the shared memory's port for 2000 clocks of a tile.
+__device__ __forceinline__ uint64_t ld_shared_pair(uint32_t at) {
+  uint64_t v;
+  asm volatile("ld.shared.u64 %0, [%1];" : "=l"(v) : "r"(at));
   return v;
 }
 
-// A tile's row: 128 scores from tensor memory, their weights back into it; the row's references m and n and its sum l.  unit: what a score
-// is worth.  low, high: what the row sees, counted from the tile's first position; there0, there1: the tile's pages.
-template <int D>
-__device__ __forceinline__ void softmax_tile(ChunkShared& sh, int slot, int stage, uint32_t t_s, uint32_t t_o, uint32_t scales, bool masked, int low, int high,
-                                             float unit, bool first, float& m, float& n, float& l) {
-  uint32_t s[4][32];
-#pragma unroll
-  for (int c = 0; c < 4; ++c) tmem_ld32(t_s + 32 * c, s[c]);
+// What the softmax of a tile works with.
+struct TileRows {
+  uint32_t t_s, t_o;                   // tensor memory: scores (weights over their first half), sums
+  uint32_t scales;                     // shared memory: this lane's first of 128 scales of keys, then of values
+  uint32_t bounds;                     // shared memory: lowest and highest position that this lane's first row sees, eight rows on the next
+  int offset;                          // of the tile in those
+  bool masked, there0, there1;         // whether any of that matters for the warp's rows; the tile's pages
+  float unit[4];                       // what a score is worth
+};
+__device__ __forceinline__ int2 row_bounds(const TileRows& r, int row) {
+  const uint64_t v = ld_shared_pair(r.bounds + row * 64);
+  return make_int2(static_cast<int>(v) - r.offset, static_cast<int>(v >> 32) - r.offset);
+}
+__device__ __forceinline__ float quad_max(float x) {
+  x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+  return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+}
+
+// 64 scores of this lane's four rows, from position 64 h of the tile on
+__device__ __forceinline__ void load_scores(const TileRows& r, int h, uint32_t (&s)[2][32]) {
+  tmem_ld_16x256b(r.t_s + 64 * h, s[0]);
+  tmem_ld_16x256b(r.t_s + 64 * h + (16u << 16), s[1]);
+}
+__device__ __forceinline__ void scores_landed(uint32_t (&s)[2][32]) {
   tmem_ld_wait_for(s[0]);
+  tmem_landed(s[1]);
+}
+
+// O of the warp's rows times `fade`.
+template <int D>
+__device__ __forceinline__ void rescale_sums(uint32_t t_o, const float (&fade)[4]) {
+#pragma unroll 1
+  for (int k = 0; k < 2 * (D / 64); ++k) {
+    const uint32_t at = t_o + (k & 1 ? 16u << 16 : 0u) + k / 2 * 64;
+    uint32_t o[32];
+    tmem_ld_16x256b(at, o);
+    tmem_ld_wait_for(o);
 #pragma unroll
-  for (int c = 1; c < 4; ++c) tmem_landed(s[c]);
-  // times the keys' scales: in units of the row's
+    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * (k & 1 ? fade[2 + e / 2 % 2] : fade[e / 2 % 2]));
+    tmem_st_16x256b(at, o);
+  }
+  tmem_st_wait();
+}
+
+// The rows' largest scores of 64 positions, times the keys' scales and in units of the rows'.
+__device__ __forceinline__ void largest_scores(const TileRows& r, int h, const uint32_t (&s)[2][32], float (&top)[4]) {
+  const int column = 64 * h + threadIdx.x % 4 * 2;
+  const bool there = h == 0 ? r.there0 : r.there1;
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
+  for (int row = 0; row < 4; ++row) {
+    const int2 see = row_bounds(r, row);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const ulonglong2 ks = ld_shared_pairs(scales + 4 * (32 * c + 4 * e));
-      float x0, x1, x2, x3;
-      f32x2_unpack(f32x2_mul(f32x2_pack_bits(s[c][4 * e], s[c][4 * e + 1]), ks.x), x0, x1);
-      f32x2_unpack(f32x2_mul(f32x2_pack_bits(s[c][4 * e + 2], s[c][4 * e + 3]), ks.y), x2, x3);
-      s[c][4 * e] = __float_as_uint(x0);
-      s[c][4 * e + 1] = __float_as_uint(x1);
-      s[c][4 * e + 2] = __float_as_uint(x2);
-      s[c][4 * e + 3] = __float_as_uint(x3);
+    for (int i = 0; i < 8; ++i) {
+      float x0, x1;
+      f32x2_unpack(f32x2_mul(f32x2_pack_bits(s[row / 2][4 * i + 2 * (row % 2)], s[row / 2][4 * i + 2 * (row % 2) + 1]), ld_shared_pair(r.scales + 4 * (64 * h + 8 * i))), x0, x1);
+      const int at = column + 8 * i;
+      if (there && at >= see.x && at <= see.y) top[row] = fmaxf(top[row], x0);
+      if (there && at + 1 >= see.x && at + 1 <= see.y) top[row] = fmaxf(top[row], x1);
     }
   }
-  if (__builtin_expect(masked, 0)) {
-    const bool there[2] = {sh.there[stage][0] != 0, sh.there[stage][1] != 0};
+}
+
+// Weights of 64 positions, times the values' scales, as pairs of f16, their sums, and in `top` the largest.  GENERAL: positions that a row does
+// not see, and products times `factor`.
+template <bool GENERAL>
+__device__ __forceinline__ void half_weights(const TileRows& r, int h, const uint32_t (&s)[2][32], const float (&shift)[4], const float (&factor)[4], float (&total)[4],
+                                             float (&top)[4], uint32_t (&p)[2][16]) {
+  uint64_t sums[4];
+  int2 see[4];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int first_bit = low - 32 * c, last_bit = high - 32 * c;
-      uint32_t bits = last_bit < 0 || first_bit > 31 || !there[c / 2] ? 0u : 0xffffffffu;
-      if (last_bit >= 0 && last_bit < 31) bits &= (2u << last_bit) - 1u;
-      if (first_bit > 0 && first_bit <= 31) bits &= 0xffffffffu << first_bit;
-#pragma unroll
-      for (int b = 0; b < 32; ++b)
-        if (!(bits >> b & 1u)) s[c][b] = 0xff800000u;
+  for (int row = 0; row < 4; ++row) {
+    sums[row] = 0ull;
+    top[row] = 0.0f;
+    see[row] = make_int2(0, 0);
+    if (GENERAL) {
+      see[row] = row_bounds(r, row);
+      if (!(h == 0 ? r.there0 : r.there1)) see[row].y = -1;
     }
   }
-  float tops[4];
+  const int column = 64 * h + threadIdx.x % 4 * 2;
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    tops[c] = fmaxf(__uint_as_float(s[c][0]), __uint_as_float(s[c][1]));
+  for (int i = 0; i < 8; ++i) {
+    const uint64_t ks = ld_shared_pair(r.scales + 4 * (64 * h + 8 * i)), vs = ld_shared_pair(r.scales + 4 * (kTile + 64 * h + 8 * i));
 #pragma unroll
-    for (int b = 2; b < 32; b += 2) tops[c] = fmaxf(tops[c], fmaxf(__uint_as_float(s[c][b]), __uint_as_float(s[c][b + 1])));
+    for (int row = 0; row < 4; ++row) {
+      const uint64_t x = f32x2_mul(f32x2_pack_bits(s[row / 2][4 * i + 2 * (row % 2)], s[row / 2][4 * i + 2 * (row % 2) + 1]), ks);
+      float x0, x1;
+      f32x2_unpack(f32x2_fma(x, f32x2_pack(r.unit[row], r.unit[row]), f32x2_pack(shift[row], shift[row])), x0, x1);
+      x0 = ex2(x0);
+      x1 = ex2(x1);
+      if (GENERAL) {
+        const int at = column + 8 * i;
+        x0 = at >= see[row].x && at <= see[row].y ? x0 : 0.0f;
+        x1 = at + 1 >= see[row].x && at + 1 <= see[row].y ? x1 : 0.0f;
+      }
+      uint64_t w = f32x2_pack(x0, x1);
+      sums[row] = f32x2_add(sums[row], w);
+      w = f32x2_mul(w, vs);
+      if (GENERAL) w = f32x2_mul(w, f32x2_pack(factor[row], factor[row]));
+      f32x2_unpack(w, x0, x1);
+      top[row] = fmaxf(top[row], fmaxf(x0, x1));
+      p[row / 2][2 * i + row % 2] = pack_half2(x0, x1);
+    }
   }
-  const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * unit;
-  const float4 v_high = *reinterpret_cast<const float4*>(sh.largest[stage]), v_low = *reinterpret_cast<const float4*>(sh.smallest[stage]);
-  const float largest = fmaxf(fmaxf(v_high.x, v_high.y), fmaxf(v_high.z, v_high.w)), smallest = fminf(fminf(v_low.x, v_low.y), fminf(v_low.z, v_low.w));
-  if (top > m + kSumGrowth) {
-    l *= ex2(m - top);                 // (0 for a row that had seen nothing)
-    m = top;
+#pragma unroll
+  for (int row = 0; row < 4; ++row) {
+    float a0, a1;
+    f32x2_unpack(sums[row], a0, a1);
+    total[row] = a0 + a1;
   }
-  float bound = top + lg2(largest);
-  const bool near = smallest >= kNear * largest && largest >= 1e-18f && largest <= 1e18f;     // (no scale of zero among them)
-  const uint64_t unit2 = f32x2_pack(unit, unit);
-  const bool slow = !near || __any_sync(0xffffffffu, bound < n - kFarBelow && top != -INFINITY);      // (not for a row that is not finite)
-  const uint32_t v_scales = scales + kTile * 4;
-  if (__builtin_expect(slow, 0)) {
-    // the products themselves: weights in units of m, then times the values' scales
-    const float shift = -finite_or_zero(m);
-    float sum = 0.0f, most = 0.0f;
+}
+
+// References for a tile from its scores themselves: m, with l in its units, and n from the bound, or with `products` from the products' own
+// largest.  fade: what O becomes smaller by.
+__device__ __forceinline__ void set_references(const TileRows& r, float largest, bool products, float (&m)[4], float (&n)[4], float (&l)[4], float (&fade)[4]) {
+  float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, bound[4];
+#pragma unroll 1
+  for (int h = 0; h < 2; ++h) {
+    uint32_t s[2][32];
+    load_scores(r, h, s);
+    scores_landed(s);
+    largest_scores(r, h, s, top);
+  }
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
+  for (int row = 0; row < 4; ++row) {
+    top[row] = quad_max(top[row]) * r.unit[row];
+    if (top[row] > m[row]) {
+      l[row] *= ex2(m[row] - top[row]);        // (0 for a row that had seen nothing)
+      m[row] = top[row];
+    }
+    bound[row] = top[row] + lg2(largest);
+  }
+  if (products) {
+    float most[4] = {}, one[4], shift[4], total[4];
 #pragma unroll
-      for (int e = 0; e < 32; e += 4) {
-        const ulonglong2 vs = ld_shared_pairs(v_scales + 4 * (32 * c + e));
-        float v[4];
-        f32x2_unpack(vs.x, v[0], v[1]);
-        f32x2_unpack(vs.y, v[2], v[3]);
+    for (int row = 0; row < 4; ++row) {
+      one[row] = 1.0f;
+      shift[row] = -finite_or_zero(m[row]);
+    }
+#pragma unroll 1
+    for (int h = 0; h < 2; ++h) {
+      uint32_t s[2][32], p[2][16];
+      load_scores(r, h, s);
+      scores_landed(s);
+      half_weights<true>(r, h, s, shift, one, total, top, p);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float p = ex2(fmaf(__uint_as_float(s[c][e + k]), unit, shift));
-          sum += p;
-          const float y = p * v[k];
-          most = fmaxf(most, y);
-          s[c][e + k] = __float_as_uint(y);
+      for (int row = 0; row < 4; ++row) most[row] = fmaxf(most[row], top[row]);
+    }
+#pragma unroll
+    for (int row = 0; row < 4; ++row) bound[row] = m[row] + fmaxf(lg2(quad_max(most[row])), -90.0f);      // (never further behind: a value may be zero)
+  }
+#pragma unroll
+  for (int row = 0; row < 4; ++row) {
+    fade[row] = 1.0f;
+    if (bound[row] > n[row] + kProductGrowth) {
+      fade[row] = ex2(n[row] - bound[row]);
+      n[row] = bound[row];
+    }
+  }
+}
+
+// The weights of a tile, half of it at a time: into tensor memory over scores that are used up.  A reference n stays what it is unless a weight
+// does not fit, which hardly ever happens; then the row's O fades, and the half is done again.  GENERAL: rows that do not see every position, and
+// `careful`: weights in units of m first, for tiles whose value scales are far apart.
+template <int D, bool GENERAL>
+__device__ __forceinline__ void tile_weights(ChunkShared& sh, const TileRows& r, int slot, uint32_t tile_parity, bool first, bool careful, float largest, float (&m)[4],
+                                             float (&n)[4], float (&l)[4]) {
+  const int lane = threadIdx.x % 32;
+  float shift[4], factor[4];
+#pragma unroll
+  for (int row = 0; row < 4; ++row) {
+    shift[row] = GENERAL && careful ? -finite_or_zero(m[row]) : kProductHeadroom - finite_or_zero(n[row]);
+    factor[row] = !(GENERAL && careful) ? 1.0f : m[row] != -INFINITY && n[row] != -INFINITY ? ex2(m[row] - n[row] + kProductHeadroom) : 0.0f;
+  }
+  uint32_t s[2][32];
+  load_scores(r, 0, s);
+#pragma unroll 1
+  for (int h = 0; h < 2; ++h) {
+    uint32_t p[2][16];
+    float total[4], top[4];
+    for (bool again = false;; again = true) {
+      scores_landed(s);
+      half_weights<GENERAL>(r, h, s, shift, factor, total, top, p);
+      if (__builtin_expect(!__any_sync(0xffffffffu, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > 32768.0f), 1) || again) break;
+      load_scores(r, h, s);
+      scores_landed(s);
+      float highest[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, fade[4];
+      largest_scores(r, h, s, highest);
+#pragma unroll
+      for (int row = 0; row < 4; ++row) {
+        // (from the scores where a weight is beyond f32, too)
+        const float most = quad_max(top[row]), bound = fmaf(quad_max(highest[row]), r.unit[row], shift[row]) + lg2(largest);
+        const float up = most > 32768.0f ? (most <= 3.402823466e38f ? lg2(most) : bound) - kProductHeadroom : 0.0f;
+        fade[row] = ex2(-up);
+        n[row] += up;
+        if (GENERAL && careful) {
+          factor[row] *= fade[row];
+        } else {
+          shift[row] -= up;
+          m[row] += up;                // (the sum's reference goes along, so that the two stay near)
+          l[row] *= fade[row];
         }
       }
+      if (h == 1) {                    // the first half's product is on its way
+        wait_whole_warp(sh, &sh.half_done[slot], tile_parity);
+        __syncwarp();
+        tc_fence_after();
+      }
+      if (!first || h == 1) rescale_sums<D>(r.t_o, fade);
+      load_scores(r, h, s);
     }
-    l += sum;
-    bound = m + fmaxf(lg2(most), -90.0f);      // (never further behind: a value may be zero)
-  }
-  float fade = 1.0f;
-  if (bound > n + kProductGrowth) {
-    fade = ex2(n - bound);
-    n = bound;
-  }
-  if (!first && __any_sync(0xffffffffu, fade != 1.0f)) {
-#pragma unroll 1
-    for (int c = 0; c < D; c += 8) {
-      uint32_t o[8];
-      tmem_ld8(t_o + c, o);
-      tmem_ld_wait_for(o);
 #pragma unroll
-      for (int b = 0; b < 8; ++b) o[b] = __float_as_uint(__uint_as_float(o[b]) * fade);
-      tmem_st8(t_o + c, o);
-    }
-  }
-  const int lane = threadIdx.x % 32;
-  if (__builtin_expect(slow, 0)) {
-    const float f = m == -INFINITY || n == -INFINITY ? 0.0f : ex2(m - n + kProductHeadroom);
-#pragma unroll
-    for (int h = 0; h < 8; ++h) {
-      uint32_t p[8];
-#pragma unroll
-      for (int b = 0; b < 8; ++b) p[b] = pack_half2(__uint_as_float(s[h / 2][16 * (h % 2) + 2 * b]) * f, __uint_as_float(s[h / 2][16 * (h % 2) + 2 * b + 1]) * f);
-      tmem_st8(t_s + 8 * h, p);
-    }
+    for (int row = 0; row < 4; ++row) l[row] += GENERAL && careful ? total[row] : total[row] * ex2(-shift[row] - finite_or_zero(m[row]));
+    if (h == 0) load_scores(r, 1, s);
+    tmem_st_16x128b(r.t_s + 32 * h, p[0]);
+    tmem_st_16x128b(r.t_s + 32 * h + (16u << 16), p[1]);
     tmem_st_wait();
     tc_fence_before();
     __syncwarp();
-    if (lane == 0) {
-      mbar_arrive(&sh.p_half[slot]);
-      mbar_arrive(&sh.p_full[slot]);
-    }
-    return;
+    if (lane == 0) mbar_arrive(h == 0 ? &sh.p_half[slot] : &sh.p_full[slot]);
   }
-  const float shift = kProductHeadroom - finite_or_zero(n);
-  const uint64_t shift2 = f32x2_pack(shift, shift);
-  uint64_t sums[2] = {0ull, 0ull};
+}
+
+// A tile of the warp's rows: scores from tensor memory, weights back into it; the rows' references m and n and this lane's part of their sums l.
+template <int D>
+__device__ __forceinline__ void softmax_tile(ChunkShared& sh, const TileRows& r, int slot, int stage, uint32_t tile_parity, bool first, float (&m)[4], float (&n)[4],
+                                             float (&l)[4]) {
+  const float4 v_high = *reinterpret_cast<const float4*>(sh.largest[stage]), v_low = *reinterpret_cast<const float4*>(sh.smallest[stage]);
+  const float largest = fmaxf(fmaxf(v_high.x, v_high.y), fmaxf(v_high.z, v_high.w)), smallest = fminf(fminf(v_low.x, v_low.y), fminf(v_low.z, v_low.w));
+  // (no scale of zero among them; the weights' sum, in units of n, is in f32's range)
+  const bool near = smallest >= kNear * largest && largest >= 1e-18f && largest <= 1e18f;
+  bool far = false, blind = false;             // (neither for a row that is not finite)
 #pragma unroll
-  for (int h = 0; h < 8; ++h) {
-    uint32_t p[8];
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const int at = 16 * (h % 2) + 4 * b;
-      const ulonglong2 vs = ld_shared_pairs(v_scales + 4 * (16 * h + 4 * b));
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        float x0, x1;
-        f32x2_unpack(f32x2_fma(f32x2_pack_bits(s[h / 2][at + 2 * k], s[h / 2][at + 2 * k + 1]), unit2, shift2), x0, x1);
-        const uint64_t w = f32x2_pack(ex2(x0), ex2(x1));
-        sums[k] = f32x2_add(sums[k], w);
-        f32x2_unpack(f32x2_mul(w, k ? vs.y : vs.x), x0, x1);
-        p[2 * b + k] = pack_half2(x0, x1);
-      }
-    }
-    tmem_st8(t_s + 8 * h, p);
-    if (h % 4 == 3) {
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(h == 3 ? &sh.p_half[slot] : &sh.p_full[slot]);
-    }
+  for (int row = 0; row < 4; ++row) {
+    far |= n[row] - m[row] > kFarAbove;
+    blind |= n[row] == -INFINITY && l[row] == l[row];
   }
-  float a0, a1;
-  f32x2_unpack(f32x2_add(sums[0], sums[1]), a0, a1);
-  l += (a0 + a1) * ex2(-shift - finite_or_zero(m));
+  const bool careful = !near || __any_sync(0xffffffffu, far);
+  if (careful || first || __any_sync(0xffffffffu, blind)) {
+    float fade[4];
+    set_references(r, largest, careful, m, n, l, fade);
+    if (!first && __any_sync(0xffffffffu, fade[0] != 1.0f || fade[1] != 1.0f || fade[2] != 1.0f || fade[3] != 1.0f)) rescale_sums<D>(r.t_o, fade);
+  }
+  if (__builtin_expect(careful || r.masked, 0)) tile_weights<D, true>(sh, r, slot, tile_parity, first, careful, largest, m, n, l);
+  else tile_weights<D, false>(sh, r, slot, tile_parity, first, false, largest, m, n, l);
 }
 
 // The warp's 32 rows of q (of which `rows` are there; mine: where this lane's row begins in q) as f16 times 2^k each, the row's largest at
@@ -675,7 +790,7 @@ __device__ __forceinline__ void join_columns(const AttentionArgs& a, int q_first
 }
 
 template <int D>
-__device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared& sh, PlanShared& s_plan, uint8_t* smem, uint32_t tmem, int ctas) {
+__device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared& sh, PlanShared& s_plan, uint8_t* smem, uint32_t tmem, const Piece& piece) {
   using Shape = ChunkShape<D>;
   // warps 0-3: slot 0, 4-7: slot 1
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, slot = warp / 4, in_slot = warp % 4 * 32 + lane;
@@ -697,7 +812,7 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
     unsigned turn = turns ? 2u + slot : g.rows <= slot * kSlotRows;
     const bool active = turn != 1u;
     const int row = (turns ? 0 : slot * kSlotRows) + in_slot;
-    float m = -INFINITY, n = -INFINITY, l = 0.0f;
+    float m = -INFINITY, n = -INFINITY, l = 0.0f;    // of this thread's row, at the segment's end
     int token_of_row = 0, column_of_row = 0;         // of this thread's row, in q and out
     {
       int low, high;
@@ -717,11 +832,25 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
       }
       __syncwarp();
       if (active && lane == 0) mbar_arrive(&sh.q_full[slot]);
-      if (turns) named_bar_sync(1, kSoftmaxThreads);       // slot 1 reads slot 0's units
-      const float unit = sh.unit[q_slot * 128 + in_slot];
       // from here on positions count from the segment's first tile
       low -= g.tile0 * kTile;
       high -= g.tile0 * kTile;
+      sh.bounds[slot][in_slot] = make_int2(low, high);
+      if (turns) named_bar_sync(1, kSoftmaxThreads);       // slot 1 reads slot 0's units
+      __syncwarp();
+      const int first_row = warp % 4 * 32 + lane / 4;      // of this lane's four in the slot
+      TileRows r;
+      r.t_s = t_s;
+      r.t_o = t_o;
+      r.bounds = smem_u32(&sh.bounds[slot][first_row]);
+      r.offset = 0;
+      float ms[4], ns[4], ls[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        r.unit[i] = sh.unit[q_slot * 128 + first_row + 8 * i];
+        ms[i] = ns[i] = -INFINITY;
+        ls[i] = 0.0f;
+      }
       bool first = true;
       for (int left = g.tiles; left > 0; --left) {
         const int stage = tile & 3;
@@ -730,8 +859,11 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
           wait_whole_warp(sh, &sh.s_full[slot], own & 1);
           __syncwarp();
           tc_fence_after();
-          const bool masked = sh.there[stage][0] == 0 || sh.there[stage][1] == 0 || __any_sync(0xffffffffu, low > 0 || high < kTile - 1);
-          softmax_tile<D>(sh, slot, stage, t_s, t_o, scales0 + stage * (2 * kTile * 4), masked, low, high, unit, first, m, n, l);
+          r.there0 = sh.there[stage][0] != 0;
+          r.there1 = sh.there[stage][1] != 0;
+          r.masked = !r.there0 || !r.there1 || __any_sync(0xffffffffu, low > 0 || high < kTile - 1);
+          r.scales = scales0 + stage * (2 * kTile * 4) + lane % 4 * 8;
+          softmax_tile<D>(sh, r, slot, stage, own & 1, first, ms, ns, ls);
           ++own;
           first = false;
         }
@@ -742,17 +874,29 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
         turn ^= turn >> 1 & 1u;
         low -= kTile;
         high -= kTile;
+        r.offset += kTile;
       }
-    }
-    // ---- the segment's end
-    if (active) {
-      wait_whole_warp(sh, &sh.o_full[slot], own_segments & 1);
-      __syncwarp();
-      tc_fence_after();
-      ++own_segments;
-      sh.end[slot][0][in_slot] = m;
-      sh.end[slot][1][in_slot] = l;
-      sh.end[slot][2][in_slot] = n;
+      // ---- the segment's end: from here on a thread has a row
+      if (active) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          ls[i] += __shfl_xor_sync(0xffffffffu, ls[i], 1);
+          ls[i] += __shfl_xor_sync(0xffffffffu, ls[i], 2);
+          if (lane % 4 == 0) {
+            sh.end[slot][0][first_row + 8 * i] = ms[i];
+            sh.end[slot][1][first_row + 8 * i] = ls[i];
+            sh.end[slot][2][first_row + 8 * i] = ns[i];
+          }
+        }
+        __syncwarp();
+        m = sh.end[slot][0][in_slot];
+        l = sh.end[slot][1][in_slot];
+        n = sh.end[slot][2][in_slot];
+        wait_whole_warp(sh, &sh.o_full[slot], own_segments & 1);
+        __syncwarp();
+        tc_fence_after();
+        ++own_segments;
+      }
     }
     if (softmax_bar_any(sh.abort_code != 0)) return;
     const bool whole = g.whole, real = row < g.rows && !(turns && slot == 1);
@@ -833,7 +977,7 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
           if (first_row + line < g.rows) *(reinterpret_cast<uint4*>(a.out + begin) + chunk) = p;
         }
       }
-      if (real && !whole) reinterpret_cast<float4*>(a.partial + 2ll * ctas * kChunkRows * D)[static_cast<long long>(part) * kChunkRows + row] = make_float4(m, l, n, 0.0f);
+      if (real && !whole) reinterpret_cast<float4*>(a.partial + 2ll * piece.ctas * kChunkRows * D)[static_cast<long long>(part) * kChunkRows + row] = make_float4(m, l, n, 0.0f);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.o_empty[slot]);
@@ -850,7 +994,7 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
       named_bar_sync(1, kSoftmaxThreads);
       if (s_plan.last) {
         __threadfence();
-        join_columns<D>(a, g.q_first, g.row0, g.head, g.rows, ctas, parts, tid, kSoftmaxThreads);
+        join_columns<D>(a, g.q_first, g.row0, g.head, g.rows, piece.ctas, parts, tid, kSoftmaxThreads);
       }
     }
     if (tid == 0) ++sh.finished;
@@ -868,17 +1012,20 @@ kv4_chunk_kernel(const __grid_constant__ AttentionArgs a, int* __restrict__ stat
   uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   __shared__ ChunkShared sh;
   __shared__ PlanShared s_plan;
+  __shared__ Piece piece;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
 
   pdl_wait();
   pdl_trigger();
   const ChunkPlan plan = {a.batch, a.cache.heads, a.group, a.window};
-  const long long total = plan.total(s_plan);
-  const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
-  if (static_cast<int>(blockIdx.x) >= ctas) return;
-  const long long w0 = piece_start(total, ctas, blockIdx.x), w1 = piece_start(total, ctas, blockIdx.x + 1);
-  const int places = static_cast<int>(w1 - w0);
-  plan.locate(s_plan, w0);
+  {
+    const long long total = plan.total(s_plan);
+    const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
+    if (static_cast<int>(blockIdx.x) >= ctas) return;
+    const long long w0 = piece_start(total, ctas, blockIdx.x), w1 = piece_start(total, ctas, blockIdx.x + 1);
+    if (tid == 0) piece = {total, w1, ctas, static_cast<int>(w1 - w0)};
+    plan.locate(s_plan, w0);
+  }
 
   if (tid == 0) {
     for (int i = 0; i < kScaleStages; ++i) {
@@ -895,6 +1042,7 @@ kv4_chunk_kernel(const __grid_constant__ AttentionArgs a, int* __restrict__ stat
       mbar_init(&sh.q_full[i], 4);
       mbar_init(&sh.s_full[i], 1);
       mbar_init(&sh.p_half[i], 4);
+      mbar_init(&sh.half_done[i], 1);
       mbar_init(&sh.p_full[i], 4);
       mbar_init(&sh.o_full[i], 1);
       mbar_init(&sh.o_empty[i], 4);
@@ -910,7 +1058,7 @@ kv4_chunk_kernel(const __grid_constant__ AttentionArgs a, int* __restrict__ stat
     sh.finished = 0;
     fence_barrier_init();
   }
-  if (warp == 16) {
+  if (warp == 12) {
     tmem_alloc(&sh.tmem, 512);
     tmem_relinquish();
   }
@@ -918,20 +1066,18 @@ kv4_chunk_kernel(const __grid_constant__ AttentionArgs a, int* __restrict__ stat
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh.tmem;                // S of slot s at columns 128 s (P over its first 64), O at 256 + 128 s
-  // 640 threads at 96 registers: 256 softmax threads at 160, 256 converting ones at 56 and 128 at 40 make 60416 of the 61440.
+  // 512 threads at 128 registers: 256 softmax threads at 184 and 256 others at 72, until the roles are done.
   if (warp < kSoftmaxWarps) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
-    softmax_role<D>(a, sh, s_plan, smem, tmem, ctas);
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
-  } else if (warp < 16) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp < 12) convert_role<D, false>(a, sh, smem);
-    else convert_role<D, true>(a, sh, smem);
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    softmax_role<D>(a, sh, s_plan, smem, tmem, piece);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 128;");
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    if (lane == 0) {
-      if (warp == 16) mma_role<D>(sh, smem, tmem);
-      if (warp == 17) plan_role(a, plan, s_plan, sh, places, w1, total, ctas, wait_limit);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp < 12) {
+      convert_role<D>(a, sh, smem);
+    } else if (lane == 0) {
+      if (warp == 12) mma_role<D>(sh, smem, tmem);
+      if (warp == 13) plan_role(a, plan, s_plan, sh, piece, wait_limit);
     }
     __syncwarp();
   }
@@ -940,10 +1086,10 @@ kv4_chunk_kernel(const __grid_constant__ AttentionArgs a, int* __restrict__ stat
   __syncthreads();
   // (Not before every role is done: an idle warp that took its registers back at once could take those that a softmax warp is
   // still to get, and the two would wait for each other.)
-  if (warp >= kSoftmaxWarps) asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
+  if (warp >= kSoftmaxWarps) asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
   if (sh.abort_code != 0) {
     // A role gave up: MMAs may still be on their way, which otherwise the roles have waited for.
-    if (tid == 16 * 32) {
+    if (tid == 12 * 32) {
       umma_commit(&sh.idle);
       mbar_wait_landed(&sh.idle, 0);
     }
@@ -951,7 +1097,7 @@ kv4_chunk_kernel(const __grid_constant__ AttentionArgs a, int* __restrict__ stat
     // What is left of the piece becomes NaN, and its units are counted, so that nobody waits for them and the next call finds the
     // counters at zero.
     ChunkCursor at;
-    at.start(plan, s_plan, places);
+    at.start(plan, s_plan, piece.places);
     bool unfinished = false;                  // (the last tile's time may run out when all that is left is to leave)
     for (int segment = 0; at.left > 0; ++segment) {
       const int n = at.tiles_here(), rows = at.rows(a.group);
@@ -964,10 +1110,10 @@ kv4_chunk_kernel(const __grid_constant__ AttentionArgs a, int* __restrict__ stat
             a.out[(at.s.first + r / a.group) * a.out_stride + (at.head * a.group + r % a.group) * D + x % D] = __float2bfloat16(__int_as_float(0x7fffffff));
           }
         } else {
-          const Parts parts(total, ctas, w1 - at.left - at.tile, at.span.tiles);
+          const Parts parts(piece.total, piece.ctas, piece.w1 - at.left - at.tile, at.span.tiles);
           const int slot_no = parts.slot(static_cast<int>(blockIdx.x));
           for (int x = tid; x < rows; x += kChunkThreads)
-            reinterpret_cast<float4*>(a.partial + 2ll * ctas * kChunkRows * D)[static_cast<long long>(slot_no) * kChunkRows + x] =
+            reinterpret_cast<float4*>(a.partial + 2ll * piece.ctas * kChunkRows * D)[static_cast<long long>(slot_no) * kChunkRows + x] =
                 make_float4(0.0f, __int_as_float(0x7fffffff), 0.0f, 0.0f);
           __threadfence();
           __syncthreads();
@@ -979,7 +1125,7 @@ kv4_chunk_kernel(const __grid_constant__ AttentionArgs a, int* __restrict__ stat
           __syncthreads();
           if (s_plan.last) {
             __threadfence();
-            join_columns<D>(a, at.s.first, at.rt * kChunkRows, at.head, rows, ctas, parts, tid, kChunkThreads);
+            join_columns<D>(a, at.s.first, at.rt * kChunkRows, at.head, rows, piece.ctas, parts, tid, kChunkThreads);
           }
           __syncthreads();
         }
@@ -989,7 +1135,7 @@ kv4_chunk_kernel(const __grid_constant__ AttentionArgs a, int* __restrict__ stat
     if (tid == 0 && unfinished) atomicExch(status, sh.abort_code);
   }
   __syncthreads();
-  if (warp == 16) {
+  if (warp == 12) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }

@@ -83,8 +83,8 @@ def random_cache(pages, heads, dim, seed=0, device="cpu"):
 
 def attention(q, cache, block_table, seq_lens, q_starts, scale=None, window=0):
     """f64 (out, spread, floor) [tokens, q_heads, D]; spread is the same average over |value|, the unit of rounding errors in the
-    weights.  floor is 2^-32 of the row's largest product of weight and value scale, times the sum of |code * group scale|: what the sums
-    are off by where every weight is off by so much (the interface lets a weight 2^-32 below the largest be left out).  Rows of no
+    weights.  floor is 2^-28 of the row's largest product of weight and value scale, times the sum of |code * group scale|: what the sums
+    are off by where every weight is off by so much (the interface lets a weight 2^-28 below the largest be left out).  Rows of no
     sequence are NaN."""
     T, HQ, D = q.shape
     group = HQ // cache.shape[2]
@@ -123,5 +123,5 @@ def attention(q, cache, block_table, seq_lens, q_starts, scale=None, window=0):
             spread[lo:hi, h] = w @ clean.abs()
             if len(j):
                 largest = (w * scales[:, h // group].nan_to_num(0.0, 0.0)).amax(-1, keepdim=True)
-                floor[lo:hi, h] = 2.0 ** -32 * largest * (seen.double() @ units[:, h // group])
+                floor[lo:hi, h] = 2.0 ** -28 * largest * (seen.double() @ units[:, h // group])
     return out, spread, floor

@@ -276,9 +276,9 @@ def _attention_inputs(kv4, q_lens, kv_lens, HQ, HK, D, seed=0, q_scale=1.5, spar
 
 
 def _check_attention(out, want, spread, floor):
-    """A weight times its value's scale is kept in f16 in units in which the row's largest is at least 2^7: below 2^-14, f16's smallest normal
-    number, it is off by up to 2^-25, which is 2^-32 of the largest (`floor`).  That shows in a dimension in which the values with large
-    weights are zero, which one code in ten is."""
+    """A weight times its value's scale is kept in f16 in units in which the row's largest is at least 2^3 (2^7 in decoding): below 2^-14, f16's
+    smallest normal number, it is off by up to 2^-25, which is 2^-28 of the largest (`floor`).  That shows in a dimension in which the values
+    with large weights are zero, which one code in ten is."""
     assert torch.equal(out.isnan(), want.isnan())
     error = (out.double() - want).abs()
     limit = want.abs() * 2.0 ** -8 * 1.01 + spread * (2.0 ** -10 + 2.0 ** -12) + floor * 1.01 + 1e-30
