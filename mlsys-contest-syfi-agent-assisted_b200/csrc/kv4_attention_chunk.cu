@@ -3,8 +3,9 @@
 // A CTA (one per SM) walks its piece of the line of 128-position tiles.  A unit's up to 256 rows are two slots of 128, the M of an MMA:
 //   S = Q K^T   tcgen05.mma kind::f16.  Keys are code * group scale, which f16 holds exactly; a row of q, scaled by a power of two, too (down
 //               to 2^-29 of its largest).
-//   P           softmax warps, four rows to a lane.  With x in units of log2 and references m (of the sum l) and n (of O) that follow the
-//               row's largest terms, l = sum 2^(x - m) and P = 2^(x - n + 5) * vscale, rounded to f16, back into tensor memory over S.
+//   P           softmax warps, four rows to a lane.  With x in units of log2 and references m (of the sum l) and n (of O) that follow a row's
+//               largest score and its largest product of weight and value scale, l = sum 2^(x - m) and P = 2^(x - n + 5) * vscale, rounded to
+//               f16, back into tensor memory over S.
 //   O += P V    kind::f16, P from tensor memory, values as code * group scale in shared memory, exact again.
 // Four converting warps, a thread per position, keep its key's and value's codes in registers while the stages in front are in use, so
 // nothing but f16 tiles lies in shared memory.  The slots are out of step by half a tile: while the softmax warps of one work, the tensor
@@ -75,9 +76,10 @@ struct ChunkShared {
   int there[kScaleStages][2];          // page p of the tile is there
   alignas(16) float largest[kScaleStages][4];    // value scales of 32 positions each that any row sees, ...
   alignas(16) float smallest[kScaleStages][4];   // ... read four at a time
-  float end[2][3][128];                // [slot][m, l, n][row], at a segment's end
+  alignas(16) float4 end[2][128];      // [slot][row] m, l and n, at a segment's end
   float unit[256];                     // of each row: what a score is worth
   int2 bounds[2][128];                 // [slot][row]: the positions that it sees, counted from the segment's first tile
+  int2 common[kSoftmaxWarps];          // the positions that all of a softmax warp's rows see
   volatile int abort_code;
   volatile uint32_t tiles_done;
   volatile int done;                   // every segment is
@@ -336,67 +338,63 @@ __device__ __forceinline__ void convert_role(const AttentionArgs& a, ChunkShared
   Ring<kSegmentRing> segments;           // of the tile to ask for
   Ring<kScaleStages> scales;
   Ring<kStages> tiles;
-  // The walk of the loads: a tile's rows are asked for when the tile in front is converted, its table entry one tile earlier.
-  int next_tile = 0, left = 0, any_low = 0, any_high = 0, all_low = 0, all_high = 0, head = 0;
-  const int32_t* table = nullptr;
-  int entry = -1, entry_head = 0;        // of the tile to ask for
-  bool entry_seen = false, entry_plain = false;
-  auto next_entry = [&]() -> bool {      // whole warp; false behind the last tile
+  // The walk of the loads: a tile's rows are asked for as soon as those of the tile in front are converted, its table entry two tiles
+  // earlier, so that neither is waited for.
+  struct Ahead {
+    int entry;                           // a page of the cache, or none
+    int head_flags;                      // key head * 4, 2: any row sees the position, 1: all rows see the tile
+  };
+  int next_tile = 0, left = 0;
+  auto look_ahead = [&](Ahead& e) -> bool {      // whole warp; false behind the last tile
+    const Segment& g = sh.segment[segments.stage];
     if (left == 0) {
       wait_whole_warp(sh, &sh.segment_full[segments.stage], segments.parity);
       __syncwarp();
-      const Segment& g = sh.segment[segments.stage];
       left = __any_sync(0xffffffffu, sh.abort_code != 0) ? 0 : g.tiles;
       if (left == 0) return false;
       next_tile = g.tile0;
-      any_low = g.any_low;
-      any_high = g.any_high;
-      all_low = g.all_low;
-      all_high = g.all_high;
-      head = g.head;
-      table = a.batch.block_table + static_cast<long long>(g.b) * a.batch.max_pages;
+    }
+    const int page = 2 * next_tile + page_of, first = next_tile * kTile;
+    e.entry = page < a.batch.max_pages && page * kKvPage <= g.any_high && (page + 1) * kKvPage > g.any_low
+                  ? __ldg(a.batch.block_table + static_cast<long long>(g.b) * a.batch.max_pages + page) : -1;
+    e.head_flags = g.head * 4 + (first + t >= g.any_low && first + t <= g.any_high ? 2 : 0) + (first >= g.all_low && first + kTile - 1 <= g.all_high ? 1 : 0);
+    ++next_tile;
+    if (--left == 0) {
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.segment_empty[segments.stage]);
       segments.next();
     }
-    const int page = 2 * next_tile + page_of, first = next_tile * kTile;
-    entry = page < a.batch.max_pages && page * kKvPage <= any_high && (page + 1) * kKvPage > any_low ? __ldg(table + page) : -1;
-    entry_head = head;
-    entry_seen = first + t >= any_low && first + t <= any_high;
-    entry_plain = first >= all_low && first + kTile - 1 <= all_high;
-    ++next_tile;
-    --left;
     return true;
   };
+  auto is_there = [&](const Ahead& e) { return e.entry >= 0 && e.entry < a.cache.num_pages; };
+  const long long to_values = static_cast<long long>(a.cache.heads) * Kv4Block<D>::kBytes;
   RawRow<D> key, value;
-  bool there = false, plain = false, seen = false;     // of the rows in registers
-  auto ask = [&]() {
-    there = entry >= 0 && entry < a.cache.num_pages;
-    seen = entry_seen;
-    plain = entry_plain;
-    if (there) {
-      const uint8_t* const block = kv4_block<D>(a.cache, entry, 0, entry_head);
-      key.ask(block, at);
-      value.ask(block + static_cast<long long>(a.cache.heads) * Kv4Block<D>::kBytes, at);
-    }
-  };
-  bool more = next_entry();
-  if (more) ask();
-  while (more) {
-    more = next_entry();                 // (of the tile behind the one in registers)
+  Ahead now, next, behind;               // of the rows in registers, and of the two tiles that follow
+  bool here = look_ahead(now);
+  if (here && is_there(now)) {
+    const uint8_t* const block = kv4_block<D>(a.cache, now.entry, 0, now.head_flags >> 2);
+    key.ask(block, at);
+    value.ask(block + to_values, at);
+  }
+  bool more = here && look_ahead(next);
+  while (here) {
+    const bool more_behind = more && look_ahead(behind), there = is_there(now);
     wait_whole_warp(sh, &sh.k_empty[tiles.stage], tiles.parity ^ 1u);
     __syncwarp();
     if (there) key.put(smem + Shape::kK + tiles.stage * Shape::kTileBytes + t * 128, t);
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) mbar_arrive(&sh.k_full[tiles.stage]);
+    float ks = there ? key.scale : 0.0f;
+    const uint8_t* const block = more && is_there(next) ? kv4_block<D>(a.cache, next.entry, 0, next.head_flags >> 2) : nullptr;
+    if (block) key.ask(block, at);
     // What a row does not see must not reach its sums, and zero times NaN is NaN: values of positions that no row sees become zeros, and
     // where some rows see a value that is not finite, the NaN goes by way of its score to those rows alone.
-    float ks = there ? key.scale : 0.0f, vs = there ? value.scale : 1.0f;
+    float vs = there ? value.scale : 1.0f;
     bool bad = !(fabsf(vs) <= 3.402823466e38f);
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) bad |= there && (((value.groups[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0u;
-    const bool valid = there && seen && (plain || !bad);
+    const bool valid = there && (now.head_flags & 2) && ((now.head_flags & 1) || !bad);
     if (bad || !(fabsf(ks) <= 3.402823466e38f)) ks = __int_as_float(0x7fffffff);
     if (!valid) vs = 1.0f;
     const unsigned bits = __float_as_uint(vs);
@@ -428,8 +426,12 @@ __device__ __forceinline__ void convert_role(const AttentionArgs& a, ChunkShared
     __syncwarp();
     if (lane == 0) mbar_arrive(&sh.v_full[tiles.stage]);
     tiles.next();
-    if (more) ask();
+    if (block) value.ask(block + to_values, at);
     if (__any_sync(0xffffffffu, sh.abort_code != 0)) return;
+    here = more;
+    now = next;
+    more = more_behind;
+    next = behind;
   }
 }
 
@@ -445,7 +447,7 @@ __device__ __forceinline__ uint64_t ld_shared_pair(uint32_t at) {
 
 // What the softmax of a tile works with.
 struct TileRows {
-  uint32_t t_s, t_o;                   // tensor memory: scores (weights over their first half), sums
+  uint32_t t_s;                        // tensor memory: scores (weights over their first half); the sums lie 256 columns on
   uint32_t scales;                     // shared memory: this lane's first of 128 scales of keys, then of values
   uint32_t bounds;                     // shared memory: lowest and highest position that this lane's first row sees, eight rows on the next
   int offset;                          // of the tile in those
@@ -605,11 +607,11 @@ __device__ __forceinline__ void set_references(const TileRows& r, float largest,
 }
 
 // The weights of a tile, half of it at a time: into tensor memory over scores that are used up.  A reference n stays what it is unless a weight
-// does not fit, which hardly ever happens; then the row's O fades, and the half is done again.  GENERAL: rows that do not see every position, and
-// `careful`: weights in units of m first, for tiles whose value scales are far apart.
+// does not fit, which hardly ever happens; then the row's O and l fade, and the half is done again.  GENERAL: rows that do not see every
+// position, and `careful`: weights in units of m first, for tiles whose value scales are far apart.
 template <int D, bool GENERAL>
-__device__ __forceinline__ void tile_weights(ChunkShared& sh, const TileRows& r, int slot, uint32_t tile_parity, bool first, bool careful, float largest, float (&m)[4],
-                                             float (&n)[4], float (&l)[4]) {
+__device__ __forceinline__ void tile_weights(ChunkShared& sh, const TileRows& r, int slot, uint32_t tile_parity, bool first, bool careful, float largest,
+                                             float (&m)[4], float (&n)[4], float (&l)[4]) {
   const int lane = threadIdx.x % 32;
   float shift[4], factor[4];
 #pragma unroll
@@ -651,14 +653,14 @@ __device__ __forceinline__ void tile_weights(ChunkShared& sh, const TileRows& r,
         __syncwarp();
         tc_fence_after();
       }
-      if (!first || h == 1) rescale_sums<D>(r.t_o, fade);
+      if (!first || h == 1) rescale_sums<D>(r.t_s + 256, fade);
       load_scores(r, h, s);
     }
-#pragma unroll
-    for (int row = 0; row < 4; ++row) l[row] += GENERAL && careful ? total[row] : total[row] * ex2(-shift[row] - finite_or_zero(m[row]));
     if (h == 0) load_scores(r, 1, s);
     tmem_st_16x128b(r.t_s + 32 * h, p[0]);
     tmem_st_16x128b(r.t_s + 32 * h + (16u << 16), p[1]);
+#pragma unroll
+    for (int row = 0; row < 4; ++row) l[row] += GENERAL && careful ? total[row] : total[row] * ex2(-shift[row] - finite_or_zero(m[row]));
     tmem_st_wait();
     tc_fence_before();
     __syncwarp();
@@ -670,6 +672,7 @@ __device__ __forceinline__ void tile_weights(ChunkShared& sh, const TileRows& r,
 template <int D>
 __device__ __forceinline__ void softmax_tile(ChunkShared& sh, const TileRows& r, int slot, int stage, uint32_t tile_parity, bool first, float (&m)[4], float (&n)[4],
                                              float (&l)[4]) {
+  // Flags first, the scores arrive meanwhile.
   const float4 v_high = *reinterpret_cast<const float4*>(sh.largest[stage]), v_low = *reinterpret_cast<const float4*>(sh.smallest[stage]);
   const float largest = fmaxf(fmaxf(v_high.x, v_high.y), fmaxf(v_high.z, v_high.w)), smallest = fminf(fminf(v_low.x, v_low.y), fminf(v_low.z, v_low.w));
   // (no scale of zero among them; the weights' sum, in units of n, is in f32's range)
@@ -680,11 +683,14 @@ __device__ __forceinline__ void softmax_tile(ChunkShared& sh, const TileRows& r,
     far |= n[row] - m[row] > kFarAbove;
     blind |= n[row] == -INFINITY && l[row] == l[row];
   }
-  const bool careful = !near || __any_sync(0xffffffffu, far);
-  if (careful || first || __any_sync(0xffffffffu, blind)) {
+  const bool careful = !near || __any_sync(0xffffffffu, far), prepare = careful || first || __any_sync(0xffffffffu, blind);
+  wait_whole_warp(sh, &sh.s_full[slot], tile_parity);
+  __syncwarp();
+  tc_fence_after();
+  if (prepare) {
     float fade[4];
     set_references(r, largest, careful, m, n, l, fade);
-    if (!first && __any_sync(0xffffffffu, fade[0] != 1.0f || fade[1] != 1.0f || fade[2] != 1.0f || fade[3] != 1.0f)) rescale_sums<D>(r.t_o, fade);
+    if (!first && __any_sync(0xffffffffu, fade[0] != 1.0f || fade[1] != 1.0f || fade[2] != 1.0f || fade[3] != 1.0f)) rescale_sums<D>(r.t_s + 256, fade);
   }
   if (__builtin_expect(careful || r.masked, 0)) tile_weights<D, true>(sh, r, slot, tile_parity, first, careful, largest, m, n, l);
   else tile_weights<D, false>(sh, r, slot, tile_parity, first, false, largest, m, n, l);
@@ -796,7 +802,7 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, slot = warp / 4, in_slot = warp % 4 * 32 + lane;
   const int across = 2 + warp % 4;                 // named barrier of the two slots' warps for the same rows
   const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
-  const uint32_t t_s = tmem + lanes + slot * 128, t_o = tmem + lanes + 256 + slot * 128, scales0 = smem_u32(smem) + Shape::kScales;
+  const uint32_t t_s = tmem + lanes + slot * 128, t_o = t_s + 256, scales0 = smem_u32(smem) + Shape::kScales;
   static_assert(kSegmentRing == 4 && kScaleStages == 4, "stage and parity are bits of a counter");
   uint32_t segment = 0, tile = 0, own = 0, own_segments = 0;       // segments and tiles so far, and those of this slot
   while (true) {
@@ -811,37 +817,34 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
     // whether the next tile is this slot's (bit 0: no), and whether that changes with each (bit 1)
     unsigned turn = turns ? 2u + slot : g.rows <= slot * kSlotRows;
     const bool active = turn != 1u;
-    const int row = (turns ? 0 : slot * kSlotRows) + in_slot;
-    float m = -INFINITY, n = -INFINITY, l = 0.0f;    // of this thread's row, at the segment's end
-    int token_of_row = 0, column_of_row = 0;         // of this thread's row, in q and out
+    // (a thread's row of the unit; rows beyond the last copy its bounds)
+    auto row_of = [&]() { return (g.turns ? 0 : slot * kSlotRows) + in_slot; };
+    auto token_of = [&](int& column) {
+      const int at = g.row0 + min(row_of(), g.rows - 1), token = at / a.group;
+      column = (g.head * a.group + at - token * a.group) * D;
+      return token;
+    };
     {
-      int low, high;
+      const int q_slot = turns ? 0 : slot, first_row = warp % 4 * 32 + lane / 4;      // the first of this lane's four in the slot
       {
-        const int r = g.row0 + min(row, g.rows - 1), token = r / a.group;        // (rows beyond the last copy its bounds)
-        token_of_row = g.q_first + token;
-        column_of_row = (g.head * a.group + r - token * a.group) * D;
-        high = g.base + token;
-        low = a.window > 0 ? max(high - a.window + 1, 0) : 0;
-      }
-      const int q_slot = turns ? 0 : slot;
-      if (active && q_slot == slot) {
-        const int in_tile = warp % 4 * 32;
-        put_queries<D>(a.q, token_of_row * a.q_stride + column_of_row, a.scale_log2, g.rows - slot * kSlotRows - in_tile,
-                       smem + Shape::kQ + slot * Shape::kTileBytes, in_tile, sh.unit + slot * 128 + in_tile);
-        fence_proxy_async_smem();
+        int column;
+        const int token = token_of(column), high = g.base + token - g.tile0 * kTile;
+        const int low = a.window > 0 ? max(g.base + token - a.window + 1, 0) - g.tile0 * kTile : -g.tile0 * kTile;
+        sh.bounds[slot][in_slot] = make_int2(low, high);      // counted from the segment's first tile
+        const int highest_low = __reduce_max_sync(0xffffffffu, low), lowest_high = __reduce_min_sync(0xffffffffu, high);
+        if (lane == 0) sh.common[warp] = make_int2(highest_low, lowest_high);
+        if (active && q_slot == slot) {
+          const int in_tile = warp % 4 * 32;
+          put_queries<D>(a.q, (g.q_first + token) * a.q_stride + column, a.scale_log2, g.rows - slot * kSlotRows - in_tile,
+                         smem + Shape::kQ + slot * Shape::kTileBytes, in_tile, sh.unit + slot * 128 + in_tile);
+          fence_proxy_async_smem();
+        }
       }
       __syncwarp();
       if (active && lane == 0) mbar_arrive(&sh.q_full[slot]);
-      // from here on positions count from the segment's first tile
-      low -= g.tile0 * kTile;
-      high -= g.tile0 * kTile;
-      sh.bounds[slot][in_slot] = make_int2(low, high);
       if (turns) named_bar_sync(1, kSoftmaxThreads);       // slot 1 reads slot 0's units
-      __syncwarp();
-      const int first_row = warp % 4 * 32 + lane / 4;      // of this lane's four in the slot
       TileRows r;
       r.t_s = t_s;
-      r.t_o = t_o;
       r.bounds = smem_u32(&sh.bounds[slot][first_row]);
       r.offset = 0;
       float ms[4], ns[4], ls[4];
@@ -856,12 +859,10 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
         const int stage = tile & 3;
         wait_whole_warp(sh, &sh.scale_full[stage], tile >> 2 & 1);
         if (!(turn & 1u)) {
-          wait_whole_warp(sh, &sh.s_full[slot], own & 1);
-          __syncwarp();
-          tc_fence_after();
+          const int2 common = sh.common[warp];
           r.there0 = sh.there[stage][0] != 0;
           r.there1 = sh.there[stage][1] != 0;
-          r.masked = !r.there0 || !r.there1 || __any_sync(0xffffffffu, low > 0 || high < kTile - 1);
+          r.masked = !r.there0 || !r.there1 || common.x > r.offset || common.y < r.offset + kTile - 1;
           r.scales = scales0 + stage * (2 * kTile * 4) + lane % 4 * 8;
           softmax_tile<D>(sh, r, slot, stage, own & 1, first, ms, ns, ls);
           ++own;
@@ -872,8 +873,6 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
         ++tile;
         if (tid == 0) sh.tiles_done = sh.tiles_done + 1u;
         turn ^= turn >> 1 & 1u;
-        low -= kTile;
-        high -= kTile;
         r.offset += kTile;
       }
       // ---- the segment's end: from here on a thread has a row
@@ -882,16 +881,8 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
         for (int i = 0; i < 4; ++i) {
           ls[i] += __shfl_xor_sync(0xffffffffu, ls[i], 1);
           ls[i] += __shfl_xor_sync(0xffffffffu, ls[i], 2);
-          if (lane % 4 == 0) {
-            sh.end[slot][0][first_row + 8 * i] = ms[i];
-            sh.end[slot][1][first_row + 8 * i] = ls[i];
-            sh.end[slot][2][first_row + 8 * i] = ns[i];
-          }
+          if (lane % 4 == 0) sh.end[slot][first_row + 8 * i] = make_float4(ms[i], ls[i], ns[i], 0.0f);
         }
-        __syncwarp();
-        m = sh.end[slot][0][in_slot];
-        l = sh.end[slot][1][in_slot];
-        n = sh.end[slot][2][in_slot];
         wait_whole_warp(sh, &sh.o_full[slot], own_segments & 1);
         __syncwarp();
         tc_fence_after();
@@ -899,19 +890,18 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
       }
     }
     if (softmax_bar_any(sh.abort_code != 0)) return;
+    const int row = row_of();
     const bool whole = g.whole, real = row < g.rows && !(turns && slot == 1);
     if (active) {
+      float4 mine = sh.end[slot][in_slot];    // m, l, n
       float f = 1.0f;
       if (turns) {                            // to the larger references of the two slots'
-        const float(&its)[3][128] = sh.end[slot ^ 1];
-        const float m_all = fmaxf(m, its[0][in_slot]), m_ref = finite_or_zero(m_all), n_all = fmaxf(n, its[2][in_slot]);
-        l = l * ex2(m - m_ref) + its[1][in_slot] * ex2(its[0][in_slot] - m_ref);
-        f = ex2(n - finite_or_zero(n_all));
-        m = m_all;
-        n = n_all;
+        const float4 its = sh.end[slot ^ 1][in_slot];
+        const float m_all = fmaxf(mine.x, its.x), m_ref = finite_or_zero(m_all), n_all = fmaxf(mine.z, its.z);
+        f = ex2(mine.z - finite_or_zero(n_all));
+        mine = make_float4(m_all, mine.y * ex2(mine.x - m_ref) + its.y * ex2(its.x - m_ref), n_all, 0.0f);
       }
-      const float inverse = l == 0.0f || n == -INFINITY ? 0.0f : ex2(n - finite_or_zero(m) - kProductHeadroom) / l;
-      if (whole) f *= inverse;
+      if (whole) f *= mine.y == 0.0f || mine.z == -INFINITY ? 0.0f : ex2(mine.z - finite_or_zero(mine.x) - kProductHeadroom) / mine.y;
       // Rows leave through the warp's own rows of the slot's q tile, which nothing reads any more.  Partial sums are kept by dimension, so that
       // a warp's 32 rows lie side by side.
       uint8_t* const own_rows = smem + Shape::kQ + slot * Shape::kTileBytes + warp % 4 * (32 * 128);
@@ -967,17 +957,19 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
       if (whole && !(turns && slot == 1)) {
         __syncwarp();
         constexpr int kLanes = D / 8, kTogether = 32 / kLanes;
-        const long long mine = token_of_row * a.out_stride + column_of_row;
+        int column;
+        const int token = token_of(column);
+        const long long place = (g.q_first + token) * a.out_stride + column;
         const int first_row = (turns ? 0 : slot * kSlotRows) + warp % 4 * 32, chunk = lane % kLanes;
 #pragma unroll 4
         for (int at = 0; at < 32; at += kTogether) {
           const int line = at + lane / kLanes;
-          const long long begin = __shfl_sync(0xffffffffu, mine, line);
+          const long long begin = __shfl_sync(0xffffffffu, place, line);
           const uint4 p = *reinterpret_cast<const uint4*>(own_rows + chunk / 8 * (kTile * 128) + line * 128 + ((chunk % 8 ^ (line & 7)) << 4));
           if (first_row + line < g.rows) *(reinterpret_cast<uint4*>(a.out + begin) + chunk) = p;
         }
       }
-      if (real && !whole) reinterpret_cast<float4*>(a.partial + 2ll * piece.ctas * kChunkRows * D)[static_cast<long long>(part) * kChunkRows + row] = make_float4(m, l, n, 0.0f);
+      if (real && !whole) reinterpret_cast<float4*>(a.partial + 2ll * piece.ctas * kChunkRows * D)[static_cast<long long>(part) * kChunkRows + row] = mine;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.o_empty[slot]);
@@ -1066,16 +1058,17 @@ kv4_chunk_kernel(const __grid_constant__ AttentionArgs a, int* __restrict__ stat
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh.tmem;                // S of slot s at columns 128 s (P over its first 64), O at 256 + 128 s
-  // 512 threads at 128 registers: 256 softmax threads at 184 and 256 others at 72, until the roles are done.
+  // 512 threads at 128 registers: 256 softmax threads at 176, 128 converting ones at 88 and 128 others at 72, until the roles are done.
   if (warp < kSoftmaxWarps) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
     softmax_role<D>(a, sh, s_plan, smem, tmem, piece);
     asm volatile("setmaxnreg.dec.sync.aligned.u32 128;");
+  } else if (warp < 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    convert_role<D>(a, sh, smem);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    if (warp < 12) {
-      convert_role<D>(a, sh, smem);
-    } else if (lane == 0) {
+    if (lane == 0) {
       if (warp == 12) mma_role<D>(sh, smem, tmem);
       if (warp == 13) plan_role(a, plan, s_plan, sh, piece, wait_limit);
     }
