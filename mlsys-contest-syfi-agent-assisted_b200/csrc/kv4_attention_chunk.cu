@@ -73,9 +73,10 @@ struct ChunkShared {
   uint64_t scale_full[kScaleStages], scale_empty[kScaleStages], k_full[4], k_empty[4], v_full[4], v_empty[4];
   uint64_t q_full[2], s_full[2], p_half[2], half_done[2], p_full[2], o_full[2], o_empty[2], idle;
   uint32_t tmem;
-  int there[kScaleStages][2];          // page p of the tile is there
-  alignas(16) float largest[kScaleStages][4];    // value scales of 32 positions each that any row sees, ...
-  alignas(16) float smallest[kScaleStages][4];   // ... read four at a time
+  int flags[kScaleStages];             // 1, 2: the tile's pages are there; 4: its value scales are near one another, none of them zero
+  float largest[kScaleStages];         // of the value scales that any row sees
+  float2 part[4];                      // largest and smallest of each converting warp's 32 positions
+  int part_there[4];
   alignas(16) float4 end[2][128];      // [slot][row] m, l and n, at a segment's end
   float unit[256];                     // of each row: what a score is worth
   int2 bounds[2][128];                 // [slot][row]: the positions that it sees, counted from the segment's first tile
@@ -292,6 +293,9 @@ __device__ __forceinline__ void ld_global_32(const void* p, uint4& a, uint4& b) 
   asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w) : "l"(p));
 }
+__device__ __forceinline__ void st_shared_16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
 // A row of codes and its scales on their way from the cache.
 template <int D>
 struct RawRow {
@@ -311,8 +315,8 @@ struct RawRow {
     }
     scale = __ldg(reinterpret_cast<const float*>(block + Kv4Block<D>::kScales) + at);
   }
-  // code * group scale as f16 into row t of a tile (`to`: the row in its first 64 dimensions)
-  __device__ __forceinline__ void put(uint8_t* to, int t) const {
+  // code * group scale as f16 into a tile's row (`to`: where its first 16 bytes lie, in rows of 128 that are swizzled)
+  __device__ __forceinline__ void put(uint32_t to) const {
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) {
       const uint32_t w[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
@@ -321,14 +325,26 @@ struct RawRow {
       const uint32_t scale[2] = {__byte_perm(both, both, 0x1010), __byte_perm(both, both, 0x3232)};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int chunk = i % 2 * 4 + k;
-        *reinterpret_cast<uint4*>(to + i / 2 * (kTile * 128) + ((chunk ^ (t & 7)) << 4)) =
-            make_uint4(hmul2_bits(e2m1x2_to_half2<0>(w[k]), scale[k / 2]), hmul2_bits(e2m1x2_to_half2<1>(w[k]), scale[k / 2]),
-                       hmul2_bits(e2m1x2_to_half2<2>(w[k]), scale[k / 2]), hmul2_bits(e2m1x2_to_half2<3>(w[k]), scale[k / 2]));
+        st_shared_16((to ^ (i % 2 * 4 + k) * 16) + i / 2 * (kTile * 128), hmul2_bits(e2m1x2_to_half2<0>(w[k]), scale[k / 2]), hmul2_bits(e2m1x2_to_half2<1>(w[k]), scale[k / 2]),
+                     hmul2_bits(e2m1x2_to_half2<2>(w[k]), scale[k / 2]), hmul2_bits(e2m1x2_to_half2<3>(w[k]), scale[k / 2]));
       }
     }
   }
 };
+
+// A barrier of the converting warps that tells all of them whether any thread's `p` holds.
+__device__ __forceinline__ bool converters_any(bool p) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, 7, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any)
+      : "r"(static_cast<uint32_t>(p))
+      : "memory");
+  return any != 0u;
+}
 
 template <int D>
 __device__ __forceinline__ void convert_role(const AttentionArgs& a, ChunkShared& sh, uint8_t* smem) {
@@ -350,7 +366,7 @@ __device__ __forceinline__ void convert_role(const AttentionArgs& a, ChunkShared
     if (left == 0) {
       wait_whole_warp(sh, &sh.segment_full[segments.stage], segments.parity);
       __syncwarp();
-      left = __any_sync(0xffffffffu, sh.abort_code != 0) ? 0 : g.tiles;
+      left = g.tiles;                    // (behind a failure an older segment's, or none: the same for the four warps)
       if (left == 0) return false;
       next_tile = g.tile0;
     }
@@ -367,27 +383,25 @@ __device__ __forceinline__ void convert_role(const AttentionArgs& a, ChunkShared
     return true;
   };
   auto is_there = [&](const Ahead& e) { return e.entry >= 0 && e.entry < a.cache.num_pages; };
-  const long long to_values = static_cast<long long>(a.cache.heads) * Kv4Block<D>::kBytes;
+  const uint32_t row = smem_u32(smem) + Shape::kK + t * 128 + (t & 7) * 16;      // in the keys' first stage
   RawRow<D> key, value;
   Ahead now, next, behind;               // of the rows in registers, and of the two tiles that follow
   bool here = look_ahead(now);
   if (here && is_there(now)) {
-    const uint8_t* const block = kv4_block<D>(a.cache, now.entry, 0, now.head_flags >> 2);
-    key.ask(block, at);
-    value.ask(block + to_values, at);
+    key.ask(kv4_block<D>(a.cache, now.entry, 0, now.head_flags >> 2), at);
+    value.ask(kv4_block<D>(a.cache, now.entry, 1, now.head_flags >> 2), at);
   }
   bool more = here && look_ahead(next);
   while (here) {
     const bool more_behind = more && look_ahead(behind), there = is_there(now);
     wait_whole_warp(sh, &sh.k_empty[tiles.stage], tiles.parity ^ 1u);
     __syncwarp();
-    if (there) key.put(smem + Shape::kK + tiles.stage * Shape::kTileBytes + t * 128, t);
+    if (there) key.put(row + tiles.stage * Shape::kTileBytes);
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) mbar_arrive(&sh.k_full[tiles.stage]);
     float ks = there ? key.scale : 0.0f;
-    const uint8_t* const block = more && is_there(next) ? kv4_block<D>(a.cache, next.entry, 0, next.head_flags >> 2) : nullptr;
-    if (block) key.ask(block, at);
+    if (more && is_there(next)) key.ask(kv4_block<D>(a.cache, next.entry, 0, next.head_flags >> 2), at);
     // What a row does not see must not reach its sums, and zero times NaN is NaN: values of positions that no row sees become zeros, and
     // where some rows see a value that is not finite, the NaN goes by way of its score to those rows alone.
     float vs = there ? value.scale : 1.0f;
@@ -406,28 +420,41 @@ __device__ __forceinline__ void convert_role(const AttentionArgs& a, ChunkShared
     to[t] = ks;
     to[kTile + t] = vs;
     if (lane == 0) {
-      sh.largest[scales.stage][warp] = __uint_as_float(high);
-      sh.smallest[scales.stage][warp] = __uint_as_float(low);
-      if (warp % 2 == 0) sh.there[scales.stage][page_of] = there;
+      sh.part[warp] = make_float2(__uint_as_float(high), __uint_as_float(low));
+      sh.part_there[warp] = there;
+    }
+    named_bar_sync(7, 128);
+    if (t == 0) {
+      float largest = 0.0f, smallest = INFINITY;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        largest = fmaxf(largest, sh.part[w].x);
+        smallest = fminf(smallest, sh.part[w].y);
+      }
+      // (the weights' sum, in units of n, is in f32's range)
+      const bool near = smallest >= kNear * largest && largest >= 1e-18f && largest <= 1e18f;
+      sh.largest[scales.stage] = largest;
+      sh.flags[scales.stage] = (sh.part_there[0] ? 1 : 0) | (sh.part_there[2] ? 2 : 0) | (near ? 4 : 0);
+      mbar_arrive(&sh.scale_full[scales.stage]);
     }
     __syncwarp();
-    if (lane == 0) mbar_arrive(&sh.scale_full[scales.stage]);
+    const bool gone = converters_any(sh.abort_code != 0);     // (and the parts are read)
     scales.next();
     wait_whole_warp(sh, &sh.v_empty[tiles.stage], tiles.parity ^ 1u);
     __syncwarp();
-    uint8_t* const row = smem + Shape::kV + tiles.stage * Shape::kTileBytes + t * 128;
+    const uint32_t to_row = row + (Shape::kV - Shape::kK) + tiles.stage * Shape::kTileBytes;
     if (valid) {
-      value.put(row, t);
+      value.put(to_row);
     } else {
 #pragma unroll 1
-      for (int chunk = 0; chunk < D / 8; ++chunk) *reinterpret_cast<uint4*>(row + chunk / 8 * (kTile * 128) + chunk % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
+      for (int chunk = 0; chunk < D / 8; ++chunk) st_shared_16((to_row ^ chunk % 8 * 16) + chunk / 8 * (kTile * 128), 0u, 0u, 0u, 0u);
     }
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) mbar_arrive(&sh.v_full[tiles.stage]);
     tiles.next();
-    if (block) value.ask(block + to_values, at);
-    if (__any_sync(0xffffffffu, sh.abort_code != 0)) return;
+    if (more && is_there(next)) value.ask(kv4_block<D>(a.cache, next.entry, 1, next.head_flags >> 2), at);
+    if (gone) return;                  // all four together
     here = more;
     now = next;
     more = more_behind;
@@ -449,14 +476,15 @@ __device__ __forceinline__ uint64_t ld_shared_pair(uint32_t at) {
 struct TileRows {
   uint32_t t_s;                        // tensor memory: scores (weights over their first half); the sums lie 256 columns on
   uint32_t scales;                     // shared memory: this lane's first of 128 scales of keys, then of values
-  uint32_t bounds;                     // shared memory: lowest and highest position that this lane's first row sees, eight rows on the next
+  const int2* bounds;                  // shared memory: lowest and highest position that each of the slots' rows sees
   int offset;                          // of the tile in those
   bool masked, there0, there1;         // whether any of that matters for the warp's rows; the tile's pages
+  bool near;                           // the tile's value scales are near one another
   float unit[4];                       // what a score is worth
 };
 __device__ __forceinline__ int2 row_bounds(const TileRows& r, int row) {
-  const uint64_t v = ld_shared_pair(r.bounds + row * 64);
-  return make_int2(static_cast<int>(v) - r.offset, static_cast<int>(v >> 32) - r.offset);
+  const int2 v = r.bounds[threadIdx.x / 32 * 32 + threadIdx.x % 32 / 4 + 8 * row];
+  return make_int2(v.x - r.offset, v.y - r.offset);
 }
 __device__ __forceinline__ float quad_max(float x) {
   x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
@@ -507,17 +535,17 @@ __device__ __forceinline__ void largest_scores(const TileRows& r, int h, const u
   }
 }
 
-// Weights of 64 positions, times the values' scales, as pairs of f16, their sums, and in `top` the largest.  GENERAL: positions that a row does
-// not see, and products times `factor`.
+// Weights of 64 positions, times the values' scales, as pairs of f16, and their sums; returns whether one does not fit (of all four rows).
+// GENERAL: positions that a row does not see, and products times `factor`.
 template <bool GENERAL>
-__device__ __forceinline__ void half_weights(const TileRows& r, int h, const uint32_t (&s)[2][32], const float (&shift)[4], const float (&factor)[4], float (&total)[4],
-                                             float (&top)[4], uint32_t (&p)[2][16]) {
+__device__ __forceinline__ bool half_weights(const TileRows& r, int h, const uint32_t (&s)[2][32], const float (&shift)[4], const float (&factor)[4], float (&total)[4],
+                                             uint32_t (&p)[2][16]) {
+  uint32_t most[2] = {0u, 0u};
   uint64_t sums[4];
   int2 see[4];
 #pragma unroll
   for (int row = 0; row < 4; ++row) {
     sums[row] = 0ull;
-    top[row] = 0.0f;
     see[row] = make_int2(0, 0);
     if (GENERAL) {
       see[row] = row_bounds(r, row);
@@ -545,8 +573,8 @@ __device__ __forceinline__ void half_weights(const TileRows& r, int h, const uin
       w = f32x2_mul(w, vs);
       if (GENERAL) w = f32x2_mul(w, f32x2_pack(factor[row], factor[row]));
       f32x2_unpack(w, x0, x1);
-      top[row] = fmaxf(top[row], fmaxf(x0, x1));
       p[row / 2][2 * i + row % 2] = pack_half2(x0, x1);
+      most[row / 2] = hmax2_bits(most[row / 2], p[row / 2][2 * i + row % 2]);
     }
   }
 #pragma unroll
@@ -554,6 +582,27 @@ __device__ __forceinline__ void half_weights(const TileRows& r, int h, const uin
     float a0, a1;
     f32x2_unpack(sums[row], a0, a1);
     total[row] = a0 + a1;
+  }
+  const uint32_t top = hmax2_bits(most[0], most[1]);
+  return (top & 0xffffu) > 0x7800u || top >> 16 > 0x7800u;      // 2^15 (the maximum of two is no NaN unless all are)
+}
+
+// The largest product of a weight, in units of `shift`, and its value's scale in 64 positions.
+__device__ __forceinline__ void largest_products(const TileRows& r, int h, const uint32_t (&s)[2][32], const float (&shift)[4], float (&most)[4]) {
+  const int column = 64 * h + threadIdx.x % 4 * 2;
+  const bool there = h == 0 ? r.there0 : r.there1;
+#pragma unroll
+  for (int row = 0; row < 4; ++row) {
+    const int2 see = row_bounds(r, row);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float x0, x1, v0, v1;
+      f32x2_unpack(f32x2_mul(f32x2_pack_bits(s[row / 2][4 * i + 2 * (row % 2)], s[row / 2][4 * i + 2 * (row % 2) + 1]), ld_shared_pair(r.scales + 4 * (64 * h + 8 * i))), x0, x1);
+      f32x2_unpack(ld_shared_pair(r.scales + 4 * (kTile + 64 * h + 8 * i)), v0, v1);
+      const int at = column + 8 * i;
+      if (there && at >= see.x && at <= see.y) most[row] = fmaxf(most[row], ex2(fmaf(x0, r.unit[row], shift[row])) * v0);
+      if (there && at + 1 >= see.x && at + 1 <= see.y) most[row] = fmaxf(most[row], ex2(fmaf(x1, r.unit[row], shift[row])) * v1);
+    }
   }
 }
 
@@ -578,20 +627,15 @@ __device__ __forceinline__ void set_references(const TileRows& r, float largest,
     bound[row] = top[row] + lg2(largest);
   }
   if (products) {
-    float most[4] = {}, one[4], shift[4], total[4];
+    float most[4] = {}, shift[4];
 #pragma unroll
-    for (int row = 0; row < 4; ++row) {
-      one[row] = 1.0f;
-      shift[row] = -finite_or_zero(m[row]);
-    }
+    for (int row = 0; row < 4; ++row) shift[row] = -finite_or_zero(m[row]);
 #pragma unroll 1
     for (int h = 0; h < 2; ++h) {
-      uint32_t s[2][32], p[2][16];
+      uint32_t s[2][32];
       load_scores(r, h, s);
       scores_landed(s);
-      half_weights<true>(r, h, s, shift, one, total, top, p);
-#pragma unroll
-      for (int row = 0; row < 4; ++row) most[row] = fmaxf(most[row], top[row]);
+      largest_products(r, h, s, shift, most);
     }
 #pragma unroll
     for (int row = 0; row < 4; ++row) bound[row] = m[row] + fmaxf(lg2(quad_max(most[row])), -90.0f);      // (never further behind: a value may be zero)
@@ -613,40 +657,36 @@ template <int D, bool GENERAL>
 __device__ __forceinline__ void tile_weights(ChunkShared& sh, const TileRows& r, int slot, uint32_t tile_parity, bool first, bool careful, float largest,
                                              float (&m)[4], float (&n)[4], float (&l)[4]) {
   const int lane = threadIdx.x % 32;
-  float shift[4], factor[4];
+  float shift[4], factor[4], worth[4];   // worth: of this tile's weights in the sum (a step of the references leaves it)
 #pragma unroll
   for (int row = 0; row < 4; ++row) {
     shift[row] = GENERAL && careful ? -finite_or_zero(m[row]) : kProductHeadroom - finite_or_zero(n[row]);
     factor[row] = !(GENERAL && careful) ? 1.0f : m[row] != -INFINITY && n[row] != -INFINITY ? ex2(m[row] - n[row] + kProductHeadroom) : 0.0f;
+    worth[row] = GENERAL && careful ? 1.0f : ex2(-shift[row] - finite_or_zero(m[row]));
   }
   uint32_t s[2][32];
   load_scores(r, 0, s);
 #pragma unroll 1
   for (int h = 0; h < 2; ++h) {
     uint32_t p[2][16];
-    float total[4], top[4];
+    float total[4];
     for (bool again = false;; again = true) {
       scores_landed(s);
-      half_weights<GENERAL>(r, h, s, shift, factor, total, top, p);
-      if (__builtin_expect(!__any_sync(0xffffffffu, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > 32768.0f), 1) || again) break;
+      const bool over = half_weights<GENERAL>(r, h, s, shift, factor, total, p);
+      // (in units of m nothing can be over that was finite)
+      if (__builtin_expect(!__any_sync(0xffffffffu, over), 1) || again || (GENERAL && careful)) break;
       load_scores(r, h, s);
       scores_landed(s);
       float highest[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, fade[4];
       largest_scores(r, h, s, highest);
 #pragma unroll
       for (int row = 0; row < 4; ++row) {
-        // (from the scores where a weight is beyond f32, too)
-        const float most = quad_max(top[row]), bound = fmaf(quad_max(highest[row]), r.unit[row], shift[row]) + lg2(largest);
-        const float up = most > 32768.0f ? (most <= 3.402823466e38f ? lg2(most) : bound) - kProductHeadroom : 0.0f;
+        const float bound = fmaf(quad_max(highest[row]), r.unit[row], shift[row]) + lg2(largest), up = bound > 15.0f ? bound - kProductHeadroom : 0.0f;
         fade[row] = ex2(-up);
         n[row] += up;
-        if (GENERAL && careful) {
-          factor[row] *= fade[row];
-        } else {
-          shift[row] -= up;
-          m[row] += up;                // (the sum's reference goes along, so that the two stay near)
-          l[row] *= fade[row];
-        }
+        shift[row] -= up;
+        m[row] += up;                  // (the sum's reference goes along, so that the two stay near)
+        l[row] *= fade[row];
       }
       if (h == 1) {                    // the first half's product is on its way
         wait_whole_warp(sh, &sh.half_done[slot], tile_parity);
@@ -660,7 +700,7 @@ __device__ __forceinline__ void tile_weights(ChunkShared& sh, const TileRows& r,
     tmem_st_16x128b(r.t_s + 32 * h, p[0]);
     tmem_st_16x128b(r.t_s + 32 * h + (16u << 16), p[1]);
 #pragma unroll
-    for (int row = 0; row < 4; ++row) l[row] += GENERAL && careful ? total[row] : total[row] * ex2(-shift[row] - finite_or_zero(m[row]));
+    for (int row = 0; row < 4; ++row) l[row] = fmaf(total[row], worth[row], l[row]);
     tmem_st_wait();
     tc_fence_before();
     __syncwarp();
@@ -668,32 +708,35 @@ __device__ __forceinline__ void tile_weights(ChunkShared& sh, const TileRows& r,
   }
 }
 
+// What the warp's rows need before a tile's weights: nothing; references, because a row has none (kBlind, as at the start); or weights in units of
+// m, because a row's n lies far above it (kFar).
+constexpr int kSettled = 0, kBlind = 1, kFar = 2;
+
 // A tile of the warp's rows: scores from tensor memory, weights back into it; the rows' references m and n and this lane's part of their sums l.
 template <int D>
-__device__ __forceinline__ void softmax_tile(ChunkShared& sh, const TileRows& r, int slot, int stage, uint32_t tile_parity, bool first, float (&m)[4], float (&n)[4],
-                                             float (&l)[4]) {
-  // Flags first, the scores arrive meanwhile.
-  const float4 v_high = *reinterpret_cast<const float4*>(sh.largest[stage]), v_low = *reinterpret_cast<const float4*>(sh.smallest[stage]);
-  const float largest = fmaxf(fmaxf(v_high.x, v_high.y), fmaxf(v_high.z, v_high.w)), smallest = fminf(fminf(v_low.x, v_low.y), fminf(v_low.z, v_low.w));
-  // (no scale of zero among them; the weights' sum, in units of n, is in f32's range)
-  const bool near = smallest >= kNear * largest && largest >= 1e-18f && largest <= 1e18f;
-  bool far = false, blind = false;             // (neither for a row that is not finite)
-#pragma unroll
-  for (int row = 0; row < 4; ++row) {
-    far |= n[row] - m[row] > kFarAbove;
-    blind |= n[row] == -INFINITY && l[row] == l[row];
-  }
-  const bool careful = !near || __any_sync(0xffffffffu, far), prepare = careful || first || __any_sync(0xffffffffu, blind);
+__device__ __forceinline__ void softmax_tile(ChunkShared& sh, const TileRows& r, int slot, int stage, uint32_t tile_parity, bool first, int& settled, float (&m)[4],
+                                             float (&n)[4], float (&l)[4]) {
+  const float largest = sh.largest[stage];
+  const bool careful = !r.near || settled == kFar;
   wait_whole_warp(sh, &sh.s_full[slot], tile_parity);
   __syncwarp();
   tc_fence_after();
-  if (prepare) {
+  if (careful || settled != kSettled) {
     float fade[4];
     set_references(r, largest, careful, m, n, l, fade);
     if (!first && __any_sync(0xffffffffu, fade[0] != 1.0f || fade[1] != 1.0f || fade[2] != 1.0f || fade[3] != 1.0f)) rescale_sums<D>(r.t_s + 256, fade);
   }
   if (__builtin_expect(careful || r.masked, 0)) tile_weights<D, true>(sh, r, slot, tile_parity, first, careful, largest, m, n, l);
   else tile_weights<D, false>(sh, r, slot, tile_parity, first, false, largest, m, n, l);
+  if (careful || settled != kSettled) {        // (neither far nor blind for a row that is not finite; steps of the references leave n - m)
+    bool far = false, blind = false;
+#pragma unroll
+    for (int row = 0; row < 4; ++row) {
+      far |= n[row] - m[row] > kFarAbove;
+      blind |= n[row] == -INFINITY && l[row] == l[row];
+    }
+    settled = __any_sync(0xffffffffu, far) ? kFar : __any_sync(0xffffffffu, blind) ? kBlind : kSettled;
+  }
 }
 
 // The warp's 32 rows of q (of which `rows` are there; mine: where this lane's row begins in q) as f16 times 2^k each, the row's largest at
@@ -845,7 +888,7 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
       if (turns) named_bar_sync(1, kSoftmaxThreads);       // slot 1 reads slot 0's units
       TileRows r;
       r.t_s = t_s;
-      r.bounds = smem_u32(&sh.bounds[slot][first_row]);
+      r.bounds = sh.bounds[0];
       r.offset = 0;
       float ms[4], ns[4], ls[4];
 #pragma unroll
@@ -854,19 +897,20 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
         ms[i] = ns[i] = -INFINITY;
         ls[i] = 0.0f;
       }
-      bool first = true;
+      int settled = kBlind;
       for (int left = g.tiles; left > 0; --left) {
         const int stage = tile & 3;
         wait_whole_warp(sh, &sh.scale_full[stage], tile >> 2 & 1);
         if (!(turn & 1u)) {
           const int2 common = sh.common[warp];
-          r.there0 = sh.there[stage][0] != 0;
-          r.there1 = sh.there[stage][1] != 0;
+          const int flags = sh.flags[stage];
+          r.there0 = flags & 1;
+          r.there1 = flags & 2;
+          r.near = flags & 4;
           r.masked = !r.there0 || !r.there1 || common.x > r.offset || common.y < r.offset + kTile - 1;
           r.scales = scales0 + stage * (2 * kTile * 4) + lane % 4 * 8;
-          softmax_tile<D>(sh, r, slot, stage, own & 1, first, ms, ns, ls);
+          softmax_tile<D>(sh, r, slot, stage, own & 1, left > g.tiles - (turns ? 2 : 1), settled, ms, ns, ls);
           ++own;
-          first = false;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.scale_empty[stage]);
@@ -1021,7 +1065,7 @@ kv4_chunk_kernel(const __grid_constant__ AttentionArgs a, int* __restrict__ stat
 
   if (tid == 0) {
     for (int i = 0; i < kScaleStages; ++i) {
-      mbar_init(&sh.scale_full[i], 4);
+      mbar_init(&sh.scale_full[i], 1);
       mbar_init(&sh.scale_empty[i], kSoftmaxWarps);
     }
     for (int i = 0; i < 4; ++i) {
@@ -1043,6 +1087,7 @@ kv4_chunk_kernel(const __grid_constant__ AttentionArgs a, int* __restrict__ stat
     for (int i = 0; i < kSegmentRing; ++i) {
       mbar_init(&sh.segment_full[i], 1);
       mbar_init(&sh.segment_empty[i], kSegmentReaders);
+      sh.segment[i].tiles = 0;
     }
     sh.abort_code = 0;
     sh.tiles_done = 0u;

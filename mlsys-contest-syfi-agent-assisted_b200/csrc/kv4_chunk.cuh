@@ -19,6 +19,11 @@ __device__ __forceinline__ uint64_t f32x2_add(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
+__device__ __forceinline__ uint32_t hmax2_bits(uint32_t a, uint32_t b) {     // a NaN is left out
+  uint32_t r;
+  asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
 // Tensor memory by 16 lanes (the warp's first or second 16, by the address): lane 4 i + j of the warp has, of every eight columns, 2 j and 2 j + 1
 // of lane i in registers 0 and 1 and of lane i + 8 in 2 and 3.  64 columns.
 __device__ __forceinline__ void tmem_ld_16x256b(uint32_t taddr, uint32_t (&r)[32]) {
