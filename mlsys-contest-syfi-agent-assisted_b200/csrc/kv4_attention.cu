@@ -14,12 +14,6 @@ namespace syfi {
 
 namespace {
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -32,119 +26,204 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {
   return r;
 }
 __device__ __forceinline__ uint32_t e4m3_pair(uint32_t lo, uint32_t hi) { return e4m3x2_to_half2(lo | hi << 8); }
+// Each half twice.  (Moves of halves: a multiplication can take either half of a register for both, where a byte permutation costs an
+// instruction; 32 sequences of 65536 positions 284 us instead of 290.)
+__device__ __forceinline__ void both_halves(uint32_t v, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tmov.b32 %0, {a, a};\n\tmov.b32 %1, {b, b};\n\t}" : "=r"(lo), "=r"(hi) : "r"(v));
+}
 
 // ---------------------------------------------------------------- few rows per sequence and key head: decoding
-// A CTA walks its piece of the pages.  A warp has half of every second page, 32 positions, in a ring of its own that cp.async fills, so
-// that no warp waits for another before the end of a unit, for 8 NT rows; mma.sync m16n8k16 in f16, whose big operand the lanes make
-// from the codes in registers, so that a row tile is as narrow as an MMA allows:
+// A CTA walks its piece of the pages.  A warp has every fourth page to itself, so that no warp waits for another before the end of a unit, for
+// 8 NT rows.  A page's two blocks come by two bulk copies into a ring of stages: the warp that has used up a stage asks for the page that
+// goes there next, whichever warp's that is.  mma.sync m16n8k16 in f16, whose big operand the lanes make from the codes in registers,
+// so that a row tile is as narrow as an MMA allows:
 //   scores:  positions (M) x rows (N) = K Q^T.  A lane has one group of 16 dimensions of two positions in each plane, whose scale it
 //            multiplies in; the MMAs' k index permutes the dimensions, alike in q.
 //   values:  dimensions (M) x rows (N) = V^T P^T.  A lane pairs the codes of two positions, a byte for each dimension; its D / 8 dimensions
 //            have one group scale.  The weights come from the scores' layout by an 8 x 8 transpose (movmatrix).
 // Which position an index of the scores stands for is chosen so that both reads of the rows of 32 bytes are free of bank conflicts: index i
 // of eight is position i ^ (i >> 2 & 1).
+// What bounds it is instructions, the conversions (half a clock's rate) first.
 constexpr int kDecodeExtra = 1;            // what a unit costs besides its pages, in pages
 constexpr float kFarBehind = 1.2676506e30f;   // 2^100 between the references of the two sums: the values' follows
-constexpr int kHalf = kKvPage / 2;         // positions of a warp's part of a page
+constexpr int kWarps = 4;
+constexpr int kStatusTimeout = 401;
 
 template <int D, int NT>
 struct Decode4Shape {
   static constexpr int kRows = 8 * NT;
-  static constexpr int kThreads = 128;
+  static constexpr int kThreads = 32 * kWarps;
   static constexpr int kBlocks = NT == 1 ? 3 : 2;          // per SM
-  static constexpr int kStages = D == 128 ? 3 : 5;
-  // of a stage and kind: [D / 64][32][32] codes, [32][D / 16] group scales, [32] scales
-  static constexpr int kCodes = kHalf * (D / 2), kGroups = kHalf * (D / kKv4Group), kKindBytes = kCodes + kGroups + kHalf * 4;
-  static constexpr int kStageBytes = 2 * kKindBytes;
-  static constexpr int kMerge = 2 * 8 * NT * D;                         // floats
-  static constexpr int kSmem = 4 * kStages * kStageBytes + kMerge * 4;
+  static constexpr int kStageBytes = 2 * Kv4Block<D>::kBytes;
+  static constexpr int kMerge = 2 * 8 * NT * D * 4;        // bytes
+  static constexpr int kRoom = (NT == 1 ? 74 : 110) * 1024 - kMerge;
+  static constexpr int kStages = kRoom / kStageBytes < 12 ? kRoom / kStageBytes : 12;
+  static constexpr int kSmem = kStages * kStageBytes + kMerge;
+};
+
+// How far the loads of a warp have come: pages `tile`, `tile` + 4, ... below `end` of a segment.
+struct LoadWalk {
+  const int32_t* table;                // of the segment's sequence, from the unit's first page on
+  int tile, end, head;
 };
 
 template <int D, int NT>
-__global__ void __launch_bounds__(Decode4Shape<D, NT>::kThreads, Decode4Shape<D, NT>::kBlocks) kv4_decode_kernel(const __grid_constant__ AttentionArgs a) {
+struct DecodeShared {
+  using Walk = Cursor<kKvPage, 8 * NT, kDecodeExtra>;
+  PlanShared plan;
+  uint64_t full[Decode4Shape<D, NT>::kStages];
+  int there[Decode4Shape<D, NT>::kStages];
+  int asked[Decode4Shape<D, NT>::kStages];       // loads of a stage so far
+  Walk load[kWarps];                   // the segment that a warp's loads are in
+  int skip[kWarps];                    // pages from its beginning to the warp's first there
+  float4 stat[kWarps][8 * NT];
+  volatile int failed;                 // a copy did not arrive in time
+};
+
+// Waits for a stage's copies, at most `limit` SM clocks, and not once another warp has waited in vain.  With a limit of one clock nothing counts as
+// there in time: pages are nearly always there before they are asked about, and a test of what follows must not depend on it.
+__device__ __forceinline__ bool landed(uint64_t* bar, uint32_t parity, volatile int* failed, long long limit) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  if (ok && limit > 1) return true;
+  const long long begun = clock64();
+  do {
+    if (*failed != 0) return false;
+    if (clock64() - begun > limit) {
+      *failed = 1;
+      return false;
+    }
+  } while (!mbar_try_wait(bar, parity));
+  return true;
+}
+
+template <int D, int NT>
+__global__ void __launch_bounds__(Decode4Shape<D, NT>::kThreads, Decode4Shape<D, NT>::kBlocks)
+kv4_decode_kernel(const __grid_constant__ AttentionArgs a, int* __restrict__ status, long long wait_limit) {
   using Shape = Decode4Shape<D, NT>;
   using Walk = Cursor<kKvPage, Shape::kRows, kDecodeExtra>;
+  using Block = Kv4Block<D>;
   constexpr int kRows = Shape::kRows, kStages = Shape::kStages, kPlanes = D / 64, kSteps = D / 16, kMmas = D / 16;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ PlanShared s_plan;
-  __shared__ float4 s_stat[4][8 * NT];
-  float* const s_merge = reinterpret_cast<float*>(smem + 4 * kStages * Shape::kStageBytes);
+  __shared__ DecodeShared<D, NT> sh;
+  float* const s_merge = reinterpret_cast<float*>(smem + kStages * Shape::kStageBytes);
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, c = lane % 4;
-  const int parity = warp / 2, half = warp % 2;          // which of a segment's pages, and of those which half
 
   pdl_wait();
   pdl_trigger();
   const Plan<kKvPage, kRows, kDecodeExtra> plan = {a.batch, a.cache.heads, a.group, a.window};
-  const long long total = plan.total(s_plan);
+  const long long total = plan.total(sh.plan);
   const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
   if (static_cast<int>(blockIdx.x) >= ctas) return;
   const long long w0 = piece_start(total, ctas, blockIdx.x), w1 = piece_start(total, ctas, blockIdx.x + 1);
-  plan.locate(s_plan, w0);
+  if (tid < kStages) {
+    mbar_init(&sh.full[tid], 1);
+    sh.asked[tid] = 0;
+    fence_barrier_init();
+  }
+  if (tid == 0) sh.failed = 0;
+  plan.locate(sh.plan, w0);                  // (ends with a barrier)
 
-  Walk load, use;
-  load.start(plan, s_plan, static_cast<int>(w1 - w0));
-  if (load.left <= 0) return;
-  use = load;
-  // The walk of this warp's loads: to its first page from `load` on that is `skip` pages ahead in its segment.
-  auto settle = [&](int skip) {
-    while (load.left > 0) {
-      const int n = load.tiles_here();
-      if (skip < n) {
-        if (skip > 0) load.advance(plan, skip);
-        return;
-      }
-      load.advance(plan, n);
-      skip = parity;
-    }
-  };
-  settle(parity);
-  auto entry_of = [&]() {
-    return load.left > 0 ? __ldg(a.batch.block_table + static_cast<long long>(load.b) * a.batch.max_pages + load.span.first + load.tile) : -1;
-  };
-  uint8_t* const ring = smem + warp * (kStages * Shape::kStageBytes);
-  const long long to_values = static_cast<long long>(a.cache.heads) * Kv4Block<D>::kBytes;
-  int stage_in = 0, stage_out = 0;           // of the page to ask for, of the page to work on
-  int entry = entry_of();                    // of the page to ask for next: read one page ahead
-  uint32_t here = 0u;                        // bit s: what stage s was asked for is there
-  auto ask = [&]() {
-    if (load.left > 0) {
-      const int stage = stage_in;
-      stage_in = stage_in + 1 == kStages ? 0 : stage_in + 1;
-      const bool there = entry >= 0 && entry < a.cache.num_pages;
-      here = there ? here | 1u << stage : here & ~(1u << stage);
-      if (there) {
-        const uint8_t* const k_block = kv4_block<D>(a.cache, entry, 0, load.head);
-        const uint32_t dst = smem_u32(ring) + stage * Shape::kStageBytes;
-#pragma unroll
-        for (int kind = 0; kind < 2; ++kind) {
-          const uint8_t* const from = k_block + (kind ? to_values : 0ll) + half * (kHalf * 32) + lane * 16;
-          const uint32_t to = dst + kind * Shape::kKindBytes + lane * 16;
-#pragma unroll
-          for (int p = 0; p < kPlanes; ++p) {
-            cp_async16(to + p * (kHalf * 32), from + p * kKv4Plane);
-            cp_async16(to + p * (kHalf * 32) + 512, from + p * kKv4Plane + 512);
-          }
+  Walk use;
+  use.start(plan, sh.plan, static_cast<int>(w1 - w0));
+  if (use.left <= 0) return;
+  // Pages of the piece are numbered: page p is warp p % 4's, in stage p % kStages.
+  if (lane == 0) {
+    sh.load[warp] = use;
+    sh.skip[warp] = warp;
+  }
+  __syncwarp();
+  LoadWalk walk = {nullptr, 0, 0, 0};
+  int entry = -1;                            // of the page to ask for next: read one page ahead
+  bool more = true;
+  // On to the walk's page, of the next segment that has any of this warp's.
+  auto settle = [&]() {
+    if (walk.tile >= walk.end) {
+      if (lane == 0) {
+        Walk& at = sh.load[warp];
+        int skip = sh.skip[warp];
+        while (at.left > 0 && skip >= at.tiles_here()) {
+          const int n = at.tiles_here();
+          skip -= n;
+          at.advance(plan, n);
         }
-        // group scales (D / 16 * 2 chunks) and scales (8 chunks) of both kinds
-        constexpr int kGroupChunks = Shape::kGroups / 16;
-        const int kind = lane / 16, l = lane % 16;
-        const uint8_t* const block = k_block + (kind ? to_values : 0ll);
-        const uint32_t to = dst + kind * Shape::kKindBytes + Shape::kCodes;
-        if (l < kGroupChunks) cp_async16(to + l * 16, block + Kv4Block<D>::kGroups + half * Shape::kGroups + l * 16);
-        if (l < 8) cp_async16(to + Shape::kGroups + l * 16, block + Kv4Block<D>::kScales + half * (kHalf * 4) + l * 16);
+        // (this lane's walk goes on behind the segment: skip counts from its end)
+        if (at.left > 0) {
+          const int n = at.tiles_here();
+          sh.skip[warp] = skip + (n - skip + kWarps - 1) / kWarps * kWarps - n;
+          walk = {a.batch.block_table + static_cast<long long>(at.b) * a.batch.max_pages + at.span.first, at.tile + skip, at.tile + n, at.head};
+          at.advance(plan, n);
+        } else {
+          walk.head = -1;
+        }
       }
-      if (load.tiles_here() > 2) {
-        load.advance(plan, 2);
-      } else {
-        load.advance(plan, load.tiles_here());
-        settle(parity);
-      }
-      entry = entry_of();
+      walk.table = reinterpret_cast<const int32_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(walk.table), 0));
+      walk.tile = __shfl_sync(0xffffffffu, walk.tile, 0);
+      walk.end = __shfl_sync(0xffffffffu, walk.end, 0);
+      walk.head = __shfl_sync(0xffffffffu, walk.head, 0);
+      more = walk.head >= 0;
     }
-    cp_async_commit();
+    if (more) entry = __ldg(walk.table + walk.tile);
   };
+  auto ask = [&](int stage) {
+    if (!more) return;
+    if (lane == 0) {
+      const bool there = entry >= 0 && entry < a.cache.num_pages;
+      sh.there[stage] = there;
+      ++sh.asked[stage];
+      if (there) {
+        mbar_arrive_expect_tx(&sh.full[stage], Shape::kStageBytes);
+        uint8_t* const to = smem + stage * Shape::kStageBytes;
+        const uint64_t policy = l2_policy_evict_first();
+        bulk_load(to, kv4_block<D>(a.cache, entry, 0, walk.head), Block::kBytes, &sh.full[stage], policy);
+        bulk_load(to + Block::kBytes, kv4_block<D>(a.cache, entry, 1, walk.head), Block::kBytes, &sh.full[stage], policy);
+      } else {
+        mbar_arrive(&sh.full[stage]);
+      }
+    }
+    walk.tile += kWarps;
+    settle();
+  };
+  settle();
+  // A warp asks for the pages that follow its own by a round of stages, so at first for its own among the first kStages, then for those.
+  constexpr int kFirst = kStages / kWarps;   // whole rounds of warps among the first stages
 #pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) ask();
+  for (int i = 0; i < kFirst; ++i) ask(i * kWarps + warp);
+  if constexpr (kStages % kWarps != 0) {
+    if (warp < kStages % kWarps) ask(kFirst * kWarps + warp);
+    // Page p + kStages is warp (p + kStages) % 4's: from here on this warp's walk is that of another, which has just asked for its first ones.
+    __syncthreads();
+    const int other = (warp + kStages) % kWarps;
+    const Walk its_load = sh.load[other];
+    const int its_skip = sh.skip[other];
+    LoadWalk* const hand = reinterpret_cast<LoadWalk*>(s_merge);
+    int* const hand_entry = reinterpret_cast<int*>(hand + kWarps);
+    if (lane == 0) {
+      hand[warp] = walk;
+      hand_entry[2 * warp] = entry;
+      hand_entry[2 * warp + 1] = more;
+    }
+    __syncthreads();
+    walk = hand[other];
+    entry = hand_entry[2 * other];
+    more = hand_entry[2 * other + 1] != 0;
+    if (lane == 0) {
+      sh.load[warp] = its_load;
+      sh.skip[warp] = its_skip;
+    }
+    __syncthreads();
+  }
+  int page0 = 0;                             // number of the segment's first page
+  int stage = warp % kStages;                // of this warp's next page, and the parity of its use
+  uint32_t parity = 0;
+  bool lost = false;                         // a page of this warp did not come in time
+  static_assert(kStages >= kWarps, "a stage for every warp's page");
 
   // This lane's positions of each 16: t0 and t0 + 8; its rows of the scores: 8 t + 2 c and 8 t + 2 c + 1.
   const int t0 = g ^ (g >> 2 & 1), v0 = (2 * c) ^ (c >> 1), v1 = (2 * c + 1) ^ (c >> 1);
@@ -199,195 +278,220 @@ __global__ void __launch_bounds__(Decode4Shape<D, NT>::kThreads, Decode4Shape<D,
         for (int e = 0; e < 4; ++e) o[t][j][e] = 0.0f;
     }
 
-    for (int tile = parity; tile < tiles; tile += 2) {
-      cp_async_wait<kStages - 2>();
-      __syncwarp();
-      ask();
-      const int stage = stage_out;
-      stage_out = stage_out + 1 == kStages ? 0 : stage_out + 1;
-      if (!(here >> stage & 1u)) continue;
-      uint8_t* const keys = ring + stage * Shape::kStageBytes;
-      uint8_t* const values = keys + Shape::kKindBytes;
-      float* const k_scale = reinterpret_cast<float*>(keys + Shape::kCodes + Shape::kGroups);
-      float* const v_scale = reinterpret_cast<float*>(values + Shape::kCodes + Shape::kGroups);
-      const int position0 = (use.span.first + use.tile + tile) * kKvPage + half * kHalf;
-      const bool plain = position0 >= all_low && position0 + kHalf - 1 <= all_high;    // every row sees every position
-      if (!plain) {
-        // What a row does not see must not reach its sums, and zero times NaN is NaN: values of positions that no row sees become zeros, and
-        // where some rows see a value that is not finite, the NaN goes by way of its score to those rows alone.  (Codes are always finite.)
-        const int position = position0 + lane;
-        uint32_t* const groups = reinterpret_cast<uint32_t*>(values + Shape::kCodes) + lane * (D / 64);
-        uint32_t over = 0u;
-#pragma unroll
-        for (int i = 0; i < D / 64; ++i) over |= (groups[i] & 0x7f7f7f7fu) + 0x01010101u;
-        const bool bad = (over & 0x80808080u) != 0u || !(fabsf(v_scale[lane]) <= 3.402823466e38f);
-        if (bad || position < any_low || position > any_high) {
-#pragma unroll
-          for (int i = 0; i < D / 64; ++i) groups[i] = 0u;
-          v_scale[lane] = 1.0f;
-          if (bad) k_scale[lane] = __int_as_float(0x7fffffff);
-        }
-        __syncwarp();
-      }
-      float x[2][NT][4];                     // element e of block b: position 16 b + t0 + 8 (e / 2), row 2 c + e % 2
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        float part[kPlanes][NT][4];          // chains of MMAs
-#pragma unroll
-        for (int p = 0; p < kPlanes; ++p) {
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) part[p][t][e] = 0.0f;
-          const uint2 w = *reinterpret_cast<const uint2*>(keys + p * (kHalf * 32) + (16 * b + t0) * 32 + c * 8);
-          const uint2 v = *reinterpret_cast<const uint2*>(keys + p * (kHalf * 32) + (16 * b + t0 + 8) * 32 + c * 8);
-          const uint8_t* const group = keys + Shape::kCodes + (16 * b + t0) * kSteps + 4 * p + c;
-          const uint32_t both = e4m3_pair(group[0], group[8 * kSteps]);
-          const uint32_t sw = __byte_perm(both, both, 0x1010), sv = __byte_perm(both, both, 0x3232);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t wi = i < 2 ? w.x : w.y, vi = i < 2 ? v.x : v.y;
-            const uint32_t ka[4] = {hmul2_bits(i % 2 ? e2m1x2_to_half2<2>(wi) : e2m1x2_to_half2<0>(wi), sw), hmul2_bits(i % 2 ? e2m1x2_to_half2<2>(vi) : e2m1x2_to_half2<0>(vi), sv),
-                                    hmul2_bits(i % 2 ? e2m1x2_to_half2<3>(wi) : e2m1x2_to_half2<1>(wi), sw), hmul2_bits(i % 2 ? e2m1x2_to_half2<3>(vi) : e2m1x2_to_half2<1>(vi), sv)};
-#pragma unroll
-            for (int t = 0; t < NT; ++t) mma_f16(part[p][t], ka, qb[t][4 * p + i][0], qb[t][4 * p + i][1]);
-          }
-        }
-        const float ks[2] = {k_scale[16 * b + t0], k_scale[16 * b + t0 + 8]};
+    const int begin = (warp - page0) & (kWarps - 1);
+    for (int tile = begin; tile < tiles; tile += kWarps) {
+      if (lost || !__all_sync(0xffffffffu, landed(&sh.full[stage], parity, &sh.failed, wait_limit))) {
+        // Not in time, for this warp or another: the rows become NaN, and nothing more is asked for, since the stage may still be written.
+        lost = true;
+        more = false;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float sum = part[0][t][e];
-            if constexpr (kPlanes == 2) sum += part[1][t][e];
-            x[b][t][e] = sum * (ks[e / 2] * unit[t][e % 2]);
+          for (int i = 0; i < 2; ++i) {
+            l[t][i] = __int_as_float(0x7fffffff);
+            n[t][i] = 0.0f;
           }
+        break;
       }
-      if (!plain) {
+      uint8_t* const keys = smem + stage * Shape::kStageBytes;
+      uint8_t* const values = keys + Block::kBytes;
+      float* const k_scale = reinterpret_cast<float*>(keys + Block::kScales);
+      float* const v_scale = reinterpret_cast<float*>(values + Block::kScales);
+      const int position0 = (use.span.first + use.tile + tile) * kKvPage;
+      const bool plain = position0 >= all_low && position0 + kKvPage - 1 <= all_high;    // every row sees every position
+      if (sh.there[stage]) {
+        if (!plain) {
+          // What a row does not see must not reach its sums, and zero times NaN is NaN: values of positions that no row sees become zeros,
+          // and where some rows see a value that is not finite, the NaN goes by way of its score to those rows alone.  (Codes are always
+          // finite.)
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+          for (int at = lane; at < kKvPage; at += 32) {
+            uint32_t* const groups = reinterpret_cast<uint32_t*>(values + Block::kGroups) + at * (D / 64);
+            uint32_t over = 0u;
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i) over |= (groups[i] & 0x7f7f7f7fu) + 0x01010101u;
+            const bool bad = (over & 0x80808080u) != 0u || !(fabsf(v_scale[at]) <= 3.402823466e38f);
+            if (bad || position0 + at < any_low || position0 + at > any_high) {
+#pragma unroll
+              for (int i = 0; i < D / 64; ++i) groups[i] = 0u;
+              v_scale[at] = 1.0f;
+              if (bad) k_scale[at] = __int_as_float(0x7fffffff);
+            }
+          }
+          fence_proxy_async_smem();          // in front of the copy that comes here next
+          __syncwarp();
+        }
+        float x[4][NT][4];                   // element e of block b: position 16 b + t0 + 8 (e / 2), row 2 c + e % 2
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          float part[kPlanes][NT][4];        // chains of MMAs
+#pragma unroll
+          for (int p = 0; p < kPlanes; ++p) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) part[p][t][e] = 0.0f;
+            const uint2 w = *reinterpret_cast<const uint2*>(keys + p * kKv4Plane + (16 * b + t0) * 32 + c * 8);
+            const uint2 v = *reinterpret_cast<const uint2*>(keys + p * kKv4Plane + (16 * b + t0 + 8) * 32 + c * 8);
+            const uint8_t* const group = keys + Block::kGroups + (16 * b + t0) * kSteps + 4 * p + c;
+            uint32_t sw, sv;
+            both_halves(e4m3_pair(group[0], group[8 * kSteps]), sw, sv);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t wi = i < 2 ? w.x : w.y, vi = i < 2 ? v.x : v.y;
+              const uint32_t ka[4] = {hmul2_bits(i % 2 ? e2m1x2_to_half2<2>(wi) : e2m1x2_to_half2<0>(wi), sw), hmul2_bits(i % 2 ? e2m1x2_to_half2<2>(vi) : e2m1x2_to_half2<0>(vi), sv),
+                                      hmul2_bits(i % 2 ? e2m1x2_to_half2<3>(wi) : e2m1x2_to_half2<1>(wi), sw), hmul2_bits(i % 2 ? e2m1x2_to_half2<3>(vi) : e2m1x2_to_half2<1>(vi), sv)};
+#pragma unroll
+              for (int t = 0; t < NT; ++t) mma_f16(part[p][t], ka, qb[t][4 * p + i][0], qb[t][4 * p + i][1]);
+            }
+          }
+          const float ks[2] = {k_scale[16 * b + t0], k_scale[16 * b + t0 + 8]};
 #pragma unroll
           for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const int position = position0 + 16 * b + t0 + 8 * (e / 2);
-              if (position < low[t][e % 2] || position > high[t][e % 2]) x[b][t][e] = -INFINITY;
+              float sum = part[0][t][e];
+              if constexpr (kPlanes == 2) sum += part[1][t][e];
+              x[b][t][e] = sum * (ks[e / 2] * unit[t][e % 2]);
             }
-      }
-      bool grown = false, late = false;
-      float top[NT][2];
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          top[t][i] = fmaxf(fmaxf(x[0][t][i], x[0][t][2 + i]), fmaxf(x[1][t][i], x[1][t][2 + i]));
-          grown |= top[t][i] > m[t][i] + kSumGrowth;
         }
-      if (__any_sync(0xffffffffu, grown)) {
-        // a row's sum in this lane follows its scores once they are 2^16 above the reference; the lanes meet at the unit's end
+        if (!plain) {
+#pragma unroll
+          for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int position = position0 + 16 * b + t0 + 8 * (e / 2);
+                if (position < low[t][e % 2] || position > high[t][e % 2]) x[b][t][e] = -INFINITY;
+              }
+        }
+        bool grown = false, late = false;
+        float top[NT][2];
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            if (top[t][i] > m[t][i] + kSumGrowth) {
-              l[t][i] *= ex2(m[t][i] - top[t][i]);
-              m[t][i] = top[t][i];
-              up[t][i] = n[t][i] == -INFINITY ? 0.0f : ex2(top[t][i] - n[t][i] + kHeadroom);
-              late |= up[t][i] > kFarBehind;
-            }
+            top[t][i] = fmaxf(x[0][t][i], x[0][t][2 + i]);
+#pragma unroll
+            for (int b = 1; b < 4; ++b) top[t][i] = fmaxf(top[t][i], fmaxf(x[b][t][i], x[b][t][2 + i]));
+            grown |= top[t][i] > m[t][i] + kSumGrowth;
           }
-      }
-      float pv[2][NT][4];                    // weights times the values' scales
+        if (__any_sync(0xffffffffu, grown)) {
+          // a row's sum in this lane follows its scores once they are 2^16 above the reference; the lanes meet at the unit's end
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const float vs[2] = {v_scale[16 * b + t0], v_scale[16 * b + t0 + 8]};
+          for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const float m_ref[2] = {finite_or_zero(m[t][0]), finite_or_zero(m[t][1])};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) pv[b][t][e] = ex2(x[b][t][e] - m_ref[e % 2]);
-          l[t][0] += pv[b][t][0] + pv[b][t][2];
-          l[t][1] += pv[b][t][1] + pv[b][t][3];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) pv[b][t][e] *= vs[e / 2];
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          top[t][i] = fmaxf(fmaxf(pv[0][t][i], pv[0][t][2 + i]), fmaxf(pv[1][t][i], pv[1][t][2 + i]));
-          late |= top[t][i] * up[t][i] > 32768.0f || (up[t][i] == 0.0f && top[t][i] > 0.0f);
-        }
-      if (__any_sync(0xffffffffu, late)) {
-        // the reference of the values' sum follows, in all lanes of a row alike
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          float fade[2];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float most = m[t][i] + fmaxf(lg2(top[t][i]), -90.0f);      // (never further behind: a value may be zero)
-#pragma unroll
-            for (int d = 4; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-            fade[i] = 1.0f;
-            if (most > n[t][i] + kGrowth) {
-              fade[i] = ex2(n[t][i] - most);
-              n[t][i] = most;
+            for (int i = 0; i < 2; ++i) {
+              if (top[t][i] > m[t][i] + kSumGrowth) {
+                l[t][i] *= ex2(m[t][i] - top[t][i]);
+                m[t][i] = top[t][i];
+                up[t][i] = n[t][i] == -INFINITY ? 0.0f : ex2(top[t][i] - n[t][i] + kHeadroom);
+                late |= up[t][i] > kFarBehind;
+              }
             }
-            up[t][i] = n[t][i] == -INFINITY || m[t][i] == -INFINITY ? 0.0f : ex2(m[t][i] - n[t][i] + kHeadroom);
-          }
-#pragma unroll
-          for (int j = 0; j < kMmas; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[t][j][e] *= fade[e % 2];
         }
-      }
+        // weights, then those times the values' scales
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        uint32_t pb[NT][2];
+        for (int b = 0; b < 4; ++b) {
+          const float vs[2] = {v_scale[16 * b + t0], v_scale[16 * b + t0 + 8]};
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[b][t][e] = ex2(x[b][t][e] - finite_or_zero(m[t][e % 2]));
+            l[t][0] += x[b][t][0] + x[b][t][2];
+            l[t][1] += x[b][t][1] + x[b][t][3];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[b][t][e] *= vs[e / 2];
+          }
+        }
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int u = 0; u < 2; ++u) pb[t][u] = transposed(pack_half2(pv[b][t][2 * u] * up[t][0], pv[b][t][2 * u + 1] * up[t][1]));
-        uint32_t even[2][D / 64], odd[2][D / 64], scale[2];
+          for (int i = 0; i < 2; ++i) {
+            top[t][i] = fmaxf(x[0][t][i], x[0][t][2 + i]);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int at0 = 16 * b + 8 * u + v0, at1 = 16 * b + 8 * u + v1;
-          const uint8_t* const groups = values + Shape::kCodes + (D == 128 ? g : g / 2);
-          scale[u] = e4m3_pair(groups[at0 * kSteps], groups[at1 * kSteps]);
-          if constexpr (D == 128) {
-            const uint8_t* const plane = values + g / 4 * (kHalf * 32) + g % 4 * 8;
-            const uint2 w = *reinterpret_cast<const uint2*>(plane + at0 * 32), r = *reinterpret_cast<const uint2*>(plane + at1 * 32);
-            even[u][0] = w.x; even[u][1] = w.y;
-            odd[u][0] = r.x; odd[u][1] = r.y;
-          } else {
-            even[u][0] = *reinterpret_cast<const uint32_t*>(values + at0 * 32 + g * 4);
-            odd[u][0] = *reinterpret_cast<const uint32_t*>(values + at1 * 32 + g * 4);
+            for (int b = 1; b < 4; ++b) top[t][i] = fmaxf(top[t][i], fmaxf(x[b][t][i], x[b][t][2 + i]));
+            late |= top[t][i] * up[t][i] > 32768.0f || (up[t][i] == 0.0f && top[t][i] > 0.0f);
+          }
+        if (__any_sync(0xffffffffu, late)) {
+          // the reference of the values' sum follows, in all lanes of a row alike
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            float fade[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              float most = m[t][i] + fmaxf(lg2(top[t][i]), -90.0f);      // (never further behind: a value may be zero)
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+              fade[i] = 1.0f;
+              if (most > n[t][i] + kGrowth) {
+                fade[i] = ex2(n[t][i] - most);
+                n[t][i] = most;
+              }
+              up[t][i] = n[t][i] == -INFINITY || m[t][i] == -INFINITY ? 0.0f : ex2(m[t][i] - n[t][i] + kHeadroom);
+            }
+#pragma unroll
+            for (int j = 0; j < kMmas; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[t][j][e] *= fade[e % 2];
           }
         }
 #pragma unroll
-        for (int w = 0; w < D / 64; ++w) {
-          // bytes that hold one dimension of both positions: dimensions 2 i, and 2 i + 1, of the word's eight
-          uint32_t first_dims[2], second_dims[2];
+        for (int b = 0; b < 4; ++b) {
+          uint32_t pb[NT][2];
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) pb[t][u] = transposed(pack_half2(x[b][t][2 * u] * up[t][0], x[b][t][2 * u + 1] * up[t][1]));
+          uint32_t even[2][D / 64], odd[2][D / 64], scale[2];
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            first_dims[u] = (even[u][w] & 0x0f0f0f0fu) | (odd[u][w] << 4 & 0xf0f0f0f0u);
-            second_dims[u] = (even[u][w] >> 4 & 0x0f0f0f0fu) | (odd[u][w] & 0xf0f0f0f0u);
+            const int at0 = 16 * b + 8 * u + v0, at1 = 16 * b + 8 * u + v1;
+            const uint8_t* const groups = values + Block::kGroups + (D == 128 ? g : g / 2);
+            scale[u] = e4m3_pair(groups[at0 * kSteps], groups[at1 * kSteps]);
+            if constexpr (D == 128) {
+              const uint8_t* const plane = values + g / 4 * kKv4Plane + g % 4 * 8;
+              const uint2 w = *reinterpret_cast<const uint2*>(plane + at0 * 32), r = *reinterpret_cast<const uint2*>(plane + at1 * 32);
+              even[u][0] = w.x; even[u][1] = w.y;
+              odd[u][0] = r.x; odd[u][1] = r.y;
+            } else {
+              even[u][0] = *reinterpret_cast<const uint32_t*>(values + at0 * 32 + g * 4);
+              odd[u][0] = *reinterpret_cast<const uint32_t*>(values + at1 * 32 + g * 4);
+            }
           }
-          auto product = [&](auto byte) {
-            constexpr int kByte = decltype(byte)::value;
-            const uint32_t va[4] = {hmul2_bits(e2m1x2_to_half2<kByte>(first_dims[0]), scale[0]), hmul2_bits(e2m1x2_to_half2<kByte>(second_dims[0]), scale[0]),
-                                    hmul2_bits(e2m1x2_to_half2<kByte>(first_dims[1]), scale[1]), hmul2_bits(e2m1x2_to_half2<kByte>(second_dims[1]), scale[1])};
 #pragma unroll
-            for (int t = 0; t < NT; ++t) mma_f16(o[t][4 * w + kByte], va, pb[t][0], pb[t][1]);
-          };
-          product(std::integral_constant<int, 0>{});
-          product(std::integral_constant<int, 1>{});
-          product(std::integral_constant<int, 2>{});
-          product(std::integral_constant<int, 3>{});
+          for (int w = 0; w < D / 64; ++w) {
+            // bytes that hold one dimension of both positions: dimensions 2 i, and 2 i + 1, of the word's eight
+            uint32_t first_dims[2], second_dims[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              first_dims[u] = (even[u][w] & 0x0f0f0f0fu) | (odd[u][w] << 4 & 0xf0f0f0f0u);
+              second_dims[u] = (even[u][w] >> 4 & 0x0f0f0f0fu) | (odd[u][w] & 0xf0f0f0f0u);
+            }
+            auto product = [&](auto byte) {
+              constexpr int kByte = decltype(byte)::value;
+              const uint32_t va[4] = {hmul2_bits(e2m1x2_to_half2<kByte>(first_dims[0]), scale[0]), hmul2_bits(e2m1x2_to_half2<kByte>(second_dims[0]), scale[0]),
+                                      hmul2_bits(e2m1x2_to_half2<kByte>(first_dims[1]), scale[1]), hmul2_bits(e2m1x2_to_half2<kByte>(second_dims[1]), scale[1])};
+#pragma unroll
+              for (int t = 0; t < NT; ++t) mma_f16(o[t][4 * w + kByte], va, pb[t][0], pb[t][1]);
+            };
+            product(std::integral_constant<int, 0>{});
+            product(std::integral_constant<int, 1>{});
+            product(std::integral_constant<int, 2>{});
+            product(std::integral_constant<int, 3>{});
+          }
         }
       }
+      __syncwarp();
+      ask(stage);
+      stage += kWarps;
+      if (stage >= kStages) {
+        stage -= kStages;
+        parity ^= 1u;
+      }
     }
+    page0 += tiles;
 
     // ---- the segment's end: lanes, then the four warps, then the unit's other pieces
 #pragma unroll
@@ -400,7 +504,7 @@ __global__ void __launch_bounds__(Decode4Shape<D, NT>::kThreads, Decode4Shape<D,
         float sum = l[t][i] * ex2(m[t][i] - finite_or_zero(top));
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        if (g == 0) s_stat[warp][8 * t + 2 * c + i] = make_float4(top, sum, n[t][i], 0.0f);
+        if (g == 0) sh.stat[warp][8 * t + 2 * c + i] = make_float4(top, sum, n[t][i], 0.0f);
       }
     __syncthreads();
 #pragma unroll
@@ -411,12 +515,12 @@ __global__ void __launch_bounds__(Decode4Shape<D, NT>::kThreads, Decode4Shape<D,
         float m_all = -INFINITY, n_all = -INFINITY, l_all = 0.0f;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          m_all = fmaxf(m_all, s_stat[w][8 * t + 2 * c + i].x);
-          n_all = fmaxf(n_all, s_stat[w][8 * t + 2 * c + i].z);
+          m_all = fmaxf(m_all, sh.stat[w][8 * t + 2 * c + i].x);
+          n_all = fmaxf(n_all, sh.stat[w][8 * t + 2 * c + i].z);
         }
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          const float4 st = s_stat[w][8 * t + 2 * c + i];
+          const float4 st = sh.stat[w][8 * t + 2 * c + i];
           l_all += st.y * ex2(st.x - finite_or_zero(m_all));
         }
         f[i] = ex2(n[t][i] - finite_or_zero(n_all));
@@ -489,15 +593,24 @@ __global__ void __launch_bounds__(Decode4Shape<D, NT>::kThreads, Decode4Shape<D,
       if (tid == 0) {
         const bool is_last = atomicAdd(a.tickets + parts.first, 1) == parts.last - parts.first;
         if (is_last) a.tickets[parts.first] = 0;
-        s_plan.last = is_last;
+        sh.plan.last = is_last;
       }
       __syncthreads();
-      if (s_plan.last) {
+      if (sh.plan.last) {
         __threadfence();
         join_parts<D, kRows>(a, use.s.first, r0, use.head, rows, ctas, parts, warp, 4);
       }
     }
     use.advance(plan, tiles);
+  }
+  if (sh.failed != 0) {
+    // Copies may still be on their way: this CTA's memory must not be the next one's before they have landed.
+    __syncthreads();
+    if (tid == 0) {
+      for (int i = 0; i < kStages; ++i)
+        if (sh.asked[i] > 0) mbar_wait_landed(&sh.full[i], (sh.asked[i] - 1) & 1);
+      atomicExch(status, kStatusTimeout);
+    }
   }
 }
 
@@ -527,12 +640,12 @@ bool take_scratch(AttentionArgs& a, Device& d, size_t partial, cudaStream_t st, 
 }
 
 template <int D, int NT>
-int launch_decode(AttentionArgs a, Device& d, int sms, cudaStream_t st) {
+int launch_decode(AttentionArgs a, Device& d, int sms, long long wait_limit, cudaStream_t st) {
   using Shape = Decode4Shape<D, NT>;
   const int ctas = sms * Shape::kBlocks;
   int rc = SYFI_KV4_OK;
   if (!take_scratch(a, d, 2ull * ctas * Shape::kRows * (D + 4) * sizeof(float), st, &rc)) return rc;
-  return launch_dependent(kv4_decode_kernel<D, NT>, dim3(ctas), dim3(Shape::kThreads), Shape::kSmem, st, a) == cudaSuccess
+  return launch_dependent(kv4_decode_kernel<D, NT>, dim3(ctas), dim3(Shape::kThreads), Shape::kSmem, st, a, d.status, wait_limit) == cudaSuccess
              ? SYFI_KV4_OK : kv_fail(SYFI_KV4_ERR_CUDA, "attention kernel launch failed");
 }
 
@@ -599,8 +712,8 @@ extern "C" int syfi_kv4_attention(const void* q, int64_t q_stride, const void* c
     if (!take_scratch(a, d, kv4_chunk_partial_bytes(head_dim, sms), st, &rc)) return rc;
     return launch_kv4_chunk(a, head_dim, sms, d.status, wait_limit, st) == cudaSuccess ? SYFI_KV4_OK : kv_fail(SYFI_KV4_ERR_CUDA, "attention kernel launch failed");
   }
-  if (head_dim == 128) return rows <= 8 ? launch_decode<128, 1>(a, d, sms, st) : launch_decode<128, 2>(a, d, sms, st);
-  return rows <= 8 ? launch_decode<64, 1>(a, d, sms, st) : launch_decode<64, 2>(a, d, sms, st);
+  if (head_dim == 128) return rows <= 8 ? launch_decode<128, 1>(a, d, sms, wait_limit, st) : launch_decode<128, 2>(a, d, sms, wait_limit, st);
+  return rows <= 8 ? launch_decode<64, 1>(a, d, sms, wait_limit, st) : launch_decode<64, 2>(a, d, sms, wait_limit, st);
 }
 
 // Test hook for the bounded waits, no part of the interface: a CTA of the next attention call's kernel on the current device may

@@ -557,7 +557,7 @@ def test_rows_that_tiny_values_decide(q_len, kv_len, octaves, D, pkg, kv4):
     assert not _attend(pkg, inputs).isnan().any()
 
 
-@pytest.mark.parametrize("q_lens,kv_lens,D", [([300, 5], [3000, 9000], 128), ([6] * 9, [4000] * 9, 64)])
+@pytest.mark.parametrize("q_lens,kv_lens,D", [([300, 5], [3000, 9000], 128), ([6] * 9, [4000] * 9, 64), ([1] * 5, [9000, 300, 64, 20000, 1], 128), ([3] * 9, [4000] * 9, 64)])
 def test_bounded_waits_run_out(q_lens, kv_lens, D, pkg, kv4):
     """A wait that runs out ends its call with a status; rows that were not computed are NaN, all others are what they are, and
     the next call is undisturbed."""
