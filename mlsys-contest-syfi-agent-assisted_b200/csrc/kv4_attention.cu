@@ -73,25 +73,23 @@ struct DecodeShared {
   PlanShared plan;
   uint64_t full[Decode4Shape<D, NT>::kStages];
   int there[Decode4Shape<D, NT>::kStages];
-  int asked[Decode4Shape<D, NT>::kStages];       // loads of a stage so far
+  volatile int holds[Decode4Shape<D, NT>::kStages];   // number of the page that a stage was last asked for
   Walk load[kWarps];                   // the segment that a warp's loads are in
   int skip[kWarps];                    // pages from its beginning to the warp's first there
   float4 stat[kWarps][8 * NT];
   volatile int failed;                 // a copy did not arrive in time
 };
 
-// Waits for a stage's copies, at most `limit` SM clocks, and not once another warp has waited in vain.  With a limit of one clock nothing counts as
-// there in time: pages are nearly always there before they are asked about, and a test of what follows must not depend on it.
-__device__ __forceinline__ bool landed(uint64_t* bar, uint32_t parity, volatile int* failed, long long limit) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  if (ok && limit > 1) return true;
+// Both addresses and the size multiples of 16 bytes; completion is counted on an mbarrier.
+__device__ __forceinline__ void bulk_copy(void* to, const void* from, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(to)), "l"(from), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+// Waits for a page's copies, at most `limit` SM clocks, and not once another warp has waited in vain.  Warps drift apart, and a phase's parity
+// says only which of two it is: so first the stage must have been asked for this very page (`holds`), which it is when the page in front of it
+// has been used up.  With a limit of one clock nothing counts as there in time: pages are nearly always there before they are asked about, and
+// a test of what follows must not depend on it.
+__device__ __forceinline__ bool landed(uint64_t* bar, uint32_t parity, const volatile int* holds, int page, volatile int* failed, long long limit) {
+  if (*holds == page && limit > 1 && mbar_try_wait(bar, parity)) return true;
   const long long begun = clock64();
   do {
     if (*failed != 0) return false;
@@ -99,7 +97,7 @@ __device__ __forceinline__ bool landed(uint64_t* bar, uint32_t parity, volatile 
       *failed = 1;
       return false;
     }
-  } while (!mbar_try_wait(bar, parity));
+  } while (*holds != page || !mbar_try_wait(bar, parity));
   return true;
 }
 
@@ -124,7 +122,7 @@ kv4_decode_kernel(const __grid_constant__ AttentionArgs a, int* __restrict__ sta
   const long long w0 = piece_start(total, ctas, blockIdx.x), w1 = piece_start(total, ctas, blockIdx.x + 1);
   if (tid < kStages) {
     mbar_init(&sh.full[tid], 1);
-    sh.asked[tid] = 0;
+    sh.holds[tid] = -1;
     fence_barrier_init();
   }
   if (tid == 0) sh.failed = 0;
@@ -171,18 +169,17 @@ kv4_decode_kernel(const __grid_constant__ AttentionArgs a, int* __restrict__ sta
     }
     if (more) entry = __ldg(walk.table + walk.tile);
   };
-  auto ask = [&](int stage) {
+  auto ask = [&](int stage, int page) {
     if (!more) return;
     if (lane == 0) {
       const bool there = entry >= 0 && entry < a.cache.num_pages;
       sh.there[stage] = there;
-      ++sh.asked[stage];
+      sh.holds[stage] = page;
       if (there) {
         mbar_arrive_expect_tx(&sh.full[stage], Shape::kStageBytes);
         uint8_t* const to = smem + stage * Shape::kStageBytes;
-        const uint64_t policy = l2_policy_evict_first();
-        bulk_load(to, kv4_block<D>(a.cache, entry, 0, walk.head), Block::kBytes, &sh.full[stage], policy);
-        bulk_load(to + Block::kBytes, kv4_block<D>(a.cache, entry, 1, walk.head), Block::kBytes, &sh.full[stage], policy);
+        bulk_copy(to, kv4_block<D>(a.cache, entry, 0, walk.head), Block::kBytes, &sh.full[stage]);
+        bulk_copy(to + Block::kBytes, kv4_block<D>(a.cache, entry, 1, walk.head), Block::kBytes, &sh.full[stage]);
       } else {
         mbar_arrive(&sh.full[stage]);
       }
@@ -194,9 +191,9 @@ kv4_decode_kernel(const __grid_constant__ AttentionArgs a, int* __restrict__ sta
   // A warp asks for the pages that follow its own by a round of stages, so at first for its own among the first kStages, then for those.
   constexpr int kFirst = kStages / kWarps;   // whole rounds of warps among the first stages
 #pragma unroll
-  for (int i = 0; i < kFirst; ++i) ask(i * kWarps + warp);
+  for (int i = 0; i < kFirst; ++i) ask(i * kWarps + warp, i * kWarps + warp);
   if constexpr (kStages % kWarps != 0) {
-    if (warp < kStages % kWarps) ask(kFirst * kWarps + warp);
+    if (warp < kStages % kWarps) ask(kFirst * kWarps + warp, kFirst * kWarps + warp);
     // Page p + kStages is warp (p + kStages) % 4's: from here on this warp's walk is that of another, which has just asked for its first ones.
     __syncthreads();
     const int other = (warp + kStages) % kWarps;
@@ -280,7 +277,7 @@ kv4_decode_kernel(const __grid_constant__ AttentionArgs a, int* __restrict__ sta
 
     const int begin = (warp - page0) & (kWarps - 1);
     for (int tile = begin; tile < tiles; tile += kWarps) {
-      if (lost || !__all_sync(0xffffffffu, landed(&sh.full[stage], parity, &sh.failed, wait_limit))) {
+      if (lost || !__all_sync(0xffffffffu, landed(&sh.full[stage], parity, &sh.holds[stage], page0 + tile, &sh.failed, wait_limit))) {
         // Not in time, for this warp or another: the rows become NaN, and nothing more is asked for, since the stage may still be written.
         lost = true;
         more = false;
@@ -484,7 +481,7 @@ kv4_decode_kernel(const __grid_constant__ AttentionArgs a, int* __restrict__ sta
         }
       }
       __syncwarp();
-      ask(stage);
+      ask(stage, page0 + tile + kStages);
       stage += kWarps;
       if (stage >= kStages) {
         stage -= kStages;
@@ -608,7 +605,7 @@ kv4_decode_kernel(const __grid_constant__ AttentionArgs a, int* __restrict__ sta
     __syncthreads();
     if (tid == 0) {
       for (int i = 0; i < kStages; ++i)
-        if (sh.asked[i] > 0) mbar_wait_landed(&sh.full[i], (sh.asked[i] - 1) & 1);
+        if (sh.holds[i] >= 0) mbar_wait_landed(&sh.full[i], sh.holds[i] / kStages & 1);
       atomicExch(status, kStatusTimeout);
     }
   }
