@@ -44,7 +44,7 @@ __device__ __forceinline__ void both_halves(uint32_t v, uint32_t& lo, uint32_t& 
 // Which position an index of the scores stands for is chosen so that both reads of the rows of 32 bytes are free of bank conflicts: index i
 // of eight is position i ^ (i >> 2 & 1).
 // What bounds it is instructions, the conversions (half a clock's rate) first.
-constexpr int kDecodeExtra = 1;            // what a unit costs besides its pages, in pages
+constexpr int kDecodeExtra = 6;            // what a unit costs besides its pages, in pages (see below)
 constexpr float kFarBehind = 1.2676506e30f;   // 2^100 between the references of the two sums: the values' follows
 constexpr int kWarps = 4;
 constexpr int kStatusTimeout = 401;
@@ -80,10 +80,6 @@ struct DecodeShared {
   volatile int failed;                 // a copy did not arrive in time
 };
 
-// Both addresses and the size multiples of 16 bytes; completion is counted on an mbarrier.
-__device__ __forceinline__ void bulk_copy(void* to, const void* from, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(to)), "l"(from), "r"(bytes), "r"(smem_u32(bar)) : "memory");
-}
 // Waits for a page's copies, at most `limit` SM clocks, and not once another warp has waited in vain.  Warps drift apart, and a phase's parity
 // says only which of two it is: so first the stage must have been asked for this very page (`holds`), which it is when the page in front of it
 // has been used up.  With a limit of one clock nothing counts as there in time: pages are nearly always there before they are asked about, and
@@ -178,8 +174,9 @@ kv4_decode_kernel(const __grid_constant__ AttentionArgs a, int* __restrict__ sta
       if (there) {
         mbar_arrive_expect_tx(&sh.full[stage], Shape::kStageBytes);
         uint8_t* const to = smem + stage * Shape::kStageBytes;
-        bulk_copy(to, kv4_block<D>(a.cache, entry, 0, walk.head), Block::kBytes, &sh.full[stage]);
-        bulk_copy(to + Block::kBytes, kv4_block<D>(a.cache, entry, 1, walk.head), Block::kBytes, &sh.full[stage]);
+        const uint64_t once = l2_policy_evict_first();       // (32 sequences of 65536 positions 256 us instead of 262)
+        bulk_load(to, kv4_block<D>(a.cache, entry, 0, walk.head), Block::kBytes, &sh.full[stage], once);
+        bulk_load(to + Block::kBytes, kv4_block<D>(a.cache, entry, 1, walk.head), Block::kBytes, &sh.full[stage], once);
       } else {
         mbar_arrive(&sh.full[stage]);
       }
