@@ -1,5 +1,7 @@
 // Writing the paged KV cache in 4 bits and reading rows of it back (include/syfi_kv4.h).  Both move bytes: what they read and write once
 // is their floor, so each is one pass with everything in between in registers.
+#include <type_traits>
+
 #include "kv4_internal.h"
 
 namespace syfi {
@@ -7,7 +9,9 @@ namespace syfi {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kWriteHeads = 4, kReadVectors = 4;   // vectors that a group of lanes has under way
+// Vectors that a group of lanes has under way.  Two instead of four: writing 8192 tokens 98 us instead of 82, reading 40,000 rows 57 instead
+// of 53; eight: 53 as well.
+constexpr int kWriteHeads = 4, kReadVectors = 4;
 constexpr int kFullGroups = 64;                    // groups per SM that are enough to keep it busy
 
 struct Write4Args {
@@ -45,12 +49,38 @@ __device__ __forceinline__ float quotient(float x, float y, float inverse) {
   return fmaf(fmaf(-q, y, x), inverse, q);
 }
 
+// A lane's eight values of a vector at `x`: eight neighbours, or four of each half.
+template <int D, int PARTS>
+__device__ __forceinline__ uint4 load8(const __nv_bfloat16* x, int lane) {
+  if constexpr (PARTS == 1) return *reinterpret_cast<const uint4*>(x + lane * 8);
+  const uint2 low = *reinterpret_cast<const uint2*>(x + lane * 4), high = *reinterpret_cast<const uint2*>(x + D / 2 + lane * 4);
+  return make_uint4(low.x, low.y, high.x, high.y);
+}
+template <int D, int PARTS>
+__device__ __forceinline__ void store8(__nv_bfloat16* x, int lane, uint4 p) {
+  if constexpr (PARTS == 1) {
+    *reinterpret_cast<uint4*>(x + lane * 8) = p;
+  } else {
+    *reinterpret_cast<uint2*>(x + lane * 4) = make_uint2(p.x, p.y);
+    *reinterpret_cast<uint2*>(x + D / 2 + lane * 4) = make_uint2(p.z, p.w);
+  }
+}
+
+// How a token's rotation pairs the dimensions: neighbours, halves of the rotated part, halves of the whole vector (or no rotation at all).
+enum Turn { kNeighbours, kHalves, kWholeHalves };
+
 // A warp takes a run of neighbouring heads of one kind (queries, keys or values) of a token, D / 8 lanes per head and HEADS heads one
 // after the other, whose loads are under way together and which share the token's cosines and sines.  A lane has eight neighbouring
 // dimensions: a word of codes, half a group.  Its partner's in a rotation of halves come by shuffles (rotary / 2 is a multiple of eight).
-template <int D, bool INTERLEAVED, int HEADS>
-__global__ void __launch_bounds__(kThreads) kv4_write_kernel(const __grid_constant__ Write4Args a) {
+// Where the whole vector is rotated by halves, or not at all, a lane has four neighbouring dimensions of each half instead: both of a pair
+// are its own, and it keeps half as many cosines and sines (8192 tokens of 64 query and 2 * 8 cache heads of 128: 82 us instead of 88).
+//
+// The bytes take 48 us there.  What keeps it from them is the instructions of a key or value (its quotients and conversions) with few warps
+// to hide their latencies; four blocks to an SM, 64 registers a thread: with three 92 us, with five (spills) 82.
+template <int D, Turn TURN, int HEADS>
+__global__ void __launch_bounds__(kThreads, HEADS > 1 ? 4 : 1) kv4_write_kernel(const __grid_constant__ Write4Args a) {
   constexpr int kLanes = D / 8, kGroups = 32 / kLanes, kRun = kGroups * HEADS;
+  constexpr int kParts = TURN == kWholeHalves ? 2 : 1, kEach = 8 / kParts;        // a lane's parts and the dimensions of each
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x % kLanes, group = (threadIdx.x & 31) / kLanes;
@@ -64,19 +94,19 @@ __global__ void __launch_bounds__(kThreads) kv4_write_kernel(const __grid_consta
   const int slot = which > 0 ? a.slots[t] : 0;
   if (which > 0 && (slot < 0 || slot / kKvPage >= a.cache.num_pages)) return;
   const int heads = which == 0 ? a.q_heads : a.cache.heads, first = static_cast<int>(run) * kRun + group;
-  const __nv_bfloat16* const from = (which == 0 ? a.q + t * a.q_stride : which == 1 ? a.k + t * a.k_stride : a.v + t * a.v_stride) + lane * 8;
+  const __nv_bfloat16* const from = which == 0 ? a.q + t * a.q_stride : which == 1 ? a.k + t * a.k_stride : a.v + t * a.v_stride;
   uint4 raw[HEADS];
 #pragma unroll
   for (int h = 0; h < HEADS; ++h)
-    raw[h] = first + h * kGroups < heads ? *reinterpret_cast<const uint4*>(from + (first + h * kGroups) * D) : make_uint4(0u, 0u, 0u, 0u);
+    raw[h] = first + h * kGroups < heads ? load8<D, kParts>(from + (first + h * kGroups) * D, lane) : make_uint4(0u, 0u, 0u, 0u);
   // what the heads share: weights, cosines and sines
   const __nv_bfloat16* const weight = which == 0 ? a.q_weight : which == 1 ? a.k_weight : nullptr;
   float w[8];
-  if (weight) floats8(*reinterpret_cast<const uint4*>(weight + lane * 8), w);
+  if (weight) floats8(load8<D, kParts>(weight, lane), w);
   const bool rotates = which < 2 && a.rotary > 0, turned = rotates && lane < a.rotary / 8;
   const int half = a.rotary / 16;               // lanes of half of the rotated dimensions
   const int partner = (threadIdx.x & 31) + (lane < half ? half : -half);
-  constexpr int kTurns = INTERLEAVED ? 4 : 8;
+  constexpr int kTurns = TURN == kHalves ? 8 : 4;
   float cs[kTurns], sn[kTurns];
 #pragma unroll
   for (int i = 0; i < kTurns; ++i) {
@@ -88,14 +118,14 @@ __global__ void __launch_bounds__(kThreads) kv4_write_kernel(const __grid_consta
     const int position = a.positions[t];
     known = position >= 0 && position < a.max_positions;
     if (turned) {
-      const float* row = a.cos_sin + (known ? position : 0) * static_cast<long long>(a.rotary) + (INTERLEAVED ? lane * 4 : (lane < half ? lane : lane - half) * 8);
+      const float* row = a.cos_sin + (known ? position : 0) * static_cast<long long>(a.rotary) + (TURN != kHalves ? lane * 4 : (lane < half ? lane : lane - half) * 8);
 #pragma unroll
       for (int i = 0; i < kTurns; i += 4) {
         const float4 c = *reinterpret_cast<const float4*>(row + i), s = *reinterpret_cast<const float4*>(row + a.rotary / 2 + i);
         cs[i] = c.x; cs[i + 1] = c.y; cs[i + 2] = c.z; cs[i + 3] = c.w;
         sn[i] = s.x; sn[i + 1] = s.y; sn[i + 2] = s.z; sn[i + 3] = s.w;
       }
-      if (!INTERLEAVED && lane < half) {
+      if (TURN == kHalves && lane < half) {
 #pragma unroll
         for (int i = 0; i < kTurns; ++i) sn[i] = -sn[i];
       }
@@ -118,13 +148,14 @@ __global__ void __launch_bounds__(kThreads) kv4_write_kernel(const __grid_consta
       for (int i = 0; i < 8; ++i) x[i] *= factor * w[i];
     }
     if (rotates) {
-      if constexpr (INTERLEAVED) {
+      if constexpr (TURN != kHalves) {
         if (turned) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float u = x[2 * i], v = x[2 * i + 1];
-            x[2 * i] = u * cs[i] - v * sn[i];
-            x[2 * i + 1] = v * cs[i] + u * sn[i];
+            float &u = x[TURN == kNeighbours ? 2 * i : i], &v = x[TURN == kNeighbours ? 2 * i + 1 : 4 + i];
+            const float turned_u = u * cs[i] - v * sn[i];
+            v = v * cs[i] + u * sn[i];
+            u = turned_u;
           }
         }
       } else {
@@ -140,37 +171,47 @@ __global__ void __launch_bounds__(kThreads) kv4_write_kernel(const __grid_consta
       for (int i = 0; i < 8; ++i) x[i] = __int_as_float(0x7fffffff);
     }
     if (which == 0) {
-      if (real) *reinterpret_cast<uint4*>(a.q_out + t * a.q_out_stride + head * D + lane * 8) = bf16x8(x);
+      if (real) store8<D, kParts>(a.q_out + t * a.q_out_stride + head * D, lane, bf16x8(x));
       continue;
     }
-    // Largest magnitudes as bits: unlike the largest float they keep a NaN.
-    unsigned top = 0u;
+    // Largest magnitudes as bits: unlike the largest float they keep a NaN.  A group is in 2 * kParts lanes.
+    unsigned top = 0u, tops[kParts];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    const float group_top = __uint_as_float(top);
+    for (int p = 0; p < kParts; ++p) {
+      tops[p] = 0u;
 #pragma unroll
-    for (int d = 2; d < kLanes; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+      for (int i = 0; i < kEach; ++i) tops[p] = max(tops[p], __float_as_uint(x[p * kEach + i]) & 0x7fffffffu);
+#pragma unroll
+      for (int d = 1; d < 2 * kParts; d <<= 1) tops[p] = max(tops[p], __shfl_xor_sync(0xffffffffu, tops[p], d));
+      top = max(top, tops[p]);
+    }
+#pragma unroll
+    for (int d = 2 * kParts; d < kLanes; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
     if (!real) continue;
     const float largest = __uint_as_float(top);
     float scale = quotient(largest < 1e-12f ? 1e-12f : largest, 2688.0f, 1.0f / 2688.0f);
-    const float six = 6.0f * scale;
-    uint32_t group_byte = cvt_e4m3x2(quotient(group_top, six, 1.0f / six), 0.0f) & 0x7fu;
-    const float unit = e4m3x2_to_float2(static_cast<uint16_t>(group_byte)).x * scale, inverse = 1.0f / unit;
-    uint32_t codes = 0u;
-    if (top >= 0x7f800000u) {                 // not finite: read back as NaN
-      scale = __int_as_float(0x7fffffff);
-      group_byte = 0u;
-    } else if (group_byte != 0u) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = quotient(x[i], unit, inverse);
-      codes = cvt_e2m1x8(x);
-    }
+    const float six = 6.0f * scale, over_six = 1.0f / six;
+    const bool finite = top < 0x7f800000u;
     uint8_t* const block = kv4_block<D>(a.cache, slot / kKvPage, which - 1, head);
     const int at = slot % kKvPage;
-    *reinterpret_cast<uint32_t*>(block + lane / 8 * kKv4Plane + at * 32 + lane % 8 * 4) = codes;
-    if (lane % 2 == 0) block[Kv4Block<D>::kGroups + at * (D / kKv4Group) + lane / 2] = static_cast<uint8_t>(group_byte);
-    if (lane == 0) *reinterpret_cast<float*>(block + Kv4Block<D>::kScales + at * 4) = scale;
+    uint32_t group_bytes[kParts];
+#pragma unroll
+    for (int p = 0; p < kParts; ++p) {
+      group_bytes[p] = finite ? cvt_e4m3x2(quotient(__uint_as_float(tops[p]), six, over_six), 0.0f) & 0x7fu : 0u;
+      const float unit = e4m3x2_to_float2(static_cast<uint16_t>(group_bytes[p])).x * scale, inverse = 1.0f / unit;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) x[p * kEach + i] = group_bytes[p] != 0u ? quotient(x[p * kEach + i], unit, inverse) : 0.0f;
+      if (lane % (2 * kParts) == 0) block[Kv4Block<D>::kGroups + at * (D / kKv4Group) + p * (D / kKv4Group / 2) + lane / (2 * kParts)] = static_cast<uint8_t>(group_bytes[p]);
+    }
+    const uint32_t codes = cvt_e2m1x8(x);
+    if constexpr (kParts == 1) {
+      *reinterpret_cast<uint32_t*>(block + lane / 8 * kKv4Plane + at * 32 + lane % 8 * 4) = codes;
+    } else {
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+        *reinterpret_cast<uint16_t*>(block + (D == 128 ? p * kKv4Plane : p * 16) + at * 32 + lane * 2) = static_cast<uint16_t>(codes >> (16 * p));
+    }
+    if (lane == 0) *reinterpret_cast<float*>(block + Kv4Block<D>::kScales + at * 4) = finite ? scale : __int_as_float(0x7fffffff);
   }
 }
 
@@ -280,10 +321,14 @@ extern "C" int syfi_kv4_write(const void* q, const void* k, const void* v, const
   const dim3 grid(static_cast<unsigned>((groups + per_block - 1) / per_block));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto run = [&](auto* kernel) { return launch_dependent(kernel, grid, dim3(kThreads), 0, st, a) == cudaSuccess; };
-  const bool ok = head_dim == 128 ? (interleaved ? (each > 1 ? run(kv4_write_kernel<128, true, kWriteHeads>) : run(kv4_write_kernel<128, true, 1>))
-                                                 : (each > 1 ? run(kv4_write_kernel<128, false, kWriteHeads>) : run(kv4_write_kernel<128, false, 1>)))
-                                  : (interleaved ? (each > 1 ? run(kv4_write_kernel<64, true, kWriteHeads>) : run(kv4_write_kernel<64, true, 1>))
-                                                 : (each > 1 ? run(kv4_write_kernel<64, false, kWriteHeads>) : run(kv4_write_kernel<64, false, 1>)));
+  const Turn turn = rotary_dim == 0 || (!interleaved && rotary_dim == head_dim) ? kWholeHalves : interleaved ? kNeighbours : kHalves;
+  auto pick = [&](auto dim, auto heads_each) {
+    constexpr int D = decltype(dim)::value, HEADS = decltype(heads_each)::value;
+    return turn == kWholeHalves ? run(kv4_write_kernel<D, kWholeHalves, HEADS>) : turn == kNeighbours ? run(kv4_write_kernel<D, kNeighbours, HEADS>) : run(kv4_write_kernel<D, kHalves, HEADS>);
+  };
+  using std::integral_constant;
+  const bool ok = head_dim == 128 ? (each > 1 ? pick(integral_constant<int, 128>(), integral_constant<int, kWriteHeads>()) : pick(integral_constant<int, 128>(), integral_constant<int, 1>()))
+                                  : (each > 1 ? pick(integral_constant<int, 64>(), integral_constant<int, kWriteHeads>()) : pick(integral_constant<int, 64>(), integral_constant<int, 1>()));
   return ok ? SYFI_KV4_OK : kv_fail(SYFI_KV4_ERR_CUDA, "write kernel launch failed");
 }
 
