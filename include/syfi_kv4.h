@@ -51,9 +51,10 @@ int syfi_kv4_read(const void* cache, int64_t num_pages, int64_t page_stride, int
  * what a query sees are syfi_paged_attention's (syfi_kv.h):
  *   out = sum_j softmax_j(scale * q . key_j) * value_j;  a query that sees nothing gets zeros; rows of no sequence are left alone.
  * Positions that a query does not see do not touch its result, whatever the cache holds there.  Scales and group scales are not
- * negative.  A query or a seen position that is not finite makes its heads' results NaN.
+ * negative.  A query, or a seen position with a scale or a key's group scale that is not finite, makes its heads' results NaN; a value's
+ * group scale that is not finite those of its dimensions at least.
  * Sums are in f32.  A weight times its value's scale is rounded to f16 (2^-12 of it on average); one 2^-28 below the row's largest
- * may not be added, with up to 16 rows per sequence and key head on average one 2^-32 below.  Codes times group scales are exact.
+ * may not be added, with up to 32 rows per sequence and key head on average one 2^-32 below.  Codes times group scales are exact.
  * Scratch memory by stream and by captured graph as for syfi_paged_attention, in buffers of its own. */
 int syfi_kv4_attention(const void* q, int64_t q_stride, const void* cache, int64_t num_pages, int64_t page_stride,
                        const int32_t* block_table, int32_t max_pages, const int32_t* seq_lens, const int32_t* q_starts,

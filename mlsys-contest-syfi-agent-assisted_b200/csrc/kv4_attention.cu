@@ -43,8 +43,14 @@ __device__ __forceinline__ void both_halves(uint32_t v, uint32_t& lo, uint32_t& 
 //            have one group scale.  The weights come from the scores' layout by an 8 x 8 transpose (movmatrix).
 // Which position an index of the scores stands for is chosen so that both reads of the rows of 32 bytes are free of bank conflicts: index i
 // of eight is position i ^ (i >> 2 & 1).
-// What bounds it is instructions, the conversions (half a clock's rate) first.
-constexpr int kDecodeExtra = 6;            // what a unit costs besides its pages, in pages (see below)
+//
+// What bounds it is instructions: 1221 of a warp for a page of 64 positions of 128 dimensions, a third of them conversions, which issue at
+// half a clock's rate; 62 % of the issue slots are taken.  32 sequences of 65536 positions, 4 key heads: 256 us, where the loads alone
+// take 210 and the bytes 195 at the rate of a copy.  Three blocks of 168 registers to an SM; four of 128: 264.
+//
+// kDecodeExtra is what a unit costs besides its pages, in pages: the prologue, its end, the join.  24 sequences of 300 to 30000 positions, 8 key
+// heads, with 1, 3, 6, 8 and 12: 78, 73, 64, 64 and 65 us (of which the plan has since lost 9).
+constexpr int kDecodeExtra = 6;
 constexpr float kFarBehind = 1.2676506e30f;   // 2^100 between the references of the two sums: the values' follows
 constexpr int kWarps = 4;
 constexpr int kStatusTimeout = 401;
@@ -340,13 +346,14 @@ kv4_decode_kernel(const __grid_constant__ AttentionArgs a, int* __restrict__ sta
             }
           }
           const float ks[2] = {k_scale[16 * b + t0], k_scale[16 * b + t0 + 8]};
+          const float zero[2] = {ks[0] - ks[0], ks[1] - ks[1]};      // or NaN: a score that is minus infinity would count as not seen
 #pragma unroll
           for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               float sum = part[0][t][e];
               if constexpr (kPlanes == 2) sum += part[1][t][e];
-              x[b][t][e] = sum * (ks[e / 2] * unit[t][e % 2]);
+              x[b][t][e] = fmaf(sum, ks[e / 2] * unit[t][e % 2], zero[e / 2]);
             }
         }
         if (!plain) {
@@ -699,9 +706,16 @@ extern "C" int syfi_kv4_attention(const void* q, int64_t q_stride, const void* c
   const long long wait_limit = d.next_wait_limit > 0 ? d.next_wait_limit : kWaitLimit;
   d.next_wait_limit = 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // Rows per sequence and key head, on average (the lengths themselves are on the device).
+  // Rows per sequence and key head, on average (the lengths themselves are on the device).  The decoding kernel reads a sequence's pages for
+  // every 8 or 16 of them, the chunk kernel for every 256, but a tile costs it as much for 8 rows as for 256.  32 sequences of 16384 positions,
+  // 8 key heads, us by rows:
+  //                      4    8   12   16   24   32
+  //   decoding, 8 rows  141  141  258  258  373  489
+  //   decoding, 16           142  202  202  370  372
+  //   chunks            494  495  495  495  498  499
+  // One sequence of 65536: 38, 40, 51, 52, 64, 78 - 53, 53, 68, 71 from 12 rows - 111 to 125.
   const int64_t rows = (tokens * a.group + batch - 1) / batch;
-  if (rows > 16) {
+  if (rows > 32) {
     int rc = SYFI_KV4_OK;
     if (!take_scratch(a, d, kv4_chunk_partial_bytes(head_dim, sms), st, &rc)) return rc;
     return launch_kv4_chunk(a, head_dim, sms, d.status, wait_limit, st) == cudaSuccess ? SYFI_KV4_OK : kv_fail(SYFI_KV4_ERR_CUDA, "attention kernel launch failed");

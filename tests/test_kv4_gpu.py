@@ -361,6 +361,20 @@ def test_what_is_not_seen_does_not_matter(q_lens, kv_lens, D, pkg, kv4):
     assert torch.equal(_attend(pkg, inputs, window=100), clean)
 
 
+@pytest.mark.parametrize("q_len", [1, 3, 300])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("what", ["keys", "values"])
+def test_an_infinite_scale_that_is_seen(what, D, q_len, pkg, kv4):
+    """Its key head's results are NaN, whichever sign its scores have; other heads keep every bit."""
+    inputs = _attention_inputs(kv4, [q_len], [2000], 16, 4, D, seed=13)
+    clean = _attend(pkg, inputs)
+    _, _, scales = kv4.views(inputs[1])
+    scales[int(inputs[2][0, 7]), 0 if what == "keys" else 1, 2, 33] = float("inf")
+    out = _attend(pkg, inputs)
+    assert out[:, 8:12].isnan().all()
+    assert torch.equal(out[:, :8], clean[:, :8]) and torch.equal(out[:, 12:], clean[:, 12:])
+
+
 @pytest.mark.parametrize("q_lens,kv_lens", [([1, 1, 1, 1], [400, 64, 5000, 65]), ([300, 64, 100], [1000, 64, 100])])
 @pytest.mark.parametrize("HQ,HK,D", [(16, 4, 128), (8, 1, 64)])
 def test_absent_pages_and_rows_that_see_nothing(q_lens, kv_lens, HQ, HK, D, pkg, kv4):
