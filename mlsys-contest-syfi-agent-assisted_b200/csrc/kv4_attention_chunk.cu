@@ -117,6 +117,10 @@ struct Ring {
   }
 };
 
+__device__ __forceinline__ void prefetch_l2(const void* p, int bytes) {      // both multiples of 16
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
+}
+
 // ---------------------------------------------------------------- planning, and the clock (one thread)
 struct Watch {
   long long limit, since;
@@ -133,6 +137,7 @@ struct Watch {
   }
 };
 
+template <int D>
 __device__ __forceinline__ void plan_role(const AttentionArgs& a, const ChunkPlan& plan, const PlanShared& s_plan, ChunkShared& sh, const Piece& piece, long long wait_limit) {
   Watch watch = {wait_limit, clock64(), 0u};
   ChunkCursor at;
@@ -174,6 +179,9 @@ __device__ __forceinline__ void plan_role(const AttentionArgs& a, const ChunkPla
     }
     mbar_arrive(&sh.segment_full[ring.stage]);
     if (!more) break;
+    // Its queries, for the softmax warps to find in L2: they ask for them only when the unit in front is done.
+    for (int token = g.row0 / a.group; token <= (g.row0 + g.rows - 1) / a.group; ++token)
+      prefetch_l2(a.q + (g.q_first + token) * a.q_stride + g.head * a.group * D, a.group * D * 2);
     ring.next();
     at.advance(plan, here);
   }
@@ -742,41 +750,48 @@ __device__ __forceinline__ void softmax_tile(ChunkShared& sh, const TileRows& r,
 }
 
 // The warp's 32 rows of q (of which `rows` are there; mine: where this lane's row begins in q) as f16 times 2^k each, the row's largest at
-// 2^14 .. 2^15, into rows row0 and on of a tile.  D / 8 lanes read a row.  units: what a score of each row is worth.
+// 2^14 .. 2^15, into rows row0 and on of a tile.  Four lanes have a row, which takes two shuffles for its largest and the exponent's arithmetic
+// for eight rows at a time; each second row starts with its other half, so that stores hit all banks.  units: what a score of each row is worth.
 template <int D>
 __device__ __forceinline__ void put_queries(const __nv_bfloat16* q, long long mine, float scale_log2, int rows, uint8_t* tile, int row0, float* units) {
-  constexpr int kLanes = D / 8, kTogether = 32 / kLanes, kBatch = 4;      // rows at a time, loads under way
-  const int lane = threadIdx.x % 32, part = lane % kLanes;
-#pragma unroll 1
-  for (int at = 0; at < 32; at += kTogether * kBatch) {
-    uint4 raw[kBatch];
+  constexpr int kChunks = D / 32;          // of eight dimensions, a lane's
+  const int lane = threadIdx.x % 32, part = lane % 4;
+#pragma unroll 2
+  for (int at = 0; at < 32; at += 8) {
+    const int row = at + lane / 4, in_tile = row0 + row;
+    const uint4* const from = reinterpret_cast<const uint4*>(q + __shfl_sync(0xffffffffu, mine, row)) + part;
+    uint4 raw[kChunks];
+    uint32_t most = 0u;
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int row = at + b * kTogether + lane / kLanes;
-      const long long from = __shfl_sync(0xffffffffu, mine, row);
-      raw[b] = make_uint4(0u, 0u, 0u, 0u);
-      if (row < rows) raw[b] = __ldg(reinterpret_cast<const uint4*>(q + from) + part);
+    for (int j = 0; j < kChunks; ++j) raw[j] = row < rows ? __ldg(from + 4 * (j ^ (row & 1))) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int j = 0; j < kChunks; ++j) {
+      most = __vmaxu2(__vmaxu2(most, raw[j].x & 0x7fff7fffu), raw[j].y & 0x7fff7fffu);
+      most = __vmaxu2(__vmaxu2(most, raw[j].z & 0x7fff7fffu), raw[j].w & 0x7fff7fffu);
     }
+    most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    const unsigned top = max(most & 0xffffu, most >> 16);
+    const int k = top == 0u ? 0 : min(14 - (static_cast<int>(top >> 7) - 127), 120);
+    const float up = copysignf(__int_as_float((k + 127) << 23), scale_log2);
+    const uint64_t ups = f32x2_pack(up, up);
+    // (a row that is not finite is NaN throughout, so that the mask takes its scores out like any other's)
+    const uint32_t spoilt = top >= 0x7f80u ? 0x7fff7fffu : 0u;
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int row = at + b * kTogether + lane / kLanes;
-      const uint32_t w[4] = {raw[b].x, raw[b].y, raw[b].z, raw[b].w};
-      unsigned top = 0u;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) top = max(top, max(w[e] & 0x7fffu, w[e] >> 16 & 0x7fffu));
-#pragma unroll
-      for (int d = kLanes / 2; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
-      const int k = top == 0u ? 0 : min(14 - (static_cast<int>(top >> 7) - 127), 120);
-      const float up = copysignf(__int_as_float((k + 127) << 23), scale_log2);
+    for (int j = 0; j < kChunks; ++j) {
+      const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
       uint32_t h[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) h[e] = pack_half2(__uint_as_float(w[e] << 16) * up, __uint_as_float(w[e] & 0xffff0000u) * up);
-      // (a row that is not finite is NaN throughout, so that the mask takes its scores out like any other's)
-      if (top >= 0x7f80u) h[0] = h[1] = h[2] = h[3] = 0x7fff7fffu;
-      *reinterpret_cast<uint4*>(tile + part / 8 * (kTile * 128) + (row0 + row) * 128 + ((part % 8 ^ ((row0 + row) & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-      // (a scale of zero keeps a factor, f32's smallest normal number, so that -infinity stays what it is)
-      if (part == 0) units[row] = fmaxf(fabsf(scale_log2) * __int_as_float((127 - k) << 23), 1.17549435e-38f);
+      for (int e = 0; e < 4; ++e) {
+        float x0, x1;
+        f32x2_unpack(f32x2_mul(f32x2_pack_bits(w[e] << 16, w[e] & 0xffff0000u), ups), x0, x1);
+        h[e] = pack_half2(x0, x1) | spoilt;
+      }
+      const int chunk = 4 * (j ^ (row & 1)) + part;
+      *reinterpret_cast<uint4*>(tile + chunk / 8 * (kTile * 128) + in_tile * 128 + ((chunk % 8 ^ (in_tile & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
     }
+    // (a scale of zero keeps a factor, f32's smallest normal number, so that -infinity stays what it is)
+    if (part == 0) units[row] = fmaxf(fabsf(scale_log2) * __int_as_float((127 - k) << 23), 1.17549435e-38f);
   }
 }
 
@@ -1117,7 +1132,7 @@ kv4_chunk_kernel(const __grid_constant__ AttentionArgs a, int* __restrict__ stat
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (lane == 0) {
       if (warp == 12) mma_role<D>(sh, smem, tmem);
-      if (warp == 13) plan_role(a, plan, s_plan, sh, piece, wait_limit);
+      if (warp == 13) plan_role<D>(a, plan, s_plan, sh, piece, wait_limit);
     }
     __syncwarp();
   }
