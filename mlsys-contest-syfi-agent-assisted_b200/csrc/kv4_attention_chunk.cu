@@ -40,6 +40,7 @@ constexpr int kStatusTimeout = 401;
 // standard deviation 1.5: 618 us).
 constexpr float kProductHeadroom = 5.0f;
 constexpr float kProductGrowth = 9.0f;      // (where the reference is set from a bound that may be twice too low)
+constexpr float kBlindGrowth = 1.0f;        // (where few positions gave it: 2^9 too low, it would not last)
 constexpr float kNear = 0.25f;              // a tile's value scales are so near one another, or the products themselves are asked
 constexpr float kFarAbove = 60.0f;          // a row whose n lies so many octaves above m, because of a huge value, keeps its weights in units of m
 
@@ -653,7 +654,7 @@ __device__ __forceinline__ void set_references(const TileRows& r, float largest,
 #pragma unroll
   for (int row = 0; row < 4; ++row) {
     fade[row] = 1.0f;
-    if (bound[row] > n[row] + kProductGrowth) {
+    if (bound[row] > n[row] + (products ? kProductGrowth : kBlindGrowth)) {
       fade[row] = ex2(n[row] - bound[row]);
       n[row] = bound[row];
     }
@@ -718,9 +719,11 @@ __device__ __forceinline__ void tile_weights(ChunkShared& sh, const TileRows& r,
   }
 }
 
-// What the warp's rows need before a tile's weights: nothing; references, because a row has none (kBlind, as at the start); or weights in units of
-// m, because a row's n lies far above it (kFar).
+// What the warp's rows need before a tile's weights: nothing; references, because a row has none (kBlind, as at the start) or one from fewer than
+// kEnough positions; or weights in units of m, because a row's n lies far above it (kFar).  (At a window's lower edge a row may see a few
+// positions of its first tile, and of 256 rows one or another then had weights 2^10 larger in a later tile, done again at 5000 clocks and more.)
 constexpr int kSettled = 0, kBlind = 1, kFar = 2;
+constexpr int kEnough = 32;
 
 // A tile of the warp's rows: scores from tensor memory, weights back into it; the rows' references m and n and this lane's part of their sums l.
 template <int D>
@@ -744,6 +747,10 @@ __device__ __forceinline__ void softmax_tile(ChunkShared& sh, const TileRows& r,
     for (int row = 0; row < 4; ++row) {
       far |= n[row] - m[row] > kFarAbove;
       blind |= n[row] == -INFINITY && l[row] == l[row];
+      if (r.masked) {
+        const int2 see = row_bounds(r, row);
+        blind |= see.y >= kTile - 1 && see.x > kTile - kEnough;
+      }
     }
     settled = __any_sync(0xffffffffu, far) ? kFar : __any_sync(0xffffffffu, blind) ? kBlind : kSettled;
   }
