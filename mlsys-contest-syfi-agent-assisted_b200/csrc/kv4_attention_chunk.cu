@@ -529,19 +529,20 @@ __device__ __forceinline__ void rescale_sums(uint32_t t_o, const float (&fade)[4
 }
 
 // The rows' largest scores of 64 positions, times the keys' scales and in units of the rows'.
+template <bool MASKED>
 __device__ __forceinline__ void largest_scores(const TileRows& r, int h, const uint32_t (&s)[2][32], float (&top)[4]) {
   const int column = 64 * h + threadIdx.x % 4 * 2;
   const bool there = h == 0 ? r.there0 : r.there1;
 #pragma unroll
   for (int row = 0; row < 4; ++row) {
-    const int2 see = row_bounds(r, row);
+    const int2 see = MASKED ? row_bounds(r, row) : make_int2(0, 0);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       float x0, x1;
       f32x2_unpack(f32x2_mul(f32x2_pack_bits(s[row / 2][4 * i + 2 * (row % 2)], s[row / 2][4 * i + 2 * (row % 2) + 1]), ld_shared_pair(r.scales + 4 * (64 * h + 8 * i))), x0, x1);
       const int at = column + 8 * i;
-      if (there && at >= see.x && at <= see.y) top[row] = fmaxf(top[row], x0);
-      if (there && at + 1 >= see.x && at + 1 <= see.y) top[row] = fmaxf(top[row], x1);
+      if (!MASKED || (there && at >= see.x && at <= see.y)) top[row] = fmaxf(top[row], x0);
+      if (!MASKED || (there && at + 1 >= see.x && at + 1 <= see.y)) top[row] = fmaxf(top[row], x1);
     }
   }
 }
@@ -626,7 +627,8 @@ __device__ __forceinline__ void set_references(const TileRows& r, float largest,
     uint32_t s[2][32];
     load_scores(r, h, s);
     scores_landed(s);
-    largest_scores(r, h, s, top);
+    if (r.masked) largest_scores<true>(r, h, s, top);
+    else largest_scores<false>(r, h, s, top);
   }
 #pragma unroll
   for (int row = 0; row < 4; ++row) {
@@ -689,7 +691,7 @@ __device__ __forceinline__ void tile_weights(ChunkShared& sh, const TileRows& r,
       load_scores(r, h, s);
       scores_landed(s);
       float highest[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, fade[4];
-      largest_scores(r, h, s, highest);
+      largest_scores<true>(r, h, s, highest);
 #pragma unroll
       for (int row = 0; row < 4; ++row) {
         const float bound = fmaf(quad_max(highest[row]), r.unit[row], shift[row]) + lg2(largest), up = bound > 15.0f ? bound - kProductHeadroom : 0.0f;
