@@ -26,8 +26,9 @@ constexpr int kTile = 128;             // positions per tile: two pages
 constexpr int kChunkRows = 256;
 constexpr int kChunkThreads = 512;     // 8 softmax warps, 4 converting ones, then MMAs, planning, two idle ones
 constexpr int kSoftmaxWarps = 8, kSoftmaxThreads = 256;
-// What a unit costs besides its tiles, in tiles.  With 1, 2, 4, 6 and 10: a prompt of 8192 tokens 1197, 998, 729, 730 and 756 us (a piece that
-// ends inside a unit pays for a join), eight sequences of 1 to 250 new tokens 85, 79, 87, 91 and 101.
+// What a unit costs besides its tiles, in tiles.  With 2, 3 and 4: prompts of 8192 tokens in all 812, 681 and 660 us (a piece that ends inside a
+// unit pays for a join, and pieces of few units each get one more), eight sequences of 1 to 250 new tokens 77, 81 and 85; with 6 and 10 both
+// lost, 4 and 16 % more for the latter.
 constexpr int kChunkExtra = 4;
 constexpr int kSlotRows = 128;         // units of at most so many rows use one slot for their even tiles and one for their odd ones
 using ChunkPlan = Plan<kTile, kChunkRows, kChunkExtra, kSlotRows>;
@@ -52,7 +53,8 @@ struct ChunkShape {
   static constexpr int kK = kQ + 2 * kTileBytes;
   static constexpr int kV = kK + kStages * kTileBytes;
   static constexpr int kScales = kV + kStages * kTileBytes;       // [K 128 f32][V 128 f32] per stage
-  static constexpr int kSmem = 1024 + kScales + kScaleStages * 2 * kTile * 4;
+  static constexpr int kHandOver = kScales + kScaleStages * 2 * kTile * 4;      // [4 warps][4][32 lanes] of four f32
+  static constexpr int kSmem = 1024 + kHandOver + 4 * 4 * 32 * 16;
 };
 
 // A piece of a unit, as the planning warp describes it to the others.
@@ -864,62 +866,174 @@ __device__ __forceinline__ void join_columns(const AttentionArgs& a, int q_first
   }
 }
 
+// The thread's number, in a form from which nothing is computed ahead of a loop: what a segment's ends need would take the tiles' registers, and
+// a register of theirs in local memory costs 600 clocks a use (the L1 is small beside this much shared memory).
+__device__ __forceinline__ int thread_here() {
+  int t = threadIdx.x;
+  asm volatile("" : "+r"(t));
+  return t;
+}
+
 template <int D>
-__device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared& sh, PlanShared& s_plan, uint8_t* smem, uint32_t tmem, const Piece& piece) {
+__device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared& sh, PlanShared& s_plan, uint8_t* smem, const Piece& piece) {
   using Shape = ChunkShape<D>;
   // warps 0-3: slot 0, 4-7: slot 1
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, slot = warp / 4, in_slot = warp % 4 * 32 + lane;
-  const int across = 2 + warp % 4;                 // named barrier of the two slots' warps for the same rows
-  const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
-  const uint32_t t_s = tmem + lanes + slot * 128, t_o = t_s + 256, scales0 = smem_u32(smem) + Shape::kScales;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, slot = warp / 4;
+  const uint32_t scales0 = smem_u32(smem) + Shape::kScales;
   static_assert(kSegmentRing == 4 && kScaleStages == 4, "stage and parity are bits of a counter");
-  uint32_t segment = 0, tile = 0, own = 0, own_segments = 0;       // segments and tiles so far, and those of this slot
+  uint32_t segment = 0, tile = 0, own = 0;       // segments and tiles so far; parities of this slot's tiles (bit 0) and segments (bit 1)
+  // A thread's row of a unit (rows beyond the last copy its bounds), and where it lies.
+  auto row_of = [&](const Segment& g, int thread) { return g.turns ? thread % 128 : thread; };
+  auto token_of = [&](const Segment& g, int row, int& column) {
+    const int at = g.row0 + min(row, g.rows - 1), token = at / a.group;
+    column = (g.head * a.group + at - token * a.group) * D;
+    return token;
+  };
+  auto is_active = [&](const Segment& g, int slot) { return g.turns || g.rows > slot * kSlotRows; };
+  // What a segment's tiles need of its rows: their bounds, and q in shared memory, where the MMAs of the one in front no longer read.
+  auto begin = [&](const Segment& g) {
+    const int thread = thread_here(), warp = thread / 32, lane = thread % 32, slot = warp / 4, in_slot = thread % 128;
+    int column;
+    const int token = token_of(g, row_of(g, thread), column), high = g.base + token - g.tile0 * kTile;
+    const int low = a.window > 0 ? max(g.base + token - a.window + 1, 0) - g.tile0 * kTile : -g.tile0 * kTile;
+    sh.bounds[slot][in_slot] = make_int2(low, high);      // counted from the segment's first tile
+    const int highest_low = __reduce_max_sync(0xffffffffu, low), lowest_high = __reduce_min_sync(0xffffffffu, high);
+    if (lane == 0) sh.common[warp] = make_int2(highest_low, lowest_high);
+    if (is_active(g, slot)) {
+      if (!(g.turns && slot == 1)) {
+        const int in_tile = warp % 4 * 32;
+        put_queries<D>(a.q, (g.q_first + token) * a.q_stride + column, a.scale_log2, g.rows - slot * kSlotRows - in_tile,
+                       smem + Shape::kQ + slot * Shape::kTileBytes, in_tile, sh.unit + slot * 128 + in_tile);
+        fence_proxy_async_smem();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.q_full[slot]);
+    }
+    __syncwarp();
+  };
   while (true) {
     wait_whole_warp(sh, &sh.segment_full[segment & 3], segment >> 2 & 1);
     if (softmax_bar_any(sh.abort_code != 0)) return;      // all eight warps meet here whatever failed, and leave together
-    const Segment& g = sh.segment[segment & 3];
-    if (g.tiles == 0) {
+    // A segment's q goes to shared memory before the results of the one in front leave tensor memory, so that its first scores do not have to
+    // be waited for.
+    const bool more = sh.segment[segment & 3].tiles > 0;
+    if (more) begin(sh.segment[segment & 3]);
+    if (segment > 0) {
+      const Segment& g = sh.segment[(segment - 1) & 3];
+      const int thread = thread_here(), warp = thread / 32, lane = thread % 32, slot = warp / 4, in_slot = thread % 128;
+      const int row = row_of(g, thread), across = 2 + warp % 4;      // named barrier of the two slots' warps for the same rows
+      const uint32_t t_o = sh.tmem + (static_cast<uint32_t>(warp % 4 * 32) << 16) + slot * 128 + 256;
+      const bool turns = g.turns, whole = g.whole, real = row < g.rows && !(turns && slot == 1);
+      if (is_active(g, slot)) {
+        float4 mine = sh.end[slot][in_slot];    // m, l, n
+        float f = 1.0f;
+        if (turns) {                            // to the larger references of the two slots'
+          const float4 its = sh.end[slot ^ 1][in_slot];
+          const float m_all = fmaxf(mine.x, its.x), m_ref = finite_or_zero(m_all), n_all = fmaxf(mine.z, its.z);
+          f = ex2(mine.z - finite_or_zero(n_all));
+          mine = make_float4(m_all, mine.y * ex2(mine.x - m_ref) + its.y * ex2(its.x - m_ref), n_all, 0.0f);
+        }
+        if (whole) f *= mine.y == 0.0f || mine.z == -INFINITY ? 0.0f : ex2(mine.z - finite_or_zero(mine.x) - kProductHeadroom) / mine.y;
+        float4* const its = reinterpret_cast<float4*>(smem + Shape::kHandOver) + warp % 4 * 128 + lane;      // slot 1's sums on their way to slot 0
+        float4* const to = reinterpret_cast<float4*>(a.partial);       // (kept by dimension, so that a warp's 32 rows lie side by side)
+        const int part = parts_of(g).slot(static_cast<int>(blockIdx.x));
+        // Two neighbouring lanes write 32 bytes of one's row, then of the other's.
+        int column;
+        const int token = token_of(g, row, column);
+        const long long place = (g.q_first + token) * a.out_stride + column, place_other = __shfl_xor_sync(0xffffffffu, place, 1);
+        const bool odd = lane % 2 != 0, real_other = (row ^ 1) < g.rows;
+        __nv_bfloat16* const even_row = a.out + (odd ? place_other : place) + 8 * odd;
+        __nv_bfloat16* const odd_row = a.out + (odd ? place : place_other) + 8 * odd;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 16) {
+          uint32_t o[16];
+          tmem_ld16(t_o + c, o);
+          tmem_ld_wait_for(o);
+#pragma unroll
+          for (int b = 0; b < 16; ++b) o[b] = __float_as_uint(__uint_as_float(o[b]) * f);
+          if (turns) {                          // slot 0 adds slot 1's sums to its own
+            if (slot == 1) {
+#pragma unroll
+              for (int b = 0; b < 4; ++b)
+                its[32 * b] = make_float4(__uint_as_float(o[4 * b]), __uint_as_float(o[4 * b + 1]), __uint_as_float(o[4 * b + 2]), __uint_as_float(o[4 * b + 3]));
+            }
+            named_bar_sync(across, 64);
+            if (slot == 0) {
+#pragma unroll
+              for (int b = 0; b < 4; ++b) {
+                const float4 x = its[32 * b];
+                o[4 * b] = __float_as_uint(__uint_as_float(o[4 * b]) + x.x);
+                o[4 * b + 1] = __float_as_uint(__uint_as_float(o[4 * b + 1]) + x.y);
+                o[4 * b + 2] = __float_as_uint(__uint_as_float(o[4 * b + 2]) + x.z);
+                o[4 * b + 3] = __float_as_uint(__uint_as_float(o[4 * b + 3]) + x.w);
+              }
+            }
+            named_bar_sync(across, 64);
+            if (slot == 1) continue;
+          }
+          if (whole) {
+            uint32_t low[4], high[4];           // this lane's row: its first eight of sixteen dimensions, the others
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const __nv_bfloat162 x = __floats2bfloat162_rn(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1]));
+              const __nv_bfloat162 y = __floats2bfloat162_rn(__uint_as_float(o[8 + 2 * e]), __uint_as_float(o[9 + 2 * e]));
+              low[e] = *reinterpret_cast<const uint32_t*>(&x);
+              high[e] = *reinterpret_cast<const uint32_t*>(&y);
+              const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? low[e] : high[e], 1);
+              if (odd) low[e] = got;            // the even row's second half
+              else high[e] = got;               // the odd row's first half
+            }
+            if (odd ? real_other : real) *reinterpret_cast<uint4*>(even_row + c) = make_uint4(low[0], low[1], low[2], low[3]);
+            if (odd ? real : real_other) *reinterpret_cast<uint4*>(odd_row + c) = make_uint4(high[0], high[1], high[2], high[3]);
+          } else if (real) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              to[(static_cast<long long>(part) * (D / 4) + c / 4 + e) * kChunkRows + row] =
+                  make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
+          }
+        }
+        if (real && !whole) reinterpret_cast<float4*>(a.partial + 2ll * piece.ctas * kChunkRows * D)[static_cast<long long>(part) * kChunkRows + row] = mine;
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.o_empty[slot]);
+      }
+      if (!whole) {
+        const Parts parts = parts_of(g);
+        __threadfence();
+        named_bar_sync(1, kSoftmaxThreads);
+        if (tid == 0) {
+          const bool is_last = atomicAdd(a.tickets + parts.first, 1) == parts.last - parts.first;
+          if (is_last) a.tickets[parts.first] = 0;
+          s_plan.last = is_last;
+        }
+        named_bar_sync(1, kSoftmaxThreads);
+        if (s_plan.last) {
+          __threadfence();
+          join_columns<D>(a, g.q_first, g.row0, g.head, g.rows, piece.ctas, parts, tid, kSoftmaxThreads);
+        }
+      }
+      if (tid == 0) ++sh.finished;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.segment_empty[(segment - 1) & 3]);
+    }
+    if (!more) {
       if (tid == 0) sh.done = 1;
       return;
     }
+    const Segment& g = sh.segment[segment & 3];
     const bool turns = g.turns;
     // whether the next tile is this slot's (bit 0: no), and whether that changes with each (bit 1)
-    unsigned turn = turns ? 2u + slot : g.rows <= slot * kSlotRows;
-    const bool active = turn != 1u;
-    // (a thread's row of the unit; rows beyond the last copy its bounds)
-    auto row_of = [&]() { return (g.turns ? 0 : slot * kSlotRows) + in_slot; };
-    auto token_of = [&](int& column) {
-      const int at = g.row0 + min(row_of(), g.rows - 1), token = at / a.group;
-      column = (g.head * a.group + at - token * a.group) * D;
-      return token;
-    };
+    unsigned turn = turns ? 2u + slot : !is_active(g, slot);
     {
-      const int q_slot = turns ? 0 : slot, first_row = warp % 4 * 32 + lane / 4;      // the first of this lane's four in the slot
-      {
-        int column;
-        const int token = token_of(column), high = g.base + token - g.tile0 * kTile;
-        const int low = a.window > 0 ? max(g.base + token - a.window + 1, 0) - g.tile0 * kTile : -g.tile0 * kTile;
-        sh.bounds[slot][in_slot] = make_int2(low, high);      // counted from the segment's first tile
-        const int highest_low = __reduce_max_sync(0xffffffffu, low), lowest_high = __reduce_min_sync(0xffffffffu, high);
-        if (lane == 0) sh.common[warp] = make_int2(highest_low, lowest_high);
-        if (active && q_slot == slot) {
-          const int in_tile = warp % 4 * 32;
-          put_queries<D>(a.q, (g.q_first + token) * a.q_stride + column, a.scale_log2, g.rows - slot * kSlotRows - in_tile,
-                         smem + Shape::kQ + slot * Shape::kTileBytes, in_tile, sh.unit + slot * 128 + in_tile);
-          fence_proxy_async_smem();
-        }
-      }
-      __syncwarp();
-      if (active && lane == 0) mbar_arrive(&sh.q_full[slot]);
       if (turns) named_bar_sync(1, kSoftmaxThreads);       // slot 1 reads slot 0's units
       TileRows r;
-      r.t_s = t_s;
       r.bounds = sh.bounds[0];
       r.offset = 0;
+      const int first_row = warp % 4 * 32 + lane / 4;      // the first of this lane's four in the slot
       float ms[4], ns[4], ls[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        r.unit[i] = sh.unit[q_slot * 128 + first_row + 8 * i];
+        r.unit[i] = sh.unit[(turns ? 0 : slot) * 128 + first_row + 8 * i];
         ms[i] = ns[i] = -INFINITY;
         ls[i] = 0.0f;
       }
@@ -928,140 +1042,41 @@ __device__ __forceinline__ void softmax_role(const AttentionArgs& a, ChunkShared
         const int stage = tile & 3;
         wait_whole_warp(sh, &sh.scale_full[stage], tile >> 2 & 1);
         if (!(turn & 1u)) {
-          const int2 common = sh.common[warp];
+          const int thread = thread_here();
+          const int2 common = sh.common[thread / 32];
           const int flags = sh.flags[stage];
           r.there0 = flags & 1;
           r.there1 = flags & 2;
           r.near = flags & 4;
           r.masked = !r.there0 || !r.there1 || common.x > r.offset || common.y < r.offset + kTile - 1;
-          r.scales = scales0 + stage * (2 * kTile * 4) + lane % 4 * 8;
-          softmax_tile<D>(sh, r, slot, stage, own & 1, left > g.tiles - (turns ? 2 : 1), settled, ms, ns, ls);
-          ++own;
+          r.scales = scales0 + stage * (2 * kTile * 4) + thread % 4 * 8;
+          r.t_s = sh.tmem + (static_cast<uint32_t>(thread / 32 % 4 * 32) << 16) + thread / 128 * 128;
+          const Segment& now = sh.segment[segment & 3];
+          softmax_tile<D>(sh, r, thread / 128, stage, own & 1, left > now.tiles - (now.turns ? 2 : 1), settled, ms, ns, ls);
+          own ^= 1u;
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.scale_empty[stage]);
+        if (thread_here() % 32 == 0) mbar_arrive(&sh.scale_empty[stage]);
         ++tile;
-        if (tid == 0) sh.tiles_done = sh.tiles_done + 1u;
+        if (thread_here() == 0) sh.tiles_done = sh.tiles_done + 1u;
         turn ^= turn >> 1 & 1u;
         r.offset += kTile;
       }
       // ---- the segment's end: from here on a thread has a row
-      if (active) {
+      if (is_active(g, thread_here() / 128)) {
+        const int thread = thread_here(), warp = thread / 32, lane = thread % 32, slot = warp / 4;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           ls[i] += __shfl_xor_sync(0xffffffffu, ls[i], 1);
           ls[i] += __shfl_xor_sync(0xffffffffu, ls[i], 2);
-          if (lane % 4 == 0) sh.end[slot][first_row + 8 * i] = make_float4(ms[i], ls[i], ns[i], 0.0f);
+          if (lane % 4 == 0) sh.end[slot][warp % 4 * 32 + lane / 4 + 8 * i] = make_float4(ms[i], ls[i], ns[i], 0.0f);
         }
-        wait_whole_warp(sh, &sh.o_full[slot], own_segments & 1);
+        wait_whole_warp(sh, &sh.o_full[slot], own >> 1 & 1);
         __syncwarp();
         tc_fence_after();
-        ++own_segments;
+        own ^= 2u;
       }
     }
-    if (softmax_bar_any(sh.abort_code != 0)) return;
-    const int row = row_of();
-    const bool whole = g.whole, real = row < g.rows && !(turns && slot == 1);
-    if (active) {
-      float4 mine = sh.end[slot][in_slot];    // m, l, n
-      float f = 1.0f;
-      if (turns) {                            // to the larger references of the two slots'
-        const float4 its = sh.end[slot ^ 1][in_slot];
-        const float m_all = fmaxf(mine.x, its.x), m_ref = finite_or_zero(m_all), n_all = fmaxf(mine.z, its.z);
-        f = ex2(mine.z - finite_or_zero(n_all));
-        mine = make_float4(m_all, mine.y * ex2(mine.x - m_ref) + its.y * ex2(its.x - m_ref), n_all, 0.0f);
-      }
-      if (whole) f *= mine.y == 0.0f || mine.z == -INFINITY ? 0.0f : ex2(mine.z - finite_or_zero(mine.x) - kProductHeadroom) / mine.y;
-      // Rows leave through the warp's own rows of the slot's q tile, which nothing reads any more.  Partial sums are kept by dimension, so that
-      // a warp's 32 rows lie side by side.
-      uint8_t* const own_rows = smem + Shape::kQ + slot * Shape::kTileBytes + warp % 4 * (32 * 128);
-      float4* const its = reinterpret_cast<float4*>(smem + Shape::kQ + Shape::kTileBytes + warp % 4 * (32 * 128)) + lane;   // of slot 1's q tile
-      float4* const to = reinterpret_cast<float4*>(a.partial);
-      const int part = parts_of(g).slot(static_cast<int>(blockIdx.x));
-#pragma unroll 1
-      for (int c = 0; c < D; c += 16) {
-        uint32_t o[16];
-        tmem_ld16(t_o + c, o);
-        tmem_ld_wait_for(o);
-#pragma unroll
-        for (int b = 0; b < 16; ++b) o[b] = __float_as_uint(__uint_as_float(o[b]) * f);
-        if (turns) {                          // slot 0 adds slot 1's sums to its own
-          if (slot == 1) {
-#pragma unroll
-            for (int b = 0; b < 4; ++b)
-              its[32 * b] = make_float4(__uint_as_float(o[4 * b]), __uint_as_float(o[4 * b + 1]), __uint_as_float(o[4 * b + 2]), __uint_as_float(o[4 * b + 3]));
-          }
-          named_bar_sync(across, 64);
-          if (slot == 0) {
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-              const float4 x = its[32 * b];
-              o[4 * b] = __float_as_uint(__uint_as_float(o[4 * b]) + x.x);
-              o[4 * b + 1] = __float_as_uint(__uint_as_float(o[4 * b + 1]) + x.y);
-              o[4 * b + 2] = __float_as_uint(__uint_as_float(o[4 * b + 2]) + x.z);
-              o[4 * b + 3] = __float_as_uint(__uint_as_float(o[4 * b + 3]) + x.w);
-            }
-          }
-          named_bar_sync(across, 64);
-          if (slot == 1) continue;
-        }
-        if (whole) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(o[8 * h + 2 * e]), __uint_as_float(o[8 * h + 2 * e + 1]));
-              w[e] = *reinterpret_cast<const uint32_t*>(&b);
-            }
-            const int chunk = c / 8 + h;
-            *reinterpret_cast<uint4*>(own_rows + chunk / 8 * (kTile * 128) + lane * 128 + ((chunk % 8 ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        } else if (real) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            to[(static_cast<long long>(part) * (D / 4) + c / 4 + e) * kChunkRows + row] =
-                make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
-        }
-      }
-      if (whole && !(turns && slot == 1)) {
-        __syncwarp();
-        constexpr int kLanes = D / 8, kTogether = 32 / kLanes;
-        int column;
-        const int token = token_of(column);
-        const long long place = (g.q_first + token) * a.out_stride + column;
-        const int first_row = (turns ? 0 : slot * kSlotRows) + warp % 4 * 32, chunk = lane % kLanes;
-#pragma unroll 4
-        for (int at = 0; at < 32; at += kTogether) {
-          const int line = at + lane / kLanes;
-          const long long begin = __shfl_sync(0xffffffffu, place, line);
-          const uint4 p = *reinterpret_cast<const uint4*>(own_rows + chunk / 8 * (kTile * 128) + line * 128 + ((chunk % 8 ^ (line & 7)) << 4));
-          if (first_row + line < g.rows) *(reinterpret_cast<uint4*>(a.out + begin) + chunk) = p;
-        }
-      }
-      if (real && !whole) reinterpret_cast<float4*>(a.partial + 2ll * piece.ctas * kChunkRows * D)[static_cast<long long>(part) * kChunkRows + row] = mine;
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.o_empty[slot]);
-    }
-    if (!whole) {
-      const Parts parts = parts_of(g);
-      __threadfence();
-      named_bar_sync(1, kSoftmaxThreads);
-      if (tid == 0) {
-        const bool is_last = atomicAdd(a.tickets + parts.first, 1) == parts.last - parts.first;
-        if (is_last) a.tickets[parts.first] = 0;
-        s_plan.last = is_last;
-      }
-      named_bar_sync(1, kSoftmaxThreads);
-      if (s_plan.last) {
-        __threadfence();
-        join_columns<D>(a, g.q_first, g.row0, g.head, g.rows, piece.ctas, parts, tid, kSoftmaxThreads);
-      }
-    }
-    if (tid == 0) ++sh.finished;
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&sh.segment_empty[segment & 3]);
     ++segment;
   }
 }
@@ -1132,7 +1147,7 @@ kv4_chunk_kernel(const __grid_constant__ AttentionArgs a, int* __restrict__ stat
   // 512 threads at 128 registers: 256 softmax threads at 176, 128 converting ones at 88 and 128 others at 72, until the roles are done.
   if (warp < kSoftmaxWarps) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
-    softmax_role<D>(a, sh, s_plan, smem, tmem, piece);
+    softmax_role<D>(a, sh, s_plan, smem, piece);
     asm volatile("setmaxnreg.dec.sync.aligned.u32 128;");
   } else if (warp < 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
