@@ -15,6 +15,12 @@
 // n comes from a bound, the row's largest score of the first tile times that tile's largest value scale.  That is near enough while the tile's
 // scales are within a factor of 4 (the largest P is then 2^3 at least, and what f16 drops 2^-28 of it at most); a tile whose scales are
 // further apart takes the products' own largest, as decoding does.
+//
+// What bounds it is a slot's chain of scores, weights and product: a tile of 256 rows takes 4700 clocks, in which the exponentials' units work for
+// 2048 and the tensor core for 2048 (heads of 128); leaving all exponentials out gains 9 %, seven of eight MMAs 6 %.  A tile of a unit that takes
+// turns takes 3700: its conversion 2800, and loads that find as much on its way as the L1 beside 214 KB of shared memory holds.  A unit costs
+// some 14000 clocks besides its tiles.  A prompt of 8192 tokens, 32 heads over 8: 660 us, 833 TFLOP/s of what is visible; 512 tokens behind 40000
+// positions with heads of 64: 338 us, 493 TFLOP/s (softmax work is twice that of heads of 128 per flop).
 #include "kv4_chunk.cuh"
 #include "stream_scratch.h"
 
@@ -26,9 +32,8 @@ constexpr int kTile = 128;             // positions per tile: two pages
 constexpr int kChunkRows = 256;
 constexpr int kChunkThreads = 512;     // 8 softmax warps, 4 converting ones, then MMAs, planning, two idle ones
 constexpr int kSoftmaxWarps = 8, kSoftmaxThreads = 256;
-// What a unit costs besides its tiles, in tiles.  With 2, 3 and 4: prompts of 8192 tokens in all 812, 681 and 660 us (a piece that ends inside a
-// unit pays for a join, and pieces of few units each get one more), eight sequences of 1 to 250 new tokens 77, 81 and 85; with 6 and 10 both
-// lost, 4 and 16 % more for the latter.
+// What a unit costs besides its tiles, in tiles.  With 2, 3 and 4: a prompt of 8192 tokens 812, 681 and 660 us (its first pieces hold many short
+// units), eight sequences of 1 to 250 new tokens 77, 81 and 85; with 6 and 10 both took longer.
 constexpr int kChunkExtra = 4;
 constexpr int kSlotRows = 128;         // units of at most so many rows use one slot for their even tiles and one for their odd ones
 // (To the plan a tile of those is a tile like any other: its conversion, 3700 clocks, is hidden behind nothing, and a tile of 256 rows takes 4700.

@@ -12,7 +12,7 @@ constexpr int kThreads = 256;
 // Vectors that a group of lanes has under way.  Two instead of four: writing 8192 tokens 98 us instead of 82, reading 40,000 rows 57 instead
 // of 53; eight: 53 as well.
 constexpr int kWriteHeads = 4, kReadVectors = 4;
-constexpr int kFullGroups = 64;                    // groups per SM that are enough to keep it busy
+constexpr int kFullGroups = 64;                    // groups per SM that are enough to keep it busy: fewer take one vector each
 
 struct Write4Args {
   const __nv_bfloat16 *q, *k, *v, *q_weight, *k_weight;
@@ -216,6 +216,8 @@ __global__ void __launch_bounds__(kThreads, HEADS > 1 ? 4 : 1) kv4_write_kernel(
 }
 
 // D / 8 lanes have a vector, eight dimensions each, and EACH neighbouring ones (heads of keys, then of values) of a row at a time.
+// 40,000 rows of 8 key heads of 128, in bf16: 46 to 53 us.  The bytes take 32, but rows from all over the cache bring whole sectors of 32 bytes
+// for 8 of group scales and 4 of a scale: 116 MB are read for 49.
 template <int D, typename Out, int EACH>
 __global__ void __launch_bounds__(kThreads) kv4_read_kernel(KvCache c, const int32_t* __restrict__ slots, unsigned rows, int first_kind, int kinds,
                                                             Out* __restrict__ k_out, Out* __restrict__ v_out) {
