@@ -311,6 +311,14 @@ def test_chunks_match_the_definition(q_lens, kv_lens, window, HQ, HK, D, pkg, kv
     _check_attention(_attend(pkg, inputs, window=window), *kv4.attention(*inputs, window=window))
 
 
+@pytest.mark.parametrize("window", [130, 257, 389, 1000, 1027])
+@pytest.mark.parametrize("HQ,HK,D", [(16, 4, 128), (16, 16, 64), (64, 1, 128)])
+def test_windows_whose_first_tile_shows_a_few_positions(window, HQ, HK, D, pkg, kv4):
+    """Scores far apart, and rows whose references come from one position, two, three of a tile."""
+    inputs = _attention_inputs(kv4, [300, 140], [3000, 1500], HQ, HK, D, seed=14, q_scale=8.0)
+    _check_attention(_attend(pkg, inputs, window=window), *kv4.attention(*inputs, window=window))
+
+
 @pytest.mark.parametrize("batch", [128, 129, 300, 1000])
 @pytest.mark.parametrize("new_tokens", ["one", "few", "chunk"])
 @pytest.mark.parametrize("D", [64, 128])
