@@ -32,9 +32,9 @@ constexpr int kTile = 128;             // positions per tile: two pages
 constexpr int kChunkRows = 256;
 constexpr int kChunkThreads = 512;     // 8 softmax warps, 4 converting ones, then MMAs, planning, two idle ones
 constexpr int kSoftmaxWarps = 8, kSoftmaxThreads = 256;
-// What a unit costs besides its tiles, in tiles.  With 2, 3 and 4: a prompt of 8192 tokens 812, 681 and 660 us (its first pieces hold many short
-// units), eight sequences of 1 to 250 new tokens 77, 81 and 85; with 6 and 10 both took longer.
-constexpr int kChunkExtra = 4;
+// What a unit costs besides its tiles, in tiles.  With 2, 3, 4 and 5: a prompt of 8192 tokens 789, 660, 662 and 656 us (its first pieces hold many
+// short units), two chunks with a window 142, 146, 141 and 140, eight sequences of 1 to 250 new tokens 85, 81, 83 and 82.
+constexpr int kChunkExtra = 5;
 constexpr int kSlotRows = 128;         // units of at most so many rows use one slot for their even tiles and one for their odd ones
 // (To the plan a tile of those is a tile like any other: its conversion, 3700 clocks, is hidden behind nothing, and a tile of 256 rows takes 4700.
 // Counted as half of one: eight sequences of 1 to 250 new tokens 84 us instead of 82.)
@@ -828,8 +828,9 @@ template <int D>
 __device__ __forceinline__ void join_columns(const AttentionArgs& a, int q_first, int unit_row0, int head, int rows, int ctas, const Parts& parts, int thread, int threads) {
   const float4* const stats = reinterpret_cast<const float4*>(a.partial + 2ll * ctas * kChunkRows * D);
   const float4* const sums = reinterpret_cast<const float4*>(a.partial);
-  for (int i = thread; i < kChunkRows * (D / 16); i += threads) {
-    const int row = i % kChunkRows, d16 = i / kChunkRows;
+  const int across = (rows + 31) / 32 * 32;      // (whole warps of neighbouring rows: the join of a unit of 4 rows 2 us instead of 10, of 256 rows 8)
+  for (int i = thread; i < across * (D / 16); i += threads) {
+    const int row = i % across, d16 = i / across;
     if (row >= rows) continue;
     float m = -INFINITY, n = -INFINITY, l = 0.0f, o[16] = {};
 #pragma unroll 2
