@@ -303,10 +303,12 @@ __device__ __forceinline__ void mma_role(ChunkShared& sh, uint8_t* smem, uint32_
 }
 
 // ---------------------------------------------------------------- codes to f16, a thread per position (four warps)
-// 32 bytes that are read once
+// 32 bytes that are read once.  Two loads, since a cache and its pages begin at any multiple of 16 bytes.  (One of 32, where they begin at multiples
+// of that, is no faster: 512 tokens behind 40000 positions 343 us by one and 342 by two, with heads of 128 379 and 374; and in lines that
+// stay in the L1 383.)
 __device__ __forceinline__ void ld_global_32(const void* p, uint4& a, uint4& b) {
-  asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w) : "l"(p));
+  asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w) : "l"(p));
+  asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4 + 16];" : "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w) : "l"(p));
 }
 __device__ __forceinline__ void st_shared_16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
