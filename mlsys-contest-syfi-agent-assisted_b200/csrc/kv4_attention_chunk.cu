@@ -534,7 +534,10 @@ __device__ __forceinline__ void rescale_sums(uint32_t t_o, const float (&fade)[4
   tmem_st_wait();
 }
 
-// The rows' largest scores of 64 positions, times the keys' scales and in units of the rows'.
+// A score is S times (its key's scale times its row's unit), here and below: a row of q is kept at most 2^120 times its size, so that S times the
+// key's scale alone can run over where tiny queries meet huge keys, although the score is an ordinary number.
+
+// The rows' largest scores of 64 positions.
 template <bool MASKED>
 __device__ __forceinline__ void largest_scores(const TileRows& r, int h, const uint32_t (&s)[2][32], float (&top)[4]) {
   const int column = 64 * h + threadIdx.x % 4 * 2;
@@ -542,10 +545,12 @@ __device__ __forceinline__ void largest_scores(const TileRows& r, int h, const u
 #pragma unroll
   for (int row = 0; row < 4; ++row) {
     const int2 see = MASKED ? row_bounds(r, row) : make_int2(0, 0);
+    const uint64_t unit = f32x2_pack(r.unit[row], r.unit[row]);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
+      const uint64_t worth = f32x2_mul(ld_shared_pair(r.scales + 4 * (64 * h + 8 * i)), unit);
       float x0, x1;
-      f32x2_unpack(f32x2_mul(f32x2_pack_bits(s[row / 2][4 * i + 2 * (row % 2)], s[row / 2][4 * i + 2 * (row % 2) + 1]), ld_shared_pair(r.scales + 4 * (64 * h + 8 * i))), x0, x1);
+      f32x2_unpack(f32x2_mul(f32x2_pack_bits(s[row / 2][4 * i + 2 * (row % 2)], s[row / 2][4 * i + 2 * (row % 2) + 1]), worth), x0, x1);
       const int at = column + 8 * i;
       if (!MASKED || (there && at >= see.x && at <= see.y)) top[row] = fmaxf(top[row], x0);
       if (!MASKED || (there && at + 1 >= see.x && at + 1 <= see.y)) top[row] = fmaxf(top[row], x1);
@@ -576,9 +581,9 @@ __device__ __forceinline__ bool half_weights(const TileRows& r, int h, const uin
     const uint64_t ks = ld_shared_pair(r.scales + 4 * (64 * h + 8 * i)), vs = ld_shared_pair(r.scales + 4 * (kTile + 64 * h + 8 * i));
 #pragma unroll
     for (int row = 0; row < 4; ++row) {
-      const uint64_t x = f32x2_mul(f32x2_pack_bits(s[row / 2][4 * i + 2 * (row % 2)], s[row / 2][4 * i + 2 * (row % 2) + 1]), ks);
+      const uint64_t worth = f32x2_mul(ks, f32x2_pack(r.unit[row], r.unit[row]));
       float x0, x1;
-      f32x2_unpack(f32x2_fma(x, f32x2_pack(r.unit[row], r.unit[row]), f32x2_pack(shift[row], shift[row])), x0, x1);
+      f32x2_unpack(f32x2_fma(f32x2_pack_bits(s[row / 2][4 * i + 2 * (row % 2)], s[row / 2][4 * i + 2 * (row % 2) + 1]), worth, f32x2_pack(shift[row], shift[row])), x0, x1);
       x0 = ex2(x0);
       x1 = ex2(x1);
       if (GENERAL) {
@@ -612,14 +617,16 @@ __device__ __forceinline__ void largest_products(const TileRows& r, int h, const
 #pragma unroll
   for (int row = 0; row < 4; ++row) {
     const int2 see = row_bounds(r, row);
+    const uint64_t unit = f32x2_pack(r.unit[row], r.unit[row]), from = f32x2_pack(shift[row], shift[row]);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
+      const uint64_t worth = f32x2_mul(ld_shared_pair(r.scales + 4 * (64 * h + 8 * i)), unit);
       float x0, x1, v0, v1;
-      f32x2_unpack(f32x2_mul(f32x2_pack_bits(s[row / 2][4 * i + 2 * (row % 2)], s[row / 2][4 * i + 2 * (row % 2) + 1]), ld_shared_pair(r.scales + 4 * (64 * h + 8 * i))), x0, x1);
+      f32x2_unpack(f32x2_fma(f32x2_pack_bits(s[row / 2][4 * i + 2 * (row % 2)], s[row / 2][4 * i + 2 * (row % 2) + 1]), worth, from), x0, x1);
       f32x2_unpack(ld_shared_pair(r.scales + 4 * (kTile + 64 * h + 8 * i)), v0, v1);
       const int at = column + 8 * i;
-      if (there && at >= see.x && at <= see.y) most[row] = fmaxf(most[row], ex2(fmaf(x0, r.unit[row], shift[row])) * v0);
-      if (there && at + 1 >= see.x && at + 1 <= see.y) most[row] = fmaxf(most[row], ex2(fmaf(x1, r.unit[row], shift[row])) * v1);
+      if (there && at >= see.x && at <= see.y) most[row] = fmaxf(most[row], ex2(x0) * v0);
+      if (there && at + 1 >= see.x && at + 1 <= see.y) most[row] = fmaxf(most[row], ex2(x1) * v1);
     }
   }
 }
@@ -638,7 +645,7 @@ __device__ __forceinline__ void set_references(const TileRows& r, float largest,
   }
 #pragma unroll
   for (int row = 0; row < 4; ++row) {
-    top[row] = quad_max(top[row]) * r.unit[row];
+    top[row] = quad_max(top[row]);
     if (top[row] > m[row]) {
       l[row] *= ex2(m[row] - top[row]);        // (0 for a row that had seen nothing)
       m[row] = top[row];
@@ -700,7 +707,7 @@ __device__ __forceinline__ void tile_weights(ChunkShared& sh, const TileRows& r,
       largest_scores<true>(r, h, s, highest);
 #pragma unroll
       for (int row = 0; row < 4; ++row) {
-        const float bound = fmaf(quad_max(highest[row]), r.unit[row], shift[row]) + lg2(largest), up = bound > 15.0f ? bound - kProductHeadroom : 0.0f;
+        const float bound = quad_max(highest[row]) + shift[row] + lg2(largest), up = bound > 15.0f ? bound - kProductHeadroom : 0.0f;
         fade[row] = ex2(-up);
         n[row] += up;
         shift[row] -= up;
@@ -805,8 +812,7 @@ __device__ __forceinline__ void put_queries(const __nv_bfloat16* q, long long mi
       const int chunk = 4 * (j ^ (row & 1)) + part;
       *reinterpret_cast<uint4*>(tile + chunk / 8 * (kTile * 128) + in_tile * 128 + ((chunk % 8 ^ (in_tile & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
     }
-    // (a scale of zero keeps a factor, f32's smallest normal number, so that -infinity stays what it is)
-    if (part == 0) units[row] = fmaxf(fabsf(scale_log2) * __int_as_float((127 - k) << 23), 1.17549435e-38f);
+    if (part == 0) units[row] = fabsf(scale_log2) * __int_as_float((127 - k) << 23);
   }
 }
 
