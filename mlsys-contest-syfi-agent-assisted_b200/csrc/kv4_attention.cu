@@ -44,12 +44,15 @@ __device__ __forceinline__ void both_halves(uint32_t v, uint32_t& lo, uint32_t& 
 // Which position an index of the scores stands for is chosen so that both reads of the rows of 32 bytes are free of bank conflicts: index i
 // of eight is position i ^ (i >> 2 & 1).
 //
-// What bounds it is instructions: 1221 of a warp for a page of 64 positions of 128 dimensions, a third of them conversions, which issue at
-// half a clock's rate; 62 % of the issue slots are taken.  32 sequences of 65536 positions, 4 key heads: 256 us, where the loads alone
-// take 210 and the bytes 195 at the rate of a copy.  Three blocks of 168 registers to an SM; four of 128: 264.
+// What bounds it is the latency of a page's steps with three warps to a scheduler: 1221 instructions of a warp for 64 positions of 128
+// dimensions, a third of them conversions, which issue at half a clock's rate, take 60 % of the issue slots, and the warps' conversions, MMAs and
+// exponentials overlap one another's no further.  32 sequences of 65536 positions, 4 key heads: 252 to 264 us, where the loads alone take
+// 210 and the bytes 195 at the rate of a copy; with heads of 64 170.  Three blocks of 168 registers to an SM; four of 128: 264.  With 16 rows
+// (two blocks of 255 registers, two of them in local memory for a while: 16 bytes) a page's conversions serve twice the rows.
 //
-// kDecodeExtra is what a unit costs besides its pages, in pages: the prologue, its end, the join.  24 sequences of 300 to 30000 positions, 8 key
-// heads, with 1, 3, 6, 8 and 12: 78, 73, 64, 64 and 65 us (of which the plan has since lost 9).
+// kDecodeExtra is what a unit costs besides its pages, in pages: the prologue, its end, the join.  With 3, 6 and 9: 24 sequences of 300 to 30000
+// positions with 8 key heads 64, 58 and 58 us (8 rows), 98, 83 and 80 (16 rows), with heads of 64 47, 42 and 41 (4 rows), 74, 62 and 58
+// (16 rows); 200 sequences of 100 to 3000 positions, heads of 64, 64, 55 and 56.
 constexpr int kDecodeExtra = 6;
 constexpr float kFarBehind = 1.2676506e30f;   // 2^100 between the references of the two sums: the values' follows
 constexpr int kWarps = 4;
@@ -713,7 +716,11 @@ extern "C" int syfi_kv4_attention(const void* q, int64_t q_stride, const void* c
   //   decoding, 8 rows  141  141  258  258  373  489
   //   decoding, 16           142  202  202  370  372
   //   chunks            494  495  495  495  498  499
-  // One sequence of 65536: 38, 40, 51, 52, 64, 78 - 53, 53, 68, 71 from 12 rows - 111 to 125.
+  // One sequence of 65536: 38, 40, 51, 52, 64, 78 - 53, 53, 68, 71 from 12 rows - 111 to 125.  Heads of 64, with the kernel that is taken: 104 (4 and
+  // 8 rows), 147 (12, 16), 262 (24), 265 (32), 396 (from 33 on); one sequence 36, 37, 44, 43, 55, 56 and 73.
+  // The average is of all rows of q, those of no sequence among them.  It is far from right where few sequences of many rows meet many of few: 60
+  // sequences of one token beside 400 tokens behind 60000 positions go to decoding and take 1948 us, in two calls 501; 64 sequences of 16384
+  // positions beside a prompt of 2048 tokens go to the chunk kernel, 1093 and 347.
   const int64_t rows = (tokens * a.group + batch - 1) / batch;
   if (rows > 32) {
     int rc = SYFI_KV4_OK;

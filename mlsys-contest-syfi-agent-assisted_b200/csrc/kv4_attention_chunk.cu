@@ -14,13 +14,20 @@
 //
 // n comes from a bound, the row's largest score of the first tile times that tile's largest value scale.  That is near enough while the tile's
 // scales are within a factor of 4 (the largest P is then 2^3 at least, and what f16 drops 2^-28 of it at most); a tile whose scales are
-// further apart takes the products' own largest, as decoding does.
+// further apart takes the products' own largest, as decoding does.  That reads the scores three times instead of once and takes the exponentials
+// twice, and the value scales of a model's tokens seldom lie within a factor of 4 over 128 positions: the times below, of scales within a factor of 3, are
+// then 1600 us (the prompt), 860 (the chunk with heads of 64), 910 (with heads of 128, 375), 240 (two chunks with a window, 139) and 130 (eight
+// sequences of 1 to 250 new tokens, 80), whether the scales have a log-normal spread by factors of 2 or 4 or are those that the writing kernel
+// leaves of normal vectors times 0.3 .. 1.3.  One scale far below the others costs its own tile only.
+// Scores that are far apart let weights outgrow the reference, which are then done again: with a standard deviation of 4 instead of 1.5
+// 1245 us (the prompt), 528, 598, 254 and 125, with 8 1366, 576, 664, 254 and 135.
 //
 // What bounds it is a slot's chain of scores, weights and product: a tile of 256 rows takes 4700 clocks, in which the exponentials' units work for
-// 2048 and the tensor core for 2048 (heads of 128); leaving all exponentials out gains 9 %, seven of eight MMAs 6 %.  A tile of a unit that takes
-// turns takes 3700: its conversion 2800, and loads that find as much on its way as the L1 beside 214 KB of shared memory holds.  A unit costs
-// some 14000 clocks besides its tiles.  A prompt of 8192 tokens, 32 heads over 8: 660 us, 833 TFLOP/s of what is visible; 512 tokens behind 40000
-// positions with heads of 64: 338 us, 493 TFLOP/s (softmax work is twice that of heads of 128 per flop).
+// 2048 and the tensor core for 2048 (heads of 128); leaving all exponentials out gains 9 %, seven of eight MMAs 6 %: half of the issue slots are
+// empty, each slot waits for itself.  A tile of a unit that takes turns takes 3700: its conversion 2800, and loads that find as much on its way as
+// the L1 beside 214 KB of shared memory holds.  A unit costs some 14000 clocks besides its tiles.  A prompt of 8192 tokens, 32 heads over 8:
+// 647 to 660 us, 833 TFLOP/s and more of what is visible; 512 tokens behind 40000 positions with heads of 64: 328 to 338 us, 493 TFLOP/s
+// and more (softmax work is twice that of heads of 128 per flop).
 #include "kv4_chunk.cuh"
 #include "stream_scratch.h"
 
@@ -32,11 +39,13 @@ constexpr int kTile = 128;             // positions per tile: two pages
 constexpr int kChunkRows = 256;
 constexpr int kChunkThreads = 512;     // 8 softmax warps, 4 converting ones, then MMAs, planning, two idle ones
 constexpr int kSoftmaxWarps = 8, kSoftmaxThreads = 256;
-// What a unit costs besides its tiles, in tiles.  With 2, 3, 4 and 5: a prompt of 8192 tokens 789, 660, 662 and 656 us (its first pieces hold many
-// short units), two chunks with a window 142, 146, 141 and 140, eight sequences of 1 to 250 new tokens 85, 81, 83 and 82.
+// What a unit counts besides its tiles, in tiles: by its clocks three, fitted five, which is flat around there.  With 3, 5 and 8: a prompt of 8192
+// tokens 661, 647 and 670 us (its first pieces hold many short units), three of 1000 85, 84 and 88, two of 2500 with heads of 64 130, 131 and
+// 138; two chunks with a window of 1024 141, 138 and 137, one of 2000 tokens with a window of 4096 202, 199 and 201; eight sequences of 1 to
+// 250 new tokens 78, 75 and 73, twelve with heads of 64 89, 86 and 85.
 constexpr int kChunkExtra = 5;
 constexpr int kSlotRows = 128;         // units of at most so many rows use one slot for their even tiles and one for their odd ones
-// (To the plan a tile of those is a tile like any other: its conversion, 3700 clocks, is hidden behind nothing, and a tile of 256 rows takes 4700.
+// (To the plan a tile of those is a tile like any other: it takes 3700 clocks, as its conversion is hidden behind nothing, and a tile of 256 rows 4700.
 // Counted as half of one: eight sequences of 1 to 250 new tokens 84 us instead of 82.)
 using ChunkPlan = Plan<kTile, kChunkRows, kChunkExtra>;
 using ChunkCursor = Cursor<kTile, kChunkRows, kChunkExtra>;
@@ -49,7 +58,7 @@ constexpr int kStatusTimeout = 401;
 constexpr float kProductHeadroom = 5.0f;
 constexpr float kProductGrowth = 9.0f;      // (where the reference is set from a bound that may be twice too low)
 constexpr float kBlindGrowth = 1.0f;        // (where few positions gave it: 2^9 too low, it would not last)
-constexpr float kNear = 0.25f;              // a tile's value scales are so near one another, or the products themselves are asked
+constexpr float kNear = 0.25f;              // a tile's value scales are so near one another, or the products themselves are asked (both sides: at the top)
 constexpr float kFarAbove = 60.0f;          // a row whose n lies so many octaves above m, because of a huge value, keeps its weights in units of m
 
 template <int D>

@@ -78,8 +78,9 @@ enum Turn { kNeighbours, kHalves, kWholeHalves };
 // Where the whole vector is rotated by halves, or not at all, a lane has four neighbouring dimensions of each half instead: both of a pair
 // are its own, and it keeps half as many cosines and sines (8192 tokens of 64 query and 2 * 8 cache heads of 128: 82 us instead of 88).
 //
-// The bytes take 48 us there.  What keeps it from them is the instructions of a key or value (its quotients and conversions) with few warps
-// to hide their latencies; four blocks to an SM, 64 registers a thread: with three 92 us, with five (spills) 82.
+// The bytes take 48 us there.  What keeps it from them is the latency of a key's or value's instructions (its quotients and conversions: 67 % of the
+// issue slots) with few warps to hide it, and those registers set the occupancy of the queries' warps too; four blocks to an SM, 64 registers a
+// thread: with three 92 us, with five (spills) 82.  With halves of part of the dimensions four heads spill 12 bytes.
 template <int D, Turn TURN, int HEADS>
 __global__ void __launch_bounds__(kThreads, HEADS > 1 ? 4 : 1) kv4_write_kernel(const __grid_constant__ Write4Args a) {
   constexpr int kLanes = D / 8, kGroups = 32 / kLanes, kRun = kGroups * HEADS;
@@ -219,8 +220,9 @@ __global__ void __launch_bounds__(kThreads, HEADS > 1 ? 4 : 1) kv4_write_kernel(
 }
 
 // D / 8 lanes have a vector, eight dimensions each, and EACH neighbouring ones (heads of keys, then of values) of a row at a time.
-// 40,000 rows of 8 key heads of 128, in bf16: 46 to 53 us.  The bytes take 32, but rows from all over the cache bring whole sectors of 32 bytes
-// for 8 of group scales and 4 of a scale: 116 MB are read for 49.
+// 40,000 rows of 8 key heads of 128, in bf16: 46 to 53 us, in f32 102.  The bytes take 32; rows from all over the cache bring whole sectors of 32
+// bytes for 8 of group scales and 4 of a scale, 116 MB for 49, which makes it 35.  The rest is instructions: 31 million of a warp, 65 % of the
+// issue slots (a lane's address arithmetic, byte loads of group scales, a scale that every lane of a vector loads).
 template <int D, typename Out, int EACH>
 __global__ void __launch_bounds__(kThreads) kv4_read_kernel(KvCache c, const int32_t* __restrict__ slots, unsigned rows, int first_kind, int kinds,
                                                             Out* __restrict__ k_out, Out* __restrict__ v_out) {
