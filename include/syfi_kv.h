@@ -70,8 +70,8 @@ int syfi_kv_read(const void* cache, int64_t num_pages, int64_t page_stride, int3
  * Sums are in f32.  A weight is rounded to f16 (2^-12 of it on average); one 2^-32 below the row's largest may not be added, nor,
  * with few rows, one whose value is 2^-32 below the row's largest.  With more than 16 rows per sequence and key head on average
  * q is held to 2^-17 of its row's largest dimension.
- * There a head of q whose largest dimension is below 2^-100 may give NaN where a score is beyond 2^4 (it is kept at most 2^120 times its size, and
- * that times a key's scale is to stay in f32's range).
+ * There the product of a query and a key is formed with the query's largest dimension brought to 2^7 .. 2^8 (by 2^120 at most); where that
+ * product is beyond f32's range, results may be NaN.
  * Calls on different streams may run at the same time: every stream has a scratch buffer of its own (up to 45 MB), which
  * grows on demand (that waits for the device).  Up to eight streams of a device hold one; a ninth waits for the device and takes
  * over the least recently used.  A captured graph has buffers of its own, one for each stream that was captured into it, until it is

@@ -53,7 +53,8 @@ int syfi_kv4_read(const void* cache, int64_t num_pages, int64_t page_stride, int
  * Positions that a query does not see do not touch its result, whatever the cache holds there.  Scales and group scales are not
  * negative.  A query, or a seen position with a scale or a key's group scale that is not finite, makes its heads' results NaN; a value's
  * group scale that is not finite those of its dimensions at least.
- * Where `scale` times a query's largest dimension, or that times a seen key's largest, is beyond f32's range, results may be NaN.
+ * Where `scale` times a query's largest dimension, or that times a seen key's largest, is beyond f32's range, results may be NaN; where the
+ * first is below 2^-110, scores are coarser than f32.
  * Sums are in f32.  A weight times its value's scale is rounded to f16 (2^-12 of it on average); one 2^-28 below the row's largest
  * may not be added, with up to 32 rows per sequence and key head on average one 2^-32 below.  Codes times group scales are exact.
  * Scratch memory by stream and by captured graph as for syfi_paged_attention, in buffers of its own. */
