@@ -194,8 +194,10 @@ __device__ __forceinline__ void plan_role(const AttentionArgs& a, const ChunkPla
     mbar_arrive(&sh.segment_full[ring.stage]);
     if (!more) break;
     // Its queries, for the softmax warps to find in L2: they ask for them only when the unit in front is done.
-    for (int token = g.row0 / a.group; token <= (g.row0 + g.rows - 1) / a.group; ++token)
-      prefetch_l2(a.q + (g.q_first + token) * a.q_stride + g.head * a.group * D, a.group * D * 2);
+    for (int token = g.row0 / a.group; token <= (g.row0 + g.rows - 1) / a.group; ++token) {
+      const int from = max(g.row0 - token * a.group, 0), to = min(g.row0 + g.rows - token * a.group, a.group);      // of the token's query heads
+      prefetch_l2(a.q + (g.q_first + token) * a.q_stride + (g.head * a.group + from) * D, (to - from) * D * 2);
+    }
     ring.next();
     at.advance(plan, here);
   }
